@@ -8,7 +8,7 @@ from __future__ import annotations
 
 __all__ = ["HotSketch", "SKEmbeddingBag", "SKEmbeddingGroup", "attach_optimizer", "sizing", "synthetic", "CafeError",
            "INSERT_PARALLEL", "INSERT_SEQUENTIAL", "load_library", "profile", "SigmodSketch", "SigmodSKEmbeddingBag",
-           "dlrm_harness", "sharded"]
+           "dlrm_harness", "sharded", "fused_linear", "fused_mlp", "FusedMLP", "AdamW"]
 
 INSERT_PARALLEL, INSERT_SEQUENTIAL = 0, 1
 
@@ -33,10 +33,18 @@ def __getattr__(name):
         load_library()
         from . import sigmod
         return getattr(sigmod, name)
+    if name in ("fused_linear", "fused_mlp", "FusedMLP"):
+        load_library()
+        from . import dense
+        return getattr(dense, name)
+    if name == "AdamW":
+        load_library()
+        from .optim import AdamW
+        return AdamW
     if name == "CafeError":
         from ._lib import CafeError
         return CafeError
-    if name in ("sizing", "synthetic", "profile", "sharded", "dlrm_harness", "sigmod"):
+    if name in ("sizing", "synthetic", "profile", "sharded", "dlrm_harness", "sigmod", "dense", "optim"):
         import importlib
         return importlib.import_module(f".{name}", __name__)
     raise AttributeError(f"module 'cafe_b200' has no attribute {name!r}")

@@ -1,0 +1,274 @@
+"""The dense layers around the embedding path on the library's kernels (csrc/dense_cuda.cu).
+
+fused_linear   y = act(x W^T + b) + residual, differentiable
+fused_mlp      a run of such layers as one node of the autograd graph: one call per direction
+FusedMLP       the Sequential of Linear and activation modules that the reference's create_mlp builds
+               (dlrm_s_pytorch.py:213-251), computed by fused_mlp; same parameters, same state_dict
+
+Tensors are CUDA tensors of one type (fp32, bf16 or fp16); sums are fp32.  Kernels go to the current stream of the tensors'
+device.  The gradients are those of first order: differentiating them again raises.  Captured into a CUDA graph, forward and
+backward follow torch's rules for whole-network capture (warm-up on a side stream, no autograd graph of the same leaves alive
+from outside the capture)."""
+from __future__ import annotations
+
+import ctypes
+from contextlib import nullcontext
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .sketch import _stream
+
+ACTIVATIONS = {"none": 0, "relu": 1, "sigmoid": 2, "gelu": 3, "silu": 4}
+_NONE, _RELU = 0, 1
+_SLOPE_NONE, _SLOPE_VALUES, _SLOPE_OUTPUT = 0, 1, 2
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+MAX_SIZE, MAX_LAYERS = 8388608, 32
+
+
+def _on(device: torch.device):
+    """The tensors' device as the current one."""
+    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _rows(t: torch.Tensor, cols: int, repeated: bool = False):
+    """t as rows of `cols` contiguous elements at one pitch: (tensor, rows, pitch).  Other layouts are copied; `repeated`:
+    pitch 0 (a row that stands for all) is one."""
+    if t.dim() != 2:
+        t = t.reshape(-1, cols) if cols else t.reshape(t.numel(), 0)
+    m = t.shape[0]
+    if t.numel() == 0:
+        return t, m, cols
+    if cols == 1 or t.stride(1) == 1:
+        ld = t.stride(0)
+        if m == 1:
+            return t, m, cols
+        if ld >= cols or (repeated and ld == 0):
+            return t, m, ld
+    return t.contiguous(), m, cols
+
+
+def _check(x, tensors, what):
+    if not x.is_cuda or x.dtype not in DTYPES:
+        raise ValueError(f"{what} needs CUDA tensors of fp32, bf16 or fp16")
+    for t in tensors:
+        if t is not None and (t.dtype != x.dtype or t.device != x.device):
+            raise ValueError(f"{what}: all tensors must have one type and be on one device")
+
+
+def _check_layer(cols, weight, bias, what):
+    if weight.dim() != 2 or weight.shape[1] != cols:
+        raise ValueError(f"{what}: weight must be [out, {cols}], got {list(weight.shape)}")
+    if bias is not None and (bias.dim() != 1 or bias.shape[0] != weight.shape[0]):
+        raise ValueError(f"{what}: bias must be [{weight.shape[0]}], got {list(bias.shape)}")
+    if max(cols, weight.shape[0]) > MAX_SIZE:
+        raise ValueError(f"{what}: sizes up to {MAX_SIZE}")
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _slope_type(dtype):
+    return torch.float32 if dtype == torch.float32 else torch.float16
+
+
+def _contiguous(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+def _linear(x, weight, bias, residual, act, keep):
+    """The forward call: (x, weight as rows, y, what the backward needs of the activation)."""
+    n, k = weight.shape
+    x2, m, ldx = _rows(x, k)
+    if m > MAX_SIZE:
+        raise ValueError(f"fused_linear: up to {MAX_SIZE} rows")
+    w2, _, ldw = _rows(weight, k)
+    y = torch.empty(*x.shape[:-1], n, dtype=x.dtype, device=x.device)
+    r2, ldr = None, 0
+    if residual is not None:
+        r2, _, ldr = _rows(residual, n, True)
+    slope = None
+    if keep and act != _NONE and not (act == _RELU and residual is None):
+        slope = torch.empty(m, n, dtype=_slope_type(x.dtype), device=x.device)
+    b = _contiguous(bias)
+    with _on(x.device):
+        _lib.check(_lib.load().cafe_linear_forward(x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(b), _ptr(r2), ldr, m, n, k, DTYPES[x.dtype],
+                                                   act, y.data_ptr(), n, _ptr(slope), n, _stream()), "cafe_linear_forward")
+    return x2, w2, y, slope
+
+
+class _FusedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        x2, w2, y, slope = _linear(x, weight, bias, residual, act, True)
+        need = ctx.needs_input_grad
+        kind = _SLOPE_NONE if act == _NONE else _SLOPE_VALUES if slope is not None else _SLOPE_OUTPUT
+        ctx.kind, ctx.shape, ctx.bias = kind, x.shape, bias is not None
+        ctx.save_for_backward(x2 if need[1] else None, w2 if need[0] else None,
+                              None if kind == _SLOPE_NONE else slope if kind == _SLOPE_VALUES else y)
+        ctx.sizes = weight.shape
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_y):
+        x, w, slope = ctx.saved_tensors
+        n, k = ctx.sizes
+        need = ctx.needs_input_grad
+        g, m, ldg = _rows(grad_y, n, True)
+        gx = torch.empty(ctx.shape, dtype=g.dtype, device=g.device) if need[0] else None
+        gw = torch.empty(n, k, dtype=g.dtype, device=g.device) if need[1] else None
+        gb = torch.empty(n, dtype=g.dtype, device=g.device) if need[2] else None
+        if need[0] or need[1] or need[2]:
+            with _on(g.device):
+                _lib.check(_lib.load().cafe_linear_backward(
+                    g.data_ptr(), ldg, _ptr(slope), n, ctx.kind, _ptr(x), k if x is None else _rows(x, k)[2], _ptr(w),
+                    k if w is None else _rows(w, k)[2], m, n, k, DTYPES[g.dtype], _ptr(gx), k, _ptr(gw), k, _ptr(gb), _stream()),
+                    "cafe_linear_backward")
+        return gx, gw, gb, grad_y if need[3] else None, None
+
+
+def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, activation: str = "none",
+                 residual: torch.Tensor | None = None) -> torch.Tensor:
+    """act(x W^T + b) + residual.  x [..., K], weight [N, K], bias [N]; residual broadcasts to [..., N]; activation is one of
+    none, relu, sigmoid, gelu (with erf) and silu.  x, weight and residual may be slices of wider tensors (any pitch
+    between rows).  For the backward the call keeps x, weight and, with an activation, its derivative (fp32 or fp16); of a ReLU
+    without residual the output."""
+    _check(x, (weight, bias, residual), "fused_linear")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"fused_linear: activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
+    if x.dim() < 1:
+        raise ValueError("fused_linear: x must have a last dimension")
+    _check_layer(x.shape[-1], weight, bias, "fused_linear")
+    if residual is not None:
+        shape = x.shape[:-1] + weight.shape[:1]
+        if residual.shape != shape:
+            residual = torch.broadcast_to(residual, shape)   # (raises if it cannot)
+    act = ACTIVATIONS[activation]
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
+                                    (residual is not None and residual.requires_grad)):
+        return _FusedLinear.apply(x, weight, bias, residual, act)
+    return _linear(x, weight, bias, residual, act, False)[2]
+
+
+# ---- a run of layers ---------------------------------------------------------------------------------------
+def _pointers(tensors):
+    return (ctypes.c_void_p * len(tensors))(*[_ptr(t) for t in tensors])
+
+
+def _mlp(x, weights, biases, acts, keep):
+    """The forward call: (x and weights as rows, y of every layer, slope of every layer or None)."""
+    n = len(weights)
+    widths = [weights[0].shape[1]] + [w.shape[0] for w in weights]
+    x2, m, ldx = _rows(x, widths[0])
+    if m > MAX_SIZE:
+        raise ValueError(f"fused_mlp: up to {MAX_SIZE} rows")
+    ws = [_rows(w, w.shape[1]) for w in weights]
+    bs = [_contiguous(b) for b in biases]
+    # rows between the layers start on 16-byte boundaries
+    pitch = [(v + 7) // 8 * 8 for v in widths[1:-1]] + [widths[-1]]
+    ys = [torch.empty(m, p, dtype=x.dtype, device=x.device) for p in pitch[:-1]]
+    ys.append(torch.empty(*x.shape[:-1], widths[-1], dtype=x.dtype, device=x.device))
+    slopes = [torch.empty(m, p, dtype=_slope_type(x.dtype), device=x.device) if keep and a not in (_NONE, _RELU) else None
+              for p, a in zip(pitch, acts)]
+    call = ((ctypes.c_int32 * (n + 1))(*widths), m, x2.data_ptr(), ldx, _pointers([w for w, _, _ in ws]), (ctypes.c_int64 * n)(*[ld for _, _, ld in ws]))
+    with _on(x.device):
+        _lib.check(_lib.load().cafe_mlp_forward(n, *call, _pointers(bs), (ctypes.c_int32 * n)(*acts), DTYPES[x.dtype], _pointers(ys),
+                                                (ctypes.c_int64 * n)(*pitch), _pointers(slopes) if keep else None, _stream()),
+                   "cafe_mlp_forward")
+    return x2, [w for w, _, _ in ws], ys, slopes, pitch
+
+
+class _FusedMLP(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, acts, *params):
+        n = len(params) // 2
+        x2, ws, ys, slopes, pitch = _mlp(x, params[:n], params[n:], acts, True)
+        ctx.acts, ctx.shape, ctx.pitch = acts, x.shape, pitch
+        ctx.save_for_backward(x2, *ws, *ys, *slopes)
+        return ys[-1]
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_y):
+        n, acts = len(ctx.acts), ctx.acts
+        x, *rest = ctx.saved_tensors
+        ws, ys, slopes = rest[:n], rest[n:2 * n], rest[2 * n:]
+        widths = [ws[0].shape[1]] + [w.shape[0] for w in ws]
+        need = ctx.needs_input_grad
+        g, m, ldg = _rows(grad_y, widths[-1], True)
+        new = lambda *shape: torch.empty(*shape, dtype=g.dtype, device=g.device)   # noqa: E731
+        gx = new(*ctx.shape) if need[0] else None
+        gws = [new(*w.shape) if need[2 + l] else None for l, w in enumerate(ws)]
+        gbs = [new(w.shape[0]) if need[2 + n + l] else None for l, w in enumerate(ws)]
+        lib = _lib.load()
+        cw = (ctypes.c_int32 * (n + 1))(*widths)
+        size = lib.cafe_mlp_backward_work(n, cw, m, DTYPES[g.dtype])
+        work = torch.empty(size, dtype=torch.uint8, device=g.device)
+        with _on(g.device):
+            _lib.check(lib.cafe_mlp_backward(
+                n, cw, m, g.data_ptr(), ldg, x.data_ptr(), _rows(x, widths[0])[2], _pointers(ws),
+                (ctypes.c_int64 * n)(*[_rows(w, w.shape[1])[2] for w in ws]), (ctypes.c_int32 * n)(*acts), DTYPES[g.dtype], _pointers(ys),
+                (ctypes.c_int64 * n)(*ctx.pitch), _pointers(slopes), _ptr(gx), widths[0], _pointers(gws), _pointers(gbs),
+                work.data_ptr(), size, _stream()), "cafe_mlp_backward")
+        return (gx, None, *gws, *gbs)
+
+
+def fused_mlp(x: torch.Tensor, weights, biases, activations) -> torch.Tensor:
+    """Layer after layer of act(x W^T + b): weights [N_l, N_{l-1}], biases [N_l] or None, activations by name (see
+    fused_linear).  The values are those of fused_linear layer by layer; between the layers they are held in x's type."""
+    weights, biases, activations = list(weights), list(biases), list(activations)
+    n = len(weights)
+    if not 1 <= n <= MAX_LAYERS or len(biases) != n or len(activations) != n:
+        raise ValueError(f"fused_mlp: one bias (or None) and one activation for each of 1 to {MAX_LAYERS} weights")
+    _check(x, weights + biases, "fused_mlp")
+    if x.dim() < 1:
+        raise ValueError("fused_mlp: x must have a last dimension")
+    cols = x.shape[-1]
+    for w, b, a in zip(weights, biases, activations):
+        if a not in ACTIVATIONS:
+            raise ValueError(f"fused_mlp: activations must be among {sorted(ACTIVATIONS)}, got {a!r}")
+        _check_layer(cols, w, b, "fused_mlp")
+        cols = w.shape[0]
+    acts = [ACTIVATIONS[a] for a in activations]
+    if torch.is_grad_enabled() and (x.requires_grad or any(w.requires_grad for w in weights) or any(b is not None and b.requires_grad for b in biases)):
+        return _FusedMLP.apply(x, acts, *weights, *biases)
+    return _mlp(x, weights, biases, acts, False)[2][-1]
+
+
+_MODULES = {nn.ReLU: "relu", nn.Sigmoid: "sigmoid", nn.SiLU: "silu", nn.Identity: "none"}
+
+
+def _module_activation(m: nn.Module) -> str:
+    if type(m) is nn.GELU and m.approximate == "none":
+        return "gelu"
+    if type(m) not in _MODULES:
+        raise ValueError(f"FusedMLP: no kernel for {m}")
+    return _MODULES[type(m)]
+
+
+class FusedMLP(nn.Sequential):
+    """nn.Sequential of nn.Linear layers, each followed by an activation module or none, computed by fused_mlp."""
+
+    def __init__(self, *layers):
+        super().__init__(*layers)
+        self._plan()
+
+    def _plan(self):
+        linears, acts = [], []
+        for m in self._modules.values():
+            if type(m) is nn.Linear:
+                linears.append(m)
+                acts.append(None)
+            elif not linears or acts[-1] is not None:
+                raise ValueError("FusedMLP: every activation follows a Linear layer")
+            else:
+                acts[-1] = _module_activation(m)
+        return linears, [a or "none" for a in acts]
+
+    def forward(self, x):
+        linears, acts = self._plan()
+        return fused_mlp(x, [m.weight for m in linears], [m.bias for m in linears], acts)

@@ -326,6 +326,52 @@ int cafe_dot_interaction_backward(const float* x_dev, const float* emb_dev, int6
                                   int F, int D, int itself, const float* grad_out_dev, int64_t out_stride, float* grad_x_dev,
                                   float* grad_emb_dev, int64_t gfield_stride, int64_t gsample_stride, void* stream);
 
+/* ---- dense layers (the MLPs around the embedding path: dlrm_s_pytorch.py:213-251, dcn.py:410-422) ------------------
+ * z = x W^T + b, y = act(z) + res for x [M, K], W [N, K], rows `ld` elements apart (ld >= the row's length; elements of a
+ * row are contiguous).  All tensors of a call have one type; sums are fp32.  bias, res and slope may be null; ldr = 0: one
+ * row of res for all.  slope_dev receives act'(z) for the backward, fp32 beside fp32 and fp16 beside 16-bit types.
+ * M, N, K <= CAFE_LINEAR_MAX.  No host synchronisation, no device memory of its own. */
+enum { CAFE_F32 = 0, CAFE_BF16 = 1, CAFE_F16 = 2 };
+enum { CAFE_ACT_NONE = 0, CAFE_ACT_RELU = 1, CAFE_ACT_SIGMOID = 2, CAFE_ACT_GELU = 3, CAFE_ACT_SILU = 4 };
+/* what slope_dev of a backward holds: nothing (no activation), act'(z), or y of a ReLU without residual (y > 0) */
+enum { CAFE_SLOPE_NONE = 0, CAFE_SLOPE_VALUES = 1, CAFE_SLOPE_OUTPUT = 2 };
+#define CAFE_LINEAR_MAX 8388608
+#define CAFE_MLP_MAX_LAYERS 32
+int cafe_linear_forward(const void* x_dev, int64_t ldx, const void* w_dev, int64_t ldw, const void* bias_dev, const void* res_dev, int64_t ldr,
+                        int M, int N, int K, int dtype, int act, void* y_dev, int64_t ldy, void* slope_dev, int64_t lds, void* stream);
+/* gz = gy * act'(z); gx = gz W, gW = gz^T x, gb = column sums of gz; each of the three may be null (not wanted).  ldg = 0: one
+ * row of gy for all. */
+int cafe_linear_backward(const void* gy_dev, int64_t ldg, const void* slope_dev, int64_t lds, int slope_kind, const void* x_dev, int64_t ldx,
+                         const void* w_dev, int64_t ldw, int M, int N, int K, int dtype, void* gx_dev, int64_t ldgx, void* gw_dev, int64_t ldgw,
+                         void* gb_dev, void* stream);
+/* `layers` layers one behind the other: layer l maps widths[l] to widths[l + 1] with acts[l]; its output goes to y_dev[l]
+ * (pitch ldy[l]) and, where slope_dev[l] is not null, act'(z) to slope_dev[l] (same pitch). */
+int cafe_mlp_forward(int layers, const int* widths, int M, const void* x_dev, int64_t ldx, const void* const* w_dev, const int64_t* ldw,
+                     const void* const* bias_dev, const int* acts, int dtype, void* const* y_dev, const int64_t* ldy, void* const* slope_dev,
+                     void* stream);
+/* Its backward: a layer without slope_dev[l] has no activation or a ReLU (taken from y_dev[l]).  gw_dev[l] is [widths[l + 1],
+ * widths[l]] contiguous; gx_dev, gw_dev[l] and gb_dev[l] may be null.  work_dev: cafe_mlp_backward_work bytes, 16-byte aligned,
+ * free again once the call's work on `stream` is done. */
+int64_t cafe_mlp_backward_work(int layers, const int* widths, int M, int dtype);
+int cafe_mlp_backward(int layers, const int* widths, int M, const void* gy_dev, int64_t ldg, const void* x_dev, int64_t ldx,
+                      const void* const* w_dev, const int64_t* ldw, const int* acts, int dtype, const void* const* y_dev, const int64_t* ldy,
+                      const void* const* slope_dev, void* gx_dev, int64_t ldgx, void* const* gw_dev, void* const* gb_dev, void* work_dev,
+                      int64_t work_bytes, void* stream);
+
+/* ---- AdamW over many tensors (the reference's scripts use torch.optim; dlrm_s_pytorch.py:1468-1478) -----------------
+ * One step over `count` tensors of one type: m <- beta1 m + (1 - beta1) g, v <- beta2 v + (1 - beta2) g^2,
+ * p <- p (1 - lr wd) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps), with t = *step_dev[i] + 1, which the call
+ * also writes back.  bits = 32: m, v fp32.  bits = 8: m_dev[i] holds codes of m and v_dev[i] codes of sqrt(v), a byte per
+ * element (8-byte aligned arrays), and mtop_dev[i] / vtop_dev[i] a byte per 256 elements; all zero is the start.  Codes are
+ * rounded at random by (seed, index[i], t, element); index null: i.  ticket_dev: an int that is 0 before the first call and
+ * that no two calls in flight share.  Nothing is read back: the call can be captured into a graph (lr is then fixed). */
+int cafe_adamw_step(int count, void* const* p_dev, const void* const* g_dev, void* const* m_dev, void* const* v_dev, uint8_t* const* mtop_dev,
+                    uint8_t* const* vtop_dev, int64_t* const* step_dev, const int64_t* numel, const int* index, int dtype, int bits,
+                    double lr, double beta1, double beta2, double eps, double weight_decay, uint32_t seed, int* ticket_dev, void* stream);
+/* The values that 8-bit moments stand for: m and sqrt(v) as bf16 (exact). */
+int cafe_adamw_moments(int count, const uint8_t* const* m_dev, const uint8_t* const* mtop_dev, const uint8_t* const* r_dev,
+                       const uint8_t* const* rtop_dev, const int64_t* numel, void* const* m_out_dev, void* const* r_out_dev, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
