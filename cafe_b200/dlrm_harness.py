@@ -1,7 +1,7 @@
 """A DLRM / DCN training harness around the CAFE drop-in, with the reference's flags and step order.
 
 What the reference's model scripts do around the compressed-embedding path (dlrm_s_pytorch.py, dcn.py), kept
-thin and with the dense side on stock PyTorch:
+thin and with the dense side on stock PyTorch unless --fused-interaction, --fused-mlp or --optimizer adamw say otherwise:
 
   * flags  --sketch-flag --compress-rate --hash-rate --sketch-threshold --adjust-threshold --sketch-alpha
            --notinsert-test with the reference's defaults (dlrm_s_pytorch.py:1017-1020, 1114, 1126-1128);
@@ -31,6 +31,8 @@ import torch.nn as nn
 from torch.autograd.profiler import record_function
 
 from . import _lib, sizing, synthetic
+from .dense import FusedMLP, fused_linear
+from .optim import AdamW
 from .sketch import _stream
 from .sk_embedding_bag import SKEmbeddingGroup
 
@@ -46,12 +48,17 @@ def add_cafe_arguments(parser: argparse.ArgumentParser) -> argparse.ArgumentPars
     parser.add_argument("--notinsert-test", action="store_true", default=False)
     # not a flag of the reference: its dot interaction (dlrm_s_pytorch.py:779-812) as one library kernel per direction
     parser.add_argument("--fused-interaction", action="store_true", default=False)
+    # nor these: the MLPs' layers as library kernels, and AdamW for the dense parameters (the tables keep SGD)
+    parser.add_argument("--fused-mlp", action="store_true", default=False)
+    parser.add_argument("--optimizer", default="sgd", choices=["sgd", "adamw"])
+    parser.add_argument("--dense-learning-rate", type=float, default=1e-3)
+    parser.add_argument("--adamw-state-bits", type=int, default=32, choices=[8, 32])
     return parser
 
 
-def create_mlp(ln, sigmoid_layer: int, rng: np.random.Generator) -> nn.Sequential:
+def create_mlp(ln, sigmoid_layer: int, rng: np.random.Generator, fused: bool = False) -> nn.Sequential:
     """dlrm_s_pytorch.py:213-251: Linear layers with normal(0, sqrt(2/(m+n))) weights and normal(0, sqrt(1/m))
-    biases, ReLU after each except a Sigmoid after layer `sigmoid_layer`."""
+    biases, ReLU after each except a Sigmoid after layer `sigmoid_layer`.  `fused`: computed by the library (FusedMLP)."""
     layers = []
     for i in range(len(ln) - 1):
         n, m = int(ln[i]), int(ln[i + 1])
@@ -60,7 +67,7 @@ def create_mlp(ln, sigmoid_layer: int, rng: np.random.Generator) -> nn.Sequentia
         lin.bias.data = torch.from_numpy(rng.normal(0.0, np.sqrt(1 / m), size=m).astype(np.float32))
         layers.append(lin)
         layers.append(nn.Sigmoid() if i == sigmoid_layer else nn.ReLU())
-    return nn.Sequential(*layers)
+    return FusedMLP(*layers) if fused else nn.Sequential(*layers)
 
 
 class CafeEmbeddingLayer(nn.Module):
@@ -262,9 +269,10 @@ def fused_dot_interaction(x: torch.Tensor, emb: torch.Tensor) -> torch.Tensor:
 
 class DLRMNet(nn.Module):
     """DLRM_Net of dlrm_s_pytorch.py with the CAFE embedding layer: bottom MLP, dot interaction, top MLP.
-    `fused_interaction`: the interaction through the library's kernels instead of torch's cat / bmm / index ops."""
+    `fused_interaction`: the interaction through the library's kernels instead of torch's cat / bmm / index ops; `fused_mlp`:
+    the same for the MLPs."""
 
-    def __init__(self, ln_emb, dim, ln_bot, ln_top_hidden, emb_layer, seed=123, fused_interaction=False):
+    def __init__(self, ln_emb, dim, ln_bot, ln_top_hidden, emb_layer, seed=123, fused_interaction=False, fused_mlp=False):
         super().__init__()
         self.fused_interaction = bool(fused_interaction)
         rng = np.random.default_rng(seed)
@@ -272,10 +280,10 @@ class DLRMNet(nn.Module):
         ln_bot = [int(v) for v in ln_bot]
         if ln_bot[-1] != dim:
             raise ValueError("the bottom MLP must end at the embedding dimension")
-        self.bot = create_mlp(ln_bot, -1, rng)
+        self.bot = create_mlp(ln_bot, -1, rng, fused_mlp)
         nf = len(ln_emb) + 1
         ln_top = [nf * (nf - 1) // 2 + dim] + [int(v) for v in ln_top_hidden]
-        self.top = create_mlp(ln_top, len(ln_top) - 2, rng)
+        self.top = create_mlp(ln_top, len(ln_top) - 2, rng, fused_mlp)
         dev = self.emb.device
         self.bot.to(dev)
         self.top.to(dev)
@@ -293,13 +301,14 @@ class DCNNet(nn.Module):
     """The deep & cross head of dcn.py:410-422, 712-742 over the CAFE embedding layer: three cross layers
     x_{l+1} = x_0 * (x_l w_l) + b_l, a deep MLP, and a final linear layer over both, then a sigmoid."""
 
-    def __init__(self, ln_emb, dim, num_dense, deep, emb_layer, cross_layers=3, seed=123):
+    def __init__(self, ln_emb, dim, num_dense, deep, emb_layer, cross_layers=3, seed=123, fused_mlp=False):
         super().__init__()
         rng = np.random.default_rng(seed)
         self.emb = emb_layer
+        self.fused_mlp = bool(fused_mlp)
         self.num_dense = int(num_dense)
         d_in = dim * len(ln_emb) + self.num_dense
-        self.deep = create_mlp([d_in] + [int(v) for v in deep], -1, rng)
+        self.deep = create_mlp([d_in] + [int(v) for v in deep], -1, rng, fused_mlp)
         g = torch.Generator().manual_seed(seed)
         self.cross_weight = nn.ParameterList([nn.Parameter(torch.randn(d_in, 1, generator=g) * 0.0001) for _ in range(cross_layers)])
         self.cross_bias = nn.ParameterList([nn.Parameter(torch.zeros(d_in)) for _ in range(cross_layers)])
@@ -318,7 +327,10 @@ class DCNNet(nn.Module):
             x1 = z
             for w, b in zip(self.cross_weight, self.cross_bias):
                 x1 = z * (x1 @ w) + b
-            return torch.sigmoid(self.last(torch.cat([self.deep(z), x1], dim=1)))
+            both = torch.cat([self.deep(z), x1], dim=1)
+            if self.fused_mlp:
+                return fused_linear(both, self.last.weight, self.last.bias, "sigmoid")
+            return torch.sigmoid(self.last(both))
 
 
 def dense_and_plain_parameters(model: nn.Module):
@@ -328,6 +340,45 @@ def dense_and_plain_parameters(model: nn.Module):
     if getattr(model.emb, "group", None) is not None:
         skip = {id(p) for p in model.emb.group.parameters()}
     return [p for p in model.parameters() if id(p) not in skip]
+
+
+class TableSGDDenseAdamW:
+    """One optimizer made of two, for train_step: SGD at `lr` for the embedding tables outside the sketch (the sketch fields'
+    own SGD runs at the same rate inside the backward), AdamW at `dense_lr` for everything else.  param_groups[0] is the
+    tables' group, so that its lr is the one that train_step hands to the embedding layer."""
+
+    def __init__(self, model: nn.Module, lr: float, dense_lr: float = 1e-3, state_bits: int = 32, **adamw):
+        mine = dense_and_plain_parameters(model)
+        of_tables = {id(p) for p in model.emb.parameters()}
+        tables = [p for p in mine if id(p) in of_tables]
+        self.tables = torch.optim.SGD([dict(params=tables)], lr=lr)
+        self.dense = AdamW([p for p in mine if id(p) not in of_tables], lr=dense_lr, state_bits=state_bits, **adamw)
+
+    @property
+    def param_groups(self):
+        return self.tables.param_groups + self.dense.param_groups
+
+    def zero_grad(self, set_to_none: bool = True):
+        self.tables.zero_grad(set_to_none)
+        self.dense.zero_grad(set_to_none)
+
+    def step(self):
+        self.tables.step()
+        self.dense.step()
+
+    def state_dict(self):
+        return dict(tables=self.tables.state_dict(), dense=self.dense.state_dict())
+
+    def load_state_dict(self, state):
+        self.tables.load_state_dict(state["tables"])
+        self.dense.load_state_dict(state["dense"])
+
+
+def build_optimizer(args, model: nn.Module):
+    """The optimizer the arguments name: the reference's SGD for everything, or AdamW for the dense parameters."""
+    if getattr(args, "optimizer", "sgd") == "adamw":
+        return TableSGDDenseAdamW(model, args.learning_rate, args.dense_learning_rate, args.adamw_state_bits, seed=args.numpy_rand_seed)
+    return torch.optim.SGD(dense_and_plain_parameters(model), lr=args.learning_rate)
 
 
 def train_step(model, optimizer, dense_x, lS_o, lS_i, target, loss_fn=None):
@@ -428,18 +479,18 @@ def build_model(args, device="cuda", group_of_ranks=None):
         emb = CafeEmbeddingLayer(cards, dim, **emb_kwargs)
     if args.model == "dcn":
         deep = [int(v) for v in (args.arch_mlp_top or top).split("-")]
-        return DCNNet(cards, dim, nd, deep, emb, seed=args.numpy_rand_seed)
+        return DCNNet(cards, dim, nd, deep, emb, seed=args.numpy_rand_seed, fused_mlp=getattr(args, "fused_mlp", False))
     ln_bot = [int(v) for v in (args.arch_mlp_bot or bot).split("-")]
     ln_top = [int(v) for v in (args.arch_mlp_top or top).split("-")]
     return DLRMNet(cards, dim, ln_bot, ln_top, emb, seed=args.numpy_rand_seed,
-                   fused_interaction=getattr(args, "fused_interaction", False))
+                   fused_interaction=getattr(args, "fused_interaction", False), fused_mlp=getattr(args, "fused_mlp", False))
 
 
 def run(args) -> dict:
     """Trains args.nbatches steps on synthetic data of args.data_set; returns losses, AUC and samples/s."""
     dev = torch.device("cuda", torch.cuda.current_device())
     model = build_model(args, dev)
-    opt = torch.optim.SGD(dense_and_plain_parameters(model), lr=args.learning_rate)
+    opt = build_optimizer(args, model)
     B = args.mini_batch_size
     batches = [synthetic_batch(args.data_set, B, 2024, s, dev) for s in range(args.nbatches)]
     losses, preds, ys = [], [], []
@@ -474,7 +525,7 @@ def run_data_parallel(args, group=None) -> dict:
     dev = torch.device("cuda", torch.cuda.current_device())
     world, rank = dist.get_world_size(group), dist.get_rank(group)
     model = build_model(args, dev, group_of_ranks=(group,))
-    opt = torch.optim.SGD(dense_and_plain_parameters(model), lr=args.learning_rate)
+    opt = build_optimizer(args, model)
     B = args.mini_batch_size
     # rank r takes batches r, r + world, ... of the seeded stream: distinct samples on every rank
     batches = [synthetic_batch(args.data_set, B, 2024, s * world + rank, dev) for s in range(args.nbatches)]
