@@ -285,6 +285,8 @@ def _own(s):
     if s["case"]["kind"] == "adamw":
         s["opt"].step()
         moments = s["opt"].moments()
+        if s["case"]["bits"] == 8:   # (as the plain form holds them: one axis)
+            moments = [(m.view(-1), v.view(-1)) for m, v in moments]
         return dict(p=[p.data for p in s["params"]], m=[m for m, _ in moments], v=[v for _, v in moments])
     mlp, train = s["case"]["kind"] == "mlp", s["case"]["train"]
     if not train:
