@@ -72,7 +72,7 @@ def _ptr(t):
 
 
 def _slope_type(dtype):
-    return torch.float32 if dtype == torch.float32 else torch.float16
+    return torch.float16 if dtype == torch.bfloat16 else torch.float32
 
 
 def _contiguous(t):

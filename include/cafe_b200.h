@@ -329,7 +329,7 @@ int cafe_dot_interaction_backward(const float* x_dev, const float* emb_dev, int6
 /* ---- dense layers (the MLPs around the embedding path: dlrm_s_pytorch.py:213-251, dcn.py:410-422) ------------------
  * z = x W^T + b, y = act(z) + res for x [M, K], W [N, K], rows `ld` elements apart (ld >= the row's length; elements of a
  * row are contiguous).  All tensors of a call have one type; sums are fp32.  bias, res and slope may be null; ldr = 0: one
- * row of res for all.  slope_dev receives act'(z) for the backward, fp32 beside fp32 and fp16 beside 16-bit types.
+ * row of res for all.  slope_dev receives act'(z) for the backward: fp16 beside bf16, else fp32.
  * M, N, K <= CAFE_LINEAR_MAX.  No host synchronisation, no device memory of its own. */
 enum { CAFE_F32 = 0, CAFE_BF16 = 1, CAFE_F16 = 2 };
 enum { CAFE_ACT_NONE = 0, CAFE_ACT_RELU = 1, CAFE_ACT_SIGMOID = 2, CAFE_ACT_GELU = 3, CAFE_ACT_SILU = 4 };

@@ -2,8 +2,9 @@
 
 Sums: a sum of n products in fp32, in any order, with every operation rounded or cut off, is off by at most (n + 8) 2^-23
 times the sum of the products' magnitudes; an operand split into three 8-bit parts loses less than one further unit of 2^-23.
-Results rounded to type t: eps(t) / 2 relative, or half the smallest step of fp16 / bf16.  Derivatives kept in fp16: 2^-12
-relative or 2^-25.  gz rounded to a 16-bit type before its products: eps / 2 relative."""
+Results rounded to type t: eps(t) / 2 relative, or half the smallest step of fp16 / bf16.  Derivatives kept in fp16 beside bf16:
+fp16 has 11 significant bits, so 2^-11 relative (finfo(fp16).eps / 2 = 2^-10 / 2), or 2^-25 near zero.  gz rounded to a 16-bit
+type before its products: eps / 2 relative.  A rounding is relative to the value that is rounded, which is itself off already."""
 import math
 
 import torch
@@ -46,7 +47,7 @@ def forward(x, w, b, act, r, dtype, x_off=None):
     far = off * LIPSCHITZ[act][0] + (8 * U) * (a.abs() + (0 if act in ("none", "relu") else z.abs() * 2.0 ** -10)) + 1e-37
     y = a if r is None else a + r.double()
     far = far + U * y.abs()
-    return y, far + half_step(y, dtype), z, off
+    return y, far + half_step(y.abs() + far, dtype), z, off
 
 
 def backward(gy, z, z_off, x, w, act, dtype, mask=None, g_off=None, x_off=None):
@@ -55,13 +56,13 @@ def backward(gy, z, z_off, x, w, act, dtype, mask=None, g_off=None, x_off=None):
     d = activation(z, act)[1] if mask is None else mask.double()
     gz = gy * d
     d_off = z_off * LIPSCHITZ[act][1] + (16 * U * (1 + z.abs()) if act not in ("none", "relu") else 0)
-    if dtype != torch.float32 and act not in ("none", "relu"):
-        d_off = d_off + d.abs() * 2.0 ** -12 + 2.0 ** -25
+    if dtype == torch.bfloat16 and act not in ("none", "relu"):
+        d_off = d_off + (d.abs() + d_off) * 2.0 ** -11 + 2.0 ** -25
     off = gy.abs() * d_off + U * gz.abs()
     if g_off is not None:
         off = off + g_off * (d.abs() + d_off)
     if dtype != torch.float32:
-        off = off + half_step(gz, dtype)
+        off = off + half_step(gz.abs() + off, dtype)
     a = gz.abs() + off
     out = {}
     M, N = gz.shape
@@ -69,7 +70,8 @@ def backward(gy, z, z_off, x, w, act, dtype, mask=None, g_off=None, x_off=None):
                                      ("gw", gz.t() @ x, a.t() @ (x.abs() + (0 if x_off is None else x_off)),
                                       off.t() @ x.abs() + (0 if x_off is None else a.t() @ x_off), M),
                                      ("gb", gz.sum(0), a.sum(0), off.sum(0), M)):
-        out[name] = (value, far + mag * ((n + 8) * U) + half_step(value, dtype))
+        far = far + mag * ((n + 8) * U)
+        out[name] = (value, far + half_step(value.abs() + far, dtype))
     return out
 
 
