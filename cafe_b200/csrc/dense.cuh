@@ -1,0 +1,192 @@
+// dense.cuh -- what the kernels of the dense layers share: activations, the description of a product, its end.
+#pragma once
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "../../include/cafe_b200.h"
+#include "cafe_internal.h"
+#include "cafe_float.cuh"
+#include "tcgen05.cuh"
+
+#define CAFE_LIN_BM 128   // rows of a block's outputs
+
+// act(z), and its derivative.  FAST (results of 16 bits): exponentials and reciprocals of 2^-22 relative error instead of exact
+// rounding.
+template <bool FAST> __device__ __forceinline__ float cafe_exp(float x) { return FAST ? __expf(x) : expf(x); }
+template <bool FAST> __device__ __forceinline__ float cafe_inverse(float x) { return FAST ? __fdividef(1.f, x) : __frcp_rn(x); }
+template <bool FAST> __device__ __forceinline__ float cafe_act(float z, int act, float* slope) {
+    switch (act) {
+        case CAFE_ACT_RELU: *slope = z > 0.f ? 1.f : 0.f; return z > 0.f ? z : (z != z ? z : 0.f);
+        case CAFE_ACT_SIGMOID: case CAFE_ACT_SILU: {
+            // e = exp(-|z|) never overflows; s and t = 1 - s keep their relative precision in both tails
+            const float e = cafe_exp<FAST>(-fabsf(z)), d = cafe_inverse<FAST>(1.f + e);
+            const float s = z >= 0.f ? d : e * d, t = z >= 0.f ? e * d : d;
+            if (act == CAFE_ACT_SIGMOID) { *slope = s * t; return s; }
+            *slope = s * (1.f + z * t);
+            return z * s;
+        }
+        case CAFE_ACT_GELU: {
+            // the normal distribution's tail below -|z|: half of exp(-z^2 / 2) times exp(y^2) erfc(y), y = |z| / sqrt(2), for which
+            // a polynomial of degree 9 in t = 1 / (1 + y / 2) without constant term was fitted here (least largest relative error
+            // on [0, 12]: 4.4e-8; evaluated in fp32 3.2e-7).  The derivative takes the same exponential.
+            const float e = cafe_exp<FAST>(-0.5f * z * z), t = cafe_inverse<FAST>(1.f + 0.353553391f * fabsf(z));
+            float q = -0.0593632702f;
+            q = fmaf(q, t, 0.286011492f); q = fmaf(q, t, -0.490175051f); q = fmaf(q, t, 0.28147069f); q = fmaf(q, t, -0.0289692743f);
+            q = fmaf(q, t, 0.203677501f); q = fmaf(q, t, 0.242853828f); q = fmaf(q, t, 0.282409568f); q = fmaf(q, t, 0.282084473f);
+            const float h = 0.5f * e * (q * t), c = z > 0.f ? 1.f - h : h;
+            *slope = c + z * e * 0.398942280f;
+            return z * c;
+        }
+        default: *slope = 1.f; return z;
+    }
+}
+// the derivative kept for the backward, always finer than the type it multiplies, so that gz's own rounding stays the only
+// one that counts: fp16 (11 bits; it lies in [-0.2, 1.2]) beside bf16 (8 bits), else fp32
+template <typename T> struct CafeSlopeOf { typedef float type; };
+template <> struct CafeSlopeOf<__nv_bfloat16> { typedef __half type; };
+
+struct CafeJob {
+    const void *a, *as, *b;
+    int64_t lda, ldas, ldb;
+    int a_kc, b_kc, a_vec, as_vec, b_vec;   // k contiguous; 16-byte loads allowed
+    int slope_kind, rows, cols, depth;
+    int tiles_n, tiles;
+    const void *bias, *res;
+    int64_t ldr, ldo, lds;
+    int act, out_vec, res_vec;
+    void *out, *slope_out, *gb;             // gb: sums over k of A(i, k), by the blocks of the first column of tiles
+};
+struct CafeJobs {
+    CafeJob job[2];
+    int count;
+};
+
+__device__ __forceinline__ void cafe_put16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// A(i, k) B(j, k) added up in the plain order, for sums that the split operands turned into a NaN: an infinite part times a
+// lower part that is zero is one, where infinity times the whole number is not
+static __device__ __noinline__ float cafe_plain_dot(const CafeJob& J, int64_t i, int64_t j, int k0, int k1) {
+    const float *a = static_cast<const float*>(J.a), *b = static_cast<const float*>(J.b), *s = static_cast<const float*>(J.as);
+    float sum = 0.f;
+    for (int64_t k = k0; k < k1 && sum == sum; ++k) {
+        float x = __ldg(a + (J.a_kc ? i * J.lda + k : k * J.lda + i));
+        if (J.slope_kind != CAFE_SLOPE_NONE) {
+            const float t = __ldg(s + (J.a_kc ? i * J.ldas + k : k * J.ldas + i));
+            x = J.slope_kind == CAFE_SLOPE_VALUES ? x * t : t > 0.f ? x : 0.f;
+        }
+        sum += x * __ldg(b + (J.b_kc ? j * J.ldb + k : k * J.ldb + j));
+    }
+    return sum;
+}
+
+// ---- the end of a product --------------------------------------------------------------------------------------------
+// A thread's 4 * QUADS consecutive columns of row r of the block's sums to shared memory; a NaN of split operands is looked into.
+template <bool SPLIT, int N>
+__device__ __forceinline__ void cafe_sums_put(const CafeJob& J, const float* acc, uint32_t at, int64_t row, int64_t col, int k0, int k1, bool look) {
+    bool nan = false;
+#pragma unroll
+    for (int c = 0; c < N; c += 4) {
+        cafe_put16(at + 4 * c, __float_as_uint(acc[c]), __float_as_uint(acc[c + 1]), __float_as_uint(acc[c + 2]), __float_as_uint(acc[c + 3]));
+        if (SPLIT) nan |= !(acc[c] == acc[c]) | !(acc[c + 1] == acc[c + 1]) | !(acc[c + 2] == acc[c + 2]) | !(acc[c + 3] == acc[c + 3]);
+    }
+    if (SPLIT && nan && look && row < J.rows)
+        for (int c = 0; c < N && col + c < J.cols; ++c) {
+            float x;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(at + 4 * c) : "memory");
+            if (x != x) {
+                x = cafe_plain_dot(J, row, col + c, k0, k1);
+                asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + 4 * c), "f"(x) : "memory");
+            }
+        }
+}
+// This block's share of the tile's rows (of a cluster of `splits` blocks, by rank): the blocks' sums in the order of ranks, then
+// bias, activation, residual and the stores.  COLS columns at a pitch of COLS + 4 floats from `base` of every block.
+template <typename T, int COLS>
+__device__ __forceinline__ void cafe_finish(const CafeJob& J, uint32_t base, int row0, int col0, int rank, int splits, int threads) {
+    typedef typename CafeSlopeOf<T>::type ST;
+    constexpr int pitch = COLS + 4, quads = COLS / 4;
+    const int per = CAFE_LIN_BM / splits;
+    for (int e = threadIdx.x; e < per * quads; e += threads) {
+        const int r = rank * per + e / quads, c = (e % quads) * 4;
+        const int64_t i = row0 + r, j = col0 + c;
+        if (i >= J.rows || j >= J.cols) continue;
+        const uint32_t at = base + (uint32_t)(r * pitch + c) * 4u;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        if (splits == 1) asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(at) : "memory");
+        else
+            for (int q = 0; q < splits; ++q) {
+                const float4 x = cafe_cluster_load4(cafe_cluster_map(at, q));
+                v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+            }
+        const int n = (int)min((int64_t)4, J.cols - j);
+        const bool vec = J.out_vec && n == 4;
+        float bias[4] = {0.f, 0.f, 0.f, 0.f}, res[4] = {0.f, 0.f, 0.f, 0.f};
+        if (J.bias) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) if (q < n) bias[q] = cafe_to_float(__ldg(static_cast<const T*>(J.bias) + j + q));
+        }
+        if (J.res) {
+            const T* p = static_cast<const T*>(J.res) + i * J.ldr + j;
+            if (J.res_vec && n == 4) {
+                alignas(16) T x[4];
+                if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(x) = __ldg(reinterpret_cast<const uint4*>(p));
+                else *reinterpret_cast<uint2*>(x) = __ldg(reinterpret_cast<const uint2*>(p));
+#pragma unroll
+                for (int q = 0; q < 4; ++q) res[q] = cafe_to_float(x[q]);
+            } else {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) if (q < n) res[q] = cafe_to_float(__ldg(p + q));
+            }
+        }
+        alignas(16) T o[4];
+        alignas(16) ST sl[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            float z = v[q] + bias[q], d = 1.f;
+            if (J.act != CAFE_ACT_NONE) z = cafe_act<sizeof(T) == 2>(z, J.act, &d);
+            o[q] = cafe_from_float<T>(z + res[q]);
+            sl[q] = cafe_from_float<ST>(d);
+        }
+        T* out = static_cast<T*>(J.out) + i * J.ldo + j;
+        if (vec) {
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(o);
+            else *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(o);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) if (q < n) out[q] = o[q];
+        }
+        if (J.slope_out) {
+            ST* so = static_cast<ST*>(J.slope_out) + i * J.lds + j;
+            if (vec) {
+                if constexpr (sizeof(ST) == 4) *reinterpret_cast<uint4*>(so) = *reinterpret_cast<const uint4*>(sl);
+                else *reinterpret_cast<uint2*>(so) = *reinterpret_cast<const uint2*>(sl);
+            } else {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) if (q < n) so[q] = sl[q];
+            }
+        }
+    }
+}
+
+// ---- the calls -------------------------------------------------------------------------------------------------------
+struct CafeForward {
+    const void *x, *w, *bias, *res;
+    int64_t ldx, ldw, ldr;
+    int M, N, K, act;
+    void *y, *slope;
+    int64_t ldy, lds;
+};
+struct CafeBackward {
+    const void *gy, *slope, *x, *w;
+    int64_t ldg, lds, ldx, ldw;
+    int slope_kind, M, N, K;
+    void *gx, *gw, *gb;
+    int64_t ldgx, ldgw;
+};
+// dense_tiles.cu: large layers.  Bytes of workspace that a call would take (0: not one for it), and the calls.
+int64_t cafe_tiles_forward_work(const CafeForward& f, int dtype);
+int64_t cafe_tiles_backward_work(const CafeBackward& f, int dtype);
+cudaError_t cafe_tiles_forward(const CafeForward& f, int dtype, const CafeJob& job, void* work, cudaStream_t st);
+cudaError_t cafe_tiles_backward(const CafeBackward& f, int dtype, const CafeJob* gw, const CafeJob* gx, void* work, cudaStream_t st);

@@ -4,40 +4,7 @@
 //   gz = gy * act'(z)  gx = gz W   gW = gz^T x   gb = sum over rows of gz   gr = gy
 //
 // for x [M, K], W [N, K], rows of any pitch, in fp32, bf16 or fp16 with sums in fp32.
-#include <cuda_runtime.h>
-#include <math.h>
-#include <stdint.h>
-
-#include "../../include/cafe_b200.h"
-#include "cafe_internal.h"
-#include "cafe_float.cuh"
-#include "tcgen05.cuh"
-
-// act(z), and its derivative
-__device__ __forceinline__ float cafe_act(float z, int act, float* slope) {
-    switch (act) {
-        case CAFE_ACT_RELU: *slope = z > 0.f ? 1.f : 0.f; return z > 0.f ? z : (z != z ? z : 0.f);
-        case CAFE_ACT_SIGMOID: case CAFE_ACT_SILU: {
-            // e = exp(-|z|) never overflows; s and t = 1 - s keep their relative precision in both tails
-            const float e = expf(-fabsf(z)), d = 1.f / (1.f + e);
-            const float s = z >= 0.f ? d : e * d, t = z >= 0.f ? e * d : d;
-            if (act == CAFE_ACT_SIGMOID) { *slope = s * t; return s; }
-            *slope = s * (1.f + z * t);
-            return z * s;
-        }
-        case CAFE_ACT_GELU: {
-            const float c = 0.5f * erfcf(z * -0.70710678118654752f);
-            *slope = c + z * expf(-0.5f * z * z) * 0.39894228040143268f;
-            return z * c;
-        }
-        default: *slope = 1.f; return z;
-    }
-}
-
-// the derivative kept for the backward, always finer than the type it multiplies, so that gz's own rounding stays the only
-// one that counts: fp16 (11 bits; it lies in [-0.2, 1.2]) beside bf16 (8 bits), else fp32
-template <typename T> struct CafeSlopeOf { typedef float type; };
-template <> struct CafeSlopeOf<__nv_bfloat16> { typedef __half type; };
+#include "dense.cuh"
 
 // ---- one matrix product: C(i, j) = sum_k A(i, k) B(j, k) ---------------------------------------------------------------
 // The three products of a layer differ only in which index of each operand is contiguous (y: k of both; gx: k of gz, j of W; gW:
@@ -53,7 +20,6 @@ template <> struct CafeSlopeOf<__nv_bfloat16> { typedef __half type; };
 // rounded: nothing overflows), and six of the nine products are added: hh, and hm + mh + mm + hl + lh in sums of their own.
 // What is left out is below 2^-23 of a product.  The tensor cores cut sums off instead of rounding them, so hh, whose sums
 // are as large as the result, is taken out and added in registers every CHUNK of k; the others are 2^-8 of it and are not.
-#define CAFE_LIN_BM 128
 #define CAFE_LIN_THREADS 512       // 8 warps that load, 8 that take sums out, the first of which issues the products
 
 template <typename T> struct CafeLin {   // 16-bit types
@@ -70,21 +36,6 @@ template <typename T, int BN> struct CafeLinShape {
     static constexpr int tm_cols = CafeLin<T>::parts == 3 ? 2 * BN : BN;
 };
 
-struct CafeJob {
-    const void *a, *as, *b;
-    int64_t lda, ldas, ldb;
-    int a_kc, b_kc, a_vec, as_vec, b_vec;   // k contiguous; 16-byte loads allowed
-    int slope_kind, rows, cols, depth;
-    int tiles_n, tiles;
-    const void *bias, *res;
-    int64_t ldr, ldo, lds;
-    int act, out_vec;
-    void *out, *slope_out, *gb;             // gb: sums over k of A(i, k), by the blocks of the first column of tiles
-};
-struct CafeJobs {
-    CafeJob job[2];
-    int count;
-};
 __device__ int g_dense_gave_up;   // a wait ran out (its outputs are not numbers)
 
 // eight values along k of one row: fp32, or 16-bit values two to a register
@@ -147,9 +98,6 @@ __device__ __forceinline__ void cafe_piece_mask(CafePiece<T>& p, const CafePiece
         cafe_piece_set<T>(p, 2 * j + 1, cafe_to_float(cafe_piece_get<T>(y, 2 * j + 1)) > 0.f ? b : cafe_from_float<T>(0.f));
     }
 }
-__device__ __forceinline__ void cafe_put16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
-}
 // a piece to its place in the operand's part(s), `part` bytes apart
 __device__ __forceinline__ void cafe_piece_store(const CafePiece<float>& p, uint32_t at, int part) {
     uint32_t h[4], m[4], l[4];
@@ -191,22 +139,6 @@ template <typename T, int R, int BK = CafeLin<T>::BK> struct CafeTurn {
         }
     }
 };
-
-// A(i, k) B(j, k) added up in the plain order, for sums that the split operands turned into a NaN: an infinite part times a
-// lower part that is zero is one, where infinity times the whole number is not
-__device__ __noinline__ float cafe_plain_dot(const CafeJob& J, int64_t i, int64_t j, int k0, int k1) {
-    const float *a = static_cast<const float*>(J.a), *b = static_cast<const float*>(J.b), *s = static_cast<const float*>(J.as);
-    float sum = 0.f;
-    for (int64_t k = k0; k < k1 && sum == sum; ++k) {
-        float x = __ldg(a + (J.a_kc ? i * J.lda + k : k * J.lda + i));
-        if (J.slope_kind != CAFE_SLOPE_NONE) {
-            const float t = __ldg(s + (J.a_kc ? i * J.ldas + k : k * J.ldas + i));
-            x = J.slope_kind == CAFE_SLOPE_VALUES ? x * t : t > 0.f ? x : 0.f;
-        }
-        sum += x * __ldg(b + (J.b_kc ? j * J.ldb + k : k * J.ldb + j));
-    }
-    return sum;
-}
 
 template <typename T, int BN>
 __global__ void __launch_bounds__(CAFE_LIN_THREADS, 1) k_linear(const __grid_constant__ CafeJobs P, int splits) {
@@ -382,72 +314,14 @@ __global__ void __launch_bounds__(CAFE_LIN_THREADS, 1) k_linear(const __grid_con
     cafe_tc_after();
     if (warp == 8) cafe_tm_free(tmem, Sh::tm_cols);
 
-    // ---- the block's sums, 128 x BN, to shared memory
-    constexpr int pitch = BN + 4;
+    // ---- the block's sums to shared memory, and what belongs at the end
     if (warp >= 8) {
         const int r = (warp & 3) * 32 + lane, c0 = (warp - 8) / 4 * half_cols;
-        const uint32_t at = base + (uint32_t)(r * pitch + c0) * 4u;
-        bool nan = false;
-#pragma unroll
-        for (int c = 0; c < half_cols; c += 4) {
-            cafe_put16(at + 4 * c, __float_as_uint(acc[c]), __float_as_uint(acc[c + 1]), __float_as_uint(acc[c + 2]), __float_as_uint(acc[c + 3]));
-            if (L::parts == 3) nan |= !(acc[c] == acc[c]) | !(acc[c + 1] == acc[c + 1]) | !(acc[c + 2] == acc[c + 2]) | !(acc[c + 3] == acc[c + 3]);
-        }
-        if constexpr (L::parts == 3) {
-            if (nan && !bail && row0 + r < J.rows) {
-                const int k0 = t0 * L::BK, k1 = min(J.depth, (t0 + turns) * L::BK);
-                for (int c = 0; c < half_cols && col0 + c0 + c < J.cols; ++c) {
-                    float x;
-                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(at + 4 * c));
-                    if (x != x) {
-                        x = cafe_plain_dot(J, row0 + r, col0 + c0 + c, k0, k1);
-                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + 4 * c), "f"(x) : "memory");
-                    }
-                }
-            }
-        }
+        cafe_sums_put<L::parts == 3, half_cols>(J, acc, base + (uint32_t)(r * (BN + 4) + c0) * 4u, row0 + r, col0 + c0, t0 * L::BK,
+                                                min(J.depth, (t0 + turns) * L::BK), !bail);
     }
     if (splits > 1) cafe_cluster_sync(); else __syncthreads();
-
-    // ---- this block's share of the rows: the cluster's sums in the order of ranks, then what belongs at the end
-    const int per = CAFE_LIN_BM / splits;
-    constexpr int quads = BN / 4;
-    for (int e = threadIdx.x; e < per * quads; e += CAFE_LIN_THREADS) {
-        const int r = rank * per + e / quads, c = (e % quads) * 4;
-        const int64_t i = row0 + r, j = col0 + c;
-        if (i >= J.rows || j >= J.cols) continue;
-        const uint32_t at = base + (uint32_t)(r * pitch + c) * 4u;
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int q = 0; q < splits; ++q) {
-            const float4 x = cafe_cluster_load4(splits > 1 ? cafe_cluster_map(at, q) : cafe_cluster_map(at, cafe_cluster_rank()));
-            v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
-        }
-        const int n = min((int64_t)4, J.cols - j);
-        alignas(16) T o[4];
-        alignas(16) ST sl[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            if (q >= n) break;
-            float z = v[q], d = 1.f;
-            if (J.bias) z += cafe_to_float(__ldg(static_cast<const T*>(J.bias) + j + q));
-            if (J.act != CAFE_ACT_NONE) z = cafe_act(z, J.act, &d);
-            if (J.res) z += cafe_to_float(__ldg(static_cast<const T*>(J.res) + i * J.ldr + j + q));
-            o[q] = cafe_from_float<T>(z);
-            sl[q] = cafe_from_float<ST>(d);
-        }
-        T* out = static_cast<T*>(J.out) + i * J.ldo + j;
-        if (J.out_vec && n == 4) {
-            if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(o);
-            else *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(o);
-        } else for (int q = 0; q < n; ++q) out[q] = o[q];
-        if (J.slope_out) {
-            ST* so = static_cast<ST*>(J.slope_out) + i * J.lds + j;
-            if (J.out_vec && n == 4) {
-                if constexpr (sizeof(ST) == 4) *reinterpret_cast<uint4*>(so) = *reinterpret_cast<const uint4*>(sl);
-                else *reinterpret_cast<uint2*>(so) = *reinterpret_cast<const uint2*>(sl);
-            } else for (int q = 0; q < n; ++q) so[q] = sl[q];
-        }
-    }
+    cafe_finish<T, BN>(J, base, row0, col0, rank, splits, CAFE_LIN_THREADS);
     if (J.gb && tn == 0 && rank == 0 && threadIdx.x < CAFE_LIN_BM && row0 + (int)threadIdx.x < J.rows) {
         float x = 0.f;
         for (int q = 0; q < splits; ++q) {
@@ -524,22 +398,8 @@ static int dense_done(cudaError_t e) {
     return CAFE_OK;
 }
 
-struct CafeForward {
-    const void *x, *w, *bias, *res;
-    int64_t ldx, ldw, ldr;
-    int M, N, K, act;
-    void *y, *slope;
-    int64_t ldy, lds;
-};
-struct CafeBackward {
-    const void *gy, *slope, *x, *w;
-    int64_t ldg, lds, ldx, ldw;
-    int slope_kind, M, N, K;
-    void *gx, *gw, *gb;
-    int64_t ldgx, ldgw;
-};
 template <typename T>
-static cudaError_t dense_forward(const CafeForward& f, cudaStream_t st) {
+static cudaError_t dense_forward(const CafeForward& f, int dtype, void* work, int64_t work_bytes, cudaStream_t st) {
     if (f.M == 0 || f.N == 0) return cudaSuccess;
     CafeJobs P = {};
     CafeJob& J = P.job[0];
@@ -550,11 +410,14 @@ static cudaError_t dense_forward(const CafeForward& f, cudaStream_t st) {
     J.rows = f.M; J.cols = f.N; J.depth = f.K;
     J.bias = f.bias; J.res = f.res; J.ldr = f.ldr; J.act = f.act; J.out = f.y; J.ldo = f.ldy; J.slope_out = f.slope; J.lds = f.lds;
     const int ssize = sizeof(typename CafeSlopeOf<T>::type);
+    J.res_vec = f.res && dense_on(f.res, f.ldr, size, 4 * size);
     J.out_vec = dense_on(f.y, f.ldy, size, 4 * size) && (!f.slope || dense_on(f.slope, f.lds, ssize, 4 * ssize));
+    const int64_t need = cafe_tiles_forward_work(f, dtype);
+    if (need > 0 && work && work_bytes >= need) return cafe_tiles_forward(f, dtype, J, work, st);
     return dense_launch<T>(P, st);
 }
 template <typename T>
-static cudaError_t dense_backward(const CafeBackward& f, cudaStream_t st) {
+static cudaError_t dense_backward(const CafeBackward& f, int dtype, void* work, int64_t work_bytes, cudaStream_t st) {
     CafeJobs P = {};
     const int size = sizeof(T), ssize = f.slope_kind == CAFE_SLOPE_VALUES ? (int)sizeof(typename CafeSlopeOf<T>::type) : size;
     const int g_vec = dense_on(f.gy, f.ldg, size, 16), s_vec = f.slope_kind != CAFE_SLOPE_NONE && dense_on(f.slope, f.lds, ssize, 16);
@@ -573,6 +436,9 @@ static cudaError_t dense_backward(const CafeBackward& f, cudaStream_t st) {
         J.rows = f.M; J.cols = f.K; J.depth = f.N;
         J.out = f.gx; J.ldo = f.ldgx; J.out_vec = dense_on(f.gx, f.ldgx, size, 4 * size);
     }
+    const int64_t need = cafe_tiles_backward_work(f, dtype);
+    if (need > 0 && work && work_bytes >= need)
+        return cafe_tiles_backward(f, dtype, f.gw || f.gb ? &P.job[0] : nullptr, f.gx ? &P.job[P.count - 1] : nullptr, work, st);
     return P.count ? dense_launch<T>(P, st) : cudaSuccess;
 }
 #define DENSE_TYPED(dtype, ...)                                              \
@@ -602,31 +468,67 @@ static int dense_backward_ok(const CafeBackward& f) {
     return 1;
 }
 
+// (work that is there must be on 16 bytes)
+static int dense_work_ok(const void* work, int64_t bytes) { return !work || (bytes >= 0 && ((uintptr_t)work & 15) == 0); }
+static int64_t dense_half(int layers, const int* widths, int M, int dtype) {
+    int64_t most = 0;
+    for (int l = 1; l < layers; ++l) most = widths[l] > most ? widths[l] : most;
+    return (((most + 7) & ~(int64_t)7) * M * (dtype == CAFE_F32 ? 4 : 2) + 255) & ~(int64_t)255;
+}
+// what lies between the layers of an MLP is on 16 bytes, rows and all
+static const void* const k_aligned = (const void*)256;
+
 extern "C" {
 
+int64_t cafe_linear_forward_work(const void* x_dev, int64_t ldx, const void* w_dev, int64_t ldw, int M, int N, int K, int dtype) {
+    CafeForward f = {};
+    f.x = x_dev; f.ldx = ldx; f.w = w_dev; f.ldw = ldw; f.M = M; f.N = N; f.K = K;
+    return dense_type_ok(dtype) && dense_sizes_ok(M, N, K) ? cafe_tiles_forward_work(f, dtype) : 0;
+}
+
 int cafe_linear_forward(const void* x_dev, int64_t ldx, const void* w_dev, int64_t ldw, const void* bias_dev, const void* res_dev, int64_t ldr,
-                        int M, int N, int K, int dtype, int act, void* y_dev, int64_t ldy, void* slope_dev, int64_t lds, void* stream) {
+                        int M, int N, int K, int dtype, int act, void* y_dev, int64_t ldy, void* slope_dev, int64_t lds, void* work_dev,
+                        int64_t work_bytes, void* stream) {
     const CafeForward f = {x_dev, w_dev, bias_dev, res_dev, ldx, ldw, ldr, M, N, K, act, y_dev, slope_dev, ldy, lds};
-    if (!dense_type_ok(dtype) || !dense_forward_ok(f)) return CAFE_ERR_ARG;
+    if (!dense_type_ok(dtype) || !dense_forward_ok(f) || !dense_work_ok(work_dev, work_bytes)) return CAFE_ERR_ARG;
     cudaError_t e;
-    DENSE_TYPED(dtype, e = dense_forward<T>(f, (cudaStream_t)stream));
+    DENSE_TYPED(dtype, e = dense_forward<T>(f, dtype, work_dev, work_bytes, (cudaStream_t)stream));
     return dense_done(e);
+}
+
+int64_t cafe_linear_backward_work(const void* gy_dev, int64_t ldg, int slope_kind, const void* x_dev, int64_t ldx, const void* w_dev, int64_t ldw,
+                                  int M, int N, int K, int dtype, int want_gx, int want_gw, int want_gb) {
+    CafeBackward f = {};
+    f.gy = gy_dev; f.ldg = ldg; f.slope_kind = slope_kind; f.x = x_dev; f.ldx = ldx; f.w = w_dev; f.ldw = ldw; f.M = M; f.N = N; f.K = K;
+    f.gx = want_gx ? (void*)k_aligned : nullptr; f.gw = want_gw ? (void*)k_aligned : nullptr; f.gb = want_gb ? (void*)k_aligned : nullptr;
+    return dense_type_ok(dtype) && dense_sizes_ok(M, N, K) ? cafe_tiles_backward_work(f, dtype) : 0;
 }
 
 int cafe_linear_backward(const void* gy_dev, int64_t ldg, const void* slope_dev, int64_t lds, int slope_kind, const void* x_dev, int64_t ldx,
                          const void* w_dev, int64_t ldw, int M, int N, int K, int dtype, void* gx_dev, int64_t ldgx, void* gw_dev, int64_t ldgw,
-                         void* gb_dev, void* stream) {
+                         void* gb_dev, void* work_dev, int64_t work_bytes, void* stream) {
     const CafeBackward f = {gy_dev, slope_dev, x_dev, w_dev, ldg, lds, ldx, ldw, slope_kind, M, N, K, gx_dev, gw_dev, gb_dev, ldgx, ldgw};
-    if (!dense_type_ok(dtype) || !dense_backward_ok(f)) return CAFE_ERR_ARG;
+    if (!dense_type_ok(dtype) || !dense_backward_ok(f) || !dense_work_ok(work_dev, work_bytes)) return CAFE_ERR_ARG;
     cudaError_t e;
-    DENSE_TYPED(dtype, e = dense_backward<T>(f, (cudaStream_t)stream));
+    DENSE_TYPED(dtype, e = dense_backward<T>(f, dtype, work_dev, work_bytes, (cudaStream_t)stream));
     return dense_done(e);
+}
+
+int64_t cafe_mlp_forward_work(int layers, const int* widths, int M, const void* x_dev, int64_t ldx, const void* const* w_dev, const int64_t* ldw, int dtype) {
+    if (layers < 1 || layers > CAFE_MLP_MAX_LAYERS || !widths || !w_dev || !ldw) return 0;
+    int64_t most = 0;
+    for (int l = 0; l < layers; ++l) {
+        const int64_t need = cafe_linear_forward_work(l ? k_aligned : x_dev, l ? (widths[l] + 7) & ~7 : ldx, w_dev[l], ldw[l], M, widths[l + 1], widths[l], dtype);
+        most = need > most ? need : most;
+    }
+    return most;
 }
 
 int cafe_mlp_forward(int layers, const int* widths, int M, const void* x_dev, int64_t ldx, const void* const* w_dev, const int64_t* ldw,
                      const void* const* bias_dev, const int* acts, int dtype, void* const* y_dev, const int64_t* ldy, void* const* slope_dev,
-                     void* stream) {
+                     void* work_dev, int64_t work_bytes, void* stream) {
     if (!dense_type_ok(dtype) || layers < 1 || layers > CAFE_MLP_MAX_LAYERS || !widths || !w_dev || !ldw || !bias_dev || !acts || !y_dev || !ldy) return CAFE_ERR_ARG;
+    if (!dense_work_ok(work_dev, work_bytes)) return CAFE_ERR_ARG;
     CafeForward f[CAFE_MLP_MAX_LAYERS];
     for (int l = 0; l < layers; ++l) {
         f[l] = {l ? y_dev[l - 1] : x_dev, w_dev[l], bias_dev[l], nullptr, l ? ldy[l - 1] : ldx, ldw[l], 0, M, widths[l + 1], widths[l], acts[l],
@@ -634,14 +536,21 @@ int cafe_mlp_forward(int layers, const int* widths, int M, const void* x_dev, in
         if (!dense_forward_ok(f[l])) return CAFE_ERR_ARG;
     }
     cudaError_t e = cudaSuccess;
-    for (int l = 0; l < layers && e == cudaSuccess; ++l) DENSE_TYPED(dtype, e = dense_forward<T>(f[l], (cudaStream_t)stream));
+    for (int l = 0; l < layers && e == cudaSuccess; ++l) DENSE_TYPED(dtype, e = dense_forward<T>(f[l], dtype, work_dev, work_bytes, (cudaStream_t)stream));
     return dense_done(e);
 }
 
-int64_t cafe_mlp_backward_work(int layers, const int* widths, int M, int dtype) {
+int64_t cafe_mlp_backward_work(int layers, const int* widths, int M, const void* gy_dev, int64_t ldg, const void* x_dev, int64_t ldx,
+                               const void* const* w_dev, const int64_t* ldw, int dtype) {
+    if (!dense_type_ok(dtype) || layers < 1 || layers > CAFE_MLP_MAX_LAYERS || !widths || !w_dev || !ldw || M < 0 || M > CAFE_LINEAR_MAX) return 0;
     int64_t most = 0;
-    for (int l = 1; l < layers; ++l) most = widths[l] > most ? widths[l] : most;
-    return 2 * ((((most + 7) & ~(int64_t)7) * M * (dtype == CAFE_F32 ? 4 : 2) + 255) & ~(int64_t)255);
+    for (int l = 0; l < layers; ++l) {
+        const int64_t ldn = (widths[l + 1] + 7) & ~7, ldk = (widths[l] + 7) & ~7;
+        const int64_t need = cafe_linear_backward_work(l == layers - 1 ? gy_dev : k_aligned, l == layers - 1 ? ldg : ldn, CAFE_SLOPE_VALUES,
+                                                       l ? k_aligned : x_dev, l ? ldk : ldx, w_dev[l], ldw[l], M, widths[l + 1], widths[l], dtype, 1, 1, 1);
+        most = need > most ? need : most;
+    }
+    return 2 * dense_half(layers, widths, M, dtype) + most;
 }
 
 int cafe_mlp_backward(int layers, const int* widths, int M, const void* gy_dev, int64_t ldg, const void* x_dev, int64_t ldx,
@@ -649,14 +558,17 @@ int cafe_mlp_backward(int layers, const int* widths, int M, const void* gy_dev, 
                       const void* const* slope_dev, void* gx_dev, int64_t ldgx, void* const* gw_dev, void* const* gb_dev, void* work_dev,
                       int64_t work_bytes, void* stream) {
     if (!dense_type_ok(dtype) || layers < 1 || layers > CAFE_MLP_MAX_LAYERS || !widths || !w_dev || !ldw || !acts || !y_dev || !ldy || !gw_dev || !gb_dev) return CAFE_ERR_ARG;
-    const int64_t need = cafe_mlp_backward_work(layers, widths, M, dtype);
-    if (need > 0 && (!work_dev || work_bytes < need || ((uintptr_t)work_dev & 15))) return CAFE_ERR_ARG;
+    if (M < 0 || M > CAFE_LINEAR_MAX) return CAFE_ERR_ARG;
+    for (int l = 0; l <= layers; ++l) if (widths[l] < 0 || widths[l] > CAFE_LINEAR_MAX) return CAFE_ERR_ARG;
+    const int64_t half_bytes = dense_half(layers, widths, M, dtype);
+    if (half_bytes > 0 && (!work_dev || work_bytes < 2 * half_bytes)) return CAFE_ERR_ARG;
+    if (!dense_work_ok(work_dev, work_bytes)) return CAFE_ERR_ARG;
+    char* const half[2] = {(char*)work_dev, (char*)work_dev + half_bytes};
     CafeBackward f[CAFE_MLP_MAX_LAYERS];
     for (int l = layers - 1; l >= 0; --l) {
         const bool last = l == layers - 1;
         const int kind = acts[l] == CAFE_ACT_NONE ? CAFE_SLOPE_NONE : slope_dev && slope_dev[l] ? CAFE_SLOPE_VALUES : CAFE_SLOPE_OUTPUT;
         if (kind == CAFE_SLOPE_OUTPUT && acts[l] != CAFE_ACT_RELU) return CAFE_ERR_ARG;
-        char* const half[2] = {(char*)work_dev, (char*)work_dev + need / 2};
         const int64_t ldn = (widths[l + 1] + 7) & ~7, ldk = (widths[l] + 7) & ~7;
         f[l] = {last ? gy_dev : half[l & 1], kind == CAFE_SLOPE_VALUES ? slope_dev[l] : y_dev[l], l ? y_dev[l - 1] : x_dev, w_dev[l],
                 last ? ldg : ldn, ldy[l], l ? ldy[l - 1] : ldx, ldw[l], kind, M, widths[l + 1], widths[l],
@@ -664,7 +576,8 @@ int cafe_mlp_backward(int layers, const int* widths, int M, const void* gy_dev, 
         if (!dense_backward_ok(f[l])) return CAFE_ERR_ARG;
     }
     cudaError_t e = cudaSuccess;
-    for (int l = layers - 1; l >= 0 && e == cudaSuccess; --l) DENSE_TYPED(dtype, e = dense_backward<T>(f[l], (cudaStream_t)stream));
+    for (int l = layers - 1; l >= 0 && e == cudaSuccess; --l)
+        DENSE_TYPED(dtype, e = dense_backward<T>(f[l], dtype, half[1] + half_bytes, work_bytes - 2 * half_bytes, (cudaStream_t)stream));
     return dense_done(e);
 }
 

@@ -1,0 +1,511 @@
+// dense_tiles.cu -- the products of large layers: operands laid out for the copy engine first, then tiles that nothing but copies
+// and matrix instructions work on.
+//
+// dense_cuda.cu's kernel cuts and stores its operands itself, once for every tile that reads them; its loading warps set its
+// pace.  Where a product is large that work is done once: k_parts writes x, W or gz = gy * act'(z) as bf16 parts (three of fp32,
+// pitch rounded up to 16 bytes; 16-bit tensors only where their rows are not on 16 bytes or a slope belongs to them, otherwise
+// they are read in place), with the column sums of gz on the way, and k_tiles fetches boxes of them by cp.async.bulk.tensor
+// in the order the tensor cores read, whichever index is contiguous.
+//
+// k_tiles: a block makes 128 x BN outputs; one thread fetches, one issues products, four warps take the sums out (and meanwhile
+// add up the bias gradient).  Two blocks share an SM, so that one's end runs beside the other's products; two stages of 48 KB
+// each.  Blocks of a cluster share the depth of a tile as in dense_cuda.cu.
+#include <cuda.h>
+
+#include "dense.cuh"
+
+#define CAFE_TILES_THREADS 192
+#define CAFE_PARTS_ROWS 128    // rows of a block of k_parts: a row of partial column sums each
+#define CAFE_PARTS_COLS 256
+
+__device__ int g_tiles_gave_up;   // a wait ran out (its outputs are not numbers)
+
+template <typename T> struct CafeTiles {
+    static constexpr int parts = 1, BK = 64, type = 0;
+    typedef T part;
+};
+template <> struct CafeTiles<__nv_bfloat16> { static constexpr int parts = 1, BK = 64, type = 1; typedef __nv_bfloat16 part; };
+template <> struct CafeTiles<float> { static constexpr int parts = 3, BK = 32, type = 1; typedef __nv_bfloat16 part; };
+#define CAFE_TILES_CHUNK 8     // fp32: turns of 32 between two times that the large sums are taken out
+
+// ---- operands as parts ---------------------------------------------------------------------------------------------------
+struct CafePartsJob {
+    const void *src, *slope;
+    int64_t ld, lds, pitch, plane;   // pitch and plane of dst in elements
+    int kind, vec, slope_vec, rows, cols, blocks_x, blocks;
+    void* dst;                       // null: sums only
+    float* sums;                     // [row blocks][cols] sums of the rows of each block, or null
+};
+struct CafeParts {
+    CafePartsJob job[3];
+    int count;
+};
+template <typename T> __device__ __forceinline__ void cafe_read8(const T* p, int n, bool vec, float* v) {
+    if (vec && n == 8) {
+        alignas(16) T x[8];
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(x)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = cafe_to_float(x[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = j < n ? cafe_to_float(__ldg(p + j)) : 0.f;
+    }
+}
+// Bound by its bytes: fp32 4 in (8 with a slope) and 6 out an element.
+template <typename T>
+__global__ void __launch_bounds__(256) k_parts(const __grid_constant__ CafeParts P) {
+    typedef typename CafeSlopeOf<T>::type ST;
+    __shared__ float part[8][CAFE_PARTS_COLS];
+    int block = blockIdx.x, q = 0;
+    while (q + 1 < P.count && block >= P.job[q].blocks) block -= P.job[q++].blocks;
+    const CafePartsJob& J = P.job[q];
+    const int by = block / J.blocks_x, bx = block - by * J.blocks_x;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int col = bx * CAFE_PARTS_COLS + lane * 8, n = min(8, J.cols - col);
+    float sum[8] = {};
+    const int64_t r0 = (int64_t)by * CAFE_PARTS_ROWS, r1 = min(r0 + CAFE_PARTS_ROWS, (int64_t)J.rows);
+    if (n > 0) {
+#pragma unroll 2
+        for (int64_t r = r0 + warp; r < r1; r += 8) {
+            alignas(16) float v[8];
+            cafe_read8(static_cast<const T*>(J.src) + r * J.ld + col, n, J.vec, v);
+            if (J.kind == CAFE_SLOPE_VALUES) {
+                float s[8];
+                cafe_read8(static_cast<const ST*>(J.slope) + r * J.lds + col, n, J.slope_vec, s);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] *= s[j];
+            } else if (J.kind == CAFE_SLOPE_OUTPUT) {
+                float s[8];
+                cafe_read8(static_cast<const T*>(J.slope) + r * J.lds + col, n, J.slope_vec, s);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = s[j] > 0.f ? v[j] : 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum[j] += v[j];
+            if (!J.dst) continue;
+            uint4* out = reinterpret_cast<uint4*>(static_cast<typename CafeTiles<T>::part*>(J.dst) + r * J.pitch + col);
+            if constexpr (sizeof(T) == 2) {
+                alignas(16) T o[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) o[j] = cafe_from_float<T>(v[j]);
+                *out = *reinterpret_cast<const uint4*>(o);
+            } else {
+#pragma unroll
+                for (int p = 0; p < 3; ++p) {   // the next 8 bits of each, cut off
+                    uint32_t o[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        o[j] = __byte_perm(__float_as_uint(v[2 * j]), __float_as_uint(v[2 * j + 1]), 0x7632);
+                        v[2 * j] -= __uint_as_float(__float_as_uint(v[2 * j]) & 0xffff0000u);
+                        v[2 * j + 1] -= __uint_as_float(__float_as_uint(v[2 * j + 1]) & 0xffff0000u);
+                    }
+                    out[(int64_t)p * J.plane / 8] = make_uint4(o[0], o[1], o[2], o[3]);
+                }
+            }
+        }
+    }
+    if (!J.sums) return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) part[warp][lane * 8 + j] = sum[j];
+    __syncthreads();
+    const int c = bx * CAFE_PARTS_COLS + threadIdx.x;
+    if (c >= J.cols) return;
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) s += part[w][threadIdx.x];
+    J.sums[(int64_t)by * J.cols + c] = s;
+}
+
+// ---- tiles ---------------------------------------------------------------------------------------------------------------
+template <typename T, int BN> struct CafeTilesShape {
+    typedef CafeTiles<T> L;
+    static constexpr int rowb = L::BK * 2;
+    static constexpr int a_part = CAFE_LIN_BM * rowb, b_part = BN * rowb, stage = L::parts * (a_part + b_part);
+    static constexpr int tile = CAFE_LIN_BM * (128 + 4) * 4;
+    static constexpr int stages = 98304 / stage < 6 ? 98304 / stage : 6;
+    static constexpr int bytes = (stage * stages > tile ? stage * stages : tile) + 1024;
+    static constexpr int tm_cols = L::parts == 3 ? 2 * BN : BN;
+};
+struct CafeTilesArgs {
+    CUtensorMap a, b;
+    CafeJob job;
+    const float* sums;   // partial column sums of A for job.gb
+    int sum_rows, splits;
+};
+
+template <typename T, int BN>
+__global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_constant__ CafeTilesArgs P) {
+    typedef CafeTiles<T> L;
+    typedef CafeTilesShape<T, BN> Sh;
+    extern __shared__ char sh_raw[];
+    __shared__ __align__(8) uint64_t bars[2 * Sh::stages + 3];
+    __shared__ uint32_t tm_at;
+    __shared__ volatile int bail;
+    const uint32_t base = (cafe_smem(sh_raw) + 1023u) & ~1023u;
+    const uint32_t bar0 = cafe_smem(bars);
+    auto full = [&](int s) { return bar0 + 8u * s; };
+    auto empty = [&](int s) { return bar0 + 8u * (Sh::stages + s); };
+    const uint32_t acc_full = bar0 + 8u * (2 * Sh::stages), acc_empty = acc_full + 8, all_done = acc_full + 16;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const CafeJob& J = P.job;
+    const int splits = P.splits, tile = blockIdx.x / splits, rank = blockIdx.x - tile * splits;
+    const int tm = tile / J.tiles_n, tn = tile - tm * J.tiles_n, row0 = tm * CAFE_LIN_BM, col0 = tn * BN;
+    const int turns_all = (J.depth + L::BK - 1) / L::BK, share = (turns_all + splits - 1) / splits;
+    const int t0 = min(rank * share, turns_all), turns = min(share, turns_all - t0);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < Sh::stages; ++s) { cafe_bar_init(full(s), 1); cafe_bar_init(empty(s), 1); }
+        cafe_bar_init(acc_full, 1);
+        cafe_bar_init(acc_empty, 4);
+        cafe_bar_init(all_done, 1);
+        cafe_fence_barrier_init();
+        bail = 0;
+    }
+    if (warp == 1) cafe_tm_alloc(cafe_smem(&tm_at), Sh::tm_cols);
+    cafe_tc_before();
+    __syncthreads();
+    cafe_tc_after();
+    const uint32_t tmem = tm_at;
+
+    constexpr int taken = L::parts == 3 ? BN : 32;
+    float acc[taken];
+    const uint32_t from = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    bool fine = true;
+    if (warp == 0) {
+        if (lane == 0) {
+            // ---- boxes of the operands
+            int t = 0;
+            for (; t < turns; ++t) {
+                const int s = t % Sh::stages, k0 = (t0 + t) * L::BK;
+                if (t >= Sh::stages && !cafe_bar_wait(empty(s), (uint32_t)(t / Sh::stages - 1) & 1u, &bail)) break;
+                const uint32_t a = base + s * Sh::stage, b = a + L::parts * Sh::a_part;
+                cafe_bar_expect(full(s), Sh::stage);
+                if (J.a_kc) cafe_box_load(a, &P.a, k0, row0, 0, full(s));
+                else
+#pragma unroll
+                    for (int q = 0; q < CAFE_LIN_BM / 64; ++q) cafe_box_load(a + q * L::parts * L::BK * 128, &P.a, row0 + 64 * q, k0, 0, full(s));
+                if (J.b_kc) cafe_box_load(b, &P.b, k0, col0, 0, full(s));
+                else
+#pragma unroll
+                    for (int q = 0; q < BN / 64; ++q) cafe_box_load(b + q * L::parts * L::BK * 128, &P.b, col0 + 64 * q, k0, 0, full(s));
+            }
+            if (t < turns)   // given up: the copies in flight end before the block does
+                for (int u = max(0, t - Sh::stages); u < t; ++u)
+                    for (int i = 0; i < (1 << 20) && !cafe_bar_try(full(u % Sh::stages), (uint32_t)(u / Sh::stages) & 1u); ++i) {}
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            // ---- products
+            const uint32_t instr = cafe_mma_instr(L::type, CAFE_LIN_BM, BN) | (J.a_kc ? 0u : 1u << 15) | (J.b_kc ? 0u : 1u << 16);
+            const uint64_t da = J.a_kc ? cafe_operand<Sh::rowb>(base) : cafe_operand_mn(base, L::parts * L::BK * 128);
+            const uint64_t db = J.b_kc ? cafe_operand<Sh::rowb>(base + L::parts * Sh::a_part) : cafe_operand_mn(base + L::parts * Sh::a_part, L::parts * L::BK * 128);
+            // offsets in 16-byte units: from a part to the next, from 16 k to the next 16
+            const uint32_t ap = (J.a_kc ? Sh::a_part : L::BK * 128) >> 4, bp = (J.b_kc ? Sh::b_part : L::BK * 128) >> 4;
+            const uint32_t ak = (J.a_kc ? 32 : 2048) >> 4, bk = (J.b_kc ? 32 : 2048) >> 4;
+            for (int t = 0; t < turns; ++t) {
+                const int s = t % Sh::stages;
+                if (!(fine = cafe_bar_wait(full(s), (uint32_t)(t / Sh::stages) & 1u, &bail))) break;
+                const bool opens = L::parts == 3 ? t % CAFE_TILES_CHUNK == 0 : t == 0;
+                if (L::parts == 3 && opens && t > 0 && !(fine = cafe_bar_wait(acc_empty, (uint32_t)(t / CAFE_TILES_CHUNK - 1) & 1u, &bail))) break;
+                cafe_tc_after();
+                const uint64_t a = da + (uint32_t)(s * Sh::stage >> 4), b = db + (uint32_t)(s * Sh::stage >> 4);
+#pragma unroll
+                for (int k = 0; k < L::BK / 16; ++k) cafe_mma(tmem, a + ak * k, b + bk * k, instr, !opens || k > 0);
+                if constexpr (L::parts == 3) {
+                    if (t % CAFE_TILES_CHUNK == CAFE_TILES_CHUNK - 1 || t == turns - 1) cafe_mma_commit(acc_full);
+#pragma unroll
+                    for (int q = 0; q < 5; ++q) {
+                        constexpr int ia[5] = {0, 1, 1, 0, 2}, ib[5] = {1, 0, 1, 2, 0};
+#pragma unroll
+                        for (int k = 0; k < L::BK / 16; ++k)
+                            cafe_mma(tmem + BN, a + ia[q] * ap + ak * k, b + ib[q] * bp + bk * k, instr, t > 0 || q > 0 || k > 0);
+                    }
+                }
+                cafe_mma_commit(empty(s));
+            }
+            cafe_mma_commit(all_done);
+        }
+    } else {
+        // ---- sums out of tensor memory, 32 rows a warp; before that the bias gradient from its partial sums
+        if (P.sums && tn == 0 && rank == 0) {
+            const int r = row0 + (int)threadIdx.x - 64;
+            if (r < J.rows) {
+                float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+                int q = 0;
+                for (; q + 4 <= P.sum_rows; q += 4) {
+                    s0 += __ldg(P.sums + (int64_t)q * J.rows + r);
+                    s1 += __ldg(P.sums + (int64_t)(q + 1) * J.rows + r);
+                    s2 += __ldg(P.sums + (int64_t)(q + 2) * J.rows + r);
+                    s3 += __ldg(P.sums + (int64_t)(q + 3) * J.rows + r);
+                }
+                for (; q < P.sum_rows; ++q) s0 += __ldg(P.sums + (int64_t)q * J.rows + r);
+                static_cast<T*>(J.gb)[r] = cafe_from_float<T>((s0 + s1) + (s2 + s3));
+            }
+            __syncwarp();
+        }
+        if constexpr (L::parts == 3) {
+            auto take = [&](uint32_t at, bool first) {
+#pragma unroll
+                for (int c = 0; c < BN; c += 16) {
+                    float v[16];
+                    cafe_tm_load16(at + c, v);
+                    cafe_tm_wait_load();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[c + i] = first ? v[i] : acc[c + i] + v[i];
+                }
+            };
+            const int chunks = (turns + CAFE_TILES_CHUNK - 1) / CAFE_TILES_CHUNK;
+            if (turns == 0) {
+#pragma unroll
+                for (int i = 0; i < BN; ++i) acc[i] = 0.f;
+            }
+            for (int c = 0; c < chunks && fine; ++c) {
+                fine = cafe_bar_wait(acc_full, (uint32_t)c & 1u, &bail);
+                cafe_tc_after();
+                fine = __all_sync(0xffffffffu, fine);
+                if (fine) take(from, c == 0);
+                cafe_tc_before();
+                __syncwarp();
+                if (lane == 0) cafe_bar_arrive(acc_empty);
+            }
+            fine = cafe_bar_wait(all_done, 0, &bail) && fine;
+            cafe_tc_after();
+            fine = __all_sync(0xffffffffu, fine);
+            if (fine && turns > 0) take(from + BN, false);
+        } else {
+            fine = cafe_bar_wait(all_done, 0, &bail);
+            cafe_tc_after();
+            fine = __all_sync(0xffffffffu, fine);
+        }
+        if (!fine) g_tiles_gave_up = 1;
+    }
+    __syncwarp();
+    // ---- 128 columns at a time: sums to shared memory (the stages are free: all products are done), then what belongs at the end
+    for (int h = 0; h < BN / 128; ++h) {
+        if (col0 + h * 128 >= J.cols) break;   // (the same for all blocks of the cluster)
+        __syncthreads();
+        if (warp >= 2) {
+            const int r = (warp & 3) * 32 + lane;
+            const uint32_t at = base + (uint32_t)(r * 132) * 4u;
+            const bool ok = fine && !bail;
+            if constexpr (L::parts == 3) {
+                if (!ok) {
+#pragma unroll
+                    for (int i = 0; i < BN; ++i) acc[i] = __uint_as_float(0x7fffffffu);
+                }
+                cafe_sums_put<true, BN>(J, acc, at, row0 + r, col0, t0 * L::BK, min(J.depth, (t0 + turns) * L::BK), ok);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 128; c += 32) {
+                    cafe_tm_load16(from + h * 128 + c, acc);
+                    cafe_tm_load16(from + h * 128 + c + 16, acc + 16);
+                    cafe_tm_wait_load();
+                    if (!ok || turns == 0) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) acc[i] = ok ? 0.f : __uint_as_float(0x7fffffffu);
+                    }
+                    cafe_sums_put<false, 32>(J, acc, at + 4 * c, 0, 0, 0, 0, false);
+                }
+            }
+        }
+        if (splits > 1) cafe_cluster_sync(); else __syncthreads();
+        cafe_finish<T, 128>(J, base, row0, col0 + h * 128, rank, splits, CAFE_TILES_THREADS);
+        if (splits > 1) cafe_cluster_sync();   // (others may still read this block's sums)
+    }
+    cafe_tc_before();
+    __syncthreads();
+    cafe_tc_after();
+    if (warp == 1) cafe_tm_free(tmem, Sh::tm_cols);
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------------
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeTiled tiles_encoder() {
+    static const EncodeTiled f = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) != cudaSuccess || r != cudaDriverEntryPointSuccess) p = nullptr;
+        return (EncodeTiled)p;
+    }();
+    return f;
+}
+
+// an operand as the copies see it: rows x cols (cols contiguous), `parts` planes
+struct TilesOperand {
+    const void* at;
+    int64_t pitch, plane;
+    int rows, cols;
+};
+// `kc`: cols is the depth
+template <typename T>
+static bool tiles_map(CUtensorMap* map, const TilesOperand& o, int kc, int box) {
+    typedef CafeTiles<T> L;
+    const cuuint64_t dims[3] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)L::parts};
+    const cuuint64_t strides[2] = {(cuuint64_t)o.pitch * 2, (cuuint64_t)(L::parts == 1 ? o.pitch : o.plane) * 2};
+    const cuuint32_t boxes[3] = {(cuuint32_t)(kc ? L::BK : 64), (cuuint32_t)(kc ? box : L::BK), (cuuint32_t)L::parts}, steps[3] = {1, 1, 1};
+    const CUtensorMapDataType type = L::type ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const CUtensorMapSwizzle sw = kc && L::BK == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+    return tiles_encoder()(map, type, 3, const_cast<void*>(o.at), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int BN>
+static cudaError_t tiles_launch_bn(CafeTilesArgs& P, const TilesOperand& a, const TilesOperand& b, cudaStream_t st) {
+    // (a bias gradient alone: no columns, no depth, nothing fetched)
+    if (P.job.depth > 0 && (!tiles_map<T>(&P.a, a, P.job.a_kc, CAFE_LIN_BM) || !tiles_map<T>(&P.b, b, P.job.b_kc, BN))) return cudaErrorInvalidValue;
+    P.job.tiles_n = P.job.cols > 0 ? (P.job.cols + BN - 1) / BN : 1;
+    P.job.tiles = ((P.job.rows + CAFE_LIN_BM - 1) / CAFE_LIN_BM) * P.job.tiles_n;
+    constexpr int bytes = CafeTilesShape<T, BN>::bytes;
+    cudaError_t e = cudaFuncSetAttribute(k_tiles<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(P.job.tiles * P.splits));
+    cfg.blockDim = dim3(CAFE_TILES_THREADS);
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)P.splits; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    CAFE_PROF(CAFE_P_LINEAR, st);
+    return cudaLaunchKernelEx(&cfg, k_tiles<T, BN>, (const CafeTilesArgs&)P);
+}
+// blocks per tile: the fewest rounds of 296 blocks for the depth that each has (a block costs 8 turns beside its own)
+template <typename T>
+static cudaError_t tiles_launch(CafeTilesArgs& P, const TilesOperand& a, const TilesOperand& b, cudaStream_t st) {
+    typedef CafeTiles<T> L;
+    const bool wide = L::parts == 1 && P.job.cols > 128;
+    const int bn = wide ? 256 : 128;
+    const int64_t tiles = (int64_t)((P.job.rows + CAFE_LIN_BM - 1) / CAFE_LIN_BM) * ((P.job.cols + bn - 1) / bn);
+    const int turns = (P.job.depth + L::BK - 1) / L::BK;
+    double best = 1e300;
+    for (int s = 1; s <= 8; s *= 2) {
+        const int64_t rounds = (tiles * s + 295) / 296;
+        const double est = (double)rounds * ((turns + s - 1) / s + 8 + (s > 1 ? 2 : 0));
+        if (est < best * 0.999) { best = est; P.splits = s; }
+    }
+    if constexpr (L::parts == 1) {
+        if (wide) return tiles_launch_bn<T, 256>(P, a, b, st);
+    }
+    return tiles_launch_bn<T, 128>(P, a, b, st);
+}
+
+static int64_t tiles_round(int64_t bytes) { return (bytes + 255) & ~(int64_t)255; }
+static int64_t tiles_pitch(int cols) { return (cols + 7) & ~7; }
+static int64_t tiles_bytes(int parts, int rows, int cols) { return tiles_round((int64_t)parts * rows * tiles_pitch(cols) * 2); }
+static bool tiles_in_place(int dtype, const void* p, int64_t ld) { return dtype != CAFE_F32 && ((uintptr_t)p & 15) == 0 && ld % 8 == 0; }
+
+// an operand: in place, or laid out at *work by a job of the next k_parts launch
+template <typename T>
+static TilesOperand tiles_operand(CafeParts* P, char** work, int dtype, const void* src, int64_t ld, int rows, int cols, const void* slope, int64_t lds,
+                                  int kind, float* sums) {
+    typedef CafeTiles<T> L;
+    const bool in_place = kind == CAFE_SLOPE_NONE && tiles_in_place(dtype, src, ld);
+    TilesOperand o = {src, ld, 0, rows, cols};
+    if (in_place && !sums) return o;
+    CafePartsJob& J = P->job[P->count++];
+    J.src = src; J.slope = slope; J.ld = ld; J.lds = lds; J.kind = kind;
+    J.vec = ((uintptr_t)src & 15) == 0 && ld * (int64_t)sizeof(T) % 16 == 0;
+    const int ss = kind == CAFE_SLOPE_VALUES ? (int)sizeof(typename CafeSlopeOf<T>::type) : (int)sizeof(T);
+    J.slope_vec = ((uintptr_t)slope & 15) == 0 && lds * ss % 16 == 0;
+    J.rows = rows; J.cols = cols; J.sums = sums;
+    J.blocks_x = (cols + CAFE_PARTS_COLS - 1) / CAFE_PARTS_COLS;
+    J.blocks = J.blocks_x * ((rows + CAFE_PARTS_ROWS - 1) / CAFE_PARTS_ROWS);
+    J.dst = nullptr;
+    if (!in_place) {
+        J.dst = *work;
+        J.pitch = o.pitch = tiles_pitch(cols);
+        J.plane = o.plane = (int64_t)rows * J.pitch;
+        o.at = *work;
+        *work += tiles_bytes(L::parts, rows, cols);
+    }
+    return o;
+}
+template <typename T>
+static cudaError_t tiles_parts(const CafeParts& P, cudaStream_t st) {
+    int blocks = 0;
+    for (int q = 0; q < P.count; ++q) blocks += P.job[q].blocks;
+    if (blocks == 0) return cudaSuccess;
+    CAFE_PROF(CAFE_P_LINEAR, st);
+    k_parts<T><<<blocks, 256, 0, st>>>(P);
+    return cudaGetLastError();
+}
+
+// Which calls: products of at least CAFE_TILES_LEAST multiply-adds that are no narrow strips.
+#define CAFE_TILES_LEAST (1ll << 29)
+// (Sums over more than 2^17 of k in one go, 2^20 over the blocks of a cluster, would lose bits of a 16-bit result.)
+static bool tiles_large(int M, int N, int K) {
+    return (int64_t)M * N * K >= CAFE_TILES_LEAST && M >= 128 && N >= 64 && K >= 64 && M <= 1 << 20 && N <= 1 << 17 && K <= 1 << 17;
+}
+
+int64_t cafe_tiles_forward_work(const CafeForward& f, int dtype) {
+    if (!tiles_large(f.M, f.N, f.K)) return 0;
+    const int parts = dtype == CAFE_F32 ? 3 : 1;
+    return 256 + (tiles_in_place(dtype, f.x, f.ldx) ? 0 : tiles_bytes(parts, f.M, f.K)) + (tiles_in_place(dtype, f.w, f.ldw) ? 0 : tiles_bytes(parts, f.N, f.K));
+}
+int64_t cafe_tiles_backward_work(const CafeBackward& f, int dtype) {
+    if (!tiles_large(f.M, f.N, f.K) || (!f.gx && !f.gw)) return 0;
+    const int parts = dtype == CAFE_F32 ? 3 : 1;
+    int64_t need = 256;
+    if (f.slope_kind != CAFE_SLOPE_NONE || !tiles_in_place(dtype, f.gy, f.ldg)) need += tiles_bytes(parts, f.M, f.N);
+    if (f.gx && !tiles_in_place(dtype, f.w, f.ldw)) need += tiles_bytes(parts, f.N, f.K);
+    if (f.gw && !tiles_in_place(dtype, f.x, f.ldx)) need += tiles_bytes(parts, f.M, f.K);
+    if (f.gb) need += tiles_round((int64_t)((f.M + CAFE_PARTS_ROWS - 1) / CAFE_PARTS_ROWS) * f.N * 4);
+    return need;
+}
+
+template <typename T>
+static cudaError_t tiles_forward(const CafeForward& f, int dtype, const CafeJob& job, char* work, cudaStream_t st) {
+    CafeParts parts = {};
+    const TilesOperand x = tiles_operand<T>(&parts, &work, dtype, f.x, f.ldx, f.M, f.K, nullptr, 0, CAFE_SLOPE_NONE, nullptr);
+    const TilesOperand w = tiles_operand<T>(&parts, &work, dtype, f.w, f.ldw, f.N, f.K, nullptr, 0, CAFE_SLOPE_NONE, nullptr);
+    cudaError_t e = tiles_parts<T>(parts, st);
+    if (e != cudaSuccess) return e;
+    CafeTilesArgs P = {};
+    P.job = job;
+    return tiles_launch<T>(P, x, w, st);
+}
+template <typename T>
+static cudaError_t tiles_backward(const CafeBackward& f, int dtype, const CafeJob* gw, const CafeJob* gx, char* work, cudaStream_t st) {
+    CafeParts parts = {};
+    float* sums = nullptr;
+    const int sum_rows = (f.M + CAFE_PARTS_ROWS - 1) / CAFE_PARTS_ROWS;
+    if (f.gb) {
+        sums = (float*)work;
+        work += tiles_round((int64_t)sum_rows * f.N * 4);
+    }
+    const TilesOperand g = tiles_operand<T>(&parts, &work, dtype, f.gy, f.ldg, f.M, f.N, f.slope, f.lds, f.slope_kind, sums);
+    TilesOperand w = {}, x = {};
+    if (gx) w = tiles_operand<T>(&parts, &work, dtype, f.w, f.ldw, f.N, f.K, nullptr, 0, CAFE_SLOPE_NONE, nullptr);
+    if (f.gw) x = tiles_operand<T>(&parts, &work, dtype, f.x, f.ldx, f.M, f.K, nullptr, 0, CAFE_SLOPE_NONE, nullptr);
+    cudaError_t e = tiles_parts<T>(parts, st);
+    if (e != cudaSuccess) return e;
+    if (gw) {
+        CafeTilesArgs P = {};
+        P.job = *gw;
+        if (!f.gw) P.job.depth = 0;
+        P.sums = sums; P.sum_rows = sum_rows;
+        if ((e = tiles_launch<T>(P, g, x, st)) != cudaSuccess) return e;
+    }
+    if (gx) {
+        CafeTilesArgs P = {};
+        P.job = *gx;
+        if ((e = tiles_launch<T>(P, g, w, st)) != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+}
+cudaError_t cafe_tiles_forward(const CafeForward& f, int dtype, const CafeJob& job, void* work, cudaStream_t st) {
+    if (!tiles_encoder()) return cudaErrorNotSupported;
+    char* const at = (char*)(((uintptr_t)work + 255) & ~(uintptr_t)255);
+    return dtype == CAFE_F32 ? tiles_forward<float>(f, dtype, job, at, st)
+                             : dtype == CAFE_BF16 ? tiles_forward<__nv_bfloat16>(f, dtype, job, at, st) : tiles_forward<__half>(f, dtype, job, at, st);
+}
+cudaError_t cafe_tiles_backward(const CafeBackward& f, int dtype, const CafeJob* gw, const CafeJob* gx, void* work, cudaStream_t st) {
+    if (!tiles_encoder()) return cudaErrorNotSupported;
+    char* const at = (char*)(((uintptr_t)work + 255) & ~(uintptr_t)255);
+    return dtype == CAFE_F32 ? tiles_backward<float>(f, dtype, gw, gx, at, st)
+                             : dtype == CAFE_BF16 ? tiles_backward<__nv_bfloat16>(f, dtype, gw, gx, at, st) : tiles_backward<__half>(f, dtype, gw, gx, at, st);
+}

@@ -84,3 +84,15 @@ __device__ __forceinline__ float cafe_cluster_load(uint32_t at) {
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
     return v;
 }
+
+// a barrier's next phase also waits for `bytes` of copies
+__device__ __forceinline__ void cafe_bar_expect(uint32_t bar, uint32_t bytes) { asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory"); }
+// a box of a tensor (three axes, the innermost first) into shared memory; what lies outside the tensor becomes zero
+__device__ __forceinline__ void cafe_box_load(uint32_t to, const void* map, int x, int y, int z, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(to), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
+// The operand whose other index is contiguous: panels of 64 of them (128 bytes, pieces exchanged as above) x k, eight k a unit;
+// `panel` bytes from one panel to the next.
+__device__ __forceinline__ uint64_t cafe_operand_mn(uint32_t at, uint32_t panel) {
+    return (uint64_t)((at & 0x3ffffu) >> 4) | (uint64_t)(panel >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}

@@ -75,6 +75,11 @@ def _slope_type(dtype):
     return torch.float16 if dtype == torch.bfloat16 else torch.float32
 
 
+def _work(size, like):
+    """Workspace of one call, from torch's allocator: free again in the stream's order."""
+    return torch.empty(size, dtype=torch.uint8, device=like.device) if size else None
+
+
 def _contiguous(t):
     return t if t is None or t.is_contiguous() else t.contiguous()
 
@@ -94,9 +99,11 @@ def _linear(x, weight, bias, residual, act, keep):
     if keep and act != _NONE and not (act == _RELU and residual is None):
         slope = torch.empty(m, n, dtype=_slope_type(x.dtype), device=x.device)
     b = _contiguous(bias)
+    lib, t = _lib.load(), DTYPES[x.dtype]
+    size = lib.cafe_linear_forward_work(x2.data_ptr(), ldx, w2.data_ptr(), ldw, m, n, k, t)
     with _on(x.device):
-        _lib.check(_lib.load().cafe_linear_forward(x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(b), _ptr(r2), ldr, m, n, k, DTYPES[x.dtype],
-                                                   act, y.data_ptr(), n, _ptr(slope), n, _stream()), "cafe_linear_forward")
+        _lib.check(lib.cafe_linear_forward(x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(b), _ptr(r2), ldr, m, n, k, t, act, y.data_ptr(), n,
+                                           _ptr(slope), n, _ptr(_work(size, x)), size, _stream()), "cafe_linear_forward")
     return x2, w2, y, slope
 
 
@@ -123,11 +130,13 @@ class _FusedLinear(torch.autograd.Function):
         gw = torch.empty(n, k, dtype=g.dtype, device=g.device) if need[1] else None
         gb = torch.empty(n, dtype=g.dtype, device=g.device) if need[2] else None
         if need[0] or need[1] or need[2]:
+            lib, t = _lib.load(), DTYPES[g.dtype]
+            ldx, ldw = k if x is None else _rows(x, k)[2], k if w is None else _rows(w, k)[2]
+            size = lib.cafe_linear_backward_work(g.data_ptr(), ldg, ctx.kind, _ptr(x), ldx, _ptr(w), ldw, m, n, k, t, need[0], need[1], need[2])
             with _on(g.device):
-                _lib.check(_lib.load().cafe_linear_backward(
-                    g.data_ptr(), ldg, _ptr(slope), n, ctx.kind, _ptr(x), k if x is None else _rows(x, k)[2], _ptr(w),
-                    k if w is None else _rows(w, k)[2], m, n, k, DTYPES[g.dtype], _ptr(gx), k, _ptr(gw), k, _ptr(gb), _stream()),
-                    "cafe_linear_backward")
+                _lib.check(lib.cafe_linear_backward(
+                    g.data_ptr(), ldg, _ptr(slope), n, ctx.kind, _ptr(x), ldx, _ptr(w), ldw, m, n, k, t, _ptr(gx), k, _ptr(gw), k, _ptr(gb),
+                    _ptr(_work(size, g)), size, _stream()), "cafe_linear_backward")
         return gx, gw, gb, grad_y if need[3] else None, None
 
 
@@ -174,11 +183,12 @@ def _mlp(x, weights, biases, acts, keep):
     ys.append(torch.empty(*x.shape[:-1], widths[-1], dtype=x.dtype, device=x.device))
     slopes = [torch.empty(m, p, dtype=_slope_type(x.dtype), device=x.device) if keep and a not in (_NONE, _RELU) else None
               for p, a in zip(pitch, acts)]
-    call = ((ctypes.c_int32 * (n + 1))(*widths), m, x2.data_ptr(), ldx, _pointers([w for w, _, _ in ws]), (ctypes.c_int64 * n)(*[ld for _, _, ld in ws]))
+    call = (n, (ctypes.c_int32 * (n + 1))(*widths), m, x2.data_ptr(), ldx, _pointers([w for w, _, _ in ws]), (ctypes.c_int64 * n)(*[ld for _, _, ld in ws]))
+    lib, t = _lib.load(), DTYPES[x.dtype]
+    size = lib.cafe_mlp_forward_work(*call, t)
     with _on(x.device):
-        _lib.check(_lib.load().cafe_mlp_forward(n, *call, _pointers(bs), (ctypes.c_int32 * n)(*acts), DTYPES[x.dtype], _pointers(ys),
-                                                (ctypes.c_int64 * n)(*pitch), _pointers(slopes) if keep else None, _stream()),
-                   "cafe_mlp_forward")
+        _lib.check(lib.cafe_mlp_forward(*call, _pointers(bs), (ctypes.c_int32 * n)(*acts), t, _pointers(ys), (ctypes.c_int64 * n)(*pitch),
+                                        _pointers(slopes) if keep else None, _ptr(_work(size, x)), size, _stream()), "cafe_mlp_forward")
     return x2, [w for w, _, _ in ws], ys, slopes, pitch
 
 
@@ -204,16 +214,14 @@ class _FusedMLP(torch.autograd.Function):
         gx = new(*ctx.shape) if need[0] else None
         gws = [new(*w.shape) if need[2 + l] else None for l, w in enumerate(ws)]
         gbs = [new(w.shape[0]) if need[2 + n + l] else None for l, w in enumerate(ws)]
-        lib = _lib.load()
-        cw = (ctypes.c_int32 * (n + 1))(*widths)
-        size = lib.cafe_mlp_backward_work(n, cw, m, DTYPES[g.dtype])
-        work = torch.empty(size, dtype=torch.uint8, device=g.device)
+        lib, t = _lib.load(), DTYPES[g.dtype]
+        call = (n, (ctypes.c_int32 * (n + 1))(*widths), m, g.data_ptr(), ldg, x.data_ptr(), _rows(x, widths[0])[2], _pointers(ws),
+                (ctypes.c_int64 * n)(*[_rows(w, w.shape[1])[2] for w in ws]))
+        size = lib.cafe_mlp_backward_work(*call, t)
         with _on(g.device):
             _lib.check(lib.cafe_mlp_backward(
-                n, cw, m, g.data_ptr(), ldg, x.data_ptr(), _rows(x, widths[0])[2], _pointers(ws),
-                (ctypes.c_int64 * n)(*[_rows(w, w.shape[1])[2] for w in ws]), (ctypes.c_int32 * n)(*acts), DTYPES[g.dtype], _pointers(ys),
-                (ctypes.c_int64 * n)(*ctx.pitch), _pointers(slopes), _ptr(gx), widths[0], _pointers(gws), _pointers(gbs),
-                work.data_ptr(), size, _stream()), "cafe_mlp_backward")
+                *call, (ctypes.c_int32 * n)(*acts), t, _pointers(ys), (ctypes.c_int64 * n)(*ctx.pitch), _pointers(slopes), _ptr(gx), widths[0],
+                _pointers(gws), _pointers(gbs), _ptr(_work(size, g)), size, _stream()), "cafe_mlp_backward")
         return (gx, None, *gws, *gbs)
 
 

@@ -330,7 +330,10 @@ int cafe_dot_interaction_backward(const float* x_dev, const float* emb_dev, int6
  * z = x W^T + b, y = act(z) + res for x [M, K], W [N, K], rows `ld` elements apart (ld >= the row's length; elements of a
  * row are contiguous).  All tensors of a call have one type; sums are fp32.  bias, res and slope may be null; ldr = 0: one
  * row of res for all.  slope_dev receives act'(z) for the backward: fp16 beside bf16, else fp32.
- * M, N, K <= CAFE_LINEAR_MAX.  No host synchronisation, no device memory of its own. */
+ * M, N, K <= CAFE_LINEAR_MAX.  No host synchronisation, no device memory of its own: work_dev (16-byte aligned, free again once
+ * the call's work on `stream` is done; two calls that may run at once need one each) lets large layers lay their operands out
+ * first; the *_work functions give its bytes for a call's arguments (0: none needed).  With less, or null, the call computes the
+ * same without. */
 enum { CAFE_F32 = 0, CAFE_BF16 = 1, CAFE_F16 = 2 };
 enum { CAFE_ACT_NONE = 0, CAFE_ACT_RELU = 1, CAFE_ACT_SIGMOID = 2, CAFE_ACT_GELU = 3, CAFE_ACT_SILU = 4 };
 /* what slope_dev of a backward holds: nothing (no activation), act'(z), or y of a ReLU without residual (y > 0) */
@@ -338,21 +341,27 @@ enum { CAFE_SLOPE_NONE = 0, CAFE_SLOPE_VALUES = 1, CAFE_SLOPE_OUTPUT = 2 };
 #define CAFE_LINEAR_MAX 8388608
 #define CAFE_MLP_MAX_LAYERS 32
 int cafe_linear_forward(const void* x_dev, int64_t ldx, const void* w_dev, int64_t ldw, const void* bias_dev, const void* res_dev, int64_t ldr,
-                        int M, int N, int K, int dtype, int act, void* y_dev, int64_t ldy, void* slope_dev, int64_t lds, void* stream);
+                        int M, int N, int K, int dtype, int act, void* y_dev, int64_t ldy, void* slope_dev, int64_t lds, void* work_dev,
+                        int64_t work_bytes, void* stream);
+int64_t cafe_linear_forward_work(const void* x_dev, int64_t ldx, const void* w_dev, int64_t ldw, int M, int N, int K, int dtype);
 /* gz = gy * act'(z); gx = gz W, gW = gz^T x, gb = column sums of gz; each of the three may be null (not wanted).  ldg = 0: one
  * row of gy for all. */
 int cafe_linear_backward(const void* gy_dev, int64_t ldg, const void* slope_dev, int64_t lds, int slope_kind, const void* x_dev, int64_t ldx,
                          const void* w_dev, int64_t ldw, int M, int N, int K, int dtype, void* gx_dev, int64_t ldgx, void* gw_dev, int64_t ldgw,
-                         void* gb_dev, void* stream);
+                         void* gb_dev, void* work_dev, int64_t work_bytes, void* stream);
+int64_t cafe_linear_backward_work(const void* gy_dev, int64_t ldg, int slope_kind, const void* x_dev, int64_t ldx, const void* w_dev, int64_t ldw,
+                                  int M, int N, int K, int dtype, int want_gx, int want_gw, int want_gb);
 /* `layers` layers one behind the other: layer l maps widths[l] to widths[l + 1] with acts[l]; its output goes to y_dev[l]
  * (pitch ldy[l]) and, where slope_dev[l] is not null, act'(z) to slope_dev[l] (same pitch). */
 int cafe_mlp_forward(int layers, const int* widths, int M, const void* x_dev, int64_t ldx, const void* const* w_dev, const int64_t* ldw,
                      const void* const* bias_dev, const int* acts, int dtype, void* const* y_dev, const int64_t* ldy, void* const* slope_dev,
-                     void* stream);
+                     void* work_dev, int64_t work_bytes, void* stream);
+int64_t cafe_mlp_forward_work(int layers, const int* widths, int M, const void* x_dev, int64_t ldx, const void* const* w_dev, const int64_t* ldw, int dtype);
 /* Its backward: a layer without slope_dev[l] has no activation or a ReLU (taken from y_dev[l]).  gw_dev[l] is [widths[l + 1],
- * widths[l]] contiguous; gx_dev, gw_dev[l] and gb_dev[l] may be null.  work_dev: cafe_mlp_backward_work bytes, 16-byte aligned,
- * free again once the call's work on `stream` is done. */
-int64_t cafe_mlp_backward_work(int layers, const int* widths, int M, int dtype);
+ * widths[l]] contiguous; gx_dev, gw_dev[l] and gb_dev[l] may be null.  work_dev also holds the gradients between the layers
+ * (two of M x the widest of them): less than that is refused. */
+int64_t cafe_mlp_backward_work(int layers, const int* widths, int M, const void* gy_dev, int64_t ldg, const void* x_dev, int64_t ldx,
+                               const void* const* w_dev, const int64_t* ldw, int dtype);
 int cafe_mlp_backward(int layers, const int* widths, int M, const void* gy_dev, int64_t ldg, const void* x_dev, int64_t ldx,
                       const void* const* w_dev, const int64_t* ldw, const int* acts, int dtype, const void* const* y_dev, const int64_t* ldy,
                       const void* const* slope_dev, void* gx_dev, int64_t ldgx, void* const* gw_dev, void* const* gb_dev, void* work_dev,

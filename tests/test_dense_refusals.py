@@ -7,19 +7,19 @@ ERR_ARG = 1
 P = 4096   # (a pointer that is never followed: every call below is refused, or has nothing to do)
 
 
-def _forward(lib, x=P, ldx=8, w=P, ldw=8, M=4, N=6, K=8, dtype=0, act=0, y=P, ldy=6, res=None, ldr=0, slope=None, lds=0):
-    return lib.cafe_linear_forward(x, ldx, w, ldw, None, res, ldr, M, N, K, dtype, act, y, ldy, slope, lds, None)
+def _forward(lib, x=P, ldx=8, w=P, ldw=8, M=4, N=6, K=8, dtype=0, act=0, y=P, ldy=6, res=None, ldr=0, slope=None, lds=0, work=None):
+    return lib.cafe_linear_forward(x, ldx, w, ldw, None, res, ldr, M, N, K, dtype, act, y, ldy, slope, lds, work, 0, None)
 
 
 def test_linear_arguments():
     from cafe_b200 import _lib
     lib = _lib.load()
     for bad in [dict(M=-1), dict(N=-1), dict(K=-1), dict(dtype=3), dict(dtype=-1), dict(act=5), dict(act=-1), dict(x=None), dict(w=None),
-                dict(y=None), dict(ldx=7), dict(ldw=7), dict(ldy=5), dict(res=P, ldr=5), dict(slope=P, lds=5), dict(M=8388609)]:
+                dict(y=None), dict(ldx=7), dict(ldw=7), dict(ldy=5), dict(res=P, ldr=5), dict(slope=P, lds=5), dict(M=8388609), dict(work=P + 8)]:
         assert _forward(lib, **bad) == ERR_ARG, bad
 
     def backward(gy=P, ldg=6, slope=P, lds=6, kind=1, x=P, ldx=8, w=P, ldw=8, M=4, N=6, K=8, dtype=0, gx=P, ldgx=8, gw=P, ldgw=8):
-        return lib.cafe_linear_backward(gy, ldg, slope, lds, kind, x, ldx, w, ldw, M, N, K, dtype, gx, ldgx, gw, ldgw, P, None)
+        return lib.cafe_linear_backward(gy, ldg, slope, lds, kind, x, ldx, w, ldw, M, N, K, dtype, gx, ldgx, gw, ldgw, P, None, 0, None)
     for bad in [dict(gy=None), dict(ldg=5), dict(slope=None), dict(lds=5), dict(kind=3), dict(kind=-1), dict(x=None), dict(ldx=7), dict(w=None),
                 dict(ldw=7), dict(ldgx=7), dict(ldgw=7), dict(dtype=7), dict(M=-2)]:
         assert backward(**bad) == ERR_ARG, bad
@@ -31,11 +31,11 @@ def test_mlp_arguments():
     i32, i64, vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p
     widths, acts = (i32 * 3)(4, 5, 6), (i32 * 2)(1, 2)
     ptrs, lds, pitch = (vp * 2)(P, P), (i64 * 2)(4, 5), (i64 * 2)(8, 6)
-    assert lib.cafe_mlp_forward(0, widths, 3, P, 4, ptrs, lds, ptrs, acts, 0, ptrs, pitch, None, None) == ERR_ARG
-    assert lib.cafe_mlp_forward(33, widths, 3, P, 4, ptrs, lds, ptrs, acts, 0, ptrs, pitch, None, None) == ERR_ARG
-    assert lib.cafe_mlp_forward(2, widths, 3, P, 3, ptrs, lds, ptrs, acts, 0, ptrs, pitch, None, None) == ERR_ARG
-    assert lib.cafe_mlp_forward(2, widths, 3, P, 4, ptrs, lds, ptrs, acts, 0, ptrs, (i64 * 2)(4, 6), None, None) == ERR_ARG
-    need = lib.cafe_mlp_backward_work(2, widths, 3, 0)
+    assert lib.cafe_mlp_forward(0, widths, 3, P, 4, ptrs, lds, ptrs, acts, 0, ptrs, pitch, None, None, 0, None) == ERR_ARG
+    assert lib.cafe_mlp_forward(33, widths, 3, P, 4, ptrs, lds, ptrs, acts, 0, ptrs, pitch, None, None, 0, None) == ERR_ARG
+    assert lib.cafe_mlp_forward(2, widths, 3, P, 3, ptrs, lds, ptrs, acts, 0, ptrs, pitch, None, None, 0, None) == ERR_ARG
+    assert lib.cafe_mlp_forward(2, widths, 3, P, 4, ptrs, lds, ptrs, acts, 0, ptrs, (i64 * 2)(4, 6), None, None, 0, None) == ERR_ARG
+    need = lib.cafe_mlp_backward_work(2, widths, 3, P, 6, P, 4, ptrs, lds, 0)
     assert need >= 2 * 3 * 5 * 4
     slopes = (vp * 2)(None, P)
 

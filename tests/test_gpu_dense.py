@@ -70,6 +70,38 @@ def test_sizes(M, N, K, dtype):
     _check(M, N, K, getattr(torch, dtype), ACTS[i % 5], seed=i)
 
 
+# rows, out, in, pitch, activation, residual: layers large enough for operands that are laid out first; ragged on every side, long
+# in each axis, one tile wide, rows on and off 16 bytes
+LARGE = [(2048, 512, 512, 0, "none", None), (2100, 700, 479, 0, "relu", None), (1030, 1100, 520, 8, "gelu", "full"), (300, 2000, 1000, 3, "silu", "row"),
+         (70000, 130, 70, 0, "sigmoid", None), (130, 64, 70000, 2, "silu", None), (128, 70001, 64, 0, "gelu", None), (4100, 129, 1025, 0, "none", "full"),
+         (1500, 640, 640, 8, "relu", "full")]
+
+
+@pytest.mark.parametrize("M,N,K,pitch,act,residual", LARGE)
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+def test_large_layers(M, N, K, pitch, act, residual, dtype):
+    import torch
+    _check(M, N, K, getattr(torch, dtype), act, seed=M, pitch=pitch, residual=residual)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_large_layers_one_gradient_alone(dtype):
+    import torch
+    from cafe_b200 import fused_linear
+    x, w, b, _, gy = _make(1100, 700, 800, getattr(torch, dtype), 12)
+    lx, lw, lb = (t.detach().requires_grad_(True) for t in (x, w, b))
+    full = torch.autograd.grad(fused_linear(lx, lw, lb, "silu"), [lx, lw, lb], gy)
+    for keep in range(1, 8):
+        leaves = [t.detach().requires_grad_(bool(keep >> i & 1)) for i, t in enumerate((x, w, b))]
+        got = torch.autograd.grad(fused_linear(*leaves, "silu"), [t for t in leaves if t.requires_grad], gy)
+        for a, c in zip(got, [f for i, f in enumerate(full) if keep >> i & 1]):
+            if keep == 4:    # (the bias gradient alone is summed by another kernel: (1100 + 8) 2^-23 of the magnitudes, or half a step)
+                assert float((a.double() - c.double()).abs().max()) <= 1108 * 2.0 ** -23 * float(gy.double().abs().sum(0).max()) * 1.1 + \
+                    float(c.double().abs().max()) * torch.finfo(c.dtype).eps
+            else:
+                assert torch.equal(a, c)
+
+
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("residual", [None, "full", "row"])
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
@@ -153,12 +185,13 @@ def test_gradient_against_differences():
 
 
 @pytest.mark.parametrize("act", ["none", "relu", "gelu"])
-def test_infinities_and_nans(act):
+@pytest.mark.parametrize("M", [140, 40000])     # (both kernels)
+def test_infinities_and_nans(act, M):
     """An element that is not finite reaches the outputs that a sum over it gives it, and no others."""
     import torch
     from cafe_b200 import fused_linear
     inf = float("inf")
-    x, w, b, _, _ = _make(140, 150, 96, torch.float32, 17)
+    x, w, b, _, _ = _make(M, 150, 96, torch.float32, 17)
     w = w.to(torch.bfloat16).float()       # (values with few bits: their lower parts are zero)
     x[3, 5], x[50, 0], x[139, 95], x[20, 7], x[20, 8] = inf, -inf, float("nan"), inf, -inf
     w[10, 5] = 0
