@@ -4,6 +4,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/cafe_b200.h"
 #include "cafe_internal.h"
 #include "cafe_float.cuh"
@@ -103,23 +105,25 @@ __device__ __forceinline__ void cafe_sums_put(const CafeJob& J, const float* acc
 }
 // This block's share of the tile's rows (of a cluster of `splits` blocks, by rank): the blocks' sums in the order of ranks, then
 // bias, activation, residual and the stores.  COLS columns at a pitch of COLS + 4 floats from `base` of every block.
-template <typename T, int COLS>
-__device__ __forceinline__ void cafe_finish(const CafeJob& J, uint32_t base, int row0, int col0, int rank, int splits, int threads) {
+template <typename T, int COLS, int SPLITS>
+__device__ __forceinline__ void cafe_finish_of(const CafeJob& J, uint32_t base, int row0, int col0, int rank, int threads) {
     typedef typename CafeSlopeOf<T>::type ST;
     constexpr int pitch = COLS + 4, quads = COLS / 4;
-    const int per = CAFE_LIN_BM / splits;
+    const int per = CAFE_LIN_BM / SPLITS;
     for (int e = threadIdx.x; e < per * quads; e += threads) {
         const int r = rank * per + e / quads, c = (e % quads) * 4;
         const int64_t i = row0 + r, j = col0 + c;
         if (i >= J.rows || j >= J.cols) continue;
         const uint32_t at = base + (uint32_t)(r * pitch + c) * 4u;
         float v[4] = {0.f, 0.f, 0.f, 0.f};
-        if (splits == 1) asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(at) : "memory");
-        else
-            for (int q = 0; q < splits; ++q) {
-                const float4 x = cafe_cluster_load4(cafe_cluster_map(at, q));
-                v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
-            }
+        if (SPLITS == 1) asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(at) : "memory");
+        else {
+            float4 x[SPLITS];
+#pragma unroll
+            for (int q = 0; q < SPLITS; ++q) x[q] = cafe_cluster_load4(cafe_cluster_map(at, q));
+#pragma unroll
+            for (int q = 0; q < SPLITS; ++q) { v[0] += x[q].x; v[1] += x[q].y; v[2] += x[q].z; v[3] += x[q].w; }
+        }
         const int n = (int)min((int64_t)4, J.cols - j);
         const bool vec = J.out_vec && n == 4;
         float bias[4] = {0.f, 0.f, 0.f, 0.f}, res[4] = {0.f, 0.f, 0.f, 0.f};
@@ -168,6 +172,23 @@ __device__ __forceinline__ void cafe_finish(const CafeJob& J, uint32_t base, int
             }
         }
     }
+}
+template <typename T, int COLS>
+__device__ __forceinline__ void cafe_finish(const CafeJob& J, uint32_t base, int row0, int col0, int rank, int splits, int threads) {
+    if (splits == 1) cafe_finish_of<T, COLS, 1>(J, base, row0, col0, rank, threads);
+    else if (splits == 2) cafe_finish_of<T, COLS, 2>(J, base, row0, col0, rank, threads);
+    else if (splits == 4) cafe_finish_of<T, COLS, 4>(J, base, row0, col0, rank, threads);
+    else cafe_finish_of<T, COLS, 8>(J, base, row0, col0, rank, threads);
+}
+
+// a kernel's limit of shared memory, once per device (always the same value: threads that do it at the same time do no harm)
+static inline cudaError_t dense_allow_shared(const void* kernel, int bytes, std::atomic<uint64_t>* devices) {
+    int d = 0;
+    cudaError_t e = cudaGetDevice(&d);
+    if (e != cudaSuccess || (d < 64 && (devices->load(std::memory_order_relaxed) >> d & 1))) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && d < 64) devices->fetch_or((uint64_t)1 << d, std::memory_order_relaxed);
+    return e;
 }
 
 // ---- the calls -------------------------------------------------------------------------------------------------------

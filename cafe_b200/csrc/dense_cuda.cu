@@ -56,27 +56,20 @@ template <typename T> __device__ __forceinline__ T cafe_piece_get(const CafePiec
         return reinterpret_cast<const T&>(b);
     }
 }
-// elements (row, k .. k + 8) of an operand; nothing outside [0, rows) x [., kend) is read
-template <typename T>
-__device__ __forceinline__ void cafe_piece_load(CafePiece<T>& p, const void* base, int64_t ld, int kc, int vec, int row, int rows, int k, int kend) {
-    const T* b = static_cast<const T*>(base);
-    if (kc) {
-        const T* src = b + (int64_t)row * ld + k;
-        if (row < rows && vec && k + 8 <= kend) {
-            const uint4 x = __ldg(reinterpret_cast<const uint4*>(src));
-            if constexpr (sizeof(T) == 4) {
-                const uint4 y = __ldg(reinterpret_cast<const uint4*>(src) + 1);
-                p.v[0] = __uint_as_float(x.x); p.v[1] = __uint_as_float(x.y); p.v[2] = __uint_as_float(x.z); p.v[3] = __uint_as_float(x.w);
-                p.v[4] = __uint_as_float(y.x); p.v[5] = __uint_as_float(y.y); p.v[6] = __uint_as_float(y.z); p.v[7] = __uint_as_float(y.w);
-            } else { p.v[0] = x.x; p.v[1] = x.y; p.v[2] = x.z; p.v[3] = x.w; }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) cafe_piece_set<T>(p, j, row < rows && k + j < kend ? __ldg(src + j) : cafe_from_float<T>(0.f));
-        }
+// Eight elements along k from `src`, the first of them, KC: contiguous, else `ld` apart.  FULL: all eight are inside; otherwise
+// `left` of them, and nothing else is read.
+template <typename T, bool KC, bool FULL>
+__device__ __forceinline__ void cafe_piece_load(CafePiece<T>& p, const T* src, int64_t ld, bool vec, int left) {
+    if (KC && FULL && vec) {
+        const uint4 x = __ldg(reinterpret_cast<const uint4*>(src));
+        if constexpr (sizeof(T) == 4) {
+            const uint4 y = __ldg(reinterpret_cast<const uint4*>(src) + 1);
+            p.v[0] = __uint_as_float(x.x); p.v[1] = __uint_as_float(x.y); p.v[2] = __uint_as_float(x.z); p.v[3] = __uint_as_float(x.w);
+            p.v[4] = __uint_as_float(y.x); p.v[5] = __uint_as_float(y.y); p.v[6] = __uint_as_float(y.z); p.v[7] = __uint_as_float(y.w);
+        } else { p.v[0] = x.x; p.v[1] = x.y; p.v[2] = x.z; p.v[3] = x.w; }
     } else {
-        const T* src = b + (int64_t)k * ld + row;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) cafe_piece_set<T>(p, j, row < rows && k + j < kend ? __ldg(src + (int64_t)j * ld) : cafe_from_float<T>(0.f));
+        for (int j = 0; j < 8; ++j) cafe_piece_set<T>(p, j, FULL || j < left ? __ldg(src + (KC ? (int64_t)j : j * ld)) : cafe_from_float<T>(0.f));
     }
 }
 template <typename T, typename S>
@@ -116,29 +109,114 @@ __device__ __forceinline__ void cafe_piece_store(const CafePiece<float>& p, uint
 }
 template <typename T> __device__ __forceinline__ void cafe_piece_store(const CafePiece<T>& p, uint32_t at, int) { cafe_put16(at, p.v[0], p.v[1], p.v[2], p.v[3]); }
 
-// One turn's pieces of this thread: `R` rows of an operand, BK deep, over 256 threads.  Piece number u: with k contiguous the
-// pieces of a row follow one another (neighbouring lanes read on in the row), else the rows do.
-template <typename T, int R, int BK = CafeLin<T>::BK> struct CafeTurn {
+// One turn's pieces of this thread: `R` rows of an operand, BK deep, over 256 threads.  With k contiguous the pieces of a row
+// follow one another (neighbouring lanes read on in the row), else the rows do.  Rows past the last one read the last one again:
+// what comes of them is not stored.
+template <typename T, int R, int BK, bool KC> struct CafeTurn {
     static constexpr int per_row = BK / 8, total = R * per_row, each = (total + 255) / 256;
     CafePiece<T> p[each];
-    __device__ __forceinline__ static int row_of(int u, int kc) { return kc ? u / per_row : u % R; }
-    __device__ __forceinline__ static int piece_of(int u, int kc) { return kc ? u % per_row : u / R; }
-    __device__ __forceinline__ void load(const void* base, int64_t ld, int kc, int vec, int row0, int rows, int k0, int kend, int tid) {
+    __device__ __forceinline__ static int row_of(int u) { return KC ? u / per_row : u % R; }
+    __device__ __forceinline__ static int piece_of(int u) { return KC ? u % per_row : u / R; }
+    __device__ __forceinline__ static bool has(int u) { return total % 256 == 0 || u < total; }
+    // base: element (row0, 0); last: rows there are from row0, less one
+    template <bool FULL> __device__ __forceinline__ void load(const T* base, int64_t ld, bool vec, int last, int k0, int kend, int tid) {
 #pragma unroll
         for (int i = 0; i < each; ++i) {
-            const int u = tid + i * 256;
-            if (total % 256 == 0 || u < total) cafe_piece_load<T>(p[i], base, ld, kc, vec, row0 + row_of(u, kc), rows, k0 + 8 * piece_of(u, kc), kend);
+            const int u = tid + i * 256, k = k0 + 8 * piece_of(u), r = min(row_of(u), last);
+            if (has(u)) cafe_piece_load<T, KC, FULL>(p[i], base + (KC ? r * ld + k : k * ld + r), ld, vec, kend - k);
         }
     }
-    __device__ __forceinline__ void store(uint32_t at, int part, int kc, int tid) const {
+    __device__ __forceinline__ void store(uint32_t at, int part, int tid) const {
 #pragma unroll
         for (int i = 0; i < each; ++i) {
             const int u = tid + i * 256;
-            if (total % 256 == 0 || u < total)
-                cafe_piece_store(p[i], at + cafe_swizzle<BK * 2>(row_of(u, kc), piece_of(u, kc)), part);
+            if (has(u)) cafe_piece_store(p[i], at + cafe_swizzle<BK * 2>(row_of(u), piece_of(u)), part);
         }
+    }
+    __device__ __forceinline__ float sum() const {
+        float x = 0.f;
+#pragma unroll
+        for (int i = 0; i < each; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x += cafe_to_float(cafe_piece_get<T>(p[i], j));
+        return x;
     }
 };
+
+// The loading warps' part of a block: AK and BK_: k contiguous in A and B; KIND: what A is multiplied by.
+template <typename T, int BN, bool AK, bool BK_, int KIND>
+__device__ __forceinline__ void cafe_produce(const CafeJob& J, uint32_t base, uint32_t full0, uint32_t empty0, volatile int* bail, int row0, int col0, int t0, int turns,
+                                             float* bias_sum) {
+    typedef CafeLin<T> L;
+    typedef CafeLinShape<T, BN> Sh;
+    typedef typename CafeSlopeOf<T>::type ST;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const T* A = static_cast<const T*>(J.a) + (AK ? row0 * J.lda : (int64_t)row0);
+    const T* B = static_cast<const T*>(J.b) + (BK_ ? col0 * J.ldb : (int64_t)col0);
+    const int64_t s0 = AK ? row0 * J.ldas : (int64_t)row0;
+    const int a_last = J.rows - 1 - row0, b_last = max(0, J.cols - 1 - col0);
+    CafeTurn<T, CAFE_LIN_BM, L::BK, AK> a[2];
+    CafeTurn<T, BN, L::BK, BK_> b[2];
+    CafeTurn<ST, CAFE_LIN_BM, L::BK, AK> sl;
+    CafeTurn<T, CAFE_LIN_BM, L::BK, AK> ym;
+    float bsum = 0.f, bchunk = 0.f;
+    const bool columns = J.cols > 0;
+    auto load = [&](int t, int h) {
+        const int k0 = (t0 + t) * L::BK;
+        if (k0 + L::BK <= J.depth) {
+            a[h].template load<true>(A, J.lda, J.a_vec, a_last, k0, J.depth, tid);
+            if (columns) b[h].template load<true>(B, J.ldb, J.b_vec, b_last, k0, J.depth, tid);
+        } else {
+            a[h].template load<false>(A, J.lda, false, a_last, k0, J.depth, tid);
+            if (columns) b[h].template load<false>(B, J.ldb, false, b_last, k0, J.depth, tid);
+        }
+    };
+    auto load_slope = [&](int t) {
+        const int k0 = (t0 + t) * L::BK;
+        if constexpr (KIND == CAFE_SLOPE_VALUES) {
+            if (k0 + L::BK <= J.depth) sl.template load<true>(static_cast<const ST*>(J.as) + s0, J.ldas, J.as_vec, a_last, k0, J.depth, tid);
+            else sl.template load<false>(static_cast<const ST*>(J.as) + s0, J.ldas, false, a_last, k0, J.depth, tid);
+        } else if constexpr (KIND == CAFE_SLOPE_OUTPUT) {
+            if (k0 + L::BK <= J.depth) ym.template load<true>(static_cast<const T*>(J.as) + s0, J.ldas, J.as_vec, a_last, k0, J.depth, tid);
+            else ym.template load<false>(static_cast<const T*>(J.as) + s0, J.ldas, false, a_last, k0, J.depth, tid);
+        }
+    };
+    load(0, 0);
+    load_slope(0);
+#pragma unroll 2
+    for (int t = 0; t < turns; ++t) {
+        const int h = t & 1, s = t % Sh::stages;
+        if (t + 1 < turns) load(t + 1, h ^ 1);
+        if constexpr (KIND == CAFE_SLOPE_VALUES) {
+            if (bias_sum) {   // (the sum takes gz before its rounding)
+                float x = 0.f;
+#pragma unroll
+                for (int i = 0; i < a[h].each; ++i)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x += cafe_to_float(cafe_piece_get<T>(a[h].p[i], j)) * cafe_to_float(cafe_piece_get<ST>(sl.p[i], j));
+                bchunk += x;
+            }
+#pragma unroll
+            for (int i = 0; i < a[h].each; ++i) cafe_piece_slope<T, ST>(a[h].p[i], sl.p[i]);
+        } else {
+            if constexpr (KIND == CAFE_SLOPE_OUTPUT) {
+#pragma unroll
+                for (int i = 0; i < a[h].each; ++i) cafe_piece_mask<T>(a[h].p[i], ym.p[i]);
+            }
+            if (bias_sum) bchunk += a[h].sum();
+        }
+        if (t + 1 < turns) load_slope(t + 1);
+        if ((t & 31) == 31) { bsum += bchunk; bchunk = 0.f; }
+        if (t >= Sh::stages && !cafe_bar_wait(empty0 + 8u * s, (uint32_t)(t / Sh::stages - 1) & 1u, bail)) break;
+        const uint32_t at = base + s * Sh::stage;
+        a[h].store(at, Sh::a_part, tid);
+        if (columns) b[h].store(at + L::parts * Sh::a_part, Sh::b_part, tid);
+        cafe_fence_async();
+        __syncwarp();
+        if (lane == 0) cafe_bar_arrive(full0 + 8u * s);
+    }
+    if (bias_sum) bias_sum[tid] = bsum + bchunk;   // (rows contiguous: a thread's pieces are all of row tid & 127)
+}
 
 template <typename T, int BN>
 __global__ void __launch_bounds__(CAFE_LIN_THREADS, 1) k_linear(const __grid_constant__ CafeJobs P, int splits) {
@@ -184,61 +262,20 @@ __global__ void __launch_bounds__(CAFE_LIN_THREADS, 1) k_linear(const __grid_con
     float acc[half_cols];
     if (warp < 8) {
         // ---- operands into shared memory
-        const int tid = threadIdx.x;
-        const bool sums = J.gb && tn == 0;
-        CafeTurn<T, CAFE_LIN_BM> a[2];
-        CafeTurn<ST, CAFE_LIN_BM, L::BK> sl;
-        CafeTurn<T, CAFE_LIN_BM> ym;
-        CafeTurn<T, BN> b[2];
-        float bsum = 0.f, bchunk = 0.f;
-        auto load = [&](int t, int h) {
-            const int k0 = (t0 + t) * L::BK;
-            a[h].load(J.a, J.lda, J.a_kc, J.a_vec, row0, J.rows, k0, J.depth, tid);
-            b[h].load(J.b, J.ldb, J.b_kc, J.b_vec, col0, J.cols, k0, J.depth, tid);
-        };
-        if (turns > 0) load(0, 0);
-#pragma unroll 2
-        for (int t = 0; t < turns; ++t) {
-            const int h = t & 1, s = t % Sh::stages;
-            const int k0 = (t0 + t) * L::BK;
-            if (J.slope_kind == CAFE_SLOPE_VALUES) sl.load(J.as, J.ldas, J.a_kc, J.as_vec, row0, J.rows, k0, J.depth, tid);
-            else if (J.slope_kind == CAFE_SLOPE_OUTPUT) ym.load(J.as, J.ldas, J.a_kc, J.as_vec, row0, J.rows, k0, J.depth, tid);
-            if (t + 1 < turns) load(t + 1, h ^ 1);
-            if (J.slope_kind == CAFE_SLOPE_VALUES) {
-                if (sums) {   // (the sum takes gz before its rounding)
-                    float x = 0.f;
-#pragma unroll
-                    for (int i = 0; i < CafeTurn<T, CAFE_LIN_BM>::each; ++i)
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) x += cafe_to_float(cafe_piece_get<T>(a[h].p[i], j)) * cafe_to_float(cafe_piece_get<ST>(sl.p[i], j));
-                    bchunk += x;
-                }
-#pragma unroll
-                for (int i = 0; i < CafeTurn<T, CAFE_LIN_BM>::each; ++i) cafe_piece_slope<T, ST>(a[h].p[i], sl.p[i]);
-            } else {
-                if (J.slope_kind == CAFE_SLOPE_OUTPUT) {
-#pragma unroll
-                    for (int i = 0; i < CafeTurn<T, CAFE_LIN_BM>::each; ++i) cafe_piece_mask<T>(a[h].p[i], ym.p[i]);
-                }
-                if (sums) {
-                    float x = 0.f;
-#pragma unroll
-                    for (int i = 0; i < CafeTurn<T, CAFE_LIN_BM>::each; ++i)
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) x += cafe_to_float(cafe_piece_get<T>(a[h].p[i], j));
-                    bchunk += x;
-                }
-            }
-            if ((t & 31) == 31) { bsum += bchunk; bchunk = 0.f; }
-            if (t >= Sh::stages && !cafe_bar_wait(empty(s), (uint32_t)(t / Sh::stages - 1) & 1u, &bail)) break;
-            const uint32_t at = base + s * Sh::stage;
-            a[h].store(at, Sh::a_part, J.a_kc, tid);
-            b[h].store(at + L::parts * Sh::a_part, Sh::b_part, J.b_kc, tid);
-            cafe_fence_async();
-            __syncwarp();
-            if (lane == 0) cafe_bar_arrive(full(s));
+        float* const sums = J.gb && tn == 0 ? &bias_sum[0][0] : nullptr;
+#define PRODUCE(AK, BK_, KIND) cafe_produce<T, BN, AK, BK_, KIND>(J, base, full(0), empty(0), &bail, row0, col0, t0, turns, sums)
+        if (turns == 0) { if (sums) sums[threadIdx.x] = 0.f; }
+        else if (J.b_kc) PRODUCE(true, true, CAFE_SLOPE_NONE);
+        else if (J.a_kc) {
+            if (J.slope_kind == CAFE_SLOPE_VALUES) PRODUCE(true, false, CAFE_SLOPE_VALUES);
+            else if (J.slope_kind == CAFE_SLOPE_OUTPUT) PRODUCE(true, false, CAFE_SLOPE_OUTPUT);
+            else PRODUCE(true, false, CAFE_SLOPE_NONE);
+        } else {
+            if (J.slope_kind == CAFE_SLOPE_VALUES) PRODUCE(false, false, CAFE_SLOPE_VALUES);
+            else if (J.slope_kind == CAFE_SLOPE_OUTPUT) PRODUCE(false, false, CAFE_SLOPE_OUTPUT);
+            else PRODUCE(false, false, CAFE_SLOPE_NONE);
         }
-        if (sums) bias_sum[tid >> 7][tid & 127] = bsum + bchunk;   // (rows contiguous: a thread's pieces are all of row tid & 127)
+#undef PRODUCE
     } else {
         // ---- products, and sums out of tensor memory: warps 8 to 11 the left half of the columns, 12 to 15 the right, 32 rows each
         const uint32_t from = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)((warp - 8) / 4 * half_cols);
@@ -346,7 +383,8 @@ static cudaError_t dense_launch_bn(CafeJobs& P, int splits, cudaStream_t st) {
     }
     if (tiles == 0) return cudaSuccess;
     constexpr int bytes = CafeLinShape<T, BN>::bytes;
-    cudaError_t e = cudaFuncSetAttribute(k_linear<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    static std::atomic<uint64_t> allowed{0};
+    const cudaError_t e = dense_allow_shared((const void*)k_linear<T, BN>, bytes, &allowed);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tiles * splits));
@@ -362,34 +400,33 @@ static cudaError_t dense_launch_bn(CafeJobs& P, int splits, cudaStream_t st) {
     return cudaLaunchKernelEx(&cfg, k_linear<T, BN>, (const CafeJobs&)P, splits);
 }
 
-// Width of the tiles and blocks per tile: the pair whose estimate is least.  A turn (BK of depth) of a 128, 64 and 32 wide tile
-// takes about 1, 0.65 and 0.5 units, a block costs 6 units beside its turns and 1 more where sums are exchanged; blocks run
-// 148 at a time, so the whole takes the longest block or all blocks' sum / 148, whichever is more.
+// Width of the tiles and blocks per tile: the pair whose estimate is least.  A turn (BK of depth) of a 64 and a 32 wide tile takes
+// about 1 and 0.75 units, a block costs 9 units beside its turns and 1 to 2 more where sums are exchanged; 148, 148,
+// 132 and 120 blocks run at a time in clusters of 1, 2, 4 and 8 (what the device says), so the whole takes the longest block or,
+// with more blocks than that, all blocks' sum over them.
 template <typename T>
 static cudaError_t dense_launch(CafeJobs& P, cudaStream_t st) {
-    static const int widths[3] = {128, 64, 32};
-    static const double unit[3] = {1.0, 0.65, 0.5};
-    int best_n = 0, best_s = 1;
+    static const int widths[2] = {64, 32}, room[4] = {148, 148, 132, 120};
+    static const double unit[2] = {1.0, 0.75}, exchange[4] = {0, 1.5, 2, 3};
+    int best_n = 0, best_s = 0;
     double best = 1e300;
-    for (int n = 0; n < 3; ++n)
-        for (int s = 1; s <= 8; s *= 2) {
+    for (int n = 0; n < 2; ++n)
+        for (int s = 0; s < 4; ++s) {
             double longest = 0, sum = 0;
             int64_t blocks = 0;
             for (int q = 0; q < P.count; ++q) {
                 const CafeJob& J = P.job[q];
                 const int turns = (J.depth + CafeLin<T>::BK - 1) / CafeLin<T>::BK;
-                const double one = (double)((turns + s - 1) / s) * unit[n] + 6 + (s > 1 ? 1 : 0);
-                const double tiles = (double)((J.rows + CAFE_LIN_BM - 1) / CAFE_LIN_BM) * (J.cols > 0 ? (J.cols + widths[n] - 1) / widths[n] : 1);
+                const double one = (double)((turns + (1 << s) - 1) >> s) * unit[n] + 9 + exchange[s];
+                const int64_t tiles = (int64_t)((J.rows + CAFE_LIN_BM - 1) / CAFE_LIN_BM) * (J.cols > 0 ? (J.cols + widths[n] - 1) / widths[n] : 1);
                 longest = one > longest ? one : longest;
-                sum += one * tiles * s;
-                blocks += (int64_t)tiles * s;
+                sum += one * (double)(tiles << s);
+                blocks += tiles << s;
             }
-            const double est = sum / 148 > longest ? sum / 148 : longest;
+            const double all = sum / room[s], est = blocks > room[s] && all + 0.5 * longest > longest ? all + 0.5 * longest : longest;
             if (est < best * 0.999 && blocks < (1 << 30)) { best = est; best_n = n; best_s = s; }
         }
-    if (best_n == 0) return dense_launch_bn<T, 128>(P, best_s, st);
-    if (best_n == 1) return dense_launch_bn<T, 64>(P, best_s, st);
-    return dense_launch_bn<T, 32>(P, best_s, st);
+    return best_n == 0 ? dense_launch_bn<T, 64>(P, 1 << best_s, st) : dense_launch_bn<T, 32>(P, 1 << best_s, st);
 }
 
 static int dense_done(cudaError_t e) {
@@ -398,9 +435,135 @@ static int dense_done(cudaError_t e) {
     return CAFE_OK;
 }
 
+// ---- a few rows against many -------------------------------------------------------------------------------------------
+// y for at most 16 rows of x (one request to score), or of W (a last layer of one output): each of the many rows is read once,
+// in plain fp32 multiply-adds; tiles of 128 would mostly be padding.  A block takes eight of the many rows at a time for every warp
+// that has a share of k of its own: `kw` warps divide k among them, the others take further rows.  A lane has four k of eight
+// many and FEW few rows at a time, so 8 + FEW loads feed 32 FEW multiply-adds; sums of a warp's lanes are halved and exchanged
+// until each lane holds FEW / 4 of them (FEW >= 4), sums of the kw warps are added in their order through shared memory.
+struct CafeFew {
+    const void *few, *many, *bias, *res;
+    int64_t ldf, ldm, ldr, ldo, lds;
+    int nfew, nmany, depth, kw, vec, act, few_is_row;   // few_is_row: the few are rows of x, so the output is [few][many]
+    void *out, *slope_out;
+};
+#define CAFE_FEW_MANY 8      // of the many rows at a time
+#define CAFE_FEW_MOST 16
+template <typename T> __device__ __forceinline__ void cafe_few_load(const T* p, bool vec, int lane, int left, float* v) {
+    if (vec) {   // lane's four k: 4 lane + {0 .. 3}
+        if (4 * lane + 4 <= left) {
+            alignas(16) T x[4];
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(x) = __ldg(reinterpret_cast<const uint4*>(p + 4 * lane));
+            else *reinterpret_cast<uint2*>(x) = __ldg(reinterpret_cast<const uint2*>(p + 4 * lane));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = cafe_to_float(x[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = 4 * lane + j < left ? cafe_to_float(__ldg(p + 4 * lane + j)) : 0.f;
+        }
+    } else {     // lane + {0, 32, 64, 96}
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = lane + 32 * j < left ? cafe_to_float(__ldg(p + lane + 32 * j)) : 0.f;
+    }
+}
+template <typename T, int FEW>
+__global__ void __launch_bounds__(256) k_few(const CafeFew P) {
+    typedef typename CafeSlopeOf<T>::type ST;
+    constexpr int N = CAFE_FEW_MANY * FEW;
+    __shared__ float part[8][N];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int groups = 8 / P.kw, group = warp / P.kw, kpart = warp % P.kw;
+    const int64_t per_block = (int64_t)groups * CAFE_FEW_MANY, first = blockIdx.x * per_block + group * CAFE_FEW_MANY;
+    // k in steps of 128, shared out among kw warps
+    float acc[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = 0.f;
+    if (first < P.nmany) {
+        const T* few = static_cast<const T*>(P.few);
+        const T* many = static_cast<const T*>(P.many) + first * P.ldm;
+        const int last = (int)min((int64_t)CAFE_FEW_MANY, P.nmany - first) - 1;
+        for (int k = kpart * 128; k < P.depth; k += P.kw * 128) {
+            const int left = P.depth - k;
+            float w[CAFE_FEW_MANY][4];
+#pragma unroll
+            for (int c = 0; c < CAFE_FEW_MANY; ++c) cafe_few_load(many + min(c, last) * P.ldm + k, P.vec, lane, left, w[c]);
+#pragma unroll
+            for (int f = 0; f < FEW; ++f) {
+                float x[4];
+                cafe_few_load(few + min(f, P.nfew - 1) * P.ldf + k, P.vec, lane, left, x);
+#pragma unroll
+                for (int c = 0; c < CAFE_FEW_MANY; ++c)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[f * CAFE_FEW_MANY + c] += x[j] * w[c][j];
+            }
+        }
+    }
+    // halving exchange: after it lane l holds, at acc[i], the whole sum number (l >> SH) * (N >> LG) + i
+    constexpr int LG = N >= 32 ? 5 : N == 16 ? 4 : 3;   // halvings that leave something to halve
+#pragma unroll
+    for (int h = 0; h < LG; ++h) {
+        const int half = N >> (h + 1), m = 16 >> h;
+        const bool up = (lane & m) != 0;
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            if (i < half) {
+                const float send = up ? acc[i] : acc[i + half], keep = up ? acc[i + half] : acc[i];
+                acc[i] = keep + __shfl_xor_sync(0xffffffffu, send, m);
+            }
+        }
+    }
+#pragma unroll
+    for (int h = LG; h < 5; ++h) acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], 16 >> h);
+    if ((lane & ((32 >> LG) - 1)) == 0) {
+#pragma unroll
+        for (int i = 0; i < (N >> LG); ++i) part[warp][(lane >> (5 - LG)) * (N >> LG) + i] = acc[i];
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < groups * N; e += 256) {
+        const int g = e / N, q = e % N;
+        // neighbouring threads write neighbouring outputs
+        const int f = P.few_is_row ? q / CAFE_FEW_MANY : q % FEW, c = P.few_is_row ? q % CAFE_FEW_MANY : q / FEW;
+        const int64_t many = blockIdx.x * per_block + g * CAFE_FEW_MANY + c;
+        if (f >= P.nfew || many >= P.nmany) continue;
+        float z = 0.f;
+        for (int w = 0; w < P.kw; ++w) z += part[g * P.kw + w][f * CAFE_FEW_MANY + c];
+        const int64_t i = P.few_is_row ? f : many, j = P.few_is_row ? many : f;
+        float d = 1.f;
+        if (P.bias) z += cafe_to_float(__ldg(static_cast<const T*>(P.bias) + j));
+        if (P.act != CAFE_ACT_NONE) z = cafe_act<sizeof(T) == 2>(z, P.act, &d);
+        if (P.res) z += cafe_to_float(__ldg(static_cast<const T*>(P.res) + i * P.ldr + j));
+        static_cast<T*>(P.out)[i * P.ldo + j] = cafe_from_float<T>(z);
+        if (P.slope_out) static_cast<ST*>(P.slope_out)[i * P.lds + j] = cafe_from_float<ST>(d);
+    }
+}
+template <typename T>
+static cudaError_t dense_few(const CafeForward& f, cudaStream_t st) {
+    CafeFew P = {};
+    P.few_is_row = f.M <= f.N;
+    const bool r = P.few_is_row;
+    P.few = r ? f.x : f.w; P.ldf = r ? f.ldx : f.ldw; P.nfew = r ? f.M : f.N;
+    P.many = r ? f.w : f.x; P.ldm = r ? f.ldw : f.ldx; P.nmany = r ? f.N : f.M;
+    P.depth = f.K; P.act = f.act; P.bias = f.bias; P.res = f.res; P.ldr = f.ldr;
+    P.out = f.y; P.ldo = f.ldy; P.slope_out = f.slope; P.lds = f.lds;
+    const int size = sizeof(T);
+    P.vec = dense_on(f.x, f.ldx, size, 4 * size) && dense_on(f.w, f.ldw, size, 4 * size);
+    // as many warps along k as have 128 of it, fewer where there are many rows to share out anyway
+    P.kw = 1;
+    while (P.kw < 8 && P.kw * 128 < f.K && (int64_t)P.nmany * P.kw < 148 * 16 * 8 * 8) P.kw *= 2;
+    const int per_block = 8 / P.kw * CAFE_FEW_MANY;
+    const unsigned grid = (unsigned)((P.nmany + per_block - 1) / per_block);
+    CAFE_PROF(CAFE_P_LINEAR, st);
+    if (P.nfew <= 1) k_few<T, 1><<<grid, 256, 0, st>>>(P);
+    else if (P.nfew <= 4) k_few<T, 4><<<grid, 256, 0, st>>>(P);
+    else if (P.nfew <= 8) k_few<T, 8><<<grid, 256, 0, st>>>(P);
+    else k_few<T, 16><<<grid, 256, 0, st>>>(P);
+    return cudaGetLastError();
+}
+
 template <typename T>
 static cudaError_t dense_forward(const CafeForward& f, int dtype, void* work, int64_t work_bytes, cudaStream_t st) {
     if (f.M == 0 || f.N == 0) return cudaSuccess;
+    if (f.M <= CAFE_FEW_MOST || f.N <= CAFE_FEW_MOST) return dense_few<T>(f, st);
     CafeJobs P = {};
     CafeJob& J = P.job[0];
     P.count = 1;

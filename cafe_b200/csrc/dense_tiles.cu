@@ -15,7 +15,9 @@
 #include "dense.cuh"
 
 #define CAFE_TILES_THREADS 192
-#define CAFE_PARTS_ROWS 128    // rows of a block of k_parts: a row of partial column sums each
+// rows of a block of k_parts (a row of partial column sums each): short blocks while they are few, so that all are under way at
+// once (1 M elements: 32 rows 3 us, 128 rows 8)
+static __host__ __device__ constexpr int cafe_parts_rows(int rows) { return rows <= 16384 ? 32 : 128; }
 #define CAFE_PARTS_COLS 256
 
 __device__ int g_tiles_gave_up;   // a wait ran out (its outputs are not numbers)
@@ -64,9 +66,10 @@ __global__ void __launch_bounds__(256) k_parts(const __grid_constant__ CafeParts
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int col = bx * CAFE_PARTS_COLS + lane * 8, n = min(8, J.cols - col);
     float sum[8] = {};
-    const int64_t r0 = (int64_t)by * CAFE_PARTS_ROWS, r1 = min(r0 + CAFE_PARTS_ROWS, (int64_t)J.rows);
+    const int per = cafe_parts_rows(J.rows);
+    const int64_t r0 = (int64_t)by * per, r1 = min(r0 + per, (int64_t)J.rows);
     if (n > 0) {
-#pragma unroll 2
+#pragma unroll 4
         for (int64_t r = r0 + warp; r < r1; r += 8) {
             alignas(16) float v[8];
             cafe_read8(static_cast<const T*>(J.src) + r * J.ld + col, n, J.vec, v);
@@ -358,7 +361,8 @@ static cudaError_t tiles_launch_bn(CafeTilesArgs& P, const TilesOperand& a, cons
     P.job.tiles_n = P.job.cols > 0 ? (P.job.cols + BN - 1) / BN : 1;
     P.job.tiles = ((P.job.rows + CAFE_LIN_BM - 1) / CAFE_LIN_BM) * P.job.tiles_n;
     constexpr int bytes = CafeTilesShape<T, BN>::bytes;
-    cudaError_t e = cudaFuncSetAttribute(k_tiles<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    static std::atomic<uint64_t> allowed{0};
+    const cudaError_t e = dense_allow_shared((const void*)k_tiles<T, BN>, bytes, &allowed);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(P.job.tiles * P.splits));
@@ -373,7 +377,8 @@ static cudaError_t tiles_launch_bn(CafeTilesArgs& P, const TilesOperand& a, cons
     CAFE_PROF(CAFE_P_LINEAR, st);
     return cudaLaunchKernelEx(&cfg, k_tiles<T, BN>, (const CafeTilesArgs&)P);
 }
-// blocks per tile: the fewest rounds of 296 blocks for the depth that each has (a block costs 8 turns beside its own)
+// blocks per tile: the fewest rounds for the depth that each has (a block costs 8 turns beside its own; 296, 296, 284 and 264 run
+// at a time in clusters of 1, 2, 4 and 8: what the device says)
 template <typename T>
 static cudaError_t tiles_launch(CafeTilesArgs& P, const TilesOperand& a, const TilesOperand& b, cudaStream_t st) {
     typedef CafeTiles<T> L;
@@ -381,11 +386,12 @@ static cudaError_t tiles_launch(CafeTilesArgs& P, const TilesOperand& a, const T
     const int bn = wide ? 256 : 128;
     const int64_t tiles = (int64_t)((P.job.rows + CAFE_LIN_BM - 1) / CAFE_LIN_BM) * ((P.job.cols + bn - 1) / bn);
     const int turns = (P.job.depth + L::BK - 1) / L::BK;
+    static const int room[4] = {296, 296, 284, 264};
     double best = 1e300;
-    for (int s = 1; s <= 8; s *= 2) {
-        const int64_t rounds = (tiles * s + 295) / 296;
-        const double est = (double)rounds * ((turns + s - 1) / s + 8 + (s > 1 ? 2 : 0));
-        if (est < best * 0.999) { best = est; P.splits = s; }
+    for (int s = 0; s < 4; ++s) {
+        const int64_t rounds = ((tiles << s) + room[s] - 1) / room[s];
+        const double est = (double)rounds * (((turns + (1 << s) - 1) >> s) + 8 + s);
+        if (est < best * 0.999) { best = est; P.splits = 1 << s; }
     }
     if constexpr (L::parts == 1) {
         if (wide) return tiles_launch_bn<T, 256>(P, a, b, st);
@@ -413,7 +419,7 @@ static TilesOperand tiles_operand(CafeParts* P, char** work, int dtype, const vo
     J.slope_vec = ((uintptr_t)slope & 15) == 0 && lds * ss % 16 == 0;
     J.rows = rows; J.cols = cols; J.sums = sums;
     J.blocks_x = (cols + CAFE_PARTS_COLS - 1) / CAFE_PARTS_COLS;
-    J.blocks = J.blocks_x * ((rows + CAFE_PARTS_ROWS - 1) / CAFE_PARTS_ROWS);
+    J.blocks = J.blocks_x * ((rows + cafe_parts_rows(rows) - 1) / cafe_parts_rows(rows));
     J.dst = nullptr;
     if (!in_place) {
         J.dst = *work;
@@ -453,7 +459,7 @@ int64_t cafe_tiles_backward_work(const CafeBackward& f, int dtype) {
     if (f.slope_kind != CAFE_SLOPE_NONE || !tiles_in_place(dtype, f.gy, f.ldg)) need += tiles_bytes(parts, f.M, f.N);
     if (f.gx && !tiles_in_place(dtype, f.w, f.ldw)) need += tiles_bytes(parts, f.N, f.K);
     if (f.gw && !tiles_in_place(dtype, f.x, f.ldx)) need += tiles_bytes(parts, f.M, f.K);
-    if (f.gb) need += tiles_round((int64_t)((f.M + CAFE_PARTS_ROWS - 1) / CAFE_PARTS_ROWS) * f.N * 4);
+    if (f.gb) need += tiles_round((int64_t)((f.M + cafe_parts_rows(f.M) - 1) / cafe_parts_rows(f.M)) * f.N * 4);
     return need;
 }
 
@@ -472,7 +478,7 @@ template <typename T>
 static cudaError_t tiles_backward(const CafeBackward& f, int dtype, const CafeJob* gw, const CafeJob* gx, char* work, cudaStream_t st) {
     CafeParts parts = {};
     float* sums = nullptr;
-    const int sum_rows = (f.M + CAFE_PARTS_ROWS - 1) / CAFE_PARTS_ROWS;
+    const int sum_rows = (f.M + cafe_parts_rows(f.M) - 1) / cafe_parts_rows(f.M);
     if (f.gb) {
         sums = (float*)work;
         work += tiles_round((int64_t)sum_rows * f.N * 4);

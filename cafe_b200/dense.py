@@ -12,7 +12,6 @@ from outside the capture)."""
 from __future__ import annotations
 
 import ctypes
-from contextlib import nullcontext
 
 import torch
 import torch.nn as nn
@@ -26,11 +25,27 @@ _NONE, _RELU = 0, 1
 _SLOPE_NONE, _SLOPE_VALUES, _SLOPE_OUTPUT = 0, 1, 2
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_SIZE, MAX_LAYERS = 8388608, 32
+_LARGE = 1 << 28   # below so many multiply-adds no call takes workspace (cafe_linear_*_work then gives 0): not asked
 
 
-def _on(device: torch.device):
-    """The tensors' device as the current one."""
-    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+_get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)   # (without the checks of the public form)
+
+
+class _on:
+    """The tensors' device as the current one; `as` its current stream."""
+    __slots__ = ("other",)
+
+    def __init__(self, device):
+        self.other = None if device.index == _get_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.other is not None:
+            self.other.__enter__()
+        return _stream()
+
+    def __exit__(self, *args):
+        if self.other is not None:
+            self.other.__exit__(*args)
 
 
 def _rows(t: torch.Tensor, cols: int, repeated: bool = False):
@@ -39,7 +54,7 @@ def _rows(t: torch.Tensor, cols: int, repeated: bool = False):
     if t.dim() != 2:
         t = t.reshape(-1, cols) if cols else t.reshape(t.numel(), 0)
     m = t.shape[0]
-    if t.numel() == 0:
+    if t.is_contiguous() or t.numel() == 0:
         return t, m, cols
     if cols == 1 or t.stride(1) == 1:
         ld = t.stride(0)
@@ -99,45 +114,60 @@ def _linear(x, weight, bias, residual, act, keep):
     if keep and act != _NONE and not (act == _RELU and residual is None):
         slope = torch.empty(m, n, dtype=_slope_type(x.dtype), device=x.device)
     b = _contiguous(bias)
-    lib, t = _lib.load(), DTYPES[x.dtype]
-    size = lib.cafe_linear_forward_work(x2.data_ptr(), ldx, w2.data_ptr(), ldw, m, n, k, t)
-    with _on(x.device):
-        _lib.check(lib.cafe_linear_forward(x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(b), _ptr(r2), ldr, m, n, k, t, act, y.data_ptr(), n,
-                                           _ptr(slope), n, _ptr(_work(size, x)), size, _stream()), "cafe_linear_forward")
-    return x2, w2, y, slope
+    lib, t, px, pw = _lib.load(), DTYPES[x.dtype], x2.data_ptr(), w2.data_ptr()
+    size = lib.cafe_linear_forward_work(px, ldx, pw, ldw, m, n, k, t) if m * n * k >= _LARGE else 0
+    with _on(x.device) as stream:
+        status = lib.cafe_linear_forward(px, ldx, pw, ldw, _ptr(b), _ptr(r2), ldr, m, n, k, t, act, y.data_ptr(), n, _ptr(slope), n,
+                                         _ptr(_work(size, x)), size, stream)
+    if status:
+        _lib.check(status, "cafe_linear_forward")
+    return x2, w2, y, slope, (m, n, k, ldx, ldw)
 
 
 class _FusedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
-        x2, w2, y, slope = _linear(x, weight, bias, residual, act, True)
+        x2, w2, y, slope, ctx.sizes = _linear(x, weight, bias, residual, act, True)
         need = ctx.needs_input_grad
-        kind = _SLOPE_NONE if act == _NONE else _SLOPE_VALUES if slope is not None else _SLOPE_OUTPUT
-        ctx.kind, ctx.shape, ctx.bias = kind, x.shape, bias is not None
+        ctx.kind = kind = _SLOPE_NONE if act == _NONE else _SLOPE_VALUES if slope is not None else _SLOPE_OUTPUT
+        ctx.shape = x.shape
         ctx.save_for_backward(x2 if need[1] else None, w2 if need[0] else None,
                               None if kind == _SLOPE_NONE else slope if kind == _SLOPE_VALUES else y)
-        ctx.sizes = weight.shape
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_y):
-        x, w, slope = ctx.saved_tensors
-        n, k = ctx.sizes
-        need = ctx.needs_input_grad
-        g, m, ldg = _rows(grad_y, n, True)
-        gx = torch.empty(ctx.shape, dtype=g.dtype, device=g.device) if need[0] else None
-        gw = torch.empty(n, k, dtype=g.dtype, device=g.device) if need[1] else None
-        gb = torch.empty(n, dtype=g.dtype, device=g.device) if need[2] else None
-        if need[0] or need[1] or need[2]:
-            lib, t = _lib.load(), DTYPES[g.dtype]
-            ldx, ldw = k if x is None else _rows(x, k)[2], k if w is None else _rows(w, k)[2]
-            size = lib.cafe_linear_backward_work(g.data_ptr(), ldg, ctx.kind, _ptr(x), ldx, _ptr(w), ldw, m, n, k, t, need[0], need[1], need[2])
-            with _on(g.device):
-                _lib.check(lib.cafe_linear_backward(
-                    g.data_ptr(), ldg, _ptr(slope), n, ctx.kind, _ptr(x), ldx, _ptr(w), ldw, m, n, k, t, _ptr(gx), k, _ptr(gw), k, _ptr(gb),
-                    _ptr(_work(size, g)), size, _stream()), "cafe_linear_backward")
-        return gx, gw, gb, grad_y if need[3] else None, None
+        # (differentiated with create_graph: gradients that refuse to be differentiated again)
+        return _linear_backward_once(ctx, grad_y) if torch.is_grad_enabled() else _linear_backward(ctx, grad_y)
+
+
+def _linear_backward(ctx, grad_y):
+    x, w, slope = ctx.saved_tensors
+    m, n, k, ldx, ldw = ctx.sizes
+    need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
+    gx = gw = gb = None
+    if need_x or need_w or need_b:
+        g, _, ldg = _rows(grad_y, n, True)
+        dtype, device = g.dtype, g.device
+        if need_x:
+            gx = torch.empty(ctx.shape, dtype=dtype, device=device)
+        if need_w:
+            gw = torch.empty(n, k, dtype=dtype, device=device)
+        if need_b:
+            gb = torch.empty(n, dtype=dtype, device=device)
+        lib, t, pg, px, pw = _lib.load(), DTYPES[dtype], g.data_ptr(), _ptr(x), _ptr(w)
+        size = 0
+        if m * n * k >= _LARGE:
+            size = lib.cafe_linear_backward_work(pg, ldg, ctx.kind, px, ldx, pw, ldw, m, n, k, t, need_x, need_w, need_b)
+        with _on(device) as stream:
+            status = lib.cafe_linear_backward(pg, ldg, _ptr(slope), n, ctx.kind, px, ldx, pw, ldw, m, n, k, t, _ptr(gx), k, _ptr(gw), k, _ptr(gb),
+                                              _ptr(_work(size, g)), size, stream)
+        if status:
+            _lib.check(status, "cafe_linear_backward")
+    return gx, gw, gb, grad_y if need_r else None, None
+
+
+_linear_backward_once = once_differentiable(_linear_backward)
 
 
 def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, activation: str = "none",
@@ -186,9 +216,9 @@ def _mlp(x, weights, biases, acts, keep):
     call = (n, (ctypes.c_int32 * (n + 1))(*widths), m, x2.data_ptr(), ldx, _pointers([w for w, _, _ in ws]), (ctypes.c_int64 * n)(*[ld for _, _, ld in ws]))
     lib, t = _lib.load(), DTYPES[x.dtype]
     size = lib.cafe_mlp_forward_work(*call, t)
-    with _on(x.device):
+    with _on(x.device) as stream:
         _lib.check(lib.cafe_mlp_forward(*call, _pointers(bs), (ctypes.c_int32 * n)(*acts), t, _pointers(ys), (ctypes.c_int64 * n)(*pitch),
-                                        _pointers(slopes) if keep else None, _ptr(_work(size, x)), size, _stream()), "cafe_mlp_forward")
+                                        _pointers(slopes) if keep else None, _ptr(_work(size, x)), size, stream), "cafe_mlp_forward")
     return x2, [w for w, _, _ in ws], ys, slopes, pitch
 
 
@@ -202,27 +232,33 @@ class _FusedMLP(torch.autograd.Function):
         return ys[-1]
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_y):
-        n, acts = len(ctx.acts), ctx.acts
-        x, *rest = ctx.saved_tensors
-        ws, ys, slopes = rest[:n], rest[n:2 * n], rest[2 * n:]
-        widths = [ws[0].shape[1]] + [w.shape[0] for w in ws]
-        need = ctx.needs_input_grad
-        g, m, ldg = _rows(grad_y, widths[-1], True)
-        new = lambda *shape: torch.empty(*shape, dtype=g.dtype, device=g.device)   # noqa: E731
-        gx = new(*ctx.shape) if need[0] else None
-        gws = [new(*w.shape) if need[2 + l] else None for l, w in enumerate(ws)]
-        gbs = [new(w.shape[0]) if need[2 + n + l] else None for l, w in enumerate(ws)]
-        lib, t = _lib.load(), DTYPES[g.dtype]
-        call = (n, (ctypes.c_int32 * (n + 1))(*widths), m, g.data_ptr(), ldg, x.data_ptr(), _rows(x, widths[0])[2], _pointers(ws),
-                (ctypes.c_int64 * n)(*[_rows(w, w.shape[1])[2] for w in ws]))
-        size = lib.cafe_mlp_backward_work(*call, t)
-        with _on(g.device):
-            _lib.check(lib.cafe_mlp_backward(
-                *call, (ctypes.c_int32 * n)(*acts), t, _pointers(ys), (ctypes.c_int64 * n)(*ctx.pitch), _pointers(slopes), _ptr(gx), widths[0],
-                _pointers(gws), _pointers(gbs), _ptr(_work(size, g)), size, _stream()), "cafe_mlp_backward")
-        return (gx, None, *gws, *gbs)
+        return _mlp_backward_once(ctx, grad_y) if torch.is_grad_enabled() else _mlp_backward(ctx, grad_y)
+
+
+def _mlp_backward(ctx, grad_y):
+    n, acts = len(ctx.acts), ctx.acts
+    x, *rest = ctx.saved_tensors
+    ws, ys, slopes = rest[:n], rest[n:2 * n], rest[2 * n:]
+    widths = [ws[0].shape[1]] + [w.shape[0] for w in ws]
+    need = ctx.needs_input_grad
+    g, m, ldg = _rows(grad_y, widths[-1], True)
+    new = lambda *shape: torch.empty(*shape, dtype=g.dtype, device=g.device)   # noqa: E731
+    gx = new(*ctx.shape) if need[0] else None
+    gws = [new(*w.shape) if need[2 + l] else None for l, w in enumerate(ws)]
+    gbs = [new(w.shape[0]) if need[2 + n + l] else None for l, w in enumerate(ws)]
+    lib, t = _lib.load(), DTYPES[g.dtype]
+    call = (n, (ctypes.c_int32 * (n + 1))(*widths), m, g.data_ptr(), ldg, x.data_ptr(), _rows(x, widths[0])[2], _pointers(ws),
+            (ctypes.c_int64 * n)(*[_rows(w, w.shape[1])[2] for w in ws]))
+    size = lib.cafe_mlp_backward_work(*call, t)
+    with _on(g.device) as stream:
+        _lib.check(lib.cafe_mlp_backward(
+            *call, (ctypes.c_int32 * n)(*acts), t, _pointers(ys), (ctypes.c_int64 * n)(*ctx.pitch), _pointers(slopes), _ptr(gx), widths[0],
+            _pointers(gws), _pointers(gbs), _ptr(_work(size, g)), size, stream), "cafe_mlp_backward")
+    return (gx, None, *gws, *gbs)
+
+
+_mlp_backward_once = once_differentiable(_mlp_backward)
 
 
 def fused_mlp(x: torch.Tensor, weights, biases, activations) -> torch.Tensor:

@@ -7,7 +7,6 @@ import torch
 
 from . import _lib
 from .dense import DTYPES, _on
-from .sketch import _stream
 
 BLOCK = 256   # elements that share the exponent of their 8-bit moments
 _CODES = ("exp_avg", "exp_avg_top", "root_avg_sq", "root_avg_sq_top")
@@ -23,10 +22,6 @@ def _dense(t: torch.Tensor) -> bool:
             return False
         at *= size
     return True
-
-
-def _array(typ, values):
-    return (typ * len(values))(*values)
 
 
 class AdamW(torch.optim.Optimizer):
@@ -115,20 +110,17 @@ class AdamW(torch.optim.Optimizer):
             ticket = self._ticket.get(device)
             if ticket is None:
                 ticket = self._ticket[device] = torch.zeros(1, dtype=torch.int32, device=device)
-            vp = ctypes.c_void_p
-            m = _array(vp, [s["exp_avg"].data_ptr() for *_, s in rows])
-            if self.state_bits == 32:
-                v, mtop, vtop = _array(vp, [s["exp_avg_sq"].data_ptr() for *_, s in rows]), None, None
-            else:
-                v = _array(vp, [s["root_avg_sq"].data_ptr() for *_, s in rows])
-                mtop = _array(vp, [s["exp_avg_top"].data_ptr() for *_, s in rows])
-                vtop = _array(vp, [s["root_avg_sq_top"].data_ptr() for *_, s in rows])
-            with _on(device):
+            n, packed = len(rows), self.state_bits == 8
+            vp = ctypes.c_void_p * n
+            names = _CODES if packed else ("exp_avg", "exp_avg_sq")
+            state = {k: vp(*[s[k].data_ptr() for _, _, _, s in rows]) for k in ("step",) + names}
+            with _on(device) as stream:
                 _lib.check(lib.cafe_adamw_step(
-                    len(rows), _array(vp, [p.data_ptr() for _, p, _, _ in rows]), _array(vp, [g.data_ptr() for _, _, g, _ in rows]), m, v,
-                    mtop, vtop, _array(vp, [s["step"].data_ptr() for *_, s in rows]), _array(ctypes.c_int64, [p.numel() for _, p, _, _ in rows]),
-                    _array(ctypes.c_int32, [k for k, *_ in rows]), DTYPES[dtype], self.state_bits, group["lr"], *group["betas"], group["eps"],
-                    group["weight_decay"], self.seed, ticket.data_ptr(), _stream()), "cafe_adamw_step")
+                    n, vp(*[p.data_ptr() for _, p, _, _ in rows]), vp(*[g.data_ptr() for _, _, g, _ in rows]), state["exp_avg"],
+                    state["root_avg_sq" if packed else "exp_avg_sq"], state.get("exp_avg_top"), state.get("root_avg_sq_top"), state["step"],
+                    (ctypes.c_int64 * n)(*[p.numel() for _, p, _, _ in rows]), (ctypes.c_int32 * n)(*[k for k, _, _, _ in rows]), DTYPES[dtype],
+                    self.state_bits, group["lr"], *group["betas"], group["eps"], group["weight_decay"], self.seed, ticket.data_ptr(), stream),
+                    "cafe_adamw_step")
         return loss
 
     @torch.no_grad()
@@ -138,18 +130,24 @@ class AdamW(torch.optim.Optimizer):
         params = [p for group in self.param_groups for p in group["params"] if "step" in self.state.get(p, ())]
         if self.state_bits == 32:
             return [(self.state[p]["exp_avg"], self.state[p]["exp_avg_sq"]) for p in params]
-        out = [tuple(torch.empty_like(p, dtype=torch.bfloat16, memory_format=torch.preserve_format) for _ in range(2)) for p in params]
         by_device = {}
-        for p, o in zip(params, out):
-            by_device.setdefault(p.device, []).append((p, o))
-        vp = ctypes.c_void_p
-        for device, rows in by_device.items():
-            codes = [_array(vp, [self.state[p][name].data_ptr() for p, _ in rows]) for name in _CODES]
-            with _on(device):
-                _lib.check(_lib.load().cafe_adamw_moments(
-                    len(rows), *codes, _array(ctypes.c_int64, [p.numel() for p, _ in rows]), _array(vp, [o[0].data_ptr() for _, o in rows]),
-                    _array(vp, [o[1].data_ptr() for _, o in rows]), _stream()), "cafe_adamw_moments")
-        return out
+        for p in params:
+            by_device.setdefault(p.device, []).append(p)
+        out = {}
+        for device, ps in by_device.items():
+            n = len(ps)
+            vp = ctypes.c_void_p * n
+            # one allocation for all, every tensor on 16 bytes
+            sizes = [-(-p.numel() // 8) * 8 for p in ps]
+            flat = torch.empty(2 * sum(sizes), dtype=torch.bfloat16, device=device)
+            values = [v.as_strided(p.shape, p.stride()) for v, p in zip(flat.split(sizes + sizes), ps + ps)]
+            codes = [vp(*[self.state[p][name].data_ptr() for p in ps]) for name in _CODES]
+            with _on(device) as stream:
+                _lib.check(_lib.load().cafe_adamw_moments(n, *codes, (ctypes.c_int64 * n)(*[p.numel() for p in ps]),
+                                                          vp(*[v.data_ptr() for v in values[:n]]), vp(*[v.data_ptr() for v in values[n:]]), stream),
+                           "cafe_adamw_moments")
+            out.update(zip(ps, zip(values[:n], values[n:])))
+        return [out[p] for p in params]
 
     def state_dict(self):
         return {**super().state_dict(), "state_bits": self.state_bits, "seed": self.seed}
