@@ -52,29 +52,52 @@ __device__ __forceinline__ uint32_t cafe_mix32(uint32_t x) {
     return x;
 }
 
-// bits of the smallest code's value for a block exponent
-template <int S> __device__ __forceinline__ uint32_t cafe_code_least(uint32_t top) { return (((top - 15u) << S) + 1u) << (23 - S); }
-template <int S> __device__ __forceinline__ float cafe_code_value(uint32_t code, uint32_t top) {
-    if (top == 255u) return __uint_as_float(0x7fffffffu);
-    const uint32_t low = S == 3 ? code & 127u : code;
-    const uint32_t bits = low ? (low + ((top - 15u) << S)) << (23 - S) : 0u;
-    return __uint_as_float(bits | (S == 3 ? (code & 128u) << 24 : 0u));
-}
-template <int S> __device__ __forceinline__ uint32_t cafe_code_ceil(float x) {   // the code grid's next point, not below |x|
-    return ((__float_as_uint(x) & 0x7fffffffu) + (1u << (23 - S)) - 1u) >> (23 - S);
-}
-template <int S> __device__ __forceinline__ uint32_t cafe_code_top(uint32_t ceil) {
-    const uint32_t t = ceil >> S;
+// A block's exponent `top` as the number that a code is counted from
+template <int S> __device__ __forceinline__ uint32_t cafe_code_base(uint32_t top) { return (top - 15u) << S; }
+// the exponent for a block whose largest magnitude has these bits: of the code grid's next point that is not below it
+template <int S> __device__ __forceinline__ uint32_t cafe_code_top(uint32_t largest) {
+    const uint32_t t = (largest + (1u << (23 - S)) - 1u) >> 23;
     return t < 16u ? 16u : t > 255u ? 255u : t;
 }
-template <int S> __device__ __forceinline__ uint32_t cafe_code(float x, uint32_t top, uint32_t rnd) {
-    if (top == 255u) return 0;
-    const uint32_t bits = __float_as_uint(x) & 0x7fffffffu, least = cafe_code_least<S>(top);
-    uint32_t c;
-    if (bits >= least) c = ((bits + (rnd << (7 - S))) >> (23 - S)) - ((top - 15u) << S);
-    else if (S == 3) c = (float)rnd * (__uint_as_float(least) * 0x1p-16f) < __uint_as_float(bits) ? 1u : 0u;
-    else c = bits ? 1u : 0u;
-    return S == 3 ? c | (__float_as_uint(x) >> 31) << 7 : c;
+// eight codes to their values
+template <int S> __device__ __forceinline__ void cafe_code_values(const uint32_t* codes, uint32_t top, float* v) {
+    const uint32_t base = cafe_code_base<S>(top);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t c = (codes[i >> 2] >> (8 * (i & 3))) & 255u, low = S == 3 ? c & 127u : c;
+        const uint32_t bits = low ? (low + base) << (23 - S) : 0u;
+        v[i] = __uint_as_float(S == 3 ? bits | (c & 128u) << 24 : bits);
+    }
+    if (top == 255u) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(0x7fffffffu);
+    }
+}
+// eight values to codes, rounded by the 16 random bits of each (S = 3 the low ones, else the high ones)
+template <int S> __device__ __forceinline__ void cafe_codes(const float* v, uint32_t top, const uint32_t* rnd, uint32_t* codes) {
+    const uint32_t base = cafe_code_base<S>(top), least = (base + 1u) << (23 - S);
+    uint32_t c[8], smallest = 0xffffffffu;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t bits = __float_as_uint(v[i]) & 0x7fffffffu, r = S == 3 ? rnd[i] & 0xffffu : rnd[i] >> 16;
+        c[i] = ((bits + (r << (7 - S))) >> (23 - S)) - base;
+        smallest = min(smallest, bits);
+    }
+    if (smallest < least) {   // below the smallest code: to it or to zero, or up to it
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t bits = __float_as_uint(v[i]) & 0x7fffffffu, r = S == 3 ? rnd[i] & 0xffffu : rnd[i] >> 16;
+            const uint32_t low = S == 3 ? ((float)r * (__uint_as_float(least) * 0x1p-16f) < __uint_as_float(bits) ? 1u : 0u) : (bits ? 1u : 0u);
+            if (bits < least) c[i] = low;
+        }
+    }
+    codes[0] = codes[1] = 0u;
+    if (top == 255u) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t x = S == 3 ? c[i] | (__float_as_uint(v[i]) >> 31) << 7 : c[i];
+        codes[i >> 2] |= x << (8 * (i & 3));
+    }
 }
 
 // eight consecutive elements, `ok` of them valid
@@ -100,15 +123,18 @@ template <typename T> __device__ __forceinline__ void cafe_store8(T* p, int ok, 
         for (int i = 0; i < 8; ++i) if (i < ok) p[i] = in[i];
     }
 }
-__device__ __forceinline__ uint64_t cafe_load_codes(const uint8_t* p, int ok) {   // (codes are the library's own arrays: on 8-byte boundaries)
-    if (ok == 8) return *reinterpret_cast<const uint64_t*>(p);
-    uint64_t c = 0;
-    for (int i = 0; i < ok; ++i) c |= (uint64_t)p[i] << (8 * i);
-    return c;
+__device__ __forceinline__ void cafe_load_codes(const uint8_t* p, int ok, uint32_t* c) {   // (codes are the library's own arrays: on 8-byte boundaries)
+    if (ok == 8) {
+        const uint2 x = *reinterpret_cast<const uint2*>(p);
+        c[0] = x.x; c[1] = x.y;
+    } else {
+        c[0] = c[1] = 0u;
+        for (int i = 0; i < ok; ++i) c[i >> 2] |= (uint32_t)p[i] << (8 * (i & 3));
+    }
 }
-__device__ __forceinline__ void cafe_store_codes(uint8_t* p, int ok, uint64_t c) {
-    if (ok == 8) *reinterpret_cast<uint64_t*>(p) = c;
-    else for (int i = 0; i < ok; ++i) p[i] = (uint8_t)(c >> (8 * i));
+__device__ __forceinline__ void cafe_store_codes(uint8_t* p, int ok, const uint32_t* c) {
+    if (ok == 8) *reinterpret_cast<uint2*>(p) = make_uint2(c[0], c[1]);
+    else for (int i = 0; i < ok; ++i) p[i] = (uint8_t)(c[i >> 2] >> (8 * (i & 3)));
 }
 
 template <int NT>
@@ -124,17 +150,27 @@ __device__ __forceinline__ int cafe_adamw_find(const CafeAdamwTensors<NT>& P, in
 // The moments' products and sums are single roundings without contraction: a block's codes are then those of the formulas
 // evaluated one operation after the other, whatever the compiler would fuse.
 template <typename T, int BITS, int NT>
-__global__ void __launch_bounds__(CAFE_ADAMW_THREADS) k_adamw(const __grid_constant__ CafeAdamwTensors<NT> P, const CafeAdamwScalars S) {
+__global__ void __launch_bounds__(CAFE_ADAMW_THREADS, 4) k_adamw(const __grid_constant__ CafeAdamwTensors<NT> P, const CafeAdamwScalars S) {
     const int lane = threadIdx.x & 31;
     const int64_t warps = (int64_t)gridDim.x * (CAFE_ADAMW_THREADS / 32);
+    int t = -1;
+    int64_t begin = 0, end = 0;       // the tensor's blocks
+    float rate = 0.f, scale = 0.f;    // lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+    uint32_t key0 = 0;
+    bool vec = false;
     for (int64_t blk = (int64_t)blockIdx.x * (CAFE_ADAMW_THREADS / 32) + (threadIdx.x >> 5); blk < P.first[P.count]; blk += warps) {
-        const int t = cafe_adamw_find(P, blk);
-        const int64_t own = blk - P.first[t], at = own * CAFE_ADAMW_BLOCK + lane * 8, left = P.n[t] - at;
+        const bool fresh = blk >= end;
+        if (fresh) {
+            t = cafe_adamw_find(P, blk);
+            begin = P.first[t];
+            end = P.first[t + 1];
+            vec = P.index[t] >= 0;
+        }
+        const int64_t own = blk - begin, at = own * CAFE_ADAMW_BLOCK + lane * 8, left = P.n[t] - at;
         const int ok = left >= 8 ? 8 : left > 0 ? (int)left : 0;
-        const int index = P.index[t] < 0 ? -1 - P.index[t] : P.index[t];
-        const bool vec = P.index[t] >= 0;
         alignas(16) T p[8], g[8];
         alignas(16) float m[8], v[8];
+        uint32_t cm[2], cv[2], tm = 0, tv = 0;
         T* pp = static_cast<T*>(P.p[t]) + at;
         cafe_load8(pp, ok, vec, p);
         cafe_load8(static_cast<const T*>(P.g[t]) + at, ok, vec, g);
@@ -142,32 +178,37 @@ __global__ void __launch_bounds__(CAFE_ADAMW_THREADS) k_adamw(const __grid_const
             cafe_load8(static_cast<const float*>(P.m[t]) + at, ok, vec, m);
             cafe_load8(static_cast<const float*>(P.v[t]) + at, ok, vec, v);
         } else {
-            const uint64_t cm = cafe_load_codes(static_cast<const uint8_t*>(P.m[t]) + at, ok);
-            const uint64_t cv = cafe_load_codes(static_cast<const uint8_t*>(P.v[t]) + at, ok);
-            const uint32_t tm = P.mtop[t][own], tv = P.vtop[t][own];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                m[i] = cafe_code_value<3>((uint32_t)(cm >> (8 * i)) & 255u, tm);
-                const float r = cafe_code_value<4>((uint32_t)(cv >> (8 * i)) & 255u, tv);
-                v[i] = __fmul_rn(r, r);
-            }
+            cafe_load_codes(static_cast<const uint8_t*>(P.m[t]) + at, ok, cm);
+            cafe_load_codes(static_cast<const uint8_t*>(P.v[t]) + at, ok, cv);
+            tm = P.mtop[t][own];
+            tv = P.vtop[t][own];
         }
-        const int64_t step = *P.step[t] + 1;
-        const float rate = S.lr / -expm1f((float)step * S.log_b1), root2 = sqrtf(-expm1f((float)step * S.log_b2));
-        uint32_t ceil_m = 0, ceil_v = 0;
+        if (fresh) {
+            const int64_t step = *P.step[t] + 1;
+            rate = S.lr / -expm1f((float)step * S.log_b1);
+            scale = rsqrtf(-expm1f((float)step * S.log_b2));
+            const int index = vec ? P.index[t] : -1 - P.index[t];
+            key0 = cafe_mix32(cafe_mix32(S.seed + 0x9E3779B9u * (uint32_t)(index + 1)) ^ (uint32_t)step);
+        }
+        if constexpr (BITS == 8) {
+            cafe_code_values<3>(cm, tm, m);
+            cafe_code_values<4>(cv, tv, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], v[i]);
+        }
+        uint32_t most_m = 0, most_v = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float gi = cafe_to_float(g[i]);
+            const float gi = cafe_to_float(g[i]), pi = cafe_to_float(p[i]);
             m[i] = __fadd_rn(__fmul_rn(m[i], S.b1), __fmul_rn(gi, S.c1));
             v[i] = __fadd_rn(__fmul_rn(v[i], S.b2), __fmul_rn(__fmul_rn(gi, S.c2), gi));
             const float r = __fsqrt_rn(v[i]);
-            const float pi = cafe_to_float(p[i]);
-            p[i] = cafe_from_float<T>(pi - (S.lr_decay * pi + rate * m[i] / (r / root2 + S.eps)));
+            p[i] = cafe_from_float<T>(pi - (S.lr_decay * pi + __fdividef(rate * m[i], r * scale + S.eps)));
             if constexpr (BITS == 8) {
                 v[i] = r;
-                if (i >= ok) m[i] = v[i] = 0.f;
-                ceil_m = max(ceil_m, cafe_code_ceil<3>(m[i]));
-                ceil_v = max(ceil_v, cafe_code_ceil<4>(r));
+                if (ok < 8 && i >= ok) m[i] = v[i] = 0.f;
+                most_m = max(most_m, __float_as_uint(m[i]) & 0x7fffffffu);
+                most_v = max(most_v, __float_as_uint(v[i]) & 0x7fffffffu);
             }
         }
         cafe_store8(pp, ok, vec, p);
@@ -175,18 +216,14 @@ __global__ void __launch_bounds__(CAFE_ADAMW_THREADS) k_adamw(const __grid_const
             cafe_store8(static_cast<float*>(P.m[t]) + at, ok, vec, m);
             cafe_store8(static_cast<float*>(P.v[t]) + at, ok, vec, v);
         } else {
-            const uint32_t tm = cafe_code_top<3>(__reduce_max_sync(0xffffffffu, ceil_m));
-            const uint32_t tv = cafe_code_top<4>(__reduce_max_sync(0xffffffffu, ceil_v));
-            uint32_t key = cafe_mix32(S.seed + 0x9E3779B9u * (uint32_t)(index + 1));
-            key = cafe_mix32(key ^ (uint32_t)step);
-            key = cafe_mix32(key + (uint32_t)(at >> 32));
-            uint64_t cm = 0, cv = 0;
+            tm = cafe_code_top<3>(__reduce_max_sync(0xffffffffu, most_m));
+            tv = cafe_code_top<4>(__reduce_max_sync(0xffffffffu, most_v));
+            const uint32_t key = cafe_mix32(key0 + (uint32_t)(at >> 32));
+            uint32_t rnd[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint32_t rnd = cafe_mix32((uint32_t)(at + i) ^ key);
-                cm |= (uint64_t)cafe_code<3>(m[i], tm, rnd & 0xffffu) << (8 * i);
-                cv |= (uint64_t)cafe_code<4>(v[i], tv, rnd >> 16) << (8 * i);
-            }
+            for (int i = 0; i < 8; ++i) rnd[i] = cafe_mix32((uint32_t)(at + i) ^ key);
+            cafe_codes<3>(m, tm, rnd, cm);
+            cafe_codes<4>(v, tv, rnd, cv);
             cafe_store_codes(static_cast<uint8_t*>(P.m[t]) + at, ok, cm);
             cafe_store_codes(static_cast<uint8_t*>(P.v[t]) + at, ok, cv);
             if (lane == 0) { P.mtop[t][own] = (uint8_t)tm; P.vtop[t][own] = (uint8_t)tv; }
@@ -216,15 +253,15 @@ __global__ void __launch_bounds__(CAFE_ADAMW_THREADS) k_adamw_moments(const __gr
         const int64_t own = blk - P.first[t], at = own * CAFE_ADAMW_BLOCK + lane * 8, left = P.n[t] - at;
         const int ok = left >= 8 ? 8 : left > 0 ? (int)left : 0;
         const bool vec = P.index[t] >= 0;
-        const uint64_t cm = cafe_load_codes(static_cast<const uint8_t*>(P.m[t]) + at, ok);
-        const uint64_t cv = cafe_load_codes(static_cast<const uint8_t*>(P.v[t]) + at, ok);
-        const uint32_t tm = P.mtop[t][own], tv = P.vtop[t][own];
+        uint32_t cm[2], cv[2];
+        cafe_load_codes(static_cast<const uint8_t*>(P.m[t]) + at, ok, cm);
+        cafe_load_codes(static_cast<const uint8_t*>(P.v[t]) + at, ok, cv);
+        float vm[8], vr[8];
+        cafe_code_values<3>(cm, P.mtop[t][own], vm);
+        cafe_code_values<4>(cv, P.vtop[t][own], vr);
         alignas(16) __nv_bfloat16 m[8], r[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            m[i] = __float2bfloat16_rn(cafe_code_value<3>((uint32_t)(cm >> (8 * i)) & 255u, tm));
-            r[i] = __float2bfloat16_rn(cafe_code_value<4>((uint32_t)(cv >> (8 * i)) & 255u, tv));
-        }
+        for (int i = 0; i < 8; ++i) { m[i] = __float2bfloat16_rn(vm[i]); r[i] = __float2bfloat16_rn(vr[i]); }
         cafe_store8(static_cast<__nv_bfloat16*>(P.p[t]) + at, ok, vec, m);
         cafe_store8(static_cast<__nv_bfloat16*>(const_cast<void*>(P.g[t])) + at, ok, vec, r);
     }

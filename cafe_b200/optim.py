@@ -137,10 +137,7 @@ class AdamW(torch.optim.Optimizer):
         for device, ps in by_device.items():
             n = len(ps)
             vp = ctypes.c_void_p * n
-            # one allocation for all, every tensor on 16 bytes
-            sizes = [-(-p.numel() // 8) * 8 for p in ps]
-            flat = torch.empty(2 * sum(sizes), dtype=torch.bfloat16, device=device)
-            values = [v.as_strided(p.shape, p.stride()) for v, p in zip(flat.split(sizes + sizes), ps + ps)]
+            values = [torch.empty_like(p, dtype=torch.bfloat16, memory_format=torch.preserve_format) for p in ps + ps]
             codes = [vp(*[self.state[p][name].data_ptr() for p in ps]) for name in _CODES]
             with _on(device) as stream:
                 _lib.check(_lib.load().cafe_adamw_moments(n, *codes, (ctypes.c_int64 * n)(*[p.numel() for p in ps]),
