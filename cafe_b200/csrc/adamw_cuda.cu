@@ -61,12 +61,12 @@ template <int S> __device__ __forceinline__ uint32_t cafe_code_top(uint32_t larg
 }
 // eight codes to their values
 template <int S> __device__ __forceinline__ void cafe_code_values(const uint32_t* codes, uint32_t top, float* v) {
-    const uint32_t base = cafe_code_base<S>(top);
+    const uint32_t base = cafe_code_base<S>(top) << (23 - S);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const uint32_t c = (codes[i >> 2] >> (8 * (i & 3))) & 255u, low = S == 3 ? c & 127u : c;
-        const uint32_t bits = low ? (low + base) << (23 - S) : 0u;
-        v[i] = __uint_as_float(S == 3 ? bits | (c & 128u) << 24 : bits);
+        const uint32_t x = codes[i >> 2] << (24 - 8 * (i & 3));   // the code in the highest byte (and others' below it)
+        const uint32_t low = S == 3 ? (x >> 4) & 0x07f00000u : (x >> 5) & 0x07f80000u, bits = low ? low + base : 0u;
+        v[i] = __uint_as_float(S == 3 ? bits | (x & 0x80000000u) : bits);
     }
     if (top == 255u) {
 #pragma unroll
@@ -75,18 +75,19 @@ template <int S> __device__ __forceinline__ void cafe_code_values(const uint32_t
 }
 // eight values to codes, rounded by the 16 random bits of each (S = 3 the low ones, else the high ones)
 template <int S> __device__ __forceinline__ void cafe_codes(const float* v, uint32_t top, const uint32_t* rnd, uint32_t* codes) {
-    const uint32_t base = cafe_code_base<S>(top), least = (base + 1u) << (23 - S);
+    const uint32_t base = cafe_code_base<S>(top) << (23 - S), least = base + (1u << (23 - S));
     uint32_t c[8], smallest = 0xffffffffu;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const uint32_t bits = __float_as_uint(v[i]) & 0x7fffffffu, r = S == 3 ? rnd[i] & 0xffffu : rnd[i] >> 16;
-        c[i] = ((bits + (r << (7 - S))) >> (23 - S)) - base;
+        const uint32_t bits = S == 3 ? __float_as_uint(v[i]) & 0x7fffffffu : __float_as_uint(v[i]);
+        const uint32_t r = S == 3 ? (rnd[i] & 0xffffu) << 4 : (rnd[i] >> 16) << 3;
+        c[i] = (bits + r - base) >> (23 - S);
         smallest = min(smallest, bits);
     }
     if (smallest < least) {   // below the smallest code: to it or to zero, or up to it
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const uint32_t bits = __float_as_uint(v[i]) & 0x7fffffffu, r = S == 3 ? rnd[i] & 0xffffu : rnd[i] >> 16;
+            const uint32_t bits = __float_as_uint(v[i]) & 0x7fffffffu, r = rnd[i] & 0xffffu;
             const uint32_t low = S == 3 ? ((float)r * (__uint_as_float(least) * 0x1p-16f) < __uint_as_float(bits) ? 1u : 0u) : (bits ? 1u : 0u);
             if (bits < least) c[i] = low;
         }
@@ -95,9 +96,22 @@ template <int S> __device__ __forceinline__ void cafe_codes(const float* v, uint
     if (top == 255u) return;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const uint32_t x = S == 3 ? c[i] | (__float_as_uint(v[i]) >> 31) << 7 : c[i];
+        const uint32_t x = S == 3 ? c[i] | ((__float_as_uint(v[i]) >> 24) & 0x80u) : c[i];
         codes[i >> 2] |= x << (8 * (i & 3));
     }
+}
+
+// Square root and reciprocal to 2^-22 of their value, for the update alone.
+__device__ __forceinline__ float cafe_root_fast(float v) { float r; asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
+__device__ __forceinline__ float cafe_inverse_fast(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+// The root that is kept: one step of Newton's iteration from the hardware's reciprocal root, x' = x + (v - x^2) y / 2 with x = v y,
+// leaves less than 2^-24 of the value beside the last rounding.  Below the normal numbers it is zero or coarse; v that overflows
+// gives a NaN, and with it its block.
+__device__ __forceinline__ float cafe_root(float v) {
+    float y;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaxf(v, 1.17549435e-38f)));
+    const float x = v * y;
+    return fmaf(fmaf(-x, x, v), 0.5f * y, x);
 }
 
 // eight consecutive elements, `ok` of them valid
@@ -202,13 +216,13 @@ __global__ void __launch_bounds__(CAFE_ADAMW_THREADS, 4) k_adamw(const __grid_co
             const float gi = cafe_to_float(g[i]), pi = cafe_to_float(p[i]);
             m[i] = __fadd_rn(__fmul_rn(m[i], S.b1), __fmul_rn(gi, S.c1));
             v[i] = __fadd_rn(__fmul_rn(v[i], S.b2), __fmul_rn(__fmul_rn(gi, S.c2), gi));
-            const float r = __fsqrt_rn(v[i]);
-            p[i] = cafe_from_float<T>(pi - (S.lr_decay * pi + __fdividef(rate * m[i], r * scale + S.eps)));
+            const float r = BITS == 8 ? cafe_root(v[i]) : cafe_root_fast(v[i]);
+            p[i] = cafe_from_float<T>(pi - fmaf(S.lr_decay, pi, rate * m[i] * cafe_inverse_fast(fmaf(r, scale, S.eps))));
             if constexpr (BITS == 8) {
                 v[i] = r;
                 if (ok < 8 && i >= ok) m[i] = v[i] = 0.f;
                 most_m = max(most_m, __float_as_uint(m[i]) & 0x7fffffffu);
-                most_v = max(most_v, __float_as_uint(v[i]) & 0x7fffffffu);
+                most_v = max(most_v, __float_as_uint(v[i]));
             }
         }
         cafe_store8(pp, ok, vec, p);
