@@ -43,6 +43,17 @@ template <bool FAST> __device__ __forceinline__ float cafe_act(float z, int act,
         default: *slope = 1.f; return z;
     }
 }
+// four at a time: z becomes act(z), d its derivative
+template <bool FAST> __device__ __forceinline__ void cafe_act4(float* z, int act, float* d) {
+    if (act == CAFE_ACT_NONE) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) d[q] = 1.f;
+        return;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) z[q] = cafe_act<FAST>(z[q], act, d + q);
+}
+
 // the derivative kept for the backward, always finer than the type it multiplies, so that gz's own rounding stays the only
 // one that counts: fp16 (11 bits; it lies in [-0.2, 1.2]) beside bf16 (8 bits), else fp32
 template <typename T> struct CafeSlopeOf { typedef float type; };
@@ -85,29 +96,84 @@ static __device__ __noinline__ float cafe_plain_dot(const CafeJob& J, int64_t i,
 
 // ---- the end of a product --------------------------------------------------------------------------------------------
 // A thread's 4 * QUADS consecutive columns of row r of the block's sums to shared memory; a NaN of split operands is looked into.
-template <bool SPLIT, int N>
-__device__ __forceinline__ void cafe_sums_put(const CafeJob& J, const float* acc, uint32_t at, int64_t row, int64_t col, int k0, int k1, bool look) {
+// EXCHANGED: the 16-byte pieces of a row (128 bytes) are exchanged by `x`.
+template <bool SPLIT, int N, bool EXCHANGED = false>
+__device__ __forceinline__ void cafe_sums_put(const CafeJob& J, const float* acc, uint32_t at, int64_t row, int64_t col, int k0, int k1, bool look, int x = 0) {
     bool nan = false;
+    auto place = [&](int c) { return at + (EXCHANGED ? (uint32_t)((((c >> 2) ^ x) << 4) + 4 * (c & 3)) : 4u * c); };
 #pragma unroll
     for (int c = 0; c < N; c += 4) {
-        cafe_put16(at + 4 * c, __float_as_uint(acc[c]), __float_as_uint(acc[c + 1]), __float_as_uint(acc[c + 2]), __float_as_uint(acc[c + 3]));
+        cafe_put16(place(c), __float_as_uint(acc[c]), __float_as_uint(acc[c + 1]), __float_as_uint(acc[c + 2]), __float_as_uint(acc[c + 3]));
         if (SPLIT) nan |= !(acc[c] == acc[c]) | !(acc[c + 1] == acc[c + 1]) | !(acc[c + 2] == acc[c + 2]) | !(acc[c + 3] == acc[c + 3]);
     }
     if (SPLIT && nan && look && row < J.rows)
         for (int c = 0; c < N && col + c < J.cols; ++c) {
-            float x;
-            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(at + 4 * c) : "memory");
-            if (x != x) {
-                x = cafe_plain_dot(J, row, col + c, k0, k1);
-                asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + 4 * c), "f"(x) : "memory");
+            float v;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(place(c)) : "memory");
+            if (v != v) {
+                v = cafe_plain_dot(J, row, col + c, k0, k1);
+                asm volatile("st.shared.f32 [%0], %1;" ::"r"(place(c)), "f"(v) : "memory");
             }
         }
+}
+// Four neighbouring outputs (row i, columns j ..): bias, activation, residual, rounding, stores.
+template <typename T>
+__device__ __forceinline__ void cafe_quad_end(const CafeJob& J, int64_t i, int64_t j, const float* v, const float* bias) {
+    typedef typename CafeSlopeOf<T>::type ST;
+    const int n = (int)min((int64_t)4, J.cols - j);
+    const bool vec = J.out_vec && n == 4;
+    float res[4] = {0.f, 0.f, 0.f, 0.f};
+    if (J.res) {
+        const T* p = static_cast<const T*>(J.res) + i * J.ldr + j;
+        if (J.res_vec && n == 4) {
+            alignas(16) T x[4];
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(x) = __ldg(reinterpret_cast<const uint4*>(p));
+            else *reinterpret_cast<uint2*>(x) = __ldg(reinterpret_cast<const uint2*>(p));
+#pragma unroll
+            for (int q = 0; q < 4; ++q) res[q] = cafe_to_float(x[q]);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) if (q < n) res[q] = cafe_to_float(__ldg(p + q));
+        }
+    }
+    alignas(16) T o[4];
+    alignas(16) ST sl[4];
+    float z[4], d[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) z[q] = v[q] + bias[q];
+    cafe_act4<sizeof(T) == 2>(z, J.act, d);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        o[q] = cafe_from_float<T>(z[q] + res[q]);
+        sl[q] = cafe_from_float<ST>(d[q]);
+    }
+    T* out = static_cast<T*>(J.out) + i * J.ldo + j;
+    if (vec) {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(o);
+        else *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(o);
+    } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) if (q < n) out[q] = o[q];
+    }
+    if (J.slope_out) {
+        ST* so = static_cast<ST*>(J.slope_out) + i * J.lds + j;
+        if (vec) {
+            if constexpr (sizeof(ST) == 4) *reinterpret_cast<uint4*>(so) = *reinterpret_cast<const uint4*>(sl);
+            else *reinterpret_cast<uint2*>(so) = *reinterpret_cast<const uint2*>(sl);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) if (q < n) so[q] = sl[q];
+        }
+    }
+}
+template <typename T> __device__ __forceinline__ void cafe_quad_bias(const CafeJob& J, int64_t j, float* bias) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) bias[q] = J.bias && j + q < J.cols ? cafe_to_float(__ldg(static_cast<const T*>(J.bias) + j + q)) : 0.f;
 }
 // This block's share of the tile's rows (of a cluster of `splits` blocks, by rank): the blocks' sums in the order of ranks, then
 // bias, activation, residual and the stores.  COLS columns at a pitch of COLS + 4 floats from `base` of every block.
 template <typename T, int COLS, int SPLITS>
 __device__ __forceinline__ void cafe_finish_of(const CafeJob& J, uint32_t base, int row0, int col0, int rank, int threads) {
-    typedef typename CafeSlopeOf<T>::type ST;
     constexpr int pitch = COLS + 4, quads = COLS / 4;
     const int per = CAFE_LIN_BM / SPLITS;
     for (int e = threadIdx.x; e < per * quads; e += threads) {
@@ -124,53 +190,9 @@ __device__ __forceinline__ void cafe_finish_of(const CafeJob& J, uint32_t base, 
 #pragma unroll
             for (int q = 0; q < SPLITS; ++q) { v[0] += x[q].x; v[1] += x[q].y; v[2] += x[q].z; v[3] += x[q].w; }
         }
-        const int n = (int)min((int64_t)4, J.cols - j);
-        const bool vec = J.out_vec && n == 4;
-        float bias[4] = {0.f, 0.f, 0.f, 0.f}, res[4] = {0.f, 0.f, 0.f, 0.f};
-        if (J.bias) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) if (q < n) bias[q] = cafe_to_float(__ldg(static_cast<const T*>(J.bias) + j + q));
-        }
-        if (J.res) {
-            const T* p = static_cast<const T*>(J.res) + i * J.ldr + j;
-            if (J.res_vec && n == 4) {
-                alignas(16) T x[4];
-                if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(x) = __ldg(reinterpret_cast<const uint4*>(p));
-                else *reinterpret_cast<uint2*>(x) = __ldg(reinterpret_cast<const uint2*>(p));
-#pragma unroll
-                for (int q = 0; q < 4; ++q) res[q] = cafe_to_float(x[q]);
-            } else {
-#pragma unroll
-                for (int q = 0; q < 4; ++q) if (q < n) res[q] = cafe_to_float(__ldg(p + q));
-            }
-        }
-        alignas(16) T o[4];
-        alignas(16) ST sl[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            float z = v[q] + bias[q], d = 1.f;
-            if (J.act != CAFE_ACT_NONE) z = cafe_act<sizeof(T) == 2>(z, J.act, &d);
-            o[q] = cafe_from_float<T>(z + res[q]);
-            sl[q] = cafe_from_float<ST>(d);
-        }
-        T* out = static_cast<T*>(J.out) + i * J.ldo + j;
-        if (vec) {
-            if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(o);
-            else *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(o);
-        } else {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) if (q < n) out[q] = o[q];
-        }
-        if (J.slope_out) {
-            ST* so = static_cast<ST*>(J.slope_out) + i * J.lds + j;
-            if (vec) {
-                if constexpr (sizeof(ST) == 4) *reinterpret_cast<uint4*>(so) = *reinterpret_cast<const uint4*>(sl);
-                else *reinterpret_cast<uint2*>(so) = *reinterpret_cast<const uint2*>(sl);
-            } else {
-#pragma unroll
-                for (int q = 0; q < 4; ++q) if (q < n) so[q] = sl[q];
-            }
-        }
+        float bias[4];
+        cafe_quad_bias<T>(J, j, bias);
+        cafe_quad_end<T>(J, i, j, v, bias);
     }
 }
 template <typename T, int COLS>

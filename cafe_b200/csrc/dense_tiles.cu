@@ -322,6 +322,222 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
     if (warp == 1) cafe_tm_free(tmem, Sh::tm_cols);
 }
 
+// ---- tiles one after the other ---------------------------------------------------------------------------------------------
+// The same products where there are tiles enough for every SM: one block an SM works through tile after tile, and two groups of
+// four warps take turns with tensor memory's two sets of sums, so that one tile is finished and stored while the next one's products
+// run.  Each warp stages its own 32 rows, 32 columns at a time, and writes them out row by row: nobody waits for anybody there.
+// Four stages of 48 KB: with three the products wait for their boxes (fp32 gx of 65536x1024x480 505 us, with two blocks of two stages
+// an SM 470).
+#define CAFE_RUN_THREADS 320
+template <typename T, int BN> struct CafeRunShape {
+    typedef CafeTiles<T> L;
+    static constexpr int rowb = L::BK * 2;
+    static constexpr int a_part = CAFE_LIN_BM * rowb, b_part = BN * rowb, stage = L::parts * (a_part + b_part);
+    static constexpr int stages = 196608 / stage < 6 ? 196608 / stage : 6;
+    static constexpr int staging = 32 * 32 * 4;   // a warp's rows, 32 columns; pieces of four exchanged by row
+    static constexpr int bytes = stage * stages + 8 * staging + 1024;
+    static constexpr int tm_set = L::parts == 3 ? 2 * BN : BN;
+};
+template <typename T, int BN>
+__global__ void __launch_bounds__(CAFE_RUN_THREADS, 1) k_tiles_run(const __grid_constant__ CafeTilesArgs P) {
+    typedef CafeTiles<T> L;
+    typedef CafeRunShape<T, BN> Sh;
+    extern __shared__ char sh_raw[];
+    __shared__ __align__(8) uint64_t bars[2 * Sh::stages + 8];
+    __shared__ uint32_t tm_at;
+    __shared__ volatile int bail;
+    const uint32_t base = (cafe_smem(sh_raw) + 1023u) & ~1023u;
+    const uint32_t bar0 = cafe_smem(bars);
+    auto full = [&](int s) { return bar0 + 8u * s; };
+    auto empty = [&](int s) { return bar0 + 8u * (Sh::stages + s); };
+    const uint32_t more = bar0 + 8u * (2 * Sh::stages);
+    // for each set of sums: a chunk's large sums are ready / taken (fp32), all of a tile's sums are ready / taken
+    auto chunk_full = [&](int g) { return more + 8u * g; };
+    auto chunk_taken = [&](int g) { return more + 16u + 8u * g; };
+    auto tile_full = [&](int g) { return more + 32u + 8u * g; };
+    auto tile_taken = [&](int g) { return more + 48u + 8u * g; };
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const CafeJob& J = P.job;
+    const int turns = (J.depth + L::BK - 1) / L::BK, tiles = J.tiles;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < Sh::stages; ++s) { cafe_bar_init(full(s), 1); cafe_bar_init(empty(s), 1); }
+        for (int g = 0; g < 2; ++g) { cafe_bar_init(chunk_full(g), 1); cafe_bar_init(chunk_taken(g), 4); cafe_bar_init(tile_full(g), 1); cafe_bar_init(tile_taken(g), 4); }
+        cafe_fence_barrier_init();
+        bail = 0;
+    }
+    if (warp == 1) cafe_tm_alloc(cafe_smem(&tm_at), 2 * Sh::tm_set);
+    cafe_tc_before();
+    __syncthreads();
+    cafe_tc_after();
+    const uint32_t tmem = tm_at;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            // ---- boxes of the operands
+            bool fine = true;
+            int64_t u = 0;   // turns so far
+            for (int tile = blockIdx.x; tile < tiles && fine; tile += gridDim.x) {
+                const int tm = tile / J.tiles_n, row0 = tm * CAFE_LIN_BM, col0 = (tile - tm * J.tiles_n) * BN;
+                for (int t = 0; t < turns; ++t, ++u) {
+                    const int s = (int)(u % Sh::stages), k0 = t * L::BK;
+                    if (u >= Sh::stages && !(fine = cafe_bar_wait(empty(s), (uint32_t)(u / Sh::stages - 1) & 1u, &bail))) break;
+                    const uint32_t a = base + s * Sh::stage, b = a + L::parts * Sh::a_part;
+                    cafe_bar_expect(full(s), Sh::stage);
+                    if (J.a_kc) cafe_box_load(a, &P.a, k0, row0, 0, full(s));
+                    else
+#pragma unroll
+                        for (int q = 0; q < CAFE_LIN_BM / 64; ++q) cafe_box_load(a + q * L::parts * L::BK * 128, &P.a, row0 + 64 * q, k0, 0, full(s));
+                    if (J.b_kc) cafe_box_load(b, &P.b, k0, col0, 0, full(s));
+                    else
+#pragma unroll
+                        for (int q = 0; q < BN / 64; ++q) cafe_box_load(b + q * L::parts * L::BK * 128, &P.b, col0 + 64 * q, k0, 0, full(s));
+                }
+            }
+            if (!fine)   // given up: the copies in flight end before the block does
+                for (int64_t v = u > Sh::stages ? u - Sh::stages : 0; v < u; ++v)
+                    for (int i = 0; i < (1 << 20) && !cafe_bar_try(full((int)(v % Sh::stages)), (uint32_t)(v / Sh::stages) & 1u); ++i) {}
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            // ---- products
+            const uint32_t instr = cafe_mma_instr(L::type, CAFE_LIN_BM, BN) | (J.a_kc ? 0u : 1u << 15) | (J.b_kc ? 0u : 1u << 16);
+            const uint64_t da = J.a_kc ? cafe_operand<Sh::rowb>(base) : cafe_operand_mn(base, L::parts * L::BK * 128);
+            const uint64_t db = J.b_kc ? cafe_operand<Sh::rowb>(base + L::parts * Sh::a_part) : cafe_operand_mn(base + L::parts * Sh::a_part, L::parts * L::BK * 128);
+            const uint32_t ap = (J.a_kc ? Sh::a_part : L::BK * 128) >> 4, bp = (J.b_kc ? Sh::b_part : L::BK * 128) >> 4;
+            const uint32_t ak = (J.a_kc ? 32 : 2048) >> 4, bk = (J.b_kc ? 32 : 2048) >> 4;
+            bool fine = true;
+            int64_t u = 0;
+            uint32_t chunks[2] = {0, 0};   // chunks handed over so far, less those that end a tile
+            int n = 0;
+            for (int tile = blockIdx.x; tile < tiles && fine; tile += gridDim.x, ++n) {
+                const int g = n & 1;
+                const uint32_t sums = tmem + g * Sh::tm_set;
+                if (n >= 2 && !(fine = cafe_bar_wait(tile_taken(g), (uint32_t)(n / 2 - 1) & 1u, &bail))) break;
+                for (int t = 0; t < turns; ++t, ++u) {
+                    const int s = (int)(u % Sh::stages);
+                    if (!(fine = cafe_bar_wait(full(s), (uint32_t)(u / Sh::stages) & 1u, &bail))) break;
+                    const bool opens = L::parts == 3 ? t % CAFE_TILES_CHUNK == 0 : t == 0;
+                    if (L::parts == 3 && opens && t > 0) {
+                        if (!(fine = cafe_bar_wait(chunk_taken(g), chunks[g] & 1u, &bail))) break;
+                        ++chunks[g];
+                    }
+                    cafe_tc_after();
+                    const uint64_t a = da + (uint32_t)(s * Sh::stage >> 4), b = db + (uint32_t)(s * Sh::stage >> 4);
+#pragma unroll
+                    for (int k = 0; k < L::BK / 16; ++k) cafe_mma(sums, a + ak * k, b + bk * k, instr, !opens || k > 0);
+                    if constexpr (L::parts == 3) {
+                        if (t % CAFE_TILES_CHUNK == CAFE_TILES_CHUNK - 1 && t < turns - 1) cafe_mma_commit(chunk_full(g));
+#pragma unroll
+                        for (int q = 0; q < 5; ++q) {
+                            constexpr int ia[5] = {0, 1, 1, 0, 2}, ib[5] = {1, 0, 1, 2, 0};
+#pragma unroll
+                            for (int k = 0; k < L::BK / 16; ++k)
+                                cafe_mma(sums + BN, a + ia[q] * ap + ak * k, b + ib[q] * bp + bk * k, instr, t > 0 || q > 0 || k > 0);
+                        }
+                    }
+                    cafe_mma_commit(empty(s));
+                }
+                cafe_mma_commit(tile_full(g));
+            }
+            if (!fine)   // given up: products in flight end before the block does
+                for (int i = 0; i < (1 << 20) && !cafe_bar_try(tile_full(n & 1), (uint32_t)(n / 2) & 1u); ++i) {}
+        }
+    } else {
+        // ---- sums out of tensor memory and out of the block: group g has every other tile, a warp 32 rows of it
+        const int g = (warp - 2) >> 2, rows = (warp & 3) * 32;
+        const uint32_t from = tmem + g * Sh::tm_set + ((uint32_t)rows << 16);
+        const uint32_t mine = base + Sh::stages * Sh::stage + (warp - 2) * Sh::staging;
+        uint32_t chunks = 0;
+        bool fine = true;
+        int n = 0;
+        for (int tile = blockIdx.x + g * gridDim.x; tile < tiles; tile += 2 * gridDim.x, ++n) {
+            const int tm = tile / J.tiles_n, row0 = tm * CAFE_LIN_BM + rows, col0 = (tile - tm * J.tiles_n) * BN;
+            float acc[L::parts == 3 ? BN : 32];
+            if constexpr (L::parts == 3) {
+                auto take = [&](uint32_t at, bool first) {
+#pragma unroll
+                    for (int c = 0; c < BN; c += 16) {
+                        float v[16];
+                        cafe_tm_load16(at + c, v);
+                        cafe_tm_wait_load();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) acc[c + i] = first ? v[i] : acc[c + i] + v[i];
+                    }
+                };
+                const int between = turns > 0 ? (turns - 1) / CAFE_TILES_CHUNK : 0;   // chunks that do not end the tile
+                for (int c = 0; c < between && fine; ++c, ++chunks) {
+                    fine = cafe_bar_wait(chunk_full(g), chunks & 1u, &bail);
+                    cafe_tc_after();
+                    fine = __all_sync(0xffffffffu, fine);
+                    if (fine) take(from, c == 0);
+                    cafe_tc_before();
+                    __syncwarp();
+                    if (lane == 0) cafe_bar_arrive(chunk_taken(g));
+                }
+                if (fine) fine = cafe_bar_wait(tile_full(g), (uint32_t)n & 1u, &bail);
+                cafe_tc_after();
+                fine = __all_sync(0xffffffffu, fine);
+                if (fine) {
+                    take(from, between == 0);
+                    take(from + BN, false);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < BN; ++i) acc[i] = __uint_as_float(0x7fffffffu);
+                }
+                cafe_tc_before();
+                __syncwarp();
+                if (lane == 0) cafe_bar_arrive(tile_taken(g));
+            } else {
+                if (fine) fine = cafe_bar_wait(tile_full(g), (uint32_t)n & 1u, &bail);
+                cafe_tc_after();
+                fine = __all_sync(0xffffffffu, fine);
+            }
+            const int columns = min(BN, J.cols - col0);
+#pragma unroll
+            for (int h = 0; h < BN / 32; ++h) {
+                if (32 * h >= columns) continue;
+                if constexpr (L::parts == 1) {
+                    cafe_tm_load16(from + 32 * h, acc);
+                    cafe_tm_load16(from + 32 * h + 16, acc + 16);
+                    cafe_tm_wait_load();
+                    if (h == BN / 32 - 1 || 32 * (h + 1) >= columns) {   // (the last columns that count have been read)
+                        cafe_tc_before();
+                        __syncwarp();
+                        if (lane == 0) cafe_bar_arrive(tile_taken(g));
+                    }
+                    if (!fine) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) acc[i] = __uint_as_float(0x7fffffffu);
+                    }
+                }
+                __syncwarp();   // the staging rows are free
+                cafe_sums_put<L::parts == 3, 32, true>(J, acc + (L::parts == 3 ? 32 * h : 0), mine + (uint32_t)lane * 128u, row0 + lane, col0 + 32 * h, 0,
+                                                       J.depth, fine, lane & 7);
+                __syncwarp();
+                const int64_t j = col0 + 32 * h + (lane & 7) * 4;
+                if (j < J.cols) {
+                    float bias[4];
+                    cafe_quad_bias<T>(J, j, bias);
+                    const int last = min(32, J.rows - row0);
+#pragma unroll 2
+                    for (int r = lane >> 3; r < last; r += 4) {
+                        float v[4];
+                        asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
+                                     : "r"(mine + (uint32_t)(r * 128 + (((lane ^ r) & 7) << 4))) : "memory");
+                        cafe_quad_end<T>(J, row0 + r, j, v, bias);
+                    }
+                }
+            }
+        }
+        if (!fine) g_tiles_gave_up = 1;
+    }
+    cafe_tc_before();
+    __syncthreads();
+    cafe_tc_after();
+    if (warp == 1) cafe_tm_free(tmem, 2 * Sh::tm_set);
+}
+
 // ---- host ----------------------------------------------------------------------------------------------------------------
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -355,11 +571,20 @@ static bool tiles_map(CUtensorMap* map, const TilesOperand& o, int kc, int box) 
 }
 
 template <typename T, int BN>
-static cudaError_t tiles_launch_bn(CafeTilesArgs& P, const TilesOperand& a, const TilesOperand& b, cudaStream_t st) {
+static cudaError_t tiles_launch_bn(CafeTilesArgs& P, const TilesOperand& a, const TilesOperand& b, bool run, cudaStream_t st) {
     // (a bias gradient alone: no columns, no depth, nothing fetched)
     if (P.job.depth > 0 && (!tiles_map<T>(&P.a, a, P.job.a_kc, CAFE_LIN_BM) || !tiles_map<T>(&P.b, b, P.job.b_kc, BN))) return cudaErrorInvalidValue;
     P.job.tiles_n = P.job.cols > 0 ? (P.job.cols + BN - 1) / BN : 1;
     P.job.tiles = ((P.job.rows + CAFE_LIN_BM - 1) / CAFE_LIN_BM) * P.job.tiles_n;
+    if (run) {
+        constexpr int bytes = CafeRunShape<T, BN>::bytes;
+        static std::atomic<uint64_t> allowed{0};
+        const cudaError_t e = dense_allow_shared((const void*)k_tiles_run<T, BN>, bytes, &allowed);
+        if (e != cudaSuccess) return e;
+        CAFE_PROF(CAFE_P_LINEAR, st);
+        k_tiles_run<T, BN><<<P.job.tiles < 148 ? P.job.tiles : 148, CAFE_RUN_THREADS, bytes, st>>>(P);
+        return cudaGetLastError();
+    }
     constexpr int bytes = CafeTilesShape<T, BN>::bytes;
     static std::atomic<uint64_t> allowed{0};
     const cudaError_t e = dense_allow_shared((const void*)k_tiles<T, BN>, bytes, &allowed);
@@ -377,26 +602,37 @@ static cudaError_t tiles_launch_bn(CafeTilesArgs& P, const TilesOperand& a, cons
     CAFE_PROF(CAFE_P_LINEAR, st);
     return cudaLaunchKernelEx(&cfg, k_tiles<T, BN>, (const CafeTilesArgs&)P);
 }
-// blocks per tile: the fewest rounds for the depth that each has (a block costs 8 turns beside its own; 296, 296, 284 and 264 run
-// at a time in clusters of 1, 2, 4 and 8: what the device says)
+// One block an SM through tile after tile, or two blocks an SM and clusters that share a tile's depth: whichever estimate is less,
+// in turns at the tensor cores' full rate.  A tile costs about 4 turns beside its own when the next one's products run meanwhile,
+// a launch's first and last 12; two blocks on an SM share its tensor cores and cost 12 each, one alone waits for its boxes a third
+// of the time.  296, 296, 284 and 264 blocks run at a
+// time in clusters of 1, 2, 4 and 8 (what the device says).
 template <typename T>
 static cudaError_t tiles_launch(CafeTilesArgs& P, const TilesOperand& a, const TilesOperand& b, cudaStream_t st) {
     typedef CafeTiles<T> L;
     const bool wide = L::parts == 1 && P.job.cols > 128;
     const int bn = wide ? 256 : 128;
-    const int64_t tiles = (int64_t)((P.job.rows + CAFE_LIN_BM - 1) / CAFE_LIN_BM) * ((P.job.cols + bn - 1) / bn);
+    const int64_t tiles = (int64_t)((P.job.rows + CAFE_LIN_BM - 1) / CAFE_LIN_BM) * (P.job.cols > 0 ? (P.job.cols + bn - 1) / bn : 1);
     const int turns = (P.job.depth + L::BK - 1) / L::BK;
     static const int room[4] = {296, 296, 284, 264};
     double best = 1e300;
     for (int s = 0; s < 4; ++s) {
-        const int64_t rounds = ((tiles << s) + room[s] - 1) / room[s];
-        const double est = (double)rounds * (((turns + (1 << s) - 1) >> s) + 8 + s);
+        const int64_t blocks = tiles << s, rounds = (blocks + room[s] - 1) / room[s];
+        const double est = (double)rounds * ((blocks > 148 ? 2.0 : 1.5) * ((turns + (1 << s) - 1) >> s) + 12 + s);
         if (est < best * 0.999) { best = est; P.splits = 1 << s; }
     }
-    if constexpr (L::parts == 1) {
-        if (wide) return tiles_launch_bn<T, 256>(P, a, b, st);
+    const bool run = P.job.depth > 0 && (double)((tiles + 147) / 148) * (turns + 4) + 12 <= best;
+    if (run && P.sums) {   // the bias gradient by itself
+        CafeTilesArgs G = P;
+        G.job.depth = G.job.cols = 0;
+        G.splits = 1;
+        const cudaError_t e = tiles_launch_bn<T, 128>(G, a, b, false, st);
+        if (e != cudaSuccess) return e;
     }
-    return tiles_launch_bn<T, 128>(P, a, b, st);
+    if constexpr (L::parts == 1) {
+        if (wide) return tiles_launch_bn<T, 256>(P, a, b, run, st);
+    }
+    return tiles_launch_bn<T, 128>(P, a, b, run, st);
 }
 
 static int64_t tiles_round(int64_t bytes) { return (bytes + 255) & ~(int64_t)255; }
