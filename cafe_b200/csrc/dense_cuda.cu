@@ -294,33 +294,31 @@ __global__ void __launch_bounds__(CAFE_LIN_THREADS, 1) k_linear(const __grid_con
         bool fine = true;
         for (int c = 0; c < chunks && fine; ++c) {
             if (warp == 8) {
-                if (lane == 0) {
-                    const int end = min(turns, (c + 1) * L::chunk);
-                    if (c > 0) fine = cafe_bar_wait(acc_empty, (uint32_t)(c - 1) & 1u, &bail);
-                    for (int t = c * L::chunk; t < end && fine; ++t) {
-                        const int s = t % Sh::stages;
-                        if (!(fine = cafe_bar_wait(full(s), (uint32_t)(t / Sh::stages) & 1u, &bail))) break;
-                        cafe_tc_after();
-                        const uint32_t a = base + s * Sh::stage, b = a + L::parts * Sh::a_part;
+                const uint32_t lead = lane == 0;
+                const int end = min(turns, (c + 1) * L::chunk);
+                if (c > 0) fine = __all_sync(0xffffffffu, cafe_bar_wait(acc_empty, (uint32_t)(c - 1) & 1u, &bail));
+                for (int t = c * L::chunk; t < end && fine; ++t) {
+                    const int s = t % Sh::stages;
+                    if (!(fine = __all_sync(0xffffffffu, cafe_bar_wait(full(s), (uint32_t)(t / Sh::stages) & 1u, &bail)))) break;
+                    cafe_tc_after();
+                    const uint32_t a = base + s * Sh::stage, b = a + L::parts * Sh::a_part;
 #pragma unroll
-                        for (int k = 0; k < L::BK / 16; ++k)
-                            cafe_mma(tmem, cafe_operand<Sh::rowb>(a + 32 * k), cafe_operand<Sh::rowb>(b + 32 * k), instr, t > c * L::chunk || k > 0);
-                        if (t == end - 1) cafe_mma_commit(acc_full);
-                        if constexpr (L::parts == 3) {
+                    for (int k = 0; k < L::BK / 16; ++k)
+                        cafe_mma(tmem, cafe_operand<Sh::rowb>(a + 32 * k), cafe_operand<Sh::rowb>(b + 32 * k), instr, t > c * L::chunk || k > 0, lead);
+                    if (t == end - 1) cafe_mma_commit(acc_full, lead);
+                    if constexpr (L::parts == 3) {
 #pragma unroll
-                            for (int q = 0; q < 5; ++q) {
-                                constexpr int ia[5] = {0, 1, 1, 0, 2}, ib[5] = {1, 0, 1, 2, 0};
+                        for (int q = 0; q < 5; ++q) {
+                            constexpr int ia[5] = {0, 1, 1, 0, 2}, ib[5] = {1, 0, 1, 2, 0};
 #pragma unroll
-                                for (int k = 0; k < L::BK / 16; ++k)
-                                    cafe_mma(tmem + BN, cafe_operand<Sh::rowb>(a + ia[q] * Sh::a_part + 32 * k),
-                                             cafe_operand<Sh::rowb>(b + ib[q] * Sh::b_part + 32 * k), instr, t > 0 || q > 0 || k > 0);
-                            }
+                            for (int k = 0; k < L::BK / 16; ++k)
+                                cafe_mma(tmem + BN, cafe_operand<Sh::rowb>(a + ia[q] * Sh::a_part + 32 * k),
+                                         cafe_operand<Sh::rowb>(b + ib[q] * Sh::b_part + 32 * k), instr, t > 0 || q > 0 || k > 0, lead);
                         }
-                        cafe_mma_commit(empty(s));
                     }
-                    if (!fine || c == chunks - 1) cafe_mma_commit(all_done);
+                    cafe_mma_commit(empty(s), lead);
                 }
-                fine = __shfl_sync(0xffffffffu, (int)fine, 0);
+                if (!fine || c == chunks - 1) cafe_mma_commit(all_done, lead);
             }
             if (fine) fine = cafe_bar_wait(acc_full, (uint32_t)c & 1u, &bail);
             cafe_tc_after();

@@ -28,7 +28,11 @@ template <typename T> struct CafeTiles {
 };
 template <> struct CafeTiles<__nv_bfloat16> { static constexpr int parts = 1, BK = 64, type = 1; typedef __nv_bfloat16 part; };
 template <> struct CafeTiles<float> { static constexpr int parts = 3, BK = 32, type = 1; typedef __nv_bfloat16 part; };
-#define CAFE_TILES_CHUNK 8     // fp32: turns of 32 between two times that the large sums are taken out
+// fp32: turns of 32 between two times that the large sums are taken out.  The tensor cores cut sums off, 2^-24 of them a turn on
+// average: relative error of 2048 x 512 outputs (norms; signed, all positive operands) over a depth of 512 in one go 1.7e-7, 2.3e-7,
+// of 2048 5.3e-7, 9.9e-7 (in plain fp32 8.1e-7, 7.0e-7), of 8192 in pieces of 256 3.4e-7, 7.0e-7 (1.6e-6, 1.4e-6) and of 65 536
+// in one go 9.4e-6, 3.6e-5.  Products are not issued while sums of a tile are taken out, so short ones go through in one.
+static int tiles_chunk(int turns) { return turns <= 32 ? 32 : turns <= 128 ? 16 : 8; }
 
 // ---- operands as parts ---------------------------------------------------------------------------------------------------
 struct CafePartsJob {
@@ -134,7 +138,7 @@ struct CafeTilesArgs {
     CUtensorMap a, b;
     CafeJob job;
     const float* sums;   // partial column sums of A for job.gb
-    int sum_rows, splits;
+    int sum_rows, splits, chunk;
 };
 
 template <typename T, int BN>
@@ -198,37 +202,40 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
                     for (int i = 0; i < (1 << 20) && !cafe_bar_try(full(u % Sh::stages), (uint32_t)(u / Sh::stages) & 1u); ++i) {}
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            // ---- products
-            const uint32_t instr = cafe_mma_instr(L::type, CAFE_LIN_BM, BN) | (J.a_kc ? 0u : 1u << 15) | (J.b_kc ? 0u : 1u << 16);
-            const uint64_t da = J.a_kc ? cafe_operand<Sh::rowb>(base) : cafe_operand_mn(base, L::parts * L::BK * 128);
-            const uint64_t db = J.b_kc ? cafe_operand<Sh::rowb>(base + L::parts * Sh::a_part) : cafe_operand_mn(base + L::parts * Sh::a_part, L::parts * L::BK * 128);
-            // offsets in 16-byte units: from a part to the next, from 16 k to the next 16
-            const uint32_t ap = (J.a_kc ? Sh::a_part : L::BK * 128) >> 4, bp = (J.b_kc ? Sh::b_part : L::BK * 128) >> 4;
-            const uint32_t ak = (J.a_kc ? 32 : 2048) >> 4, bk = (J.b_kc ? 32 : 2048) >> 4;
-            for (int t = 0; t < turns; ++t) {
-                const int s = t % Sh::stages;
-                if (!(fine = cafe_bar_wait(full(s), (uint32_t)(t / Sh::stages) & 1u, &bail))) break;
-                const bool opens = L::parts == 3 ? t % CAFE_TILES_CHUNK == 0 : t == 0;
-                if (L::parts == 3 && opens && t > 0 && !(fine = cafe_bar_wait(acc_empty, (uint32_t)(t / CAFE_TILES_CHUNK - 1) & 1u, &bail))) break;
-                cafe_tc_after();
-                const uint64_t a = da + (uint32_t)(s * Sh::stage >> 4), b = db + (uint32_t)(s * Sh::stage >> 4);
-#pragma unroll
-                for (int k = 0; k < L::BK / 16; ++k) cafe_mma(tmem, a + ak * k, b + bk * k, instr, !opens || k > 0);
-                if constexpr (L::parts == 3) {
-                    if (t % CAFE_TILES_CHUNK == CAFE_TILES_CHUNK - 1 || t == turns - 1) cafe_mma_commit(acc_full);
-#pragma unroll
-                    for (int q = 0; q < 5; ++q) {
-                        constexpr int ia[5] = {0, 1, 1, 0, 2}, ib[5] = {1, 0, 1, 2, 0};
-#pragma unroll
-                        for (int k = 0; k < L::BK / 16; ++k)
-                            cafe_mma(tmem + BN, a + ia[q] * ap + ak * k, b + ib[q] * bp + bk * k, instr, t > 0 || q > 0 || k > 0);
-                    }
-                }
-                cafe_mma_commit(empty(s));
+        // ---- products
+        const uint32_t lead = lane == 0;
+        const uint32_t instr = cafe_mma_instr(L::type, CAFE_LIN_BM, BN) | (J.a_kc ? 0u : 1u << 15) | (J.b_kc ? 0u : 1u << 16);
+        const uint64_t da = J.a_kc ? cafe_operand<Sh::rowb>(base) : cafe_operand_mn(base, L::parts * L::BK * 128);
+        const uint64_t db = J.b_kc ? cafe_operand<Sh::rowb>(base + L::parts * Sh::a_part) : cafe_operand_mn(base + L::parts * Sh::a_part, L::parts * L::BK * 128);
+        // offsets in 16-byte units: from a part to the next, from 16 k to the next 16
+        const uint32_t ap = (J.a_kc ? Sh::a_part : L::BK * 128) >> 4, bp = (J.b_kc ? Sh::b_part : L::BK * 128) >> 4;
+        const uint32_t ak = (J.a_kc ? 32 : 2048) >> 4, bk = (J.b_kc ? 32 : 2048) >> 4;
+        int s = 0, in_chunk = 0;
+        uint32_t phase = 0, chunk_phase = 1;
+        for (int t = 0; t < turns; ++t) {
+            if (!(fine = __all_sync(0xffffffffu, cafe_bar_wait(full(s), phase, &bail)))) break;
+            if (L::parts == 3 && in_chunk == 0 && t > 0) {
+                if (!(fine = __all_sync(0xffffffffu, cafe_bar_wait(acc_empty, chunk_phase & 1u, &bail)))) break;
             }
-            cafe_mma_commit(all_done);
+            cafe_tc_after();
+            const uint64_t a = da + (uint32_t)(s * Sh::stage >> 4), b = db + (uint32_t)(s * Sh::stage >> 4);
+#pragma unroll
+            for (int k = 0; k < L::BK / 16; ++k) cafe_mma(tmem, a + ak * k, b + bk * k, instr, in_chunk > 0 || k > 0, lead);
+            ++in_chunk;
+            if constexpr (L::parts == 3) {
+                if (in_chunk == P.chunk || t == turns - 1) { cafe_mma_commit(acc_full, lead); in_chunk = 0; ++chunk_phase; }
+#pragma unroll
+                for (int q = 0; q < 5; ++q) {
+                    constexpr int ia[5] = {0, 1, 1, 0, 2}, ib[5] = {1, 0, 1, 2, 0};
+#pragma unroll
+                    for (int k = 0; k < L::BK / 16; ++k)
+                        cafe_mma(tmem + BN, a + ia[q] * ap + ak * k, b + ib[q] * bp + bk * k, instr, t > 0 || q > 0 || k > 0, lead);
+                }
+            }
+            cafe_mma_commit(empty(s), lead);
+            if (++s == Sh::stages) { s = 0; phase ^= 1u; }
         }
+        cafe_mma_commit(all_done, lead);
     } else {
         // ---- sums out of tensor memory, 32 rows a warp; before that the bias gradient from its partial sums
         if (P.sums && tn == 0 && rank == 0) {
@@ -258,7 +265,7 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
                     for (int i = 0; i < 16; ++i) acc[c + i] = first ? v[i] : acc[c + i] + v[i];
                 }
             };
-            const int chunks = (turns + CAFE_TILES_CHUNK - 1) / CAFE_TILES_CHUNK;
+            const int chunks = (turns + P.chunk - 1) / P.chunk;
             if (turns == 0) {
 #pragma unroll
                 for (int i = 0; i < BN; ++i) acc[i] = 0.f;
@@ -325,16 +332,16 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
 // ---- tiles one after the other ---------------------------------------------------------------------------------------------
 // The same products where there are tiles enough for every SM: one block an SM works through tile after tile, and two groups of
 // four warps take turns with tensor memory's two sets of sums, so that one tile is finished and stored while the next one's products
-// run.  Each warp stages its own 32 rows, 32 columns at a time, and writes them out row by row: nobody waits for anybody there.
-// Four stages of 48 KB: with three the products wait for their boxes (fp32 gx of 65536x1024x480 505 us, with two blocks of two stages
-// an SM 470).
+// run.  Each warp stages its own 32 rows, 32 or 64 columns at a time, and writes them out row by row: nobody waits for anybody there.
+// A row's piece of a pass is 128 bytes of fp32 or of 16-bit output (64 bytes of bf16 cost the 16384x1024x4096 forward 30 us of 159);
+// the stages of 48 KB get what is left, four and three.
 #define CAFE_RUN_THREADS 320
 template <typename T, int BN> struct CafeRunShape {
     typedef CafeTiles<T> L;
     static constexpr int rowb = L::BK * 2;
     static constexpr int a_part = CAFE_LIN_BM * rowb, b_part = BN * rowb, stage = L::parts * (a_part + b_part);
-    static constexpr int stages = 196608 / stage < 6 ? 196608 / stage : 6;
-    static constexpr int staging = 32 * 32 * 4;   // a warp's rows, 32 columns; pieces of four exchanged by row
+    static constexpr int cols = L::parts == 3 ? 32 : 64, staging = 32 * cols * 4;   // of a pass; pieces of four exchanged by row
+    static constexpr int room = 229376 - 8 * staging, stages = room / stage < 6 ? room / stage : 6;
     static constexpr int bytes = stage * stages + 8 * staging + 1024;
     static constexpr int tm_set = L::parts == 3 ? 2 * BN : BN;
 };
@@ -399,50 +406,52 @@ __global__ void __launch_bounds__(CAFE_RUN_THREADS, 1) k_tiles_run(const __grid_
                     for (int i = 0; i < (1 << 20) && !cafe_bar_try(full((int)(v % Sh::stages)), (uint32_t)(v / Sh::stages) & 1u); ++i) {}
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            // ---- products
-            const uint32_t instr = cafe_mma_instr(L::type, CAFE_LIN_BM, BN) | (J.a_kc ? 0u : 1u << 15) | (J.b_kc ? 0u : 1u << 16);
-            const uint64_t da = J.a_kc ? cafe_operand<Sh::rowb>(base) : cafe_operand_mn(base, L::parts * L::BK * 128);
-            const uint64_t db = J.b_kc ? cafe_operand<Sh::rowb>(base + L::parts * Sh::a_part) : cafe_operand_mn(base + L::parts * Sh::a_part, L::parts * L::BK * 128);
-            const uint32_t ap = (J.a_kc ? Sh::a_part : L::BK * 128) >> 4, bp = (J.b_kc ? Sh::b_part : L::BK * 128) >> 4;
-            const uint32_t ak = (J.a_kc ? 32 : 2048) >> 4, bk = (J.b_kc ? 32 : 2048) >> 4;
-            bool fine = true;
-            int64_t u = 0;
-            uint32_t chunks[2] = {0, 0};   // chunks handed over so far, less those that end a tile
-            int n = 0;
-            for (int tile = blockIdx.x; tile < tiles && fine; tile += gridDim.x, ++n) {
-                const int g = n & 1;
-                const uint32_t sums = tmem + g * Sh::tm_set;
-                if (n >= 2 && !(fine = cafe_bar_wait(tile_taken(g), (uint32_t)(n / 2 - 1) & 1u, &bail))) break;
-                for (int t = 0; t < turns; ++t, ++u) {
-                    const int s = (int)(u % Sh::stages);
-                    if (!(fine = cafe_bar_wait(full(s), (uint32_t)(u / Sh::stages) & 1u, &bail))) break;
-                    const bool opens = L::parts == 3 ? t % CAFE_TILES_CHUNK == 0 : t == 0;
-                    if (L::parts == 3 && opens && t > 0) {
-                        if (!(fine = cafe_bar_wait(chunk_taken(g), chunks[g] & 1u, &bail))) break;
-                        ++chunks[g];
-                    }
-                    cafe_tc_after();
-                    const uint64_t a = da + (uint32_t)(s * Sh::stage >> 4), b = db + (uint32_t)(s * Sh::stage >> 4);
-#pragma unroll
-                    for (int k = 0; k < L::BK / 16; ++k) cafe_mma(sums, a + ak * k, b + bk * k, instr, !opens || k > 0);
-                    if constexpr (L::parts == 3) {
-                        if (t % CAFE_TILES_CHUNK == CAFE_TILES_CHUNK - 1 && t < turns - 1) cafe_mma_commit(chunk_full(g));
-#pragma unroll
-                        for (int q = 0; q < 5; ++q) {
-                            constexpr int ia[5] = {0, 1, 1, 0, 2}, ib[5] = {1, 0, 1, 2, 0};
-#pragma unroll
-                            for (int k = 0; k < L::BK / 16; ++k)
-                                cafe_mma(sums + BN, a + ia[q] * ap + ak * k, b + ib[q] * bp + bk * k, instr, t > 0 || q > 0 || k > 0);
-                        }
-                    }
-                    cafe_mma_commit(empty(s));
+        // ---- products
+        const uint32_t lead = lane == 0;
+        const uint32_t instr = cafe_mma_instr(L::type, CAFE_LIN_BM, BN) | (J.a_kc ? 0u : 1u << 15) | (J.b_kc ? 0u : 1u << 16);
+        const uint64_t da = J.a_kc ? cafe_operand<Sh::rowb>(base) : cafe_operand_mn(base, L::parts * L::BK * 128);
+        const uint64_t db = J.b_kc ? cafe_operand<Sh::rowb>(base + L::parts * Sh::a_part) : cafe_operand_mn(base + L::parts * Sh::a_part, L::parts * L::BK * 128);
+        const uint32_t ap = (J.a_kc ? Sh::a_part : L::BK * 128) >> 4, bp = (J.b_kc ? Sh::b_part : L::BK * 128) >> 4;
+        const uint32_t ak = (J.a_kc ? 32 : 2048) >> 4, bk = (J.b_kc ? 32 : 2048) >> 4;
+        bool fine = true;
+        int s = 0, n = 0;
+        uint32_t phase = 0, chunk_phases = 0;   // (bit g: parity of the chunks of set g that were handed over, less those that end a tile)
+        for (int tile = blockIdx.x; tile < tiles && fine; tile += gridDim.x, ++n) {
+            const int g = n & 1;
+            const uint32_t sums = tmem + g * Sh::tm_set;
+            if (n >= 2 && !(fine = __all_sync(0xffffffffu, cafe_bar_wait(tile_taken(g), (uint32_t)(n / 2 - 1) & 1u, &bail)))) break;
+            int in_chunk = 0;
+            for (int t = 0; t < turns; ++t) {
+                if (!(fine = __all_sync(0xffffffffu, cafe_bar_wait(full(s), phase, &bail)))) break;
+                if (L::parts == 3 && in_chunk == 0 && t > 0) {
+                    if (!(fine = __all_sync(0xffffffffu, cafe_bar_wait(chunk_taken(g), chunk_phases >> g & 1u, &bail)))) break;
+                    chunk_phases ^= 1u << g;
                 }
-                cafe_mma_commit(tile_full(g));
+                cafe_tc_after();
+                const uint64_t a = da + (uint32_t)(s * Sh::stage >> 4), b = db + (uint32_t)(s * Sh::stage >> 4);
+#pragma unroll
+                for (int k = 0; k < L::BK / 16; ++k) cafe_mma(sums, a + ak * k, b + bk * k, instr, in_chunk > 0 || k > 0, lead);
+                ++in_chunk;
+                if constexpr (L::parts == 3) {
+                    if (in_chunk == P.chunk) {
+                        if (t < turns - 1) cafe_mma_commit(chunk_full(g), lead);
+                        in_chunk = 0;
+                    }
+#pragma unroll
+                    for (int q = 0; q < 5; ++q) {
+                        constexpr int ia[5] = {0, 1, 1, 0, 2}, ib[5] = {1, 0, 1, 2, 0};
+#pragma unroll
+                        for (int k = 0; k < L::BK / 16; ++k)
+                            cafe_mma(sums + BN, a + ia[q] * ap + ak * k, b + ib[q] * bp + bk * k, instr, t > 0 || q > 0 || k > 0, lead);
+                    }
+                }
+                cafe_mma_commit(empty(s), lead);
+                if (++s == Sh::stages) { s = 0; phase ^= 1u; }
             }
-            if (!fine)   // given up: products in flight end before the block does
-                for (int i = 0; i < (1 << 20) && !cafe_bar_try(tile_full(n & 1), (uint32_t)(n / 2) & 1u); ++i) {}
+            cafe_mma_commit(tile_full(g), lead);
         }
+        if (!fine)   // given up: products in flight end before the block does
+            for (int i = 0; i < (1 << 20) && !cafe_bar_try(tile_full(n & 1), (uint32_t)(n / 2) & 1u); ++i) {}
     } else {
         // ---- sums out of tensor memory and out of the block: group g has every other tile, a warp 32 rows of it
         const int g = (warp - 2) >> 2, rows = (warp & 3) * 32;
@@ -453,7 +462,8 @@ __global__ void __launch_bounds__(CAFE_RUN_THREADS, 1) k_tiles_run(const __grid_
         int n = 0;
         for (int tile = blockIdx.x + g * gridDim.x; tile < tiles; tile += 2 * gridDim.x, ++n) {
             const int tm = tile / J.tiles_n, row0 = tm * CAFE_LIN_BM + rows, col0 = (tile - tm * J.tiles_n) * BN;
-            float acc[L::parts == 3 ? BN : 32];
+            constexpr int W = Sh::cols;
+            float acc[L::parts == 3 ? BN : W];
             if constexpr (L::parts == 3) {
                 auto take = [&](uint32_t at, bool first) {
 #pragma unroll
@@ -465,7 +475,7 @@ __global__ void __launch_bounds__(CAFE_RUN_THREADS, 1) k_tiles_run(const __grid_
                         for (int i = 0; i < 16; ++i) acc[c + i] = first ? v[i] : acc[c + i] + v[i];
                     }
                 };
-                const int between = turns > 0 ? (turns - 1) / CAFE_TILES_CHUNK : 0;   // chunks that do not end the tile
+                const int between = turns > 0 ? (turns - 1) / P.chunk : 0;   // chunks that do not end the tile
                 for (int c = 0; c < between && fine; ++c, ++chunks) {
                     fine = cafe_bar_wait(chunk_full(g), chunks & 1u, &bail);
                     cafe_tc_after();
@@ -495,36 +505,38 @@ __global__ void __launch_bounds__(CAFE_RUN_THREADS, 1) k_tiles_run(const __grid_
             }
             const int columns = min(BN, J.cols - col0);
 #pragma unroll
-            for (int h = 0; h < BN / 32; ++h) {
-                if (32 * h >= columns) continue;
+            for (int h = 0; h < BN / W; ++h) {
+                if (W * h >= columns) continue;
                 if constexpr (L::parts == 1) {
-                    cafe_tm_load16(from + 32 * h, acc);
-                    cafe_tm_load16(from + 32 * h + 16, acc + 16);
+#pragma unroll
+                    for (int c = 0; c < W; c += 16) cafe_tm_load16(from + W * h + c, acc + c);
                     cafe_tm_wait_load();
-                    if (h == BN / 32 - 1 || 32 * (h + 1) >= columns) {   // (the last columns that count have been read)
+                    if (h == BN / W - 1 || W * (h + 1) >= columns) {   // (the last columns that count have been read)
                         cafe_tc_before();
                         __syncwarp();
                         if (lane == 0) cafe_bar_arrive(tile_taken(g));
                     }
                     if (!fine) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) acc[i] = __uint_as_float(0x7fffffffu);
+                        for (int i = 0; i < W; ++i) acc[i] = __uint_as_float(0x7fffffffu);
                     }
                 }
                 __syncwarp();   // the staging rows are free
-                cafe_sums_put<L::parts == 3, 32, true>(J, acc + (L::parts == 3 ? 32 * h : 0), mine + (uint32_t)lane * 128u, row0 + lane, col0 + 32 * h, 0,
-                                                       J.depth, fine, lane & 7);
+                cafe_sums_put<L::parts == 3, W, true>(J, acc + (L::parts == 3 ? W * h : 0), mine + (uint32_t)lane * (W * 4), row0 + lane, col0 + W * h, 0,
+                                                      J.depth, fine, lane & 7);
                 __syncwarp();
-                const int64_t j = col0 + 32 * h + (lane & 7) * 4;
+                constexpr int lanes = W / 4;   // to a row
+                const int q = lane % lanes;
+                const int64_t j = col0 + W * h + q * 4;
                 if (j < J.cols) {
                     float bias[4];
                     cafe_quad_bias<T>(J, j, bias);
                     const int last = min(32, J.rows - row0);
 #pragma unroll 2
-                    for (int r = lane >> 3; r < last; r += 4) {
+                    for (int r = lane / lanes; r < last; r += 32 / lanes) {
                         float v[4];
                         asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
-                                     : "r"(mine + (uint32_t)(r * 128 + (((lane ^ r) & 7) << 4))) : "memory");
+                                     : "r"(mine + (uint32_t)(r * (W * 4) + ((q ^ (r & 7)) << 4))) : "memory");
                         cafe_quad_end<T>(J, row0 + r, j, v, bias);
                     }
                 }
@@ -577,6 +589,7 @@ static cudaError_t tiles_launch_bn(CafeTilesArgs& P, const TilesOperand& a, cons
     P.job.tiles_n = P.job.cols > 0 ? (P.job.cols + BN - 1) / BN : 1;
     P.job.tiles = ((P.job.rows + CAFE_LIN_BM - 1) / CAFE_LIN_BM) * P.job.tiles_n;
     if (run) {
+        P.chunk = tiles_chunk((P.job.depth + CafeTiles<T>::BK - 1) / CafeTiles<T>::BK);
         constexpr int bytes = CafeRunShape<T, BN>::bytes;
         static std::atomic<uint64_t> allowed{0};
         const cudaError_t e = dense_allow_shared((const void*)k_tiles_run<T, BN>, bytes, &allowed);
@@ -585,6 +598,7 @@ static cudaError_t tiles_launch_bn(CafeTilesArgs& P, const TilesOperand& a, cons
         k_tiles_run<T, BN><<<P.job.tiles < 148 ? P.job.tiles : 148, CAFE_RUN_THREADS, bytes, st>>>(P);
         return cudaGetLastError();
     }
+    P.chunk = tiles_chunk(((P.job.depth + CafeTiles<T>::BK - 1) / CafeTiles<T>::BK + P.splits - 1) / P.splits);
     constexpr int bytes = CafeTilesShape<T, BN>::bytes;
     static std::atomic<uint64_t> allowed{0};
     const cudaError_t e = dense_allow_shared((const void*)k_tiles<T, BN>, bytes, &allowed);

@@ -44,12 +44,16 @@ __device__ __forceinline__ void cafe_tm_load16(uint32_t at, float* v) {
                  : "r"(at));
 }
 
-// D[128 x N] (+)= A[128 x 16] B[N x 16]^T, operands in shared memory (descriptors), D in tensor memory
-__device__ __forceinline__ void cafe_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(instr), "r"((uint32_t)add) : "memory");
+// D[128 x N] (+)= A[128 x 16] B[N x 16]^T, operands in shared memory (descriptors), D in tensor memory.  Called by a whole warp,
+// issued by the lane that leads: what the warp has in common stays in uniform registers, where the instruction wants it (from one
+// lane's branch every descriptor is moved there first, and 12 products of 64 cycles a turn then wait for their issue).
+__device__ __forceinline__ void cafe_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool add, uint32_t lead) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(instr), "r"((uint32_t)add), "r"(lead) : "memory");
 }
-// the barrier's next arrival: when all products issued so far by this thread are done
-__device__ __forceinline__ void cafe_mma_commit(uint32_t bar) { asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory"); }
+// the barrier's next arrival: when all products issued so far by this lane are done
+__device__ __forceinline__ void cafe_mma_commit(uint32_t bar, uint32_t lead) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(lead) : "memory");
+}
 
 // Rows of ROWB = 64 or 128 bytes, K contiguous, one behind the other; the 16-byte pieces of a row are exchanged by
 // cafe_swizzle.  Eight rows are a unit.
