@@ -43,15 +43,20 @@ template <bool FAST> __device__ __forceinline__ float cafe_act(float z, int act,
         default: *slope = 1.f; return z;
     }
 }
-// four at a time: z becomes act(z), d its derivative
-template <bool FAST> __device__ __forceinline__ void cafe_act4(float* z, int act, float* d) {
-    if (act == CAFE_ACT_NONE) {
+// N at a time: z becomes act(z), d its derivative
+template <bool FAST, int N> __device__ __forceinline__ void cafe_act_all(float* z, int act, float* d) {
+#define CAFE_ACT_CASE(A) case A: { _Pragma("unroll") for (int q = 0; q < N; ++q) z[q] = cafe_act<FAST>(z[q], A, d + q); break; }
+    switch (act) {
+        CAFE_ACT_CASE(CAFE_ACT_RELU)
+        CAFE_ACT_CASE(CAFE_ACT_SIGMOID)
+        CAFE_ACT_CASE(CAFE_ACT_GELU)
+        CAFE_ACT_CASE(CAFE_ACT_SILU)
+        default: {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) d[q] = 1.f;
-        return;
+            for (int q = 0; q < N; ++q) d[q] = 1.f;
+        }
     }
-#pragma unroll
-    for (int q = 0; q < 4; ++q) z[q] = cafe_act<FAST>(z[q], act, d + q);
+#undef CAFE_ACT_CASE
 }
 
 // the derivative kept for the backward, always finer than the type it multiplies, so that gz's own rounding stays the only
@@ -67,7 +72,8 @@ struct CafeJob {
     int tiles_n, tiles;
     const void *bias, *res;
     int64_t ldr, ldo, lds;
-    int act, out_vec, res_vec;
+    int act, out_vec, res_vec;              // 16-byte stores of four outputs (and slopes), loads of four of the residual; ..
+    int out_row, slope_row, res_row;        // .. rows on 16 bytes
     void *out, *slope_out, *gb;             // gb: sums over k of A(i, k), by the blocks of the first column of tiles
 };
 struct CafeJobs {
@@ -96,57 +102,56 @@ static __device__ __noinline__ float cafe_plain_dot(const CafeJob& J, int64_t i,
 
 // ---- the end of a product --------------------------------------------------------------------------------------------
 // A thread's 4 * QUADS consecutive columns of row r of the block's sums to shared memory; a NaN of split operands is looked into.
-// EXCHANGED: the 16-byte pieces of a row (128 bytes) are exchanged by `x`.
-template <bool SPLIT, int N, bool EXCHANGED = false>
-__device__ __forceinline__ void cafe_sums_put(const CafeJob& J, const float* acc, uint32_t at, int64_t row, int64_t col, int k0, int k1, bool look, int x = 0) {
+template <bool SPLIT, int N>
+__device__ __forceinline__ void cafe_sums_put(const CafeJob& J, const float* acc, uint32_t at, int64_t row, int64_t col, int k0, int k1, bool look) {
     bool nan = false;
-    auto place = [&](int c) { return at + (EXCHANGED ? (uint32_t)((((c >> 2) ^ x) << 4) + 4 * (c & 3)) : 4u * c); };
 #pragma unroll
     for (int c = 0; c < N; c += 4) {
-        cafe_put16(place(c), __float_as_uint(acc[c]), __float_as_uint(acc[c + 1]), __float_as_uint(acc[c + 2]), __float_as_uint(acc[c + 3]));
+        cafe_put16(at + 4 * c, __float_as_uint(acc[c]), __float_as_uint(acc[c + 1]), __float_as_uint(acc[c + 2]), __float_as_uint(acc[c + 3]));
         if (SPLIT) nan |= !(acc[c] == acc[c]) | !(acc[c + 1] == acc[c + 1]) | !(acc[c + 2] == acc[c + 2]) | !(acc[c + 3] == acc[c + 3]);
     }
     if (SPLIT && nan && look && row < J.rows)
         for (int c = 0; c < N && col + c < J.cols; ++c) {
             float v;
-            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(place(c)) : "memory");
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at + 4 * c) : "memory");
             if (v != v) {
                 v = cafe_plain_dot(J, row, col + c, k0, k1);
-                asm volatile("st.shared.f32 [%0], %1;" ::"r"(place(c)), "f"(v) : "memory");
+                asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + 4 * c), "f"(v) : "memory");
             }
         }
 }
+// Four neighbouring elements of the residual (row i, columns j ..), as they lie.
+template <typename T> struct CafeQuad { alignas(4 * sizeof(T)) T v[4]; };
+template <typename T>
+__device__ __forceinline__ void cafe_quad_residual(const CafeJob& J, int64_t i, int64_t j, CafeQuad<T>& x) {
+    const T* p = static_cast<const T*>(J.res) + i * J.ldr + j;
+    const int n = (int)min((int64_t)4, J.cols - j);
+    if (J.res_vec && n == 4) {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(x.v) = __ldg(reinterpret_cast<const uint4*>(p));
+        else *reinterpret_cast<uint2*>(x.v) = __ldg(reinterpret_cast<const uint2*>(p));
+    } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) x.v[q] = q < n ? __ldg(p + q) : cafe_from_float<T>(0.f);
+    }
+}
 // Four neighbouring outputs (row i, columns j ..): bias, activation, residual, rounding, stores.
 template <typename T>
-__device__ __forceinline__ void cafe_quad_end(const CafeJob& J, int64_t i, int64_t j, const float* v, const float* bias) {
+__device__ __forceinline__ void cafe_quad_end(const CafeJob& J, int64_t i, int64_t j, const float* v, const float* bias, const CafeQuad<T>& res) {
     typedef typename CafeSlopeOf<T>::type ST;
     const int n = (int)min((int64_t)4, J.cols - j);
     const bool vec = J.out_vec && n == 4;
-    float res[4] = {0.f, 0.f, 0.f, 0.f};
-    if (J.res) {
-        const T* p = static_cast<const T*>(J.res) + i * J.ldr + j;
-        if (J.res_vec && n == 4) {
-            alignas(16) T x[4];
-            if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(x) = __ldg(reinterpret_cast<const uint4*>(p));
-            else *reinterpret_cast<uint2*>(x) = __ldg(reinterpret_cast<const uint2*>(p));
-#pragma unroll
-            for (int q = 0; q < 4; ++q) res[q] = cafe_to_float(x[q]);
-        } else {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) if (q < n) res[q] = cafe_to_float(__ldg(p + q));
-        }
-    }
     alignas(16) T o[4];
     alignas(16) ST sl[4];
     float z[4], d[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) z[q] = v[q] + bias[q];
-    cafe_act4<sizeof(T) == 2>(z, J.act, d);
+    cafe_act_all<sizeof(T) == 2, 4>(z, J.act, d);
+    if (J.res) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        o[q] = cafe_from_float<T>(z[q] + res[q]);
-        sl[q] = cafe_from_float<ST>(d[q]);
+        for (int q = 0; q < 4; ++q) z[q] += cafe_to_float(res.v[q]);
     }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) o[q] = cafe_from_float<T>(z[q]);
     T* out = static_cast<T*>(J.out) + i * J.ldo + j;
     if (vec) {
         if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(o);
@@ -156,6 +161,8 @@ __device__ __forceinline__ void cafe_quad_end(const CafeJob& J, int64_t i, int64
         for (int q = 0; q < 4; ++q) if (q < n) out[q] = o[q];
     }
     if (J.slope_out) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) sl[q] = cafe_from_float<ST>(d[q]);
         ST* so = static_cast<ST*>(J.slope_out) + i * J.lds + j;
         if (vec) {
             if constexpr (sizeof(ST) == 4) *reinterpret_cast<uint4*>(so) = *reinterpret_cast<const uint4*>(sl);
@@ -192,7 +199,9 @@ __device__ __forceinline__ void cafe_finish_of(const CafeJob& J, uint32_t base, 
         }
         float bias[4];
         cafe_quad_bias<T>(J, j, bias);
-        cafe_quad_end<T>(J, i, j, v, bias);
+        CafeQuad<T> res;
+        if (J.res) cafe_quad_residual<T>(J, i, j, res);
+        cafe_quad_end<T>(J, i, j, v, bias, res);
     }
 }
 template <typename T, int COLS>

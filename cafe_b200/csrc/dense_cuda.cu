@@ -572,6 +572,9 @@ static cudaError_t dense_forward(const CafeForward& f, int dtype, void* work, in
     J.bias = f.bias; J.res = f.res; J.ldr = f.ldr; J.act = f.act; J.out = f.y; J.ldo = f.ldy; J.slope_out = f.slope; J.lds = f.lds;
     const int ssize = sizeof(typename CafeSlopeOf<T>::type);
     J.res_vec = f.res && dense_on(f.res, f.ldr, size, 4 * size);
+    J.out_row = dense_on(f.y, f.ldy, size, 16);
+    J.res_row = f.res && dense_on(f.res, f.ldr, size, 16);
+    J.slope_row = f.slope && dense_on(f.slope, f.lds, sizeof(typename CafeSlopeOf<T>::type), 16);
     J.out_vec = dense_on(f.y, f.ldy, size, 4 * size) && (!f.slope || dense_on(f.slope, f.lds, ssize, 4 * ssize));
     const int64_t need = cafe_tiles_forward_work(f, dtype);
     if (need > 0 && work && work_bytes >= need) return cafe_tiles_forward(f, dtype, J, work, st);
@@ -588,14 +591,14 @@ static cudaError_t dense_backward(const CafeBackward& f, int dtype, void* work, 
         J.a = f.gy; J.lda = f.ldg; J.a_vec = g_vec; J.as = f.slope; J.ldas = f.lds; J.as_vec = s_vec; J.slope_kind = f.slope_kind;
         J.b = f.x; J.ldb = f.ldx;
         J.rows = f.N; J.cols = f.gw ? f.K : 0; J.depth = f.M;
-        J.out = f.gw; J.ldo = f.ldgw; J.out_vec = dense_on(f.gw, f.ldgw, size, 4 * size); J.gb = f.gb;
+        J.out = f.gw; J.ldo = f.ldgw; J.out_vec = dense_on(f.gw, f.ldgw, size, 4 * size); J.out_row = dense_on(f.gw, f.ldgw, size, 16); J.gb = f.gb;
     }
     if (f.gx && f.M > 0 && f.K > 0) {
         CafeJob& J = P.job[P.count++];
         J.a = f.gy; J.lda = f.ldg; J.a_kc = 1; J.a_vec = g_vec; J.as = f.slope; J.ldas = f.lds; J.as_vec = s_vec; J.slope_kind = f.slope_kind;
         J.b = f.w; J.ldb = f.ldw;
         J.rows = f.M; J.cols = f.K; J.depth = f.N;
-        J.out = f.gx; J.ldo = f.ldgx; J.out_vec = dense_on(f.gx, f.ldgx, size, 4 * size);
+        J.out = f.gx; J.ldo = f.ldgx; J.out_vec = dense_on(f.gx, f.ldgx, size, 4 * size); J.out_row = dense_on(f.gx, f.ldgx, size, 16);
     }
     const int64_t need = cafe_tiles_backward_work(f, dtype);
     if (need > 0 && work && work_bytes >= need)

@@ -29,10 +29,10 @@ template <typename T> struct CafeTiles {
 template <> struct CafeTiles<__nv_bfloat16> { static constexpr int parts = 1, BK = 64, type = 1; typedef __nv_bfloat16 part; };
 template <> struct CafeTiles<float> { static constexpr int parts = 3, BK = 32, type = 1; typedef __nv_bfloat16 part; };
 // fp32: turns of 32 between two times that the large sums are taken out.  The tensor cores cut sums off, 2^-24 of them a turn on
-// average: relative error of 2048 x 512 outputs (norms; signed, all positive operands) over a depth of 512 in one go 1.7e-7, 2.3e-7,
-// of 2048 5.3e-7, 9.9e-7 (in plain fp32 8.1e-7, 7.0e-7), of 8192 in pieces of 256 3.4e-7, 7.0e-7 (1.6e-6, 1.4e-6) and of 65 536
-// in one go 9.4e-6, 3.6e-5.  Products are not issued while sums of a tile are taken out, so short ones go through in one.
-static int tiles_chunk(int turns) { return turns <= 32 ? 32 : turns <= 128 ? 16 : 8; }
+// average: relative error (norms; signed, all positive operands) of a depth of 2048 in one go 5.3e-7, 9.9e-7, in pieces of 256
+// 2.9e-7, 4.8e-7 (in plain fp32 8.1e-7, 7.0e-7); of 65 536 in one go 9.4e-6, 3.6e-5, in pieces 5.5e-7, 1.6e-6.  Pieces of 1024
+// were not measurably faster.
+#define CAFE_TILES_CHUNK 8
 
 // ---- operands as parts ---------------------------------------------------------------------------------------------------
 struct CafePartsJob {
@@ -138,7 +138,7 @@ struct CafeTilesArgs {
     CUtensorMap a, b;
     CafeJob job;
     const float* sums;   // partial column sums of A for job.gb
-    int sum_rows, splits, chunk;
+    int sum_rows, splits;
 };
 
 template <typename T, int BN>
@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
             for (int k = 0; k < L::BK / 16; ++k) cafe_mma(tmem, a + ak * k, b + bk * k, instr, in_chunk > 0 || k > 0, lead);
             ++in_chunk;
             if constexpr (L::parts == 3) {
-                if (in_chunk == P.chunk || t == turns - 1) { cafe_mma_commit(acc_full, lead); in_chunk = 0; ++chunk_phase; }
+                if (in_chunk == CAFE_TILES_CHUNK || t == turns - 1) { cafe_mma_commit(acc_full, lead); in_chunk = 0; ++chunk_phase; }
 #pragma unroll
                 for (int q = 0; q < 5; ++q) {
                     constexpr int ia[5] = {0, 1, 1, 0, 2}, ib[5] = {1, 0, 1, 2, 0};
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
                     for (int i = 0; i < 16; ++i) acc[c + i] = first ? v[i] : acc[c + i] + v[i];
                 }
             };
-            const int chunks = (turns + P.chunk - 1) / P.chunk;
+            const int chunks = (turns + CAFE_TILES_CHUNK - 1) / CAFE_TILES_CHUNK;
             if (turns == 0) {
 #pragma unroll
                 for (int i = 0; i < BN; ++i) acc[i] = 0.f;
@@ -332,19 +332,66 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
 // ---- tiles one after the other ---------------------------------------------------------------------------------------------
 // The same products where there are tiles enough for every SM: one block an SM works through tile after tile, and two groups of
 // four warps take turns with tensor memory's two sets of sums, so that one tile is finished and stored while the next one's products
-// run.  Each warp stages its own 32 rows, 32 or 64 columns at a time, and writes them out row by row: nobody waits for anybody there.
-// A row's piece of a pass is 128 bytes of fp32 or of 16-bit output (64 bytes of bf16 cost the 16384x1024x4096 forward 30 us of 159);
-// the stages of 48 KB get what is left, four and three.
+// run.  A lane has a row: it takes sixteen of its sums at a time out of tensor memory (fp32: where it has put them back, complete),
+// adds bias, activation and residual and leaves them in its warp's staging rows, from which the warp writes 128 bytes of a row at a
+// time; the residual's rows lie there before.  Nobody waits for another warp.  (With sums staged and finished row by row instead,
+// the 16384x1024x4096 forward took 162 us with GELU and slope, 860 with a residual as well: loads that nothing hid.)
 #define CAFE_RUN_THREADS 320
 template <typename T, int BN> struct CafeRunShape {
     typedef CafeTiles<T> L;
+    typedef typename CafeSlopeOf<T>::type ST;
     static constexpr int rowb = L::BK * 2;
     static constexpr int a_part = CAFE_LIN_BM * rowb, b_part = BN * rowb, stage = L::parts * (a_part + b_part);
-    static constexpr int cols = L::parts == 3 ? 32 : 64, staging = 32 * cols * 4;   // of a pass; pieces of four exchanged by row
+    static constexpr int cols = sizeof(T) == 2 && sizeof(ST) == 2 ? 64 : 32;                  // of a pass
+    static constexpr int out_row = cols * sizeof(T), slope_row = cols * sizeof(ST);           // bytes
+    static constexpr int staging = 32 * (out_row + slope_row);
     static constexpr int room = 229376 - 8 * staging, stages = room / stage < 6 ? room / stage : 6;
     static constexpr int bytes = stage * stages + 8 * staging + 1024;
     static constexpr int tm_set = L::parts == 3 ? 2 * BN : BN;
 };
+__device__ __forceinline__ uint4 cafe_get16(uint32_t at) {
+    uint4 x;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at) : "memory");
+    return x;
+}
+// Staged rows of ROW bytes: 16-byte piece c of row r lies at piece c ^ r (of as many as a row has, at most eight).
+template <int ROW> __device__ __forceinline__ uint32_t cafe_staged(uint32_t at, int r, int c) {
+    return at + (uint32_t)(r * ROW + ((c ^ (r & (ROW >= 128 ? 7 : ROW / 16 - 1))) << 4));
+}
+// The warp's 32 rows of W columns between shared memory and rows of E elsewhere, `n` columns and `m` rows of them there.
+template <typename E, int W> __device__ __forceinline__ void cafe_rows_out(uint32_t at, E* to, int64_t ld, bool on16, int m, int n, int lane) {
+    constexpr int ROW = W * sizeof(E), per = ROW / 16, each = 16 / sizeof(E);
+#pragma unroll 2
+    for (int r = lane / per; r < m; r += 32 / per) {
+        const int c = lane % per;
+        alignas(16) E x[each];
+        *reinterpret_cast<uint4*>(x) = cafe_get16(cafe_staged<ROW>(at, r, c));
+        E* p = to + r * ld + c * each;
+        if (on16 && (c + 1) * each <= n) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(x);
+        else {
+#pragma unroll
+            for (int q = 0; q < each; ++q) if (c * each + q < n) p[q] = x[q];
+        }
+    }
+}
+template <typename E, int W> __device__ __forceinline__ void cafe_rows_in(uint32_t at, const E* from, int64_t ld, bool on16, int m, int n, int lane) {
+    constexpr int ROW = W * sizeof(E), per = ROW / 16, each = 16 / sizeof(E);
+#pragma unroll 4
+    for (int r = lane / per; r < m; r += 32 / per) {
+        const int c = lane % per;
+        const E* p = from + r * ld + c * each;
+        const uint32_t to = cafe_staged<ROW>(at, r, c);
+        if (on16 && (c + 1) * each <= n) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(p) : "memory");
+        else {
+            alignas(16) E x[each];
+#pragma unroll
+            for (int q = 0; q < each; ++q) x[q] = c * each + q < n ? __ldg(p + q) : cafe_from_float<E>(0.f);
+            const uint4 y = *reinterpret_cast<const uint4*>(x);
+            cafe_put16(to, y.x, y.y, y.z, y.w);
+        }
+    }
+}
+
 template <typename T, int BN>
 __global__ void __launch_bounds__(CAFE_RUN_THREADS, 1) k_tiles_run(const __grid_constant__ CafeTilesArgs P) {
     typedef CafeTiles<T> L;
@@ -433,7 +480,7 @@ __global__ void __launch_bounds__(CAFE_RUN_THREADS, 1) k_tiles_run(const __grid_
                 for (int k = 0; k < L::BK / 16; ++k) cafe_mma(sums, a + ak * k, b + bk * k, instr, in_chunk > 0 || k > 0, lead);
                 ++in_chunk;
                 if constexpr (L::parts == 3) {
-                    if (in_chunk == P.chunk) {
+                    if (in_chunk == CAFE_TILES_CHUNK) {
                         if (t < turns - 1) cafe_mma_commit(chunk_full(g), lead);
                         in_chunk = 0;
                     }
@@ -461,10 +508,20 @@ __global__ void __launch_bounds__(CAFE_RUN_THREADS, 1) k_tiles_run(const __grid_
         bool fine = true;
         int n = 0;
         for (int tile = blockIdx.x + g * gridDim.x; tile < tiles; tile += 2 * gridDim.x, ++n) {
-            const int tm = tile / J.tiles_n, row0 = tm * CAFE_LIN_BM + rows, col0 = (tile - tm * J.tiles_n) * BN;
+            const int tm = tile / J.tiles_n, col0 = (tile - tm * J.tiles_n) * BN;
+            const int64_t row0 = (int64_t)tm * CAFE_LIN_BM + rows;
+            typedef typename CafeSlopeOf<T>::type ST;
             constexpr int W = Sh::cols;
-            float acc[L::parts == 3 ? BN : W];
+            const uint32_t out = mine, slopes = mine + 32 * Sh::out_row;
+            const int m = (int)max((int64_t)0, min((int64_t)32, J.rows - row0));
+            auto residual = [&](int h) {
+                if (!J.res) return;
+                cafe_rows_in<T, W>(out, static_cast<const T*>(J.res) + row0 * J.ldr + col0 + h, J.ldr, J.res_row, m, min(W, J.cols - col0 - h), lane);
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+            residual(0);
             if constexpr (L::parts == 3) {
+                float acc[BN];
                 auto take = [&](uint32_t at, bool first) {
 #pragma unroll
                     for (int c = 0; c < BN; c += 16) {
@@ -475,7 +532,7 @@ __global__ void __launch_bounds__(CAFE_RUN_THREADS, 1) k_tiles_run(const __grid_
                         for (int i = 0; i < 16; ++i) acc[c + i] = first ? v[i] : acc[c + i] + v[i];
                     }
                 };
-                const int between = turns > 0 ? (turns - 1) / P.chunk : 0;   // chunks that do not end the tile
+                const int between = turns > 0 ? (turns - 1) / CAFE_TILES_CHUNK : 0;   // chunks that do not end the tile
                 for (int c = 0; c < between && fine; ++c, ++chunks) {
                     fine = cafe_bar_wait(chunk_full(g), chunks & 1u, &bail);
                     cafe_tc_after();
@@ -491,55 +548,81 @@ __global__ void __launch_bounds__(CAFE_RUN_THREADS, 1) k_tiles_run(const __grid_
                 if (fine) {
                     take(from, between == 0);
                     take(from + BN, false);
-                } else {
 #pragma unroll
-                    for (int i = 0; i < BN; ++i) acc[i] = __uint_as_float(0x7fffffffu);
+                    for (int c = 0; c < BN; c += 16) cafe_tm_store16(from + c, acc + c);
+                    cafe_tm_wait_store();
                 }
-                cafe_tc_before();
-                __syncwarp();
-                if (lane == 0) cafe_bar_arrive(tile_taken(g));
             } else {
                 if (fine) fine = cafe_bar_wait(tile_full(g), (uint32_t)n & 1u, &bail);
                 cafe_tc_after();
                 fine = __all_sync(0xffffffffu, fine);
             }
             const int columns = min(BN, J.cols - col0);
-#pragma unroll
-            for (int h = 0; h < BN / W; ++h) {
-                if (W * h >= columns) continue;
-                if constexpr (L::parts == 1) {
-#pragma unroll
-                    for (int c = 0; c < W; c += 16) cafe_tm_load16(from + W * h + c, acc + c);
+#pragma unroll 1
+            for (int h = 0; h < columns; h += W) {
+                if (J.res) asm volatile("cp.async.wait_group 0;" ::: "memory");
+                __syncwarp();
+#pragma unroll 1
+                for (int c = 0; c < W; c += 16) {
+                    float z[16], d[16];
+                    cafe_tm_load16(from + h + c, z);
                     cafe_tm_wait_load();
-                    if (h == BN / W - 1 || W * (h + 1) >= columns) {   // (the last columns that count have been read)
-                        cafe_tc_before();
-                        __syncwarp();
-                        if (lane == 0) cafe_bar_arrive(tile_taken(g));
+                    const int64_t j = col0 + h + c;
+                    if constexpr (L::parts == 3) {
+                        bool nan = false;
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) nan |= !(z[q] == z[q]);
+                        if (nan && lane < m) {
+#pragma unroll
+                            for (int q = 0; q < 16; ++q) if (z[q] != z[q] && j + q < J.cols) z[q] = cafe_plain_dot(J, row0 + lane, j + q, 0, J.depth);
+                        }
                     }
                     if (!fine) {
 #pragma unroll
-                        for (int i = 0; i < W; ++i) acc[i] = __uint_as_float(0x7fffffffu);
+                        for (int q = 0; q < 16; ++q) z[q] = __uint_as_float(0x7fffffffu);
+                    }
+                    if (J.bias) {
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) if (j + q < J.cols) z[q] += cafe_to_float(__ldg(static_cast<const T*>(J.bias) + j + q));
+                    }
+                    cafe_act_all<sizeof(T) == 2, 16>(z, J.act, d);
+                    constexpr int each = 16 / sizeof(T), slope_each = 16 / sizeof(ST);
+#pragma unroll
+                    for (int p = 0; p < 16; p += each) {
+                        const uint32_t at = cafe_staged<Sh::out_row>(out, lane, (c + p) / each);
+                        alignas(16) T x[each];
+                        if (J.res) {
+                            *reinterpret_cast<uint4*>(x) = cafe_get16(at);
+#pragma unroll
+                            for (int q = 0; q < each; ++q) z[p + q] += cafe_to_float(x[q]);
+                        }
+#pragma unroll
+                        for (int q = 0; q < each; ++q) x[q] = cafe_from_float<T>(z[p + q]);
+                        const uint4 y = *reinterpret_cast<const uint4*>(x);
+                        cafe_put16(at, y.x, y.y, y.z, y.w);
+                    }
+                    if (J.slope_out) {
+#pragma unroll
+                        for (int p = 0; p < 16; p += slope_each) {
+                            alignas(16) ST x[slope_each];
+#pragma unroll
+                            for (int q = 0; q < slope_each; ++q) x[q] = cafe_from_float<ST>(d[p + q]);
+                            const uint4 y = *reinterpret_cast<const uint4*>(x);
+                            cafe_put16(cafe_staged<Sh::slope_row>(slopes, lane, (c + p) / slope_each), y.x, y.y, y.z, y.w);
+                        }
                     }
                 }
-                __syncwarp();   // the staging rows are free
-                cafe_sums_put<L::parts == 3, W, true>(J, acc + (L::parts == 3 ? W * h : 0), mine + (uint32_t)lane * (W * 4), row0 + lane, col0 + W * h, 0,
-                                                      J.depth, fine, lane & 7);
+                if (h + W >= columns) {   // tensor memory has been read
+                    cafe_tc_before();
+                    __syncwarp();
+                    if (lane == 0) cafe_bar_arrive(tile_taken(g));
+                }
                 __syncwarp();
-                constexpr int lanes = W / 4;   // to a row
-                const int q = lane % lanes;
-                const int64_t j = col0 + W * h + q * 4;
-                if (j < J.cols) {
-                    float bias[4];
-                    cafe_quad_bias<T>(J, j, bias);
-                    const int last = min(32, J.rows - row0);
-#pragma unroll 2
-                    for (int r = lane / lanes; r < last; r += 32 / lanes) {
-                        float v[4];
-                        asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
-                                     : "r"(mine + (uint32_t)(r * (W * 4) + ((q ^ (r & 7)) << 4))) : "memory");
-                        cafe_quad_end<T>(J, row0 + r, j, v, bias);
-                    }
-                }
+                const int here = min(W, columns - h);
+                cafe_rows_out<T, W>(out, static_cast<T*>(J.out) + row0 * J.ldo + col0 + h, J.ldo, J.out_row, m, here, lane);
+                if (J.slope_out) cafe_rows_out<ST, W>(slopes, static_cast<ST*>(J.slope_out) + row0 * J.lds + col0 + h, J.lds, J.slope_row, m, here, lane);
+                __syncwarp();   // the staging rows are free
+                if (h + W < columns) residual(h + W);
             }
         }
         if (!fine) g_tiles_gave_up = 1;
@@ -589,7 +672,6 @@ static cudaError_t tiles_launch_bn(CafeTilesArgs& P, const TilesOperand& a, cons
     P.job.tiles_n = P.job.cols > 0 ? (P.job.cols + BN - 1) / BN : 1;
     P.job.tiles = ((P.job.rows + CAFE_LIN_BM - 1) / CAFE_LIN_BM) * P.job.tiles_n;
     if (run) {
-        P.chunk = tiles_chunk((P.job.depth + CafeTiles<T>::BK - 1) / CafeTiles<T>::BK);
         constexpr int bytes = CafeRunShape<T, BN>::bytes;
         static std::atomic<uint64_t> allowed{0};
         const cudaError_t e = dense_allow_shared((const void*)k_tiles_run<T, BN>, bytes, &allowed);
@@ -598,7 +680,6 @@ static cudaError_t tiles_launch_bn(CafeTilesArgs& P, const TilesOperand& a, cons
         k_tiles_run<T, BN><<<P.job.tiles < 148 ? P.job.tiles : 148, CAFE_RUN_THREADS, bytes, st>>>(P);
         return cudaGetLastError();
     }
-    P.chunk = tiles_chunk(((P.job.depth + CafeTiles<T>::BK - 1) / CafeTiles<T>::BK + P.splits - 1) / P.splits);
     constexpr int bytes = CafeTilesShape<T, BN>::bytes;
     static std::atomic<uint64_t> allowed{0};
     const cudaError_t e = dense_allow_shared((const void*)k_tiles<T, BN>, bytes, &allowed);
