@@ -294,7 +294,6 @@ __global__ void __launch_bounds__(CAFE_LIN_THREADS, 1) k_linear(const __grid_con
         bool fine = true;
         for (int c = 0; c < chunks && fine; ++c) {
             if (warp == 8) {
-                const uint32_t lead = lane == 0;
                 const int end = min(turns, (c + 1) * L::chunk);
                 if (c > 0) fine = __all_sync(0xffffffffu, cafe_bar_wait(acc_empty, (uint32_t)(c - 1) & 1u, &bail));
                 for (int t = c * L::chunk; t < end && fine; ++t) {
@@ -302,23 +301,27 @@ __global__ void __launch_bounds__(CAFE_LIN_THREADS, 1) k_linear(const __grid_con
                     if (!(fine = __all_sync(0xffffffffu, cafe_bar_wait(full(s), (uint32_t)(t / Sh::stages) & 1u, &bail)))) break;
                     cafe_tc_after();
                     const uint32_t a = base + s * Sh::stage, b = a + L::parts * Sh::a_part;
+                    if (cafe_elect()) {
 #pragma unroll
-                    for (int k = 0; k < L::BK / 16; ++k)
-                        cafe_mma(tmem, cafe_operand<Sh::rowb>(a + 32 * k), cafe_operand<Sh::rowb>(b + 32 * k), instr, t > c * L::chunk || k > 0, lead);
-                    if (t == end - 1) cafe_mma_commit(acc_full, lead);
-                    if constexpr (L::parts == 3) {
+                        for (int k = 0; k < L::BK / 16; ++k)
+                            cafe_mma(tmem, cafe_operand<Sh::rowb>(a + 32 * k), cafe_operand<Sh::rowb>(b + 32 * k), instr, t > c * L::chunk || k > 0);
+                        if (t == end - 1) cafe_mma_commit(acc_full);
+                        if constexpr (L::parts == 3) {
 #pragma unroll
-                        for (int q = 0; q < 5; ++q) {
-                            constexpr int ia[5] = {0, 1, 1, 0, 2}, ib[5] = {1, 0, 1, 2, 0};
+                            for (int q = 0; q < 5; ++q) {
+                                constexpr int ia[5] = {0, 1, 1, 0, 2}, ib[5] = {1, 0, 1, 2, 0};
 #pragma unroll
-                            for (int k = 0; k < L::BK / 16; ++k)
-                                cafe_mma(tmem + BN, cafe_operand<Sh::rowb>(a + ia[q] * Sh::a_part + 32 * k),
-                                         cafe_operand<Sh::rowb>(b + ib[q] * Sh::b_part + 32 * k), instr, t > 0 || q > 0 || k > 0, lead);
+                                for (int k = 0; k < L::BK / 16; ++k)
+                                    cafe_mma(tmem + BN, cafe_operand<Sh::rowb>(a + ia[q] * Sh::a_part + 32 * k),
+                                             cafe_operand<Sh::rowb>(b + ib[q] * Sh::b_part + 32 * k), instr, t > 0 || q > 0 || k > 0);
+                            }
                         }
+                        cafe_mma_commit(empty(s));
                     }
-                    cafe_mma_commit(empty(s), lead);
+                    __syncwarp();
                 }
-                if (!fine || c == chunks - 1) cafe_mma_commit(all_done, lead);
+                if ((!fine || c == chunks - 1) && cafe_elect()) cafe_mma_commit(all_done);
+                __syncwarp();
             }
             if (fine) fine = cafe_bar_wait(acc_full, (uint32_t)c & 1u, &bail);
             cafe_tc_after();
@@ -528,7 +531,7 @@ __global__ void __launch_bounds__(256) k_few(const CafeFew P) {
         const int64_t i = P.few_is_row ? f : many, j = P.few_is_row ? many : f;
         float d = 1.f;
         if (P.bias) z += cafe_to_float(__ldg(static_cast<const T*>(P.bias) + j));
-        if (P.act != CAFE_ACT_NONE) z = cafe_act<sizeof(T) == 2>(z, P.act, &d);
+        if (P.act != CAFE_ACT_NONE) z = cafe_act(z, P.act, &d);
         if (P.res) z += cafe_to_float(__ldg(static_cast<const T*>(P.res) + i * P.ldr + j));
         static_cast<T*>(P.out)[i * P.ldo + j] = cafe_from_float<T>(z);
         if (P.slope_out) static_cast<ST*>(P.slope_out)[i * P.lds + j] = cafe_from_float<ST>(d);

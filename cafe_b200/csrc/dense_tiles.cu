@@ -15,10 +15,12 @@
 #include "dense.cuh"
 
 #define CAFE_TILES_THREADS 192
-// rows of a block of k_parts (a row of partial column sums each): short blocks while they are few, so that all are under way at
-// once (1 M elements: 32 rows 3 us, 128 rows 8)
-static __host__ __device__ constexpr int cafe_parts_rows(int rows) { return rows <= 16384 ? 32 : 128; }
 #define CAFE_PARTS_COLS 256
+// rows of a block of k_parts (a row of partial column sums each): short blocks while they are few, so that all are under way at
+// once (1 M elements: 32 rows 3 us, 128 rows 8), long ones where there are enough (16384 x 4096: 128 rows save a third)
+static __host__ __device__ constexpr int cafe_parts_rows(int rows, int cols) {
+    return (int64_t)((rows + 127) / 128) * ((cols + CAFE_PARTS_COLS - 1) / CAFE_PARTS_COLS) >= 1024 ? 128 : 32;
+}
 
 __device__ int g_tiles_gave_up;   // a wait ran out (its outputs are not numbers)
 
@@ -70,7 +72,7 @@ __global__ void __launch_bounds__(256) k_parts(const __grid_constant__ CafeParts
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int col = bx * CAFE_PARTS_COLS + lane * 8, n = min(8, J.cols - col);
     float sum[8] = {};
-    const int per = cafe_parts_rows(J.rows);
+    const int per = cafe_parts_rows(J.rows, J.cols);
     const int64_t r0 = (int64_t)by * per, r1 = min(r0 + per, (int64_t)J.rows);
     if (n > 0) {
 #pragma unroll 4
@@ -180,30 +182,30 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
     const uint32_t from = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     bool fine = true;
     if (warp == 0) {
-        if (lane == 0) {
-            // ---- boxes of the operands
-            int t = 0;
-            for (; t < turns; ++t) {
-                const int s = t % Sh::stages, k0 = (t0 + t) * L::BK;
-                if (t >= Sh::stages && !cafe_bar_wait(empty(s), (uint32_t)(t / Sh::stages - 1) & 1u, &bail)) break;
-                const uint32_t a = base + s * Sh::stage, b = a + L::parts * Sh::a_part;
-                cafe_bar_expect(full(s), Sh::stage);
-                if (J.a_kc) cafe_box_load(a, &P.a, k0, row0, 0, full(s));
+        // ---- boxes of the operands
+        int t = 0, s = 0;
+        uint32_t phase = 1;   // (a fresh barrier's phase before its first counts as over)
+        for (int k0 = t0 * L::BK; t < turns; ++t, k0 += L::BK) {
+            if (!(fine = __all_sync(0xffffffffu, cafe_bar_wait(empty(s), phase, &bail)))) break;
+            const uint32_t a = base + s * Sh::stage, b = a + L::parts * Sh::a_part, bar = full(s);
+            if (cafe_elect()) {
+                cafe_bar_expect(bar, Sh::stage);
+                if (J.a_kc) cafe_box_load(a, &P.a, k0, row0, 0, bar);
                 else
 #pragma unroll
-                    for (int q = 0; q < CAFE_LIN_BM / 64; ++q) cafe_box_load(a + q * L::parts * L::BK * 128, &P.a, row0 + 64 * q, k0, 0, full(s));
-                if (J.b_kc) cafe_box_load(b, &P.b, k0, col0, 0, full(s));
+                    for (int q = 0; q < CAFE_LIN_BM / 64; ++q) cafe_box_load(a + q * L::parts * L::BK * 128, &P.a, row0 + 64 * q, k0, 0, bar);
+                if (J.b_kc) cafe_box_load(b, &P.b, k0, col0, 0, bar);
                 else
 #pragma unroll
-                    for (int q = 0; q < BN / 64; ++q) cafe_box_load(b + q * L::parts * L::BK * 128, &P.b, col0 + 64 * q, k0, 0, full(s));
+                    for (int q = 0; q < BN / 64; ++q) cafe_box_load(b + q * L::parts * L::BK * 128, &P.b, col0 + 64 * q, k0, 0, bar);
             }
-            if (t < turns)   // given up: the copies in flight end before the block does
-                for (int u = max(0, t - Sh::stages); u < t; ++u)
-                    for (int i = 0; i < (1 << 20) && !cafe_bar_try(full(u % Sh::stages), (uint32_t)(u / Sh::stages) & 1u); ++i) {}
+            if (++s == Sh::stages) { s = 0; phase ^= 1u; }
         }
+        if (!fine)   // given up: the copies in flight end before the block does
+            for (int u = max(0, t - Sh::stages); u < t; ++u)
+                for (int i = 0; i < (1 << 20) && !cafe_bar_try(full(u % Sh::stages), (uint32_t)(u / Sh::stages) & 1u); ++i) {}
     } else if (warp == 1) {
         // ---- products
-        const uint32_t lead = lane == 0;
         const uint32_t instr = cafe_mma_instr(L::type, CAFE_LIN_BM, BN) | (J.a_kc ? 0u : 1u << 15) | (J.b_kc ? 0u : 1u << 16);
         const uint64_t da = J.a_kc ? cafe_operand<Sh::rowb>(base) : cafe_operand_mn(base, L::parts * L::BK * 128);
         const uint64_t db = J.b_kc ? cafe_operand<Sh::rowb>(base + L::parts * Sh::a_part) : cafe_operand_mn(base + L::parts * Sh::a_part, L::parts * L::BK * 128);
@@ -219,23 +221,28 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
             }
             cafe_tc_after();
             const uint64_t a = da + (uint32_t)(s * Sh::stage >> 4), b = db + (uint32_t)(s * Sh::stage >> 4);
+            const bool ends = in_chunk == CAFE_TILES_CHUNK - 1 || t == turns - 1;
+            if (cafe_elect()) {
 #pragma unroll
-            for (int k = 0; k < L::BK / 16; ++k) cafe_mma(tmem, a + ak * k, b + bk * k, instr, in_chunk > 0 || k > 0, lead);
-            ++in_chunk;
-            if constexpr (L::parts == 3) {
-                if (in_chunk == CAFE_TILES_CHUNK || t == turns - 1) { cafe_mma_commit(acc_full, lead); in_chunk = 0; ++chunk_phase; }
+                for (int k = 0; k < L::BK / 16; ++k) cafe_mma(tmem, a + ak * k, b + bk * k, instr, in_chunk > 0 || k > 0);
+                if constexpr (L::parts == 3) {
+                    if (ends) cafe_mma_commit(acc_full);
 #pragma unroll
-                for (int q = 0; q < 5; ++q) {
-                    constexpr int ia[5] = {0, 1, 1, 0, 2}, ib[5] = {1, 0, 1, 2, 0};
+                    for (int q = 0; q < 5; ++q) {
+                        constexpr int ia[5] = {0, 1, 1, 0, 2}, ib[5] = {1, 0, 1, 2, 0};
 #pragma unroll
-                    for (int k = 0; k < L::BK / 16; ++k)
-                        cafe_mma(tmem + BN, a + ia[q] * ap + ak * k, b + ib[q] * bp + bk * k, instr, t > 0 || q > 0 || k > 0, lead);
+                        for (int k = 0; k < L::BK / 16; ++k)
+                            cafe_mma(tmem + BN, a + ia[q] * ap + ak * k, b + ib[q] * bp + bk * k, instr, t > 0 || q > 0 || k > 0);
+                    }
                 }
+                cafe_mma_commit(empty(s));
             }
-            cafe_mma_commit(empty(s), lead);
+            ++in_chunk;
+            if (L::parts == 3 && ends) { in_chunk = 0; ++chunk_phase; }
             if (++s == Sh::stages) { s = 0; phase ^= 1u; }
         }
-        cafe_mma_commit(all_done, lead);
+        __syncwarp();
+        if (cafe_elect()) cafe_mma_commit(all_done);
     } else {
         // ---- sums out of tensor memory, 32 rows a warp; before that the bias gradient from its partial sums
         if (P.sums && tn == 0 && rank == 0) {
@@ -329,25 +336,31 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
     if (warp == 1) cafe_tm_free(tmem, Sh::tm_cols);
 }
 
-// ---- tiles one after the other ---------------------------------------------------------------------------------------------
-// The same products where there are tiles enough for every SM: one block an SM works through tile after tile, and two groups of
-// four warps take turns with tensor memory's two sets of sums, so that one tile is finished and stored while the next one's products
-// run.  A lane has a row: it takes sixteen of its sums at a time out of tensor memory (fp32: where it has put them back, complete),
-// adds bias, activation and residual and leaves them in its warp's staging rows, from which the warp writes 128 bytes of a row at a
-// time; the residual's rows lie there before.  Nobody waits for another warp.  (With sums staged and finished row by row instead,
-// the 16384x1024x4096 forward took 162 us with GELU and slope, 860 with a residual as well: loads that nothing hid.)
-#define CAFE_RUN_THREADS 320
-template <typename T, int BN> struct CafeRunShape {
+// ---- tiles one after the other, by pairs of blocks --------------------------------------------------------------------------
+// Where there are tiles enough: two blocks, an SM each, work on tiles of 256 x BN, tile after tile.  Each fetches its own 128 rows of
+// A and half of B's, so an SM's boxes are half to three quarters of those of a block by itself, and the products no longer wait
+// for them (16384x1024x1024 in fp32: 48 KB for 768 cycles of products an SM came at 29 bytes a cycle, tensor cores busy 46 %).
+// Block 0 issues the products of both; block 1 tells it when its boxes are there.
+//
+// fp32: eight warps have 32 rows and half of the columns each.  They take the large sums out every 256 of k and everything when a
+// tile's products are done, into registers; tensor memory is then free for the next tile, whose products run while this one is
+// finished.  16 bits: two sets of sums in tensor memory, two groups of four warps take turns, a lane takes sixteen sums at a time.
+// Either way a lane has a row: bias, activation, residual; results go to its warp's staging rows, from which the warp writes 128
+// bytes of a row at a time.  Nobody waits for another warp.
+#define CAFE_PAIR_THREADS 320
+template <typename T, int BN> struct CafePairShape {
     typedef CafeTiles<T> L;
     typedef typename CafeSlopeOf<T>::type ST;
     static constexpr int rowb = L::BK * 2;
-    static constexpr int a_part = CAFE_LIN_BM * rowb, b_part = BN * rowb, stage = L::parts * (a_part + b_part);
+    static constexpr int a_part = CAFE_LIN_BM * rowb, b_part = BN / 2 * rowb, stage = L::parts * (a_part + b_part);
     static constexpr int cols = sizeof(T) == 2 && sizeof(ST) == 2 ? 64 : 32;                  // of a pass
     static constexpr int out_row = cols * sizeof(T), slope_row = cols * sizeof(ST);           // bytes
     static constexpr int staging = 32 * (out_row + slope_row);
     static constexpr int room = 229376 - 8 * staging, stages = room / stage < 6 ? room / stage : 6;
     static constexpr int bytes = stage * stages + 8 * staging + 1024;
-    static constexpr int tm_set = L::parts == 3 ? 2 * BN : BN;
+    static constexpr int sets = L::parts == 3 ? 1 : 2, tm_set = L::parts == 3 ? 2 * BN : BN;
+    static constexpr int takers = L::parts == 3 ? 8 : 4;                                      // warps of a block that share a tile
+    static constexpr int mine = L::parts == 3 ? BN / 2 : BN;                                  // columns of a warp
 };
 __device__ __forceinline__ uint4 cafe_get16(uint32_t at) {
     uint4 x;
@@ -358,16 +371,31 @@ __device__ __forceinline__ uint4 cafe_get16(uint32_t at) {
 template <int ROW> __device__ __forceinline__ uint32_t cafe_staged(uint32_t at, int r, int c) {
     return at + (uint32_t)(r * ROW + ((c ^ (r & (ROW >= 128 ? 7 : ROW / 16 - 1))) << 4));
 }
-// The warp's 32 rows of W columns between shared memory and rows of E elsewhere, `n` columns and `m` rows of them there.
-template <typename E, int W> __device__ __forceinline__ void cafe_rows_out(uint32_t at, E* to, int64_t ld, bool on16, int m, int n, int lane) {
+// The warp's 32 rows of W columns between shared memory and rows of E elsewhere, `n` columns and `m` rows of them there; on the way
+// out rows of `add` are added.
+template <typename E, int W>
+__device__ __forceinline__ void cafe_rows_out(uint32_t at, E* to, int64_t ld, bool on16, const E* add, int64_t lda, bool add16, int m, int n, int lane) {
     constexpr int ROW = W * sizeof(E), per = ROW / 16, each = 16 / sizeof(E);
-#pragma unroll 2
+    const int c = lane % per;
+    const bool whole = (c + 1) * each <= n;
+#pragma unroll 4
     for (int r = lane / per; r < m; r += 32 / per) {
-        const int c = lane % per;
-        alignas(16) E x[each];
+        alignas(16) E x[each], y[each];
+        if (add) {
+            const E* p = add + r * lda + c * each;
+            if (add16 && whole) *reinterpret_cast<uint4*>(y) = __ldg(reinterpret_cast<const uint4*>(p));
+            else {
+#pragma unroll
+                for (int q = 0; q < each; ++q) y[q] = c * each + q < n ? __ldg(p + q) : cafe_from_float<E>(0.f);
+            }
+        }
         *reinterpret_cast<uint4*>(x) = cafe_get16(cafe_staged<ROW>(at, r, c));
+        if (add) {
+#pragma unroll
+            for (int q = 0; q < each; ++q) x[q] = cafe_from_float<E>(cafe_to_float(x[q]) + cafe_to_float(y[q]));
+        }
         E* p = to + r * ld + c * each;
-        if (on16 && (c + 1) * each <= n) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(x);
+        if (on16 && whole) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(x);
         else {
 #pragma unroll
             for (int q = 0; q < each; ++q) if (c * each + q < n) p[q] = x[q];
@@ -392,10 +420,57 @@ template <typename E, int W> __device__ __forceinline__ void cafe_rows_in(uint32
     }
 }
 
+
+// the end of sixteen neighbouring sums of a row (columns j ..), the lane's own, r = lane: bias, activation, residual from the staged row, rounding, staging
+template <typename T, int OUT_ROW, int SLOPE_ROW, bool RES>
+__device__ __forceinline__ void cafe_row_end(const CafeJob& J, float* z, int64_t j, uint32_t out, uint32_t slopes, int r, int c) {
+    typedef typename CafeSlopeOf<T>::type ST;
+    constexpr int each = 16 / sizeof(T), slope_each = 16 / sizeof(ST);
+    float d[16];
+    if (J.bias) {   // (a lane loads one of them)
+        const int64_t i = j + (r & 15);
+        const float mine = i < J.cols ? cafe_to_float(__ldg(static_cast<const T*>(J.bias) + i)) : 0.f;
+#pragma unroll
+        for (int q = 0; q < 16; ++q) z[q] += __shfl_sync(0xffffffffu, mine, q);
+    }
+    cafe_act_all<16>(z, J.act, d);
+#pragma unroll
+    for (int p = 0; p < 16; p += each) {
+        const uint32_t at = cafe_staged<OUT_ROW>(out, r, (c + p) / each);
+        alignas(16) T x[each];
+        if (RES && J.res) {
+            *reinterpret_cast<uint4*>(x) = cafe_get16(at);
+#pragma unroll
+            for (int q = 0; q < each; ++q) z[p + q] += cafe_to_float(x[q]);
+        }
+#pragma unroll
+        for (int q = 0; q < each; ++q) x[q] = cafe_from_float<T>(z[p + q]);
+        const uint4 y = *reinterpret_cast<const uint4*>(x);
+        cafe_put16(at, y.x, y.y, y.z, y.w);
+    }
+    if (J.slope_out) {
+#pragma unroll
+        for (int p = 0; p < 16; p += slope_each) {
+            alignas(16) ST x[slope_each];
+#pragma unroll
+            for (int q = 0; q < slope_each; ++q) x[q] = cafe_from_float<ST>(d[p + q]);
+            const uint4 y = *reinterpret_cast<const uint4*>(x);
+            cafe_put16(cafe_staged<SLOPE_ROW>(slopes, r, (c + p) / slope_each), y.x, y.y, y.z, y.w);
+        }
+    }
+}
+// 32 of a lane's sums to its staging row, and back sixteen at a time
+template <int I> __device__ __forceinline__ void cafe_row_put(const float* acc, uint32_t at, int lane) {
+#pragma unroll
+    for (int c = 0; c < 32; c += 4)
+        cafe_put16(cafe_staged<128>(at, lane, c / 4), __float_as_uint(acc[I + c]), __float_as_uint(acc[I + c + 1]), __float_as_uint(acc[I + c + 2]), __float_as_uint(acc[I + c + 3]));
+}
+
 template <typename T, int BN>
-__global__ void __launch_bounds__(CAFE_RUN_THREADS, 1) k_tiles_run(const __grid_constant__ CafeTilesArgs P) {
+__global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) __cluster_dims__(2, 1, 1) k_tiles_pair(const __grid_constant__ CafeTilesArgs P) {
     typedef CafeTiles<T> L;
-    typedef CafeRunShape<T, BN> Sh;
+    typedef CafePairShape<T, BN> Sh;
+    typedef typename CafeSlopeOf<T>::type ST;
     extern __shared__ char sh_raw[];
     __shared__ __align__(8) uint64_t bars[2 * Sh::stages + 8];
     __shared__ uint32_t tm_at;
@@ -405,232 +480,253 @@ __global__ void __launch_bounds__(CAFE_RUN_THREADS, 1) k_tiles_run(const __grid_
     auto full = [&](int s) { return bar0 + 8u * s; };
     auto empty = [&](int s) { return bar0 + 8u * (Sh::stages + s); };
     const uint32_t more = bar0 + 8u * (2 * Sh::stages);
-    // for each set of sums: a chunk's large sums are ready / taken (fp32), all of a tile's sums are ready / taken
-    auto chunk_full = [&](int g) { return more + 8u * g; };
-    auto chunk_taken = [&](int g) { return more + 16u + 8u * g; };
-    auto tile_full = [&](int g) { return more + 32u + 8u * g; };
-    auto tile_taken = [&](int g) { return more + 48u + 8u * g; };
+    // a chunk's large sums are ready / taken (fp32); for each set of sums: all of a tile's are ready / taken
+    const uint32_t chunk_full = more, chunk_taken = more + 8u;
+    auto tile_full = [&](int g) { return more + 16u + 8u * g; };
+    auto tile_taken = [&](int g) { return more + 32u + 8u * g; };
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cafe_cluster_rank();
     const CafeJob& J = P.job;
     const int turns = (J.depth + L::BK - 1) / L::BK, tiles = J.tiles;
+    const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < Sh::stages; ++s) { cafe_bar_init(full(s), 1); cafe_bar_init(empty(s), 1); }
-        for (int g = 0; g < 2; ++g) { cafe_bar_init(chunk_full(g), 1); cafe_bar_init(chunk_taken(g), 4); cafe_bar_init(tile_full(g), 1); cafe_bar_init(tile_taken(g), 4); }
+        for (int s = 0; s < Sh::stages; ++s) { cafe_bar_init(full(s), 2 - rank); cafe_bar_init(empty(s), 1); }   // (block 0: its boxes and the other's)
+        cafe_bar_init(chunk_full, 1);
+        cafe_bar_init(chunk_taken, 2 * Sh::takers);
+        for (int g = 0; g < 2; ++g) { cafe_bar_init(tile_full(g), 1); cafe_bar_init(tile_taken(g), 2 * Sh::takers); }
         cafe_fence_barrier_init();
         bail = 0;
     }
-    if (warp == 1) cafe_tm_alloc(cafe_smem(&tm_at), 2 * Sh::tm_set);
+    if (warp == 1) cafe_tm_alloc2(cafe_smem(&tm_at), Sh::sets * Sh::tm_set);
     cafe_tc_before();
     __syncthreads();
+    cafe_cluster_sync();
     cafe_tc_after();
     const uint32_t tmem = tm_at;
 
     if (warp == 0) {
-        if (lane == 0) {
-            // ---- boxes of the operands
-            bool fine = true;
-            int64_t u = 0;   // turns so far
-            for (int tile = blockIdx.x; tile < tiles && fine; tile += gridDim.x) {
-                const int tm = tile / J.tiles_n, row0 = tm * CAFE_LIN_BM, col0 = (tile - tm * J.tiles_n) * BN;
-                for (int t = 0; t < turns; ++t, ++u) {
-                    const int s = (int)(u % Sh::stages), k0 = t * L::BK;
-                    if (u >= Sh::stages && !(fine = cafe_bar_wait(empty(s), (uint32_t)(u / Sh::stages - 1) & 1u, &bail))) break;
-                    const uint32_t a = base + s * Sh::stage, b = a + L::parts * Sh::a_part;
-                    cafe_bar_expect(full(s), Sh::stage);
-                    if (J.a_kc) cafe_box_load(a, &P.a, k0, row0, 0, full(s));
+        // ---- boxes of the operands: this block's rows of A, this block's half of B's
+        bool fine = true;
+        int s = 0;
+        uint32_t phase = 1;   // (a fresh barrier's phase before its first counts as over)
+        int64_t u = 0;
+        for (int tile = first; tile < tiles && fine; tile += step) {
+            const int tm = tile / J.tiles_n, row0 = tm * 256 + rank * 128, col0 = (tile - tm * J.tiles_n) * BN + rank * (BN / 2);
+            for (int k0 = 0; k0 < J.depth; k0 += L::BK, ++u) {
+                if (!(fine = __all_sync(0xffffffffu, cafe_bar_wait(empty(s), phase, &bail)))) break;
+                const uint32_t a = base + s * Sh::stage, b = a + L::parts * Sh::a_part, bar = full(s);
+                if (cafe_elect()) {
+                    cafe_bar_expect(bar, Sh::stage);
+                    if (J.a_kc) cafe_box_load(a, &P.a, k0, row0, 0, bar);
                     else
 #pragma unroll
-                        for (int q = 0; q < CAFE_LIN_BM / 64; ++q) cafe_box_load(a + q * L::parts * L::BK * 128, &P.a, row0 + 64 * q, k0, 0, full(s));
-                    if (J.b_kc) cafe_box_load(b, &P.b, k0, col0, 0, full(s));
+                        for (int q = 0; q < CAFE_LIN_BM / 64; ++q) cafe_box_load(a + q * L::parts * L::BK * 128, &P.a, row0 + 64 * q, k0, 0, bar);
+                    if (J.b_kc) cafe_box_load(b, &P.b, k0, col0, 0, bar);
                     else
 #pragma unroll
-                        for (int q = 0; q < BN / 64; ++q) cafe_box_load(b + q * L::parts * L::BK * 128, &P.b, col0 + 64 * q, k0, 0, full(s));
+                        for (int q = 0; q < BN / 128; ++q) cafe_box_load(b + q * L::parts * L::BK * 128, &P.b, col0 + 64 * q, k0, 0, bar);
                 }
+                if (++s == Sh::stages) { s = 0; phase ^= 1u; }
             }
-            if (!fine)   // given up: the copies in flight end before the block does
-                for (int64_t v = u > Sh::stages ? u - Sh::stages : 0; v < u; ++v)
-                    for (int i = 0; i < (1 << 20) && !cafe_bar_try(full((int)(v % Sh::stages)), (uint32_t)(v / Sh::stages) & 1u); ++i) {}
+        }
+        if (!fine)   // given up: the copies in flight end before the block does
+            for (int64_t v = u > Sh::stages ? u - Sh::stages : 0; v < u; ++v)
+                for (int i = 0; i < (1 << 20) && !cafe_bar_try(full((int)(v % Sh::stages)), (uint32_t)(v / Sh::stages) & 1u); ++i) {}
+    } else if (warp == 1 && rank == 1) {
+        if (lane == 0) {
+            // ---- this block's boxes are there
+            int s = 0;
+            uint32_t phase = 0;
+            bool fine = true;
+            for (int tile = first; tile < tiles && fine; tile += step)
+                for (int t = 0; t < turns; ++t) {
+                    if (!(fine = cafe_bar_wait(full(s), phase, &bail))) break;
+                    cafe_bar_arrive_at(cafe_cluster_map(full(s), 0));
+                    if (++s == Sh::stages) { s = 0; phase ^= 1u; }
+                }
         }
     } else if (warp == 1) {
         // ---- products
-        const uint32_t lead = lane == 0;
-        const uint32_t instr = cafe_mma_instr(L::type, CAFE_LIN_BM, BN) | (J.a_kc ? 0u : 1u << 15) | (J.b_kc ? 0u : 1u << 16);
+        const uint32_t instr = cafe_mma_instr(L::type, 256, BN) | (J.a_kc ? 0u : 1u << 15) | (J.b_kc ? 0u : 1u << 16);
         const uint64_t da = J.a_kc ? cafe_operand<Sh::rowb>(base) : cafe_operand_mn(base, L::parts * L::BK * 128);
         const uint64_t db = J.b_kc ? cafe_operand<Sh::rowb>(base + L::parts * Sh::a_part) : cafe_operand_mn(base + L::parts * Sh::a_part, L::parts * L::BK * 128);
+        // offsets in 16-byte units: from a part to the next, from 16 k to the next 16
         const uint32_t ap = (J.a_kc ? Sh::a_part : L::BK * 128) >> 4, bp = (J.b_kc ? Sh::b_part : L::BK * 128) >> 4;
         const uint32_t ak = (J.a_kc ? 32 : 2048) >> 4, bk = (J.b_kc ? 32 : 2048) >> 4;
         bool fine = true;
         int s = 0, n = 0;
-        uint32_t phase = 0, chunk_phases = 0;   // (bit g: parity of the chunks of set g that were handed over, less those that end a tile)
-        for (int tile = blockIdx.x; tile < tiles && fine; tile += gridDim.x, ++n) {
-            const int g = n & 1;
+        uint32_t phase = 0, chunk_phase = 0;
+        for (int tile = first; tile < tiles && fine; tile += step, ++n) {
+            const int g = n % Sh::sets;
             const uint32_t sums = tmem + g * Sh::tm_set;
-            if (n >= 2 && !(fine = __all_sync(0xffffffffu, cafe_bar_wait(tile_taken(g), (uint32_t)(n / 2 - 1) & 1u, &bail)))) break;
+            if (n >= Sh::sets && !(fine = __all_sync(0xffffffffu, cafe_bar_wait(tile_taken(g), (uint32_t)(n / Sh::sets - 1) & 1u, &bail)))) break;
             int in_chunk = 0;
             for (int t = 0; t < turns; ++t) {
                 if (!(fine = __all_sync(0xffffffffu, cafe_bar_wait(full(s), phase, &bail)))) break;
                 if (L::parts == 3 && in_chunk == 0 && t > 0) {
-                    if (!(fine = __all_sync(0xffffffffu, cafe_bar_wait(chunk_taken(g), chunk_phases >> g & 1u, &bail)))) break;
-                    chunk_phases ^= 1u << g;
+                    if (!(fine = __all_sync(0xffffffffu, cafe_bar_wait(chunk_taken, chunk_phase, &bail)))) break;
+                    chunk_phase ^= 1u;
                 }
                 cafe_tc_after();
                 const uint64_t a = da + (uint32_t)(s * Sh::stage >> 4), b = db + (uint32_t)(s * Sh::stage >> 4);
+                if (cafe_elect()) {
 #pragma unroll
-                for (int k = 0; k < L::BK / 16; ++k) cafe_mma(sums, a + ak * k, b + bk * k, instr, in_chunk > 0 || k > 0, lead);
-                ++in_chunk;
-                if constexpr (L::parts == 3) {
-                    if (in_chunk == CAFE_TILES_CHUNK) {
-                        if (t < turns - 1) cafe_mma_commit(chunk_full(g), lead);
-                        in_chunk = 0;
+                    for (int k = 0; k < L::BK / 16; ++k) cafe_mma2(sums, a + ak * k, b + bk * k, instr, in_chunk > 0 || k > 0);
+                    if constexpr (L::parts == 3) {
+                        if (in_chunk == CAFE_TILES_CHUNK - 1 && t < turns - 1) cafe_mma_commit2(chunk_full);
+#pragma unroll
+                        for (int q = 0; q < 5; ++q) {
+                            constexpr int ia[5] = {0, 1, 1, 0, 2}, ib[5] = {1, 0, 1, 2, 0};
+#pragma unroll
+                            for (int k = 0; k < L::BK / 16; ++k)
+                                cafe_mma2(sums + BN, a + ia[q] * ap + ak * k, b + ib[q] * bp + bk * k, instr, t > 0 || q > 0 || k > 0);
+                        }
                     }
-#pragma unroll
-                    for (int q = 0; q < 5; ++q) {
-                        constexpr int ia[5] = {0, 1, 1, 0, 2}, ib[5] = {1, 0, 1, 2, 0};
-#pragma unroll
-                        for (int k = 0; k < L::BK / 16; ++k)
-                            cafe_mma(sums + BN, a + ia[q] * ap + ak * k, b + ib[q] * bp + bk * k, instr, t > 0 || q > 0 || k > 0, lead);
-                    }
+                    cafe_mma_commit2(empty(s));
                 }
-                cafe_mma_commit(empty(s), lead);
+                ++in_chunk;
+                if (L::parts == 3 && in_chunk == CAFE_TILES_CHUNK) in_chunk = 0;
                 if (++s == Sh::stages) { s = 0; phase ^= 1u; }
             }
-            cafe_mma_commit(tile_full(g), lead);
+            __syncwarp();
+            if (cafe_elect()) cafe_mma_commit2(tile_full(g));
         }
         if (!fine)   // given up: products in flight end before the block does
-            for (int i = 0; i < (1 << 20) && !cafe_bar_try(tile_full(n & 1), (uint32_t)(n / 2) & 1u); ++i) {}
+            for (int i = 0; i < (1 << 20) && !cafe_bar_try(tile_full(n % Sh::sets), (uint32_t)(n / Sh::sets) & 1u); ++i) {}
     } else {
-        // ---- sums out of tensor memory and out of the block: group g has every other tile, a warp 32 rows of it
-        const int g = (warp - 2) >> 2, rows = (warp & 3) * 32;
-        const uint32_t from = tmem + g * Sh::tm_set + ((uint32_t)rows << 16);
-        const uint32_t mine = base + Sh::stages * Sh::stage + (warp - 2) * Sh::staging;
-        uint32_t chunks = 0;
+        // ---- sums out of tensor memory and out of the block
+        constexpr int W = Sh::cols;
+        const int half = (warp - 2) >> 2, rows = (warp & 3) * 32;
+        const uint32_t out = base + Sh::stages * Sh::stage + (warp - 2) * Sh::staging, slopes = out + 32 * Sh::out_row;
+        const uint32_t lanes = (uint32_t)rows << 16;
+        uint32_t chunk_phase = 0;
         bool fine = true;
-        int n = 0;
-        for (int tile = blockIdx.x + g * gridDim.x; tile < tiles; tile += 2 * gridDim.x, ++n) {
-            const int tm = tile / J.tiles_n, col0 = (tile - tm * J.tiles_n) * BN;
-            const int64_t row0 = (int64_t)tm * CAFE_LIN_BM + rows;
-            typedef typename CafeSlopeOf<T>::type ST;
-            constexpr int W = Sh::cols;
-            const uint32_t out = mine, slopes = mine + 32 * Sh::out_row;
-            const int m = (int)max((int64_t)0, min((int64_t)32, J.rows - row0));
-            auto residual = [&](int h) {
-                if (!J.res) return;
-                cafe_rows_in<T, W>(out, static_cast<const T*>(J.res) + row0 * J.ldr + col0 + h, J.ldr, J.res_row, m, min(W, J.cols - col0 - h), lane);
-                asm volatile("cp.async.commit_group;" ::: "memory");
-            };
-            residual(0);
+        // fp32: every tile, the warp's half of the columns; 16 bits: every other tile, all of them
+        int n = L::parts == 3 ? 0 : half;
+        for (int tile = first + n * step; tile < tiles; tile += L::parts == 3 ? step : 2 * step, n += L::parts == 3 ? 1 : 2) {
+            const int g = n % Sh::sets, tm = tile / J.tiles_n, col0 = (tile - tm * J.tiles_n) * BN + (L::parts == 3 ? half * Sh::mine : 0);
+            const int64_t row0 = (int64_t)tm * 256 + rank * 128 + rows;
+            const int m = (int)max((int64_t)0, min((int64_t)32, J.rows - row0)), columns = max(0, min(Sh::mine, J.cols - col0));
+            const uint32_t from = tmem + g * Sh::tm_set + lanes + (L::parts == 3 ? half * Sh::mine : 0);
+            const uint32_t taken = cafe_cluster_map(tile_taken(g), 0);
             if constexpr (L::parts == 3) {
-                float acc[BN];
-                auto take = [&](uint32_t at, bool first) {
+                float acc[Sh::mine];
+                auto take = [&](uint32_t at, bool first_sums) {
 #pragma unroll
-                    for (int c = 0; c < BN; c += 16) {
+                    for (int c = 0; c < Sh::mine; c += 16) {
                         float v[16];
                         cafe_tm_load16(at + c, v);
                         cafe_tm_wait_load();
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) acc[c + i] = first ? v[i] : acc[c + i] + v[i];
+                        for (int i = 0; i < 16; ++i) acc[c + i] = first_sums ? v[i] : acc[c + i] + v[i];
                     }
                 };
                 const int between = turns > 0 ? (turns - 1) / CAFE_TILES_CHUNK : 0;   // chunks that do not end the tile
-                for (int c = 0; c < between && fine; ++c, ++chunks) {
-                    fine = cafe_bar_wait(chunk_full(g), chunks & 1u, &bail);
+                for (int c = 0; c < between && fine; ++c, chunk_phase ^= 1u) {
+                    fine = cafe_bar_wait(chunk_full, chunk_phase, &bail);
                     cafe_tc_after();
                     fine = __all_sync(0xffffffffu, fine);
                     if (fine) take(from, c == 0);
                     cafe_tc_before();
                     __syncwarp();
-                    if (lane == 0) cafe_bar_arrive(chunk_taken(g));
+                    if (lane == 0) cafe_bar_arrive_at(cafe_cluster_map(chunk_taken, 0));
                 }
-                if (fine) fine = cafe_bar_wait(tile_full(g), (uint32_t)n & 1u, &bail);
+                if (fine) fine = cafe_bar_wait(tile_full(g), (uint32_t)(n / Sh::sets) & 1u, &bail);
                 cafe_tc_after();
                 fine = __all_sync(0xffffffffu, fine);
                 if (fine) {
                     take(from, between == 0);
                     take(from + BN, false);
+                } else {
 #pragma unroll
-                    for (int c = 0; c < BN; c += 16) cafe_tm_store16(from + c, acc + c);
-                    cafe_tm_wait_store();
+                    for (int i = 0; i < Sh::mine; ++i) acc[i] = __uint_as_float(0x7fffffffu);
                 }
-            } else {
-                if (fine) fine = cafe_bar_wait(tile_full(g), (uint32_t)n & 1u, &bail);
-                cafe_tc_after();
-                fine = __all_sync(0xffffffffu, fine);
-            }
-            const int columns = min(BN, J.cols - col0);
-#pragma unroll 1
-            for (int h = 0; h < columns; h += W) {
-                if (J.res) asm volatile("cp.async.wait_group 0;" ::: "memory");
+                cafe_tc_before();
                 __syncwarp();
+                if (lane == 0) cafe_bar_arrive_at(taken);
 #pragma unroll 1
-                for (int c = 0; c < W; c += 16) {
-                    float z[16], d[16];
-                    cafe_tm_load16(from + h + c, z);
-                    cafe_tm_wait_load();
-                    const int64_t j = col0 + h + c;
-                    if constexpr (L::parts == 3) {
+                for (int h = 0; h < columns; h += W) {
+                    switch (h) {
+                        case 0: cafe_row_put<0>(acc, out, lane); break;
+                        case 32: cafe_row_put<32 % Sh::mine>(acc, out, lane); break;
+                        case 64: cafe_row_put<64 % Sh::mine>(acc, out, lane); break;
+                        default: cafe_row_put<96 % Sh::mine>(acc, out, lane); break;
+                    }
+#pragma unroll 1
+                    for (int c = 0; c < W; c += 16) {
+                        float z[16];
                         bool nan = false;
 #pragma unroll
-                        for (int q = 0; q < 16; ++q) nan |= !(z[q] == z[q]);
-                        if (nan && lane < m) {
+                        for (int q = 0; q < 16; q += 4) {
+                            const uint4 x = cafe_get16(cafe_staged<128>(out, lane, (c + q) / 4));
+                            z[q] = __uint_as_float(x.x); z[q + 1] = __uint_as_float(x.y); z[q + 2] = __uint_as_float(x.z); z[q + 3] = __uint_as_float(x.w);
+                            nan |= !(z[q] == z[q]) | !(z[q + 1] == z[q + 1]) | !(z[q + 2] == z[q + 2]) | !(z[q + 3] == z[q + 3]);
+                        }
+                        const int64_t j = col0 + h + c;
+                        if (nan && fine && lane < m) {
 #pragma unroll
                             for (int q = 0; q < 16; ++q) if (z[q] != z[q] && j + q < J.cols) z[q] = cafe_plain_dot(J, row0 + lane, j + q, 0, J.depth);
                         }
+                        cafe_row_end<T, Sh::out_row, Sh::slope_row, false>(J, z, j, out, slopes, lane, c);
                     }
-                    if (!fine) {
-#pragma unroll
-                        for (int q = 0; q < 16; ++q) z[q] = __uint_as_float(0x7fffffffu);
-                    }
-                    if (J.bias) {
-#pragma unroll
-                        for (int q = 0; q < 16; ++q) if (j + q < J.cols) z[q] += cafe_to_float(__ldg(static_cast<const T*>(J.bias) + j + q));
-                    }
-                    cafe_act_all<sizeof(T) == 2, 16>(z, J.act, d);
-                    constexpr int each = 16 / sizeof(T), slope_each = 16 / sizeof(ST);
-#pragma unroll
-                    for (int p = 0; p < 16; p += each) {
-                        const uint32_t at = cafe_staged<Sh::out_row>(out, lane, (c + p) / each);
-                        alignas(16) T x[each];
-                        if (J.res) {
-                            *reinterpret_cast<uint4*>(x) = cafe_get16(at);
-#pragma unroll
-                            for (int q = 0; q < each; ++q) z[p + q] += cafe_to_float(x[q]);
-                        }
-#pragma unroll
-                        for (int q = 0; q < each; ++q) x[q] = cafe_from_float<T>(z[p + q]);
-                        const uint4 y = *reinterpret_cast<const uint4*>(x);
-                        cafe_put16(at, y.x, y.y, y.z, y.w);
-                    }
-                    if (J.slope_out) {
-#pragma unroll
-                        for (int p = 0; p < 16; p += slope_each) {
-                            alignas(16) ST x[slope_each];
-#pragma unroll
-                            for (int q = 0; q < slope_each; ++q) x[q] = cafe_from_float<ST>(d[p + q]);
-                            const uint4 y = *reinterpret_cast<const uint4*>(x);
-                            cafe_put16(cafe_staged<Sh::slope_row>(slopes, lane, (c + p) / slope_each), y.x, y.y, y.z, y.w);
-                        }
-                    }
-                }
-                if (h + W >= columns) {   // tensor memory has been read
-                    cafe_tc_before();
                     __syncwarp();
-                    if (lane == 0) cafe_bar_arrive(tile_taken(g));
+                    const int here = min(W, columns - h);
+                    cafe_rows_out<T, W>(out, static_cast<T*>(J.out) + row0 * J.ldo + col0 + h, J.ldo, J.out_row,
+                                        J.res ? static_cast<const T*>(J.res) + row0 * J.ldr + col0 + h : nullptr, J.ldr, J.res_row, m, here, lane);
+                    if (J.slope_out)
+                        cafe_rows_out<ST, W>(slopes, static_cast<ST*>(J.slope_out) + row0 * J.lds + col0 + h, J.lds, J.slope_row, (const ST*)nullptr, 0, 0, m, here, lane);
+                    __syncwarp();   // the staging rows are free
                 }
-                __syncwarp();
-                const int here = min(W, columns - h);
-                cafe_rows_out<T, W>(out, static_cast<T*>(J.out) + row0 * J.ldo + col0 + h, J.ldo, J.out_row, m, here, lane);
-                if (J.slope_out) cafe_rows_out<ST, W>(slopes, static_cast<ST*>(J.slope_out) + row0 * J.lds + col0 + h, J.lds, J.slope_row, m, here, lane);
-                __syncwarp();   // the staging rows are free
-                if (h + W < columns) residual(h + W);
+            } else {
+                // the residual's rows lie in the staging rows before the results do
+                auto residual = [&](int h) {
+                    if (!J.res) return;
+                    cafe_rows_in<T, W>(out, static_cast<const T*>(J.res) + row0 * J.ldr + col0 + h, J.ldr, J.res_row, m, min(W, J.cols - col0 - h), lane);
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                };
+                residual(0);
+                if (fine) fine = cafe_bar_wait(tile_full(g), (uint32_t)(n / Sh::sets) & 1u, &bail);
+                cafe_tc_after();
+                fine = __all_sync(0xffffffffu, fine);
+#pragma unroll 1
+                for (int h = 0; h < columns; h += W) {
+                    if (J.res) asm volatile("cp.async.wait_group 0;" ::: "memory");
+                    __syncwarp();
+#pragma unroll 1
+                    for (int c = 0; c < W; c += 16) {
+                        float z[16];
+                        cafe_tm_load16(from + h + c, z);
+                        cafe_tm_wait_load();
+                        if (!fine) {
+#pragma unroll
+                            for (int q = 0; q < 16; ++q) z[q] = __uint_as_float(0x7fffffffu);
+                        }
+                        cafe_row_end<T, Sh::out_row, Sh::slope_row, true>(J, z, col0 + h + c, out, slopes, lane, c);
+                    }
+                    if (h + W >= columns) {   // tensor memory has been read
+                        cafe_tc_before();
+                        __syncwarp();
+                        if (lane == 0) cafe_bar_arrive_at(taken);
+                    }
+                    __syncwarp();
+                    const int here = min(W, columns - h);
+                    cafe_rows_out<T, W>(out, static_cast<T*>(J.out) + row0 * J.ldo + col0 + h, J.ldo, J.out_row, (const T*)nullptr, 0, 0, m, here, lane);
+                    if (J.slope_out)
+                        cafe_rows_out<ST, W>(slopes, static_cast<ST*>(J.slope_out) + row0 * J.lds + col0 + h, J.lds, J.slope_row, (const ST*)nullptr, 0, 0, m, here, lane);
+                    __syncwarp();   // the staging rows are free
+                    if (h + W < columns) residual(h + W);
+                }
             }
         }
         if (!fine) g_tiles_gave_up = 1;
     }
     cafe_tc_before();
     __syncthreads();
+    cafe_cluster_sync();   // all of the pair's products are done and taken
     cafe_tc_after();
-    if (warp == 1) cafe_tm_free(tmem, 2 * Sh::tm_set);
+    if (warp == 1) cafe_tm_free2(tmem, Sh::sets * Sh::tm_set);
+    cafe_cluster_sync();
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------------
@@ -666,20 +762,11 @@ static bool tiles_map(CUtensorMap* map, const TilesOperand& o, int kc, int box) 
 }
 
 template <typename T, int BN>
-static cudaError_t tiles_launch_bn(CafeTilesArgs& P, const TilesOperand& a, const TilesOperand& b, bool run, cudaStream_t st) {
+static cudaError_t tiles_launch_bn(CafeTilesArgs& P, const TilesOperand& a, const TilesOperand& b, cudaStream_t st) {
     // (a bias gradient alone: no columns, no depth, nothing fetched)
     if (P.job.depth > 0 && (!tiles_map<T>(&P.a, a, P.job.a_kc, CAFE_LIN_BM) || !tiles_map<T>(&P.b, b, P.job.b_kc, BN))) return cudaErrorInvalidValue;
     P.job.tiles_n = P.job.cols > 0 ? (P.job.cols + BN - 1) / BN : 1;
     P.job.tiles = ((P.job.rows + CAFE_LIN_BM - 1) / CAFE_LIN_BM) * P.job.tiles_n;
-    if (run) {
-        constexpr int bytes = CafeRunShape<T, BN>::bytes;
-        static std::atomic<uint64_t> allowed{0};
-        const cudaError_t e = dense_allow_shared((const void*)k_tiles_run<T, BN>, bytes, &allowed);
-        if (e != cudaSuccess) return e;
-        CAFE_PROF(CAFE_P_LINEAR, st);
-        k_tiles_run<T, BN><<<P.job.tiles < 148 ? P.job.tiles : 148, CAFE_RUN_THREADS, bytes, st>>>(P);
-        return cudaGetLastError();
-    }
     constexpr int bytes = CafeTilesShape<T, BN>::bytes;
     static std::atomic<uint64_t> allowed{0};
     const cudaError_t e = dense_allow_shared((const void*)k_tiles<T, BN>, bytes, &allowed);
@@ -697,37 +784,53 @@ static cudaError_t tiles_launch_bn(CafeTilesArgs& P, const TilesOperand& a, cons
     CAFE_PROF(CAFE_P_LINEAR, st);
     return cudaLaunchKernelEx(&cfg, k_tiles<T, BN>, (const CafeTilesArgs&)P);
 }
-// One block an SM through tile after tile, or two blocks an SM and clusters that share a tile's depth: whichever estimate is less,
-// in turns at the tensor cores' full rate.  A tile costs about 4 turns beside its own when the next one's products run meanwhile,
-// a launch's first and last 12; two blocks on an SM share its tensor cores and cost 12 each, one alone waits for its boxes a third
-// of the time.  296, 296, 284 and 264 blocks run at a
-// time in clusters of 1, 2, 4 and 8 (what the device says).
+template <typename T, int BN>
+static cudaError_t tiles_launch_pair(CafeTilesArgs& P, const TilesOperand& a, const TilesOperand& b, cudaStream_t st) {
+    if (!tiles_map<T>(&P.a, a, P.job.a_kc, CAFE_LIN_BM) || !tiles_map<T>(&P.b, b, P.job.b_kc, BN / 2)) return cudaErrorInvalidValue;
+    P.job.tiles_n = (P.job.cols + BN - 1) / BN;
+    P.job.tiles = ((P.job.rows + 255) / 256) * P.job.tiles_n;
+    constexpr int bytes = CafePairShape<T, BN>::bytes;
+    static std::atomic<uint64_t> allowed{0};
+    const cudaError_t e = dense_allow_shared((const void*)k_tiles_pair<T, BN>, bytes, &allowed);
+    if (e != cudaSuccess) return e;
+    CAFE_PROF(CAFE_P_LINEAR, st);
+    k_tiles_pair<T, BN><<<2 * (P.job.tiles < 74 ? P.job.tiles : 74), CAFE_PAIR_THREADS, bytes, st>>>(P);
+    return cudaGetLastError();
+}
+// Pairs of blocks through tile after tile, or two blocks an SM and clusters that share a tile's depth: whichever estimate is less,
+// in turns of a 128 x 128 tile at the tensor cores' full rate.  A pair's turn takes 1.2 (fp32) or, 256 columns wide, 2.35 (16 bits)
+// of these, a tile 3 more and a launch 14; two blocks on an SM share its tensor cores and wait for their boxes, 2.7 (fp32) or 2.2 a
+// turn of 128 columns each, and cost 14 a tile, one alone 1.7.  296, 296, 284 and 264 blocks run at a time in clusters of 1, 2, 4
+// and 8 (what the device says).
 template <typename T>
 static cudaError_t tiles_launch(CafeTilesArgs& P, const TilesOperand& a, const TilesOperand& b, cudaStream_t st) {
     typedef CafeTiles<T> L;
-    const bool wide = L::parts == 1 && P.job.cols > 128;
+    constexpr bool split = L::parts == 3;
+    const bool wide = !split && P.job.cols > 128;
     const int bn = wide ? 256 : 128;
-    const int64_t tiles = (int64_t)((P.job.rows + CAFE_LIN_BM - 1) / CAFE_LIN_BM) * (P.job.cols > 0 ? (P.job.cols + bn - 1) / bn : 1);
+    const int64_t rows = P.job.rows, cols = P.job.cols;
+    const int64_t wide_tiles = cols > 0 ? (cols + bn - 1) / bn : 1, tiles = ((rows + CAFE_LIN_BM - 1) / CAFE_LIN_BM) * wide_tiles;
     const int turns = (P.job.depth + L::BK - 1) / L::BK;
     static const int room[4] = {296, 296, 284, 264};
     double best = 1e300;
     for (int s = 0; s < 4; ++s) {
         const int64_t blocks = tiles << s, rounds = (blocks + room[s] - 1) / room[s];
-        const double est = (double)rounds * ((blocks > 148 ? 2.0 : 1.5) * ((turns + (1 << s) - 1) >> s) + 12 + s);
+        const double est = (double)rounds * ((blocks > 148 ? split ? 2.7 : 2.2 : 1.7) * (bn / 128) * ((turns + (1 << s) - 1) >> s) + 14 + s);
         if (est < best * 0.999) { best = est; P.splits = 1 << s; }
     }
-    const bool run = P.job.depth > 0 && (double)((tiles + 147) / 148) * (turns + 4) + 12 <= best;
-    if (run && P.sums) {   // the bias gradient by itself
+    const int64_t rounds = (((rows + 255) / 256) * wide_tiles + 73) / 74;
+    const bool pair = P.job.depth > 0 && (double)rounds * ((split ? 1.2 : wide ? 2.35 : 2.2) * turns + 3) + 14 < best;
+    if (pair && P.sums) {   // the bias gradient by itself
         CafeTilesArgs G = P;
         G.job.depth = G.job.cols = 0;
         G.splits = 1;
-        const cudaError_t e = tiles_launch_bn<T, 128>(G, a, b, false, st);
+        const cudaError_t e = tiles_launch_bn<T, 128>(G, a, b, st);
         if (e != cudaSuccess) return e;
     }
-    if constexpr (L::parts == 1) {
-        if (wide) return tiles_launch_bn<T, 256>(P, a, b, run, st);
+    if constexpr (!split) {
+        if (wide) return pair ? tiles_launch_pair<T, 256>(P, a, b, st) : tiles_launch_bn<T, 256>(P, a, b, st);
     }
-    return tiles_launch_bn<T, 128>(P, a, b, run, st);
+    return pair ? tiles_launch_pair<T, 128>(P, a, b, st) : tiles_launch_bn<T, 128>(P, a, b, st);
 }
 
 static int64_t tiles_round(int64_t bytes) { return (bytes + 255) & ~(int64_t)255; }
@@ -750,7 +853,7 @@ static TilesOperand tiles_operand(CafeParts* P, char** work, int dtype, const vo
     J.slope_vec = ((uintptr_t)slope & 15) == 0 && lds * ss % 16 == 0;
     J.rows = rows; J.cols = cols; J.sums = sums;
     J.blocks_x = (cols + CAFE_PARTS_COLS - 1) / CAFE_PARTS_COLS;
-    J.blocks = J.blocks_x * ((rows + cafe_parts_rows(rows) - 1) / cafe_parts_rows(rows));
+    J.blocks = J.blocks_x * ((rows + cafe_parts_rows(rows, cols) - 1) / cafe_parts_rows(rows, cols));
     J.dst = nullptr;
     if (!in_place) {
         J.dst = *work;
@@ -790,7 +893,7 @@ int64_t cafe_tiles_backward_work(const CafeBackward& f, int dtype) {
     if (f.slope_kind != CAFE_SLOPE_NONE || !tiles_in_place(dtype, f.gy, f.ldg)) need += tiles_bytes(parts, f.M, f.N);
     if (f.gx && !tiles_in_place(dtype, f.w, f.ldw)) need += tiles_bytes(parts, f.N, f.K);
     if (f.gw && !tiles_in_place(dtype, f.x, f.ldx)) need += tiles_bytes(parts, f.M, f.K);
-    if (f.gb) need += tiles_round((int64_t)((f.M + cafe_parts_rows(f.M) - 1) / cafe_parts_rows(f.M)) * f.N * 4);
+    if (f.gb) need += tiles_round((int64_t)((f.M + cafe_parts_rows(f.M, f.N) - 1) / cafe_parts_rows(f.M, f.N)) * f.N * 4);
     return need;
 }
 
@@ -809,7 +912,7 @@ template <typename T>
 static cudaError_t tiles_backward(const CafeBackward& f, int dtype, const CafeJob* gw, const CafeJob* gx, char* work, cudaStream_t st) {
     CafeParts parts = {};
     float* sums = nullptr;
-    const int sum_rows = (f.M + cafe_parts_rows(f.M) - 1) / cafe_parts_rows(f.M);
+    const int sum_rows = (f.M + cafe_parts_rows(f.M, f.N) - 1) / cafe_parts_rows(f.M, f.N);
     if (f.gb) {
         sums = (float*)work;
         work += tiles_round((int64_t)sum_rows * f.N * 4);

@@ -15,13 +15,25 @@ __device__ __forceinline__ bool cafe_bar_try(uint32_t bar, uint32_t parity) {
 }
 // Waits for the phase of `parity` to end, but not for good: after about a second, or when another wait of the block has run
 // out (*bail), it gives up and says so.
+static __device__ __noinline__ bool cafe_bar_wait_on(uint32_t bar, uint32_t parity, volatile int* bail);
 __device__ __forceinline__ bool cafe_bar_wait(uint32_t bar, uint32_t parity, volatile int* bail) {
+    return cafe_bar_try(bar, parity) || cafe_bar_wait_on(bar, parity, bail);
+}
+static __device__ __noinline__ bool cafe_bar_wait_on(uint32_t bar, uint32_t parity, volatile int* bail) {
     for (int i = 0; !cafe_bar_try(bar, parity); ++i) {
         if (i > (1 << 20) || ((i & 255) == 255 && *bail)) { *bail = 1; return false; }
     }
     return true;
 }
 
+// One lane of the warp, all of whose lanes are here.  Copies, products and commits go inside a branch on it: what the instructions
+// take then stays in uniform registers.  (A lane-0 predicate on every instruction cost 45 cycles each: 1410 cycles for the twelve
+// products of 64 cycles of a turn, 910 with one branch around them.)
+__device__ __forceinline__ bool cafe_elect() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+    return p;
+}
 __device__ __forceinline__ void cafe_fence_barrier_init() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
 // this thread's writes to shared memory become visible to the tensor cores' reads
 __device__ __forceinline__ void cafe_fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -53,16 +65,12 @@ __device__ __forceinline__ void cafe_tm_store16(uint32_t at, const float* v) {
 }
 __device__ __forceinline__ void cafe_tm_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// D[128 x N] (+)= A[128 x 16] B[N x 16]^T, operands in shared memory (descriptors), D in tensor memory.  Called by a whole warp,
-// issued by the lane that leads: what the warp has in common stays in uniform registers, where the instruction wants it (from one
-// lane's branch every descriptor is moved there first, and 12 products of 64 cycles a turn then wait for their issue).
-__device__ __forceinline__ void cafe_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool add, uint32_t lead) {
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(instr), "r"((uint32_t)add), "r"(lead) : "memory");
+// D[128 x N] (+)= A[128 x 16] B[N x 16]^T, operands in shared memory (descriptors), D in tensor memory
+__device__ __forceinline__ void cafe_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(instr), "r"((uint32_t)add) : "memory");
 }
 // the barrier's next arrival: when all products issued so far by this lane are done
-__device__ __forceinline__ void cafe_mma_commit(uint32_t bar, uint32_t lead) {
-    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(lead) : "memory");
-}
+__device__ __forceinline__ void cafe_mma_commit(uint32_t bar) { asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory"); }
 
 // Rows of ROWB = 64 or 128 bytes, K contiguous, one behind the other; the 16-byte pieces of a row are exchanged by
 // cafe_swizzle.  Eight rows are a unit.
@@ -77,6 +85,25 @@ template <int ROWB> __device__ __forceinline__ uint32_t cafe_swizzle(int row, in
 __host__ __device__ constexpr uint32_t cafe_mma_instr(int type, int M, int N) {
     return 1u << 4 | (uint32_t)type << 7 | (uint32_t)type << 10 | (uint32_t)(N >> 3) << 17 | (uint32_t)(M >> 4) << 24;
 }
+
+// ---- pairs of blocks: a cluster of two whose tensor cores work on one tile.  D[256 x N] (+)= A[256 x 16] B[N x 16]^T: block 0 has
+// rows 0 to 127 of A and D and the first half of B's rows, block 1 the rest; block 0 issues.
+__device__ __forceinline__ void cafe_tm_alloc2(uint32_t to, uint32_t cols) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(to), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cafe_tm_free2(uint32_t at, uint32_t cols) { asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(cols) : "memory"); }
+__device__ __forceinline__ void cafe_mma2(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(instr), "r"((uint32_t)add) : "memory");
+}
+// the next arrival of the barrier at this place in both blocks
+__device__ __forceinline__ void cafe_mma_commit2(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+
+// An arrival at another block's barrier.  What it tells of is not in this thread's own writes (boxes that the copy engine has written,
+// tensor memory that has been read), so it needs no fence of the cluster's scope, which takes thousands of cycles.
+__device__ __forceinline__ void cafe_bar_arrive_at(uint32_t cluster_bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory"); }
 
 __device__ __forceinline__ uint32_t cafe_cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ void cafe_cluster_sync() {
