@@ -223,6 +223,32 @@ static inline cudaError_t dense_allow_shared(const void* kernel, int bytes, std:
     return e;
 }
 
+// A launch in clusters of `cluster` blocks.  EARLY: it may start while the kernel before it in the stream ends (its kernel waits:
+// cafe_wait_for_earlier); for kernels of one block an SM.  Smaller blocks would crowd onto the SMs that are free first and leave
+// others empty later (gW of 65536x1024x479 in 256 blocks: 476 or 669 us).
+template <bool EARLY, typename... P, typename... A>
+static inline cudaError_t dense_start(void (*kernel)(P...), dim3 grid, unsigned threads, int shared, int cluster, cudaStream_t st, const A&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = shared;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    int n = 0;
+    if (EARLY) {
+        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+        at[n].id = cudaLaunchAttributeClusterDimension;
+        at[n].val.clusterDim.x = (unsigned)cluster; at[n].val.clusterDim.y = 1; at[n++].val.clusterDim.z = 1;
+    }
+    cfg.attrs = at;
+    cfg.numAttrs = n;
+    CAFE_PROF(CAFE_P_LINEAR, st);
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // ---- the calls -------------------------------------------------------------------------------------------------------
 struct CafeForward {
     const void *x, *w, *bias, *res;

@@ -252,10 +252,12 @@ __global__ void __launch_bounds__(CAFE_LIN_THREADS, 1) k_linear(const __grid_con
         cafe_fence_barrier_init();
         bail = 0;
     }
+    cafe_next_may_start();
     if (warp == 8) cafe_tm_alloc(cafe_smem(&tm_at), Sh::tm_cols);
     cafe_tc_before();
     __syncthreads();
     cafe_tc_after();
+    cafe_wait_for_earlier();
     const uint32_t tmem = tm_at;
 
     constexpr int half_cols = BN / 2;
@@ -387,18 +389,7 @@ static cudaError_t dense_launch_bn(CafeJobs& P, int splits, cudaStream_t st) {
     static std::atomic<uint64_t> allowed{0};
     const cudaError_t e = dense_allow_shared((const void*)k_linear<T, BN>, bytes, &allowed);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * splits));
-    cfg.blockDim = dim3(CAFE_LIN_THREADS);
-    cfg.dynamicSmemBytes = bytes;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)splits; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    CAFE_PROF(CAFE_P_LINEAR, st);
-    return cudaLaunchKernelEx(&cfg, k_linear<T, BN>, (const CafeJobs&)P, splits);
+    return dense_start<true>(k_linear<T, BN>, dim3((unsigned)(tiles * splits)), CAFE_LIN_THREADS, bytes, splits, st, P, splits);
 }
 
 // Width of the tiles and blocks per tile: the pair whose estimate is least.  A turn (BK of depth) of a 64 and a 32 wide tile takes
@@ -475,6 +466,7 @@ __global__ void __launch_bounds__(256) k_few(const CafeFew P) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int groups = 8 / P.kw, group = warp / P.kw, kpart = warp % P.kw;
     const int64_t per_block = (int64_t)groups * CAFE_FEW_MANY, first = blockIdx.x * per_block + group * CAFE_FEW_MANY;
+    cafe_next_may_start();
     // k in steps of 128, shared out among kw warps
     float acc[N];
 #pragma unroll
@@ -553,12 +545,165 @@ static cudaError_t dense_few(const CafeForward& f, cudaStream_t st) {
     while (P.kw < 8 && P.kw * 128 < f.K && (int64_t)P.nmany * P.kw < 148 * 16 * 8 * 8) P.kw *= 2;
     const int per_block = 8 / P.kw * CAFE_FEW_MANY;
     const unsigned grid = (unsigned)((P.nmany + per_block - 1) / per_block);
-    CAFE_PROF(CAFE_P_LINEAR, st);
-    if (P.nfew <= 1) k_few<T, 1><<<grid, 256, 0, st>>>(P);
-    else if (P.nfew <= 4) k_few<T, 4><<<grid, 256, 0, st>>>(P);
-    else if (P.nfew <= 8) k_few<T, 8><<<grid, 256, 0, st>>>(P);
-    else k_few<T, 16><<<grid, 256, 0, st>>>(P);
-    return cudaGetLastError();
+    if (P.nfew <= 1) return dense_start<false>(k_few<T, 1>, dim3(grid), 256, 0, 1, st, P);
+    if (P.nfew <= 4) return dense_start<false>(k_few<T, 4>, dim3(grid), 256, 0, 1, st, P);
+    if (P.nfew <= 8) return dense_start<false>(k_few<T, 8>, dim3(grid), 256, 0, 1, st, P);
+    return dense_start<false>(k_few<T, 16>, dim3(grid), 256, 0, 1, st, P);
+}
+
+// The backward of a layer of at most 16 outputs: gx = gz W is a sum of few outer products, gW = gz^T x a few long sums, both bound
+// by the bytes of x and gx, which are read and written once here, in plain fp32 multiply-adds (2048 x 256 -> 1: 36 us as tiles of 128
+// that are padding).  A block has 256 columns of k, a thread four of them and every other row of the block's rows; sums of
+// blocks' rows go to `part` and k_few_join adds them in order.
+struct CafeFewBack {
+    const void *gy, *slope, *x, *w;
+    int64_t ldg, lds, ldx, ldw, ldgx;
+    int kind, M, N, K, rows, vec, vec_out;   // rows: of a block
+    void* gx;
+    float* part;                             // [row blocks][N][K + 1]: gW and, behind it, gb; or null
+};
+template <typename T, int FEW>
+__global__ void __launch_bounds__(128) k_few_back(const CafeFewBack P) {
+    typedef typename CafeSlopeOf<T>::type ST;
+    __shared__ float half[FEW][64][4];
+    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+    const int k = blockIdx.x * 256 + tx * 4, n4 = min(4, P.K - k);
+    const int m0 = blockIdx.y * P.rows, m1 = min(m0 + P.rows, P.M);
+    cafe_next_may_start();
+    float w[FEW][4], acc[FEW][4], gb[FEW];
+#pragma unroll
+    for (int n = 0; n < FEW; ++n) {
+        gb[n] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            acc[n][j] = 0.f;
+            w[n][j] = P.gx && n < P.N && j < n4 ? cafe_to_float(__ldg(static_cast<const T*>(P.w) + n * P.ldw + k + j)) : 0.f;
+        }
+    }
+#pragma unroll 4
+    for (int64_t m = m0 + ty; m < m1; m += 2) {
+        float g[FEW], x[4];
+#pragma unroll
+        for (int n = 0; n < FEW; ++n) {
+            float v = n < P.N ? cafe_to_float(__ldg(static_cast<const T*>(P.gy) + m * P.ldg + n)) : 0.f;
+            if (n < P.N && P.kind == CAFE_SLOPE_VALUES) v *= cafe_to_float(__ldg(static_cast<const ST*>(P.slope) + m * P.lds + n));
+            else if (n < P.N && P.kind == CAFE_SLOPE_OUTPUT) v = cafe_to_float(__ldg(static_cast<const T*>(P.slope) + m * P.lds + n)) > 0.f ? v : 0.f;
+            g[n] = v;
+            gb[n] += v;
+        }
+        if (P.part) {
+            const T* p = static_cast<const T*>(P.x) + m * P.ldx + k;
+            if (P.vec && n4 == 4) {
+                alignas(16) T v[4];
+                if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(v) = __ldg(reinterpret_cast<const uint4*>(p));
+                else *reinterpret_cast<uint2*>(v) = __ldg(reinterpret_cast<const uint2*>(p));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] = cafe_to_float(v[j]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] = P.x && j < n4 ? cafe_to_float(__ldg(p + j)) : 0.f;
+            }
+#pragma unroll
+            for (int n = 0; n < FEW; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[n][j] += g[n] * x[j];
+        }
+        if (P.gx && n4 > 0) {
+            alignas(16) T o[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float s = 0.f;
+#pragma unroll
+                for (int n = 0; n < FEW; ++n) s += g[n] * w[n][j];
+                o[j] = cafe_from_float<T>(s);
+            }
+            T* to = static_cast<T*>(P.gx) + m * P.ldgx + k;
+            if (P.vec_out && n4 == 4) {
+                if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(o);
+                else *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(o);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) if (j < n4) to[j] = o[j];
+            }
+        }
+    }
+    if (!P.part) return;
+    if (ty == 1) {
+#pragma unroll
+        for (int n = 0; n < FEW; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) half[n][tx][j] = acc[n][j];
+    }
+    __shared__ float half_gb[FEW];
+    if (threadIdx.x == 64) {
+#pragma unroll
+        for (int n = 0; n < FEW; ++n) half_gb[n] = gb[n];
+    }
+    __syncthreads();
+    if (ty == 0) {
+#pragma unroll
+        for (int n = 0; n < FEW; ++n) {
+            if (n >= P.N) break;
+            float* to = P.part + ((int64_t)blockIdx.y * P.N + n) * (P.K + 1);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) if (j < n4) to[k + j] = acc[n][j] + half[n][tx][j];
+            if (threadIdx.x == 0 && blockIdx.x == 0) to[P.K] = gb[n] + half_gb[n];
+        }
+    }
+}
+// eight warps share the row blocks of 32 neighbouring sums
+template <typename T>
+__global__ void __launch_bounds__(256) k_few_join(const float* part, int blocks, int N, int K, void* gw, int64_t ldgw, void* gb) {
+    __shared__ float sum[8][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t e = (int64_t)blockIdx.x * 32 + lane, all = (int64_t)N * (K + 1);
+    cafe_next_may_start();
+    float s = 0.f;
+    if (e < all)
+#pragma unroll 4
+        for (int b = warp; b < blocks; b += 8) s += part[b * all + e];
+    sum[warp][lane] = s;
+    __syncthreads();
+    if (warp || e >= all) return;
+#pragma unroll
+    for (int q = 1; q < 8; ++q) s += sum[q][lane];
+    const int n = (int)(e / (K + 1)), k = (int)(e - (int64_t)n * (K + 1));
+    if (k < K) { if (gw) static_cast<T*>(gw)[n * ldgw + k] = cafe_from_float<T>(s); }
+    else if (gb) static_cast<T*>(gb)[n] = cafe_from_float<T>(s);
+}
+// rows of a block: blocks for every SM several times over, but at least 16 rows each
+static int dense_few_rows(int M, int K) {
+    const int64_t across = (K + 255) / 256, want = (148 * 8 + across - 1) / across;
+    int64_t rows = (M + want - 1) / want;
+    rows = rows < 16 ? 16 : rows;
+    if (M > rows * 32768) rows = (M + 32767) / 32768;
+    return (int)rows;
+}
+static int64_t dense_few_back_work(const CafeBackward& f) {
+    if (f.N < 1 || f.N > CAFE_FEW_MOST || f.M < 1 || f.K < 1 || !(f.gw || f.gb)) return 0;
+    const int rows = dense_few_rows(f.M, f.K);
+    return (int64_t)((f.M + rows - 1) / rows) * f.N * (f.K + 1) * 4;
+}
+template <typename T>
+static cudaError_t dense_few_back(const CafeBackward& f, void* work, cudaStream_t st) {
+    CafeFewBack P = {};
+    P.gy = f.gy; P.slope = f.slope; P.x = f.gw ? f.x : nullptr; P.w = f.w;
+    P.ldg = f.ldg; P.lds = f.lds; P.ldx = f.ldx; P.ldw = f.ldw; P.ldgx = f.ldgx;
+    P.kind = f.slope_kind; P.M = f.M; P.N = f.N; P.K = f.K; P.gx = f.gx;
+    P.part = f.gw || f.gb ? (float*)work : nullptr;
+    P.rows = dense_few_rows(f.M, f.K);
+    const int size = sizeof(T);
+    P.vec = P.x && dense_on(f.x, f.ldx, size, 4 * size);
+    P.vec_out = f.gx && dense_on(f.gx, f.ldgx, size, 4 * size);
+    const int blocks = (f.M + P.rows - 1) / P.rows;
+    const dim3 grid((unsigned)((f.K + 255) / 256), (unsigned)blocks);
+    cudaError_t e;
+    if (f.N <= 1) e = dense_start<false>(k_few_back<T, 1>, grid, 128, 0, 1, st, P);
+    else if (f.N <= 4) e = dense_start<false>(k_few_back<T, 4>, grid, 128, 0, 1, st, P);
+    else if (f.N <= 8) e = dense_start<false>(k_few_back<T, 8>, grid, 128, 0, 1, st, P);
+    else e = dense_start<false>(k_few_back<T, 16>, grid, 128, 0, 1, st, P);
+    if (e != cudaSuccess || !P.part) return e;
+    return dense_start<false>(k_few_join<T>, dim3((unsigned)(((int64_t)f.N * (f.K + 1) + 31) / 32)), 256, 0, 1, st, (const float*)P.part, blocks, f.N, f.K, f.gw, f.ldgw, f.gb);
 }
 
 template <typename T>
@@ -585,6 +730,10 @@ static cudaError_t dense_forward(const CafeForward& f, int dtype, void* work, in
 }
 template <typename T>
 static cudaError_t dense_backward(const CafeBackward& f, int dtype, void* work, int64_t work_bytes, cudaStream_t st) {
+    if (f.N >= 1 && f.N <= CAFE_FEW_MOST && f.M >= 1 && f.K >= 1) {
+        const int64_t few = dense_few_back_work(f);
+        if (few == 0 || (work && work_bytes >= few)) return f.gx || few ? dense_few_back<T>(f, work, st) : cudaSuccess;
+    }
     CafeJobs P = {};
     const int size = sizeof(T), ssize = f.slope_kind == CAFE_SLOPE_VALUES ? (int)sizeof(typename CafeSlopeOf<T>::type) : size;
     const int g_vec = dense_on(f.gy, f.ldg, size, 16), s_vec = f.slope_kind != CAFE_SLOPE_NONE && dense_on(f.slope, f.lds, ssize, 16);
@@ -668,7 +817,9 @@ int64_t cafe_linear_backward_work(const void* gy_dev, int64_t ldg, int slope_kin
     CafeBackward f = {};
     f.gy = gy_dev; f.ldg = ldg; f.slope_kind = slope_kind; f.x = x_dev; f.ldx = ldx; f.w = w_dev; f.ldw = ldw; f.M = M; f.N = N; f.K = K;
     f.gx = want_gx ? (void*)k_aligned : nullptr; f.gw = want_gw ? (void*)k_aligned : nullptr; f.gb = want_gb ? (void*)k_aligned : nullptr;
-    return dense_type_ok(dtype) && dense_sizes_ok(M, N, K) ? cafe_tiles_backward_work(f, dtype) : 0;
+    if (!dense_type_ok(dtype) || !dense_sizes_ok(M, N, K)) return 0;
+    const int64_t few = dense_few_back_work(f);
+    return few ? few : cafe_tiles_backward_work(f, dtype);
 }
 
 int cafe_linear_backward(const void* gy_dev, int64_t ldg, const void* slope_dev, int64_t lds, int slope_kind, const void* x_dev, int64_t ldx,

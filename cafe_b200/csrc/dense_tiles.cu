@@ -74,6 +74,7 @@ __global__ void __launch_bounds__(256) k_parts(const __grid_constant__ CafeParts
     float sum[8] = {};
     const int per = cafe_parts_rows(J.rows, J.cols);
     const int64_t r0 = (int64_t)by * per, r1 = min(r0 + per, (int64_t)J.rows);
+    cafe_next_may_start();
     if (n > 0) {
 #pragma unroll 4
         for (int64_t r = r0 + warp; r < r1; r += 8) {
@@ -171,6 +172,7 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
         cafe_fence_barrier_init();
         bail = 0;
     }
+    cafe_next_may_start();
     if (warp == 1) cafe_tm_alloc(cafe_smem(&tm_at), Sh::tm_cols);
     cafe_tc_before();
     __syncthreads();
@@ -467,7 +469,7 @@ template <int I> __device__ __forceinline__ void cafe_row_put(const float* acc, 
 }
 
 template <typename T, int BN>
-__global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) __cluster_dims__(2, 1, 1) k_tiles_pair(const __grid_constant__ CafeTilesArgs P) {
+__global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) k_tiles_pair(const __grid_constant__ CafeTilesArgs P) {
     typedef CafeTiles<T> L;
     typedef CafePairShape<T, BN> Sh;
     typedef typename CafeSlopeOf<T>::type ST;
@@ -498,11 +500,13 @@ __global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) __cluster_dims__(2, 1, 1
         cafe_fence_barrier_init();
         bail = 0;
     }
+    cafe_next_may_start();
     if (warp == 1) cafe_tm_alloc2(cafe_smem(&tm_at), Sh::sets * Sh::tm_set);
     cafe_tc_before();
     __syncthreads();
     cafe_cluster_sync();
     cafe_tc_after();
+    cafe_wait_for_earlier();
     const uint32_t tmem = tm_at;
 
     if (warp == 0) {
@@ -771,18 +775,7 @@ static cudaError_t tiles_launch_bn(CafeTilesArgs& P, const TilesOperand& a, cons
     static std::atomic<uint64_t> allowed{0};
     const cudaError_t e = dense_allow_shared((const void*)k_tiles<T, BN>, bytes, &allowed);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(P.job.tiles * P.splits));
-    cfg.blockDim = dim3(CAFE_TILES_THREADS);
-    cfg.dynamicSmemBytes = bytes;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)P.splits; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    CAFE_PROF(CAFE_P_LINEAR, st);
-    return cudaLaunchKernelEx(&cfg, k_tiles<T, BN>, (const CafeTilesArgs&)P);
+    return dense_start<false>(k_tiles<T, BN>, dim3((unsigned)(P.job.tiles * P.splits)), CAFE_TILES_THREADS, bytes, P.splits, st, P);
 }
 template <typename T, int BN>
 static cudaError_t tiles_launch_pair(CafeTilesArgs& P, const TilesOperand& a, const TilesOperand& b, cudaStream_t st) {
@@ -793,14 +786,13 @@ static cudaError_t tiles_launch_pair(CafeTilesArgs& P, const TilesOperand& a, co
     static std::atomic<uint64_t> allowed{0};
     const cudaError_t e = dense_allow_shared((const void*)k_tiles_pair<T, BN>, bytes, &allowed);
     if (e != cudaSuccess) return e;
-    CAFE_PROF(CAFE_P_LINEAR, st);
-    k_tiles_pair<T, BN><<<2 * (P.job.tiles < 74 ? P.job.tiles : 74), CAFE_PAIR_THREADS, bytes, st>>>(P);
-    return cudaGetLastError();
+    return dense_start<true>(k_tiles_pair<T, BN>, dim3(2u * (P.job.tiles < 74 ? P.job.tiles : 74)), CAFE_PAIR_THREADS, bytes, 2, st, P);
 }
 // Pairs of blocks through tile after tile, or two blocks an SM and clusters that share a tile's depth: whichever estimate is less,
-// in turns of a 128 x 128 tile at the tensor cores' full rate.  A pair's turn takes 1.2 (fp32) or, 256 columns wide, 2.35 (16 bits)
-// of these, a tile 3 more and a launch 14; two blocks on an SM share its tensor cores and wait for their boxes, 2.7 (fp32) or 2.2 a
-// turn of 128 columns each, and cost 14 a tile, one alone 1.7.  296, 296, 284 and 264 blocks run at a time in clusters of 1, 2, 4
+// in turns of a 128 x 128 tile at the tensor cores' full rate.  A pair's turn takes 1.2 (fp32) or, 256 columns wide, 2.7 (16 bits)
+// of these, a tile 3 more and a launch 14; two blocks on an SM share its tensor cores and wait for their boxes, 2.7 (fp32) or 3.3 a
+// turn of 128 columns each, and cost 14 a tile, one alone 1.7 or 2.  (Measured both ways: 4096x4096x4096 bf16 pairs 105 us, clusters
+// 129; 2048x1024x1024 bf16 24.6 and 22.6; 65536x479x1024 fp32 364 and 433; 2048x1024x512 fp32 40 and 36.)  296, 296, 284 and 264 blocks run at a time in clusters of 1, 2, 4
 // and 8 (what the device says).
 template <typename T>
 static cudaError_t tiles_launch(CafeTilesArgs& P, const TilesOperand& a, const TilesOperand& b, cudaStream_t st) {
@@ -815,11 +807,11 @@ static cudaError_t tiles_launch(CafeTilesArgs& P, const TilesOperand& a, const T
     double best = 1e300;
     for (int s = 0; s < 4; ++s) {
         const int64_t blocks = tiles << s, rounds = (blocks + room[s] - 1) / room[s];
-        const double est = (double)rounds * ((blocks > 148 ? split ? 2.7 : 2.2 : 1.7) * (bn / 128) * ((turns + (1 << s) - 1) >> s) + 14 + s);
+        const double est = (double)rounds * ((blocks > 148 ? split ? 2.7 : 3.3 : split ? 1.7 : 2.0) * (bn / 128) * ((turns + (1 << s) - 1) >> s) + 14 + s);
         if (est < best * 0.999) { best = est; P.splits = 1 << s; }
     }
     const int64_t rounds = (((rows + 255) / 256) * wide_tiles + 73) / 74;
-    const bool pair = P.job.depth > 0 && (double)rounds * ((split ? 1.2 : wide ? 2.35 : 2.2) * turns + 3) + 14 < best;
+    const bool pair = P.job.depth > 0 && (double)rounds * ((split ? 1.2 : wide ? 2.7 : 2.2) * turns + 3) + 14 < best;
     if (pair && P.sums) {   // the bias gradient by itself
         CafeTilesArgs G = P;
         G.job.depth = G.job.cols = 0;
@@ -869,13 +861,11 @@ static cudaError_t tiles_parts(const CafeParts& P, cudaStream_t st) {
     int blocks = 0;
     for (int q = 0; q < P.count; ++q) blocks += P.job[q].blocks;
     if (blocks == 0) return cudaSuccess;
-    CAFE_PROF(CAFE_P_LINEAR, st);
-    k_parts<T><<<blocks, 256, 0, st>>>(P);
-    return cudaGetLastError();
+    return dense_start<false>(k_parts<T>, dim3((unsigned)blocks), 256, 0, 1, st, P);
 }
 
 // Which calls: products of at least CAFE_TILES_LEAST multiply-adds that are no narrow strips.
-#define CAFE_TILES_LEAST (1ll << 29)
+#define CAFE_TILES_LEAST (1ll << 27)
 // (Sums over more than 2^17 of k in one go, 2^20 over the blocks of a cluster, would lose bits of a 16-bit result.)
 static bool tiles_large(int M, int N, int K) {
     return (int64_t)M * N * K >= CAFE_TILES_LEAST && M >= 128 && N >= 64 && K >= 64 && M <= 1 << 20 && N <= 1 << 17 && K <= 1 << 17;

@@ -26,6 +26,12 @@ static __device__ __noinline__ bool cafe_bar_wait_on(uint32_t bar, uint32_t pari
     return true;
 }
 
+// Launches that follow one another closely: the next kernel of the stream may start once all blocks of this one have, and does what
+// does not depend on it; nothing that another kernel wrote is read, and nothing is written, before the wait, which ends when all
+// kernels before this one are done.
+__device__ __forceinline__ void cafe_next_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void cafe_wait_for_earlier() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // One lane of the warp, all of whose lanes are here.  Copies, products and commits go inside a branch on it: what the instructions
 // take then stays in uniform registers.  (A lane-0 predicate on every instruction cost 45 cycles each: 1410 cycles for the twelve
 // products of 64 cycles of a turn, 910 with one branch around them.)

@@ -25,7 +25,7 @@ _NONE, _RELU = 0, 1
 _SLOPE_NONE, _SLOPE_VALUES, _SLOPE_OUTPUT = 0, 1, 2
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_SIZE, MAX_LAYERS = 8388608, 32
-_LARGE = 1 << 28   # below so many multiply-adds no call takes workspace (cafe_linear_*_work then gives 0): not asked
+_LARGE, _FEW = 1 << 27, 16   # no call of fewer multiply-adds takes workspace (its size is 0), but a backward of few outputs: not asked
 
 
 _get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)   # (without the checks of the public form)
@@ -157,7 +157,7 @@ def _linear_backward(ctx, grad_y):
             gb = torch.empty(n, dtype=dtype, device=device)
         lib, t, pg, px, pw = _lib.load(), DTYPES[dtype], g.data_ptr(), _ptr(x), _ptr(w)
         size = 0
-        if m * n * k >= _LARGE:
+        if n <= _FEW or m * n * k >= _LARGE:
             size = lib.cafe_linear_backward_work(pg, ldg, ctx.kind, px, ldx, pw, ldw, m, n, k, t, need_x, need_w, need_b)
         with _on(device) as stream:
             status = lib.cafe_linear_backward(pg, ldg, _ptr(slope), n, ctx.kind, px, ldx, pw, ldw, m, n, k, t, _ptr(gx), k, _ptr(gw), k, _ptr(gb),

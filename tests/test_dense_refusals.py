@@ -41,7 +41,7 @@ def test_mlp_arguments():
 
     def backward(work=P, size=need, slopes=slopes):
         return lib.cafe_mlp_backward(2, widths, 3, P, 6, P, 4, ptrs, lds, acts, 0, ptrs, pitch, slopes, P, 4, ptrs, ptrs, work, size, None)
-    assert backward(size=need - 1) == ERR_ARG
+    assert backward(size=2 * 3 * 5 * 4 - 1) == ERR_ARG   # (less than the gradients between the layers take)
     assert backward(work=None) == ERR_ARG
     assert backward(work=P + 4) == ERR_ARG
     assert backward(slopes=None) == ERR_ARG    # a sigmoid needs its slope
