@@ -468,8 +468,32 @@ template <int I> __device__ __forceinline__ void cafe_row_put(const float* acc, 
         cafe_put16(cafe_staged<128>(at, lane, c / 4), __float_as_uint(acc[I + c]), __float_as_uint(acc[I + c + 1]), __float_as_uint(acc[I + c + 2]), __float_as_uint(acc[I + c + 3]));
 }
 
+struct CafePairArgs {
+    CUtensorMap a[2], b[2];
+    CafeJob job[2];      // the longer tiles first
+    int count;
+    const float* sums;   // [sum_rows][gb_cols]: partial sums of a bias gradient, added up on the way
+    int sum_rows, gb_cols;
+    void* gb;
+    int share[75];
+};
+// A backward's two products are one launch.  The first one's tiles (the longer) go round the pairs; the second one's are handed out
+// so that all pairs end at about the same time, pair p has those from share[p] to share[p + 1]: 2048x1024x1024 takes the time of gW
+// alone (backward 84 us as two launches, 70 as one).
+struct CafePairTiles {
+    int first, step, own, from, all;   // tiles of the first product: first, first + step, .. `own` of them; of the second: from, from + 1, ..
+    __device__ __forceinline__ CafePairTiles(const CafePairArgs& P, int pair, int pairs) {
+        first = pair; step = pairs;
+        own = pair < P.job[0].tiles ? (P.job[0].tiles - pair + pairs - 1) / pairs : 0;
+        from = P.share[pair];
+        all = own + P.share[pair + 1] - from;
+    }
+    __device__ __forceinline__ int which(int n) const { return n >= own; }
+    __device__ __forceinline__ int tile(int n) const { return n < own ? first + n * step : from + n - own; }
+};
+
 template <typename T, int BN>
-__global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) k_tiles_pair(const __grid_constant__ CafeTilesArgs P) {
+__global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) k_tiles_pair(const __grid_constant__ CafePairArgs P) {
     typedef CafeTiles<T> L;
     typedef CafePairShape<T, BN> Sh;
     typedef typename CafeSlopeOf<T>::type ST;
@@ -488,9 +512,8 @@ __global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) k_tiles_pair(const __gri
     auto tile_taken = [&](int g) { return more + 32u + 8u * g; };
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cafe_cluster_rank();
-    const CafeJob& J = P.job;
-    const int turns = (J.depth + L::BK - 1) / L::BK, tiles = J.tiles;
-    const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const CafePairTiles list(P, pair, pairs);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < Sh::stages; ++s) { cafe_bar_init(full(s), 2 - rank); cafe_bar_init(empty(s), 1); }   // (block 0: its boxes and the other's)
@@ -515,21 +538,25 @@ __global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) k_tiles_pair(const __gri
         int s = 0;
         uint32_t phase = 1;   // (a fresh barrier's phase before its first counts as over)
         int64_t u = 0;
-        for (int tile = first; tile < tiles && fine; tile += step) {
+        for (int n = 0; n < list.all && fine; ++n) {
+            const int which = list.which(n), tile = list.tile(n);
+            const CafeJob& J = P.job[which];
+            const CUtensorMap *ma = &P.a[which], *mb = &P.b[which];
             const int tm = tile / J.tiles_n, row0 = tm * 256 + rank * 128, col0 = (tile - tm * J.tiles_n) * BN + rank * (BN / 2);
+            const int a_kc = J.a_kc, b_kc = J.b_kc;
             for (int k0 = 0; k0 < J.depth; k0 += L::BK, ++u) {
                 if (!(fine = __all_sync(0xffffffffu, cafe_bar_wait(empty(s), phase, &bail)))) break;
                 const uint32_t a = base + s * Sh::stage, b = a + L::parts * Sh::a_part, bar = full(s);
                 if (cafe_elect()) {
                     cafe_bar_expect(bar, Sh::stage);
-                    if (J.a_kc) cafe_box_load(a, &P.a, k0, row0, 0, bar);
+                    if (a_kc) cafe_box_load(a, ma, k0, row0, 0, bar);
                     else
 #pragma unroll
-                        for (int q = 0; q < CAFE_LIN_BM / 64; ++q) cafe_box_load(a + q * L::parts * L::BK * 128, &P.a, row0 + 64 * q, k0, 0, bar);
-                    if (J.b_kc) cafe_box_load(b, &P.b, k0, col0, 0, bar);
+                        for (int q = 0; q < CAFE_LIN_BM / 64; ++q) cafe_box_load(a + q * L::parts * L::BK * 128, ma, row0 + 64 * q, k0, 0, bar);
+                    if (b_kc) cafe_box_load(b, mb, k0, col0, 0, bar);
                     else
 #pragma unroll
-                        for (int q = 0; q < BN / 128; ++q) cafe_box_load(b + q * L::parts * L::BK * 128, &P.b, col0 + 64 * q, k0, 0, bar);
+                        for (int q = 0; q < BN / 128; ++q) cafe_box_load(b + q * L::parts * L::BK * 128, mb, col0 + 64 * q, k0, 0, bar);
                 }
                 if (++s == Sh::stages) { s = 0; phase ^= 1u; }
             }
@@ -543,25 +570,29 @@ __global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) k_tiles_pair(const __gri
             int s = 0;
             uint32_t phase = 0;
             bool fine = true;
-            for (int tile = first; tile < tiles && fine; tile += step)
+            for (int n = 0; n < list.all && fine; ++n) {
+                const int turns = (P.job[list.which(n)].depth + L::BK - 1) / L::BK;
                 for (int t = 0; t < turns; ++t) {
                     if (!(fine = cafe_bar_wait(full(s), phase, &bail))) break;
                     cafe_bar_arrive_at(cafe_cluster_map(full(s), 0));
                     if (++s == Sh::stages) { s = 0; phase ^= 1u; }
                 }
+            }
         }
     } else if (warp == 1) {
         // ---- products
-        const uint32_t instr = cafe_mma_instr(L::type, 256, BN) | (J.a_kc ? 0u : 1u << 15) | (J.b_kc ? 0u : 1u << 16);
-        const uint64_t da = J.a_kc ? cafe_operand<Sh::rowb>(base) : cafe_operand_mn(base, L::parts * L::BK * 128);
-        const uint64_t db = J.b_kc ? cafe_operand<Sh::rowb>(base + L::parts * Sh::a_part) : cafe_operand_mn(base + L::parts * Sh::a_part, L::parts * L::BK * 128);
-        // offsets in 16-byte units: from a part to the next, from 16 k to the next 16
-        const uint32_t ap = (J.a_kc ? Sh::a_part : L::BK * 128) >> 4, bp = (J.b_kc ? Sh::b_part : L::BK * 128) >> 4;
-        const uint32_t ak = (J.a_kc ? 32 : 2048) >> 4, bk = (J.b_kc ? 32 : 2048) >> 4;
         bool fine = true;
         int s = 0, n = 0;
         uint32_t phase = 0, chunk_phase = 0;
-        for (int tile = first; tile < tiles && fine; tile += step, ++n) {
+        for (; n < list.all && fine; ++n) {
+            const CafeJob& J = P.job[list.which(n)];
+            const int turns = (J.depth + L::BK - 1) / L::BK;
+            const uint32_t instr = cafe_mma_instr(L::type, 256, BN) | (J.a_kc ? 0u : 1u << 15) | (J.b_kc ? 0u : 1u << 16);
+            const uint64_t da = J.a_kc ? cafe_operand<Sh::rowb>(base) : cafe_operand_mn(base, L::parts * L::BK * 128);
+            const uint64_t db = J.b_kc ? cafe_operand<Sh::rowb>(base + L::parts * Sh::a_part) : cafe_operand_mn(base + L::parts * Sh::a_part, L::parts * L::BK * 128);
+            // offsets in 16-byte units: from a part to the next, from 16 k to the next 16
+            const uint32_t ap = (J.a_kc ? Sh::a_part : L::BK * 128) >> 4, bp = (J.b_kc ? Sh::b_part : L::BK * 128) >> 4;
+            const uint32_t ak = (J.a_kc ? 32 : 2048) >> 4, bk = (J.b_kc ? 32 : 2048) >> 4;
             const int g = n % Sh::sets;
             const uint32_t sums = tmem + g * Sh::tm_set;
             if (n >= Sh::sets && !(fine = __all_sync(0xffffffffu, cafe_bar_wait(tile_taken(g), (uint32_t)(n / Sh::sets - 1) & 1u, &bail)))) break;
@@ -606,9 +637,24 @@ __global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) k_tiles_pair(const __gri
         const uint32_t lanes = (uint32_t)rows << 16;
         uint32_t chunk_phase = 0;
         bool fine = true;
+        if (P.sums) {
+            const int c = blockIdx.x * 256 + (int)threadIdx.x - 64;
+            if (c < P.gb_cols) {
+                float x[4] = {0.f, 0.f, 0.f, 0.f};
+                int q = 0;
+                for (; q + 4 <= P.sum_rows; q += 4)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] += __ldg(P.sums + (int64_t)(q + i) * P.gb_cols + c);
+                for (; q < P.sum_rows; ++q) x[0] += __ldg(P.sums + (int64_t)q * P.gb_cols + c);
+                static_cast<T*>(P.gb)[c] = cafe_from_float<T>((x[0] + x[1]) + (x[2] + x[3]));
+            }
+            __syncwarp();
+        }
         // fp32: every tile, the warp's half of the columns; 16 bits: every other tile, all of them
-        int n = L::parts == 3 ? 0 : half;
-        for (int tile = first + n * step; tile < tiles; tile += L::parts == 3 ? step : 2 * step, n += L::parts == 3 ? 1 : 2) {
+        for (int n = L::parts == 3 ? 0 : half; n < list.all; n += L::parts == 3 ? 1 : 2) {
+            const int tile = list.tile(n);
+            const CafeJob& J = P.job[list.which(n)];
+            const int turns = (J.depth + L::BK - 1) / L::BK;
             const int g = n % Sh::sets, tm = tile / J.tiles_n, col0 = (tile - tm * J.tiles_n) * BN + (L::parts == 3 ? half * Sh::mine : 0);
             const int64_t row0 = (int64_t)tm * 256 + rank * 128 + rows;
             const int m = (int)max((int64_t)0, min((int64_t)32, J.rows - row0)), columns = max(0, min(Sh::mine, J.cols - col0));
@@ -777,52 +823,147 @@ static cudaError_t tiles_launch_bn(CafeTilesArgs& P, const TilesOperand& a, cons
     if (e != cudaSuccess) return e;
     return dense_start<false>(k_tiles<T, BN>, dim3((unsigned)(P.job.tiles * P.splits)), CAFE_TILES_THREADS, bytes, P.splits, st, P);
 }
+// One product of a call: its job, its operands, and for gW where the bias gradient's partial sums are
+struct TilesProduct {
+    CafeJob job;
+    TilesOperand a, b;
+};
+struct TilesSums {
+    const float* at;
+    int rows, cols;
+    void* gb;
+};
+// what a pair's tile of a product takes, in the units of the estimates below
+template <typename T> static double tiles_pair_cost(const CafeJob& J, int bn) {
+    return (CafeTiles<T>::parts == 3 ? 1.2 : bn == 256 ? 2.7 : 2.2) * ((J.depth + CafeTiles<T>::BK - 1) / CafeTiles<T>::BK) + 3;
+}
+// The second product's tiles handed out to 74 pairs that have the first one's in turn: the least time in which all are done (by
+// bisection), and who has how many (share may be null).
+static double tiles_share(int64_t tiles0, double cost0, int64_t tiles1, double cost1, int pairs, int* share) {
+    double lo = 0, hi = cost0 * (double)((tiles0 + pairs - 1) / pairs) + cost1 * (double)((tiles1 + pairs - 1) / pairs);
+    auto room = [&](double t, int p) {
+        const double left = t - cost0 * (double)(tiles0 > p ? (tiles0 - p + pairs - 1) / pairs : 0);
+        return left > 0 ? (int64_t)(left / cost1 + 1e-9) : 0;
+    };
+    for (int i = 0; i < 24; ++i) {
+        const double t = 0.5 * (lo + hi);
+        int64_t n = 0;
+        for (int p = 0; p < pairs; ++p) n += room(t, p);
+        if (n >= tiles1) hi = t; else lo = t;
+    }
+    if (share) {
+        int64_t at = 0;
+        for (int p = 0; p < pairs; ++p) {
+            share[p] = (int)at;
+            at += room(hi, p);
+            at = at > tiles1 ? tiles1 : at;
+        }
+        share[pairs] = (int)tiles1;   // (room for all by construction)
+    }
+    const double first = cost0 * (double)((tiles0 + pairs - 1) / pairs);
+    return hi > first ? hi : first;
+}
 template <typename T, int BN>
-static cudaError_t tiles_launch_pair(CafeTilesArgs& P, const TilesOperand& a, const TilesOperand& b, cudaStream_t st) {
-    if (!tiles_map<T>(&P.a, a, P.job.a_kc, CAFE_LIN_BM) || !tiles_map<T>(&P.b, b, P.job.b_kc, BN / 2)) return cudaErrorInvalidValue;
-    P.job.tiles_n = (P.job.cols + BN - 1) / BN;
-    P.job.tiles = ((P.job.rows + 255) / 256) * P.job.tiles_n;
+static cudaError_t tiles_launch_pair(TilesProduct* q, int count, const TilesSums& sums, cudaStream_t st) {
+    CafePairArgs P = {};
+    P.count = count;
+    int tiles = 0;
+    for (int i = 0; i < count; ++i) {
+        CafeJob& J = q[i].job;
+        if (!tiles_map<T>(&P.a[i], q[i].a, J.a_kc, CAFE_LIN_BM) || !tiles_map<T>(&P.b[i], q[i].b, J.b_kc, BN / 2)) return cudaErrorInvalidValue;
+        J.tiles_n = (J.cols + BN - 1) / BN;
+        J.tiles = ((J.rows + 255) / 256) * J.tiles_n;
+        tiles += J.tiles;
+        P.job[i] = J;
+    }
+    int pairs = tiles < 74 ? tiles : 74;
+    if (sums.at) {
+        P.sums = sums.at; P.sum_rows = sums.rows; P.gb_cols = sums.cols; P.gb = sums.gb;
+        const int least = (sums.cols + 511) / 512;   // (256 columns a block)
+        pairs = pairs < least ? least : pairs;
+    }
+    if (count == 2) tiles_share(P.job[0].tiles, tiles_pair_cost<T>(P.job[0], BN), P.job[1].tiles, tiles_pair_cost<T>(P.job[1], BN), pairs, P.share);
     constexpr int bytes = CafePairShape<T, BN>::bytes;
     static std::atomic<uint64_t> allowed{0};
     const cudaError_t e = dense_allow_shared((const void*)k_tiles_pair<T, BN>, bytes, &allowed);
     if (e != cudaSuccess) return e;
-    return dense_start<true>(k_tiles_pair<T, BN>, dim3(2u * (P.job.tiles < 74 ? P.job.tiles : 74)), CAFE_PAIR_THREADS, bytes, 2, st, P);
+    return dense_start<true>(k_tiles_pair<T, BN>, dim3(2u * pairs), CAFE_PAIR_THREADS, bytes, 2, st, P);
 }
 // Pairs of blocks through tile after tile, or two blocks an SM and clusters that share a tile's depth: whichever estimate is less,
 // in turns of a 128 x 128 tile at the tensor cores' full rate.  A pair's turn takes 1.2 (fp32) or, 256 columns wide, 2.7 (16 bits)
 // of these, a tile 3 more and a launch 14; two blocks on an SM share its tensor cores and wait for their boxes, 2.7 (fp32) or 3.3 a
 // turn of 128 columns each, and cost 14 a tile, one alone 1.7 or 2.  (Measured both ways: 4096x4096x4096 bf16 pairs 105 us, clusters
-// 129; 2048x1024x1024 bf16 24.6 and 22.6; 65536x479x1024 fp32 364 and 433; 2048x1024x512 fp32 40 and 36.)  296, 296, 284 and 264 blocks run at a time in clusters of 1, 2, 4
-// and 8 (what the device says).
-template <typename T>
-static cudaError_t tiles_launch(CafeTilesArgs& P, const TilesOperand& a, const TilesOperand& b, cudaStream_t st) {
-    typedef CafeTiles<T> L;
-    constexpr bool split = L::parts == 3;
-    const bool wide = !split && P.job.cols > 128;
-    const int bn = wide ? 256 : 128;
-    const int64_t rows = P.job.rows, cols = P.job.cols;
-    const int64_t wide_tiles = cols > 0 ? (cols + bn - 1) / bn : 1, tiles = ((rows + CAFE_LIN_BM - 1) / CAFE_LIN_BM) * wide_tiles;
-    const int turns = (P.job.depth + L::BK - 1) / L::BK;
+// 129; 2048x1024x1024 bf16 24.6 and 22.6; 65536x479x1024 fp32 364 and 433; 2048x1024x512 fp32 40 and 36.)  296, 296, 284 and 264
+// blocks run at a time in clusters of 1, 2, 4 and 8 (what the device says).
+template <typename T> static double tiles_estimate_clusters(const CafeJob& J, int* splits) {
+    constexpr bool split = CafeTiles<T>::parts == 3;
+    const int bn = !split && J.cols > 128 ? 256 : 128;
+    const int64_t tiles = (int64_t)((J.rows + CAFE_LIN_BM - 1) / CAFE_LIN_BM) * (J.cols > 0 ? (J.cols + bn - 1) / bn : 1);
+    const int turns = (J.depth + CafeTiles<T>::BK - 1) / CafeTiles<T>::BK;
     static const int room[4] = {296, 296, 284, 264};
     double best = 1e300;
     for (int s = 0; s < 4; ++s) {
         const int64_t blocks = tiles << s, rounds = (blocks + room[s] - 1) / room[s];
         const double est = (double)rounds * ((blocks > 148 ? split ? 2.7 : 3.3 : split ? 1.7 : 2.0) * (bn / 128) * ((turns + (1 << s) - 1) >> s) + 14 + s);
-        if (est < best * 0.999) { best = est; P.splits = 1 << s; }
+        if (est < best * 0.999) { best = est; *splits = 1 << s; }
     }
-    const int64_t rounds = (((rows + 255) / 256) * wide_tiles + 73) / 74;
-    const bool pair = P.job.depth > 0 && (double)rounds * ((split ? 1.2 : wide ? 2.7 : 2.2) * turns + 3) + 14 < best;
-    if (pair && P.sums) {   // the bias gradient by itself
-        CafeTilesArgs G = P;
-        G.job.depth = G.job.cols = 0;
-        G.splits = 1;
-        const cudaError_t e = tiles_launch_bn<T, 128>(G, a, b, st);
+    return best;
+}
+template <typename T> static double tiles_estimate_pairs(const TilesProduct* q, int count, int bn) {
+    double cost[2];
+    int64_t tiles[2];
+    for (int i = 0; i < count; ++i) {
+        const CafeJob& J = q[i].job;
+        if (J.depth == 0 || J.cols == 0) return 1e300;
+        cost[i] = tiles_pair_cost<T>(J, bn);
+        tiles[i] = (int64_t)((J.rows + 255) / 256) * ((J.cols + bn - 1) / bn);
+    }
+    if (count == 1) return (double)((tiles[0] + 73) / 74) * cost[0] + 14;
+    const int a = cost[0] < cost[1];
+    return tiles_share(tiles[a], cost[a], tiles[!a], cost[!a], 74, nullptr) + 14;
+}
+template <typename T>
+static cudaError_t tiles_launch_clusters(const TilesProduct& q, int splits, const TilesSums& sums, cudaStream_t st) {
+    CafeTilesArgs P = {};
+    P.job = q.job;
+    P.splits = splits;
+    P.sums = sums.at; P.sum_rows = sums.rows;
+    if constexpr (CafeTiles<T>::parts == 1) {
+        if (q.job.cols > 128) return tiles_launch_bn<T, 256>(P, q.a, q.b, st);
+    }
+    return tiles_launch_bn<T, 128>(P, q.a, q.b, st);
+}
+// `count` products; the partial sums, if any, belong to the first
+template <typename T>
+static cudaError_t tiles_launch(TilesProduct* q, int count, const TilesSums& sums, cudaStream_t st) {
+    const TilesSums none = {};
+    bool wide = false;
+    if constexpr (CafeTiles<T>::parts == 1)
+        for (int i = 0; i < count; ++i) wide |= q[i].job.cols > 128;
+    const int bn = wide ? 256 : 128;
+    double apart = 0, each[2];
+    int splits[2];
+    for (int i = 0; i < count; ++i) {
+        const double c = tiles_estimate_clusters<T>(q[i].job, &splits[i]), p = tiles_estimate_pairs<T>(q + i, 1, bn);
+        each[i] = p;
+        apart += c < p ? c : p;
+        if (c < p) each[i] = 1e300;
+    }
+    auto pair = [&](TilesProduct* p, int n, const TilesSums& s) {
+        if constexpr (CafeTiles<T>::parts == 1) {
+            if (wide) return tiles_launch_pair<T, 256>(p, n, s, st);
+        }
+        return tiles_launch_pair<T, 128>(p, n, s, st);
+    };
+    if (count == 2 && tiles_estimate_pairs<T>(q, 2, bn) < apart) {
+        if (q[1].job.depth > q[0].job.depth) { const TilesProduct t = q[0]; q[0] = q[1]; q[1] = t; }
+        return pair(q, 2, sums);
+    }
+    for (int i = 0; i < count; ++i) {
+        const cudaError_t e = each[i] < 1e300 ? pair(q + i, 1, i ? none : sums) : tiles_launch_clusters<T>(q[i], splits[i], i ? none : sums, st);
         if (e != cudaSuccess) return e;
     }
-    if constexpr (!split) {
-        if (wide) return pair ? tiles_launch_pair<T, 256>(P, a, b, st) : tiles_launch_bn<T, 256>(P, a, b, st);
-    }
-    return pair ? tiles_launch_pair<T, 128>(P, a, b, st) : tiles_launch_bn<T, 128>(P, a, b, st);
+    return cudaSuccess;
 }
 
 static int64_t tiles_round(int64_t bytes) { return (bytes + 255) & ~(int64_t)255; }
@@ -864,20 +1005,22 @@ static cudaError_t tiles_parts(const CafeParts& P, cudaStream_t st) {
     return dense_start<false>(k_parts<T>, dim3((unsigned)blocks), 256, 0, 1, st, P);
 }
 
-// Which calls: products of at least CAFE_TILES_LEAST multiply-adds that are no narrow strips.
-#define CAFE_TILES_LEAST (1ll << 27)
+// Which calls: products of at least so many multiply-adds (the two of a backward share what is laid out: 1777x367x511 in fp16 forward
+// 28 us by this file, 21 by dense_cuda.cu's kernel, backward 45 and 50) that are no narrow strips.
+#define CAFE_TILES_LEAST (1ll << 29)
+#define CAFE_TILES_LEAST_BACK (1ll << 27)
 // (Sums over more than 2^17 of k in one go, 2^20 over the blocks of a cluster, would lose bits of a 16-bit result.)
-static bool tiles_large(int M, int N, int K) {
-    return (int64_t)M * N * K >= CAFE_TILES_LEAST && M >= 128 && N >= 64 && K >= 64 && M <= 1 << 20 && N <= 1 << 17 && K <= 1 << 17;
+static bool tiles_large(int M, int N, int K, int64_t least) {
+    return (int64_t)M * N * K >= least && M >= 128 && N >= 64 && K >= 64 && M <= 1 << 20 && N <= 1 << 17 && K <= 1 << 17;
 }
 
 int64_t cafe_tiles_forward_work(const CafeForward& f, int dtype) {
-    if (!tiles_large(f.M, f.N, f.K)) return 0;
+    if (!tiles_large(f.M, f.N, f.K, CAFE_TILES_LEAST)) return 0;
     const int parts = dtype == CAFE_F32 ? 3 : 1;
     return 256 + (tiles_in_place(dtype, f.x, f.ldx) ? 0 : tiles_bytes(parts, f.M, f.K)) + (tiles_in_place(dtype, f.w, f.ldw) ? 0 : tiles_bytes(parts, f.N, f.K));
 }
 int64_t cafe_tiles_backward_work(const CafeBackward& f, int dtype) {
-    if (!tiles_large(f.M, f.N, f.K) || (!f.gx && !f.gw)) return 0;
+    if (!tiles_large(f.M, f.N, f.K, CAFE_TILES_LEAST_BACK) || (!f.gx && !f.gw)) return 0;
     const int parts = dtype == CAFE_F32 ? 3 : 1;
     int64_t need = 256;
     if (f.slope_kind != CAFE_SLOPE_NONE || !tiles_in_place(dtype, f.gy, f.ldg)) need += tiles_bytes(parts, f.M, f.N);
@@ -894,9 +1037,8 @@ static cudaError_t tiles_forward(const CafeForward& f, int dtype, const CafeJob&
     const TilesOperand w = tiles_operand<T>(&parts, &work, dtype, f.w, f.ldw, f.N, f.K, nullptr, 0, CAFE_SLOPE_NONE, nullptr);
     cudaError_t e = tiles_parts<T>(parts, st);
     if (e != cudaSuccess) return e;
-    CafeTilesArgs P = {};
-    P.job = job;
-    return tiles_launch<T>(P, x, w, st);
+    TilesProduct q = {job, x, w};
+    return tiles_launch<T>(&q, 1, TilesSums{}, st);
 }
 template <typename T>
 static cudaError_t tiles_backward(const CafeBackward& f, int dtype, const CafeJob* gw, const CafeJob* gx, char* work, cudaStream_t st) {
@@ -913,19 +1055,15 @@ static cudaError_t tiles_backward(const CafeBackward& f, int dtype, const CafeJo
     if (f.gw) x = tiles_operand<T>(&parts, &work, dtype, f.x, f.ldx, f.M, f.K, nullptr, 0, CAFE_SLOPE_NONE, nullptr);
     cudaError_t e = tiles_parts<T>(parts, st);
     if (e != cudaSuccess) return e;
-    if (gw) {
-        CafeTilesArgs P = {};
-        P.job = *gw;
-        if (!f.gw) P.job.depth = 0;
-        P.sums = sums; P.sum_rows = sum_rows;
-        if ((e = tiles_launch<T>(P, g, x, st)) != cudaSuccess) return e;
+    TilesProduct q[2];
+    int count = 0;
+    if (gw) {   // (without gW wanted: no columns, no depth, the bias gradient alone)
+        q[count] = {*gw, g, x};
+        if (!f.gw) q[count].job.depth = 0;
+        ++count;
     }
-    if (gx) {
-        CafeTilesArgs P = {};
-        P.job = *gx;
-        if ((e = tiles_launch<T>(P, g, w, st)) != cudaSuccess) return e;
-    }
-    return cudaSuccess;
+    if (gx) q[count++] = {*gx, g, w};
+    return tiles_launch<T>(q, count, f.gb ? TilesSums{sums, sum_rows, f.N, f.gb} : TilesSums{}, st);
 }
 cudaError_t cafe_tiles_forward(const CafeForward& f, int dtype, const CafeJob& job, void* work, cudaStream_t st) {
     if (!tiles_encoder()) return cudaErrorNotSupported;
