@@ -12,6 +12,7 @@ from outside the capture)."""
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 
 import torch
 import torch.nn as nn
@@ -195,41 +196,85 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
 
 # ---- a run of layers ---------------------------------------------------------------------------------------
 def _pointers(tensors):
-    return (ctypes.c_void_p * len(tensors))(*[_ptr(t) for t in tensors])
+    return (ctypes.c_void_p * len(tensors))(*[None if t is None else t.data_ptr() for t in tensors])
+
+
+class _Plan:
+    """What a run of layers of these sizes needs besides its tensors: where the outputs between the layers and the slopes lie in
+    one buffer (rows and starts on 16 bytes), and the arrays that describe it to the library."""
+
+    def __init__(self, m, widths, acts, dtype, keep):
+        n, size = len(acts), dtype.itemsize
+        slope_size = _slope_type(dtype).itemsize
+        pitch = [(v + 7) // 8 * 8 for v in widths[1:-1]] + [widths[-1]]
+        at, self.y_at, self.slope_at = 0, [], []
+        for p in pitch[:-1]:
+            self.y_at.append(at)
+            at += -(-m * p * size // 256) * 256
+        for p, a in zip(pitch, acts):
+            held = keep and a not in (_NONE, _RELU)
+            self.slope_at.append(at if held else None)
+            if held:
+                at += -(-m * p * slope_size // 256) * 256
+        self.bytes, self.n, self.type = at, n, DTYPES[dtype]
+        self.widths, self.acts, self.pitch = (ctypes.c_int32 * (n + 1))(*widths), (ctypes.c_int32 * n)(*acts), (ctypes.c_int64 * n)(*pitch)
+
+    def outputs(self, base, last):
+        return (ctypes.c_void_p * self.n)(*[base + a for a in self.y_at], last)
+
+    def slopes(self, base):
+        return (ctypes.c_void_p * self.n)(*[None if a is None else base + a for a in self.slope_at])
+
+
+_plan = lru_cache(maxsize=256)(_Plan)
+
+
+def _weight_rows(weights):
+    """(weights as rows of contiguous elements, their pitches for the library)."""
+    ws, lds = [], []
+    for w in weights:
+        if w.is_contiguous():
+            ws.append(w)
+            lds.append(w.shape[1])
+        else:
+            w, _, ld = _rows(w, w.shape[1])
+            ws.append(w)
+            lds.append(ld)
+    return ws, (ctypes.c_int64 * len(lds))(*lds)
 
 
 def _mlp(x, weights, biases, acts, keep):
-    """The forward call: (x and weights as rows, y of every layer, slope of every layer or None)."""
-    n = len(weights)
-    widths = [weights[0].shape[1]] + [w.shape[0] for w in weights]
+    """The forward call: (x and weights as rows, output, buffer of what lies between, plan, rows, pitches)."""
+    widths = (weights[0].shape[1], *[w.shape[0] for w in weights])
     x2, m, ldx = _rows(x, widths[0])
     if m > MAX_SIZE:
         raise ValueError(f"fused_mlp: up to {MAX_SIZE} rows")
-    ws = [_rows(w, w.shape[1]) for w in weights]
+    plan = _plan(m, widths, acts, x.dtype, keep)
+    ws, lds = _weight_rows(weights)
     bs = [_contiguous(b) for b in biases]
-    # rows between the layers start on 16-byte boundaries
-    pitch = [(v + 7) // 8 * 8 for v in widths[1:-1]] + [widths[-1]]
-    ys = [torch.empty(m, p, dtype=x.dtype, device=x.device) for p in pitch[:-1]]
-    ys.append(torch.empty(*x.shape[:-1], widths[-1], dtype=x.dtype, device=x.device))
-    slopes = [torch.empty(m, p, dtype=_slope_type(x.dtype), device=x.device) if keep and a not in (_NONE, _RELU) else None
-              for p, a in zip(pitch, acts)]
-    call = (n, (ctypes.c_int32 * (n + 1))(*widths), m, x2.data_ptr(), ldx, _pointers([w for w, _, _ in ws]), (ctypes.c_int64 * n)(*[ld for _, _, ld in ws]))
-    lib, t = _lib.load(), DTYPES[x.dtype]
-    size = lib.cafe_mlp_forward_work(*call, t)
-    with _on(x.device) as stream:
-        _lib.check(lib.cafe_mlp_forward(*call, _pointers(bs), (ctypes.c_int32 * n)(*acts), t, _pointers(ys), (ctypes.c_int64 * n)(*pitch),
-                                        _pointers(slopes) if keep else None, _ptr(_work(size, x)), size, stream), "cafe_mlp_forward")
-    return x2, [w for w, _, _ in ws], ys, slopes, pitch
+    device = x.device
+    y = torch.empty(*x.shape[:-1], widths[-1], dtype=x.dtype, device=device)
+    between = torch.empty(plan.bytes, dtype=torch.uint8, device=device)
+    base = between.data_ptr()
+    lib = _lib.load()
+    call = (plan.n, plan.widths, m, x2.data_ptr(), ldx, _pointers(ws), lds)
+    size = lib.cafe_mlp_forward_work(*call, plan.type)
+    with _on(device) as stream:
+        status = lib.cafe_mlp_forward(*call, _pointers(bs), plan.acts, plan.type, plan.outputs(base, y.data_ptr()), plan.pitch,
+                                      plan.slopes(base) if keep else None, _ptr(_work(size, x)), size, stream)
+    if status:
+        _lib.check(status, "cafe_mlp_forward")
+    return x2, ws, y, between, (plan, m, ldx, lds)
 
 
 class _FusedMLP(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, acts, *params):
-        n = len(params) // 2
-        x2, ws, ys, slopes, pitch = _mlp(x, params[:n], params[n:], acts, True)
-        ctx.acts, ctx.shape, ctx.pitch = acts, x.shape, pitch
-        ctx.save_for_backward(x2, *ws, *ys, *slopes)
-        return ys[-1]
+        n = len(acts)
+        x2, ws, y, between, ctx.sizes = _mlp(x, params[:n], params[n:], acts, True)
+        ctx.shape = x.shape
+        ctx.save_for_backward(x2, y, between, *ws)
+        return y
 
     @staticmethod
     def backward(ctx, grad_y):
@@ -237,24 +282,22 @@ class _FusedMLP(torch.autograd.Function):
 
 
 def _mlp_backward(ctx, grad_y):
-    n, acts = len(ctx.acts), ctx.acts
-    x, *rest = ctx.saved_tensors
-    ws, ys, slopes = rest[:n], rest[n:2 * n], rest[2 * n:]
-    widths = [ws[0].shape[1]] + [w.shape[0] for w in ws]
-    need = ctx.needs_input_grad
-    g, m, ldg = _rows(grad_y, widths[-1], True)
-    new = lambda *shape: torch.empty(*shape, dtype=g.dtype, device=g.device)   # noqa: E731
-    gx = new(*ctx.shape) if need[0] else None
-    gws = [new(*w.shape) if need[2 + l] else None for l, w in enumerate(ws)]
-    gbs = [new(w.shape[0]) if need[2 + n + l] else None for l, w in enumerate(ws)]
-    lib, t = _lib.load(), DTYPES[g.dtype]
-    call = (n, (ctypes.c_int32 * (n + 1))(*widths), m, g.data_ptr(), ldg, x.data_ptr(), _rows(x, widths[0])[2], _pointers(ws),
-            (ctypes.c_int64 * n)(*[_rows(w, w.shape[1])[2] for w in ws]))
-    size = lib.cafe_mlp_backward_work(*call, t)
-    with _on(g.device) as stream:
-        _lib.check(lib.cafe_mlp_backward(
-            *call, (ctypes.c_int32 * n)(*acts), t, _pointers(ys), (ctypes.c_int64 * n)(*ctx.pitch), _pointers(slopes), _ptr(gx), widths[0],
-            _pointers(gws), _pointers(gbs), _ptr(_work(size, g)), size, stream), "cafe_mlp_backward")
+    x, y, between, *ws = ctx.saved_tensors
+    plan, m, ldx, lds = ctx.sizes
+    n, need = plan.n, ctx.needs_input_grad
+    g, _, ldg = _rows(grad_y, plan.widths[n], True)
+    dtype, device = g.dtype, g.device
+    gx = torch.empty(ctx.shape, dtype=dtype, device=device) if need[0] else None
+    gws = [torch.empty(w.shape, dtype=dtype, device=device) if want else None for w, want in zip(ws, need[2:2 + n])]
+    gbs = [torch.empty(w.shape[0], dtype=dtype, device=device) if want else None for w, want in zip(ws, need[2 + n:])]
+    lib, base = _lib.load(), between.data_ptr()
+    call = (n, plan.widths, m, g.data_ptr(), ldg, x.data_ptr(), ldx, _pointers(ws), lds)
+    size = lib.cafe_mlp_backward_work(*call, plan.type)
+    with _on(device) as stream:
+        status = lib.cafe_mlp_backward(*call, plan.acts, plan.type, plan.outputs(base, y.data_ptr()), plan.pitch, plan.slopes(base), _ptr(gx),
+                                       plan.widths[0], _pointers(gws), _pointers(gbs), _ptr(_work(size, g)), size, stream)
+    if status:
+        _lib.check(status, "cafe_mlp_backward")
     return (gx, None, *gws, *gbs)
 
 
@@ -264,7 +307,7 @@ _mlp_backward_once = once_differentiable(_mlp_backward)
 def fused_mlp(x: torch.Tensor, weights, biases, activations) -> torch.Tensor:
     """Layer after layer of act(x W^T + b): weights [N_l, N_{l-1}], biases [N_l] or None, activations by name (see
     fused_linear).  The values are those of fused_linear layer by layer; between the layers they are held in x's type."""
-    weights, biases, activations = list(weights), list(biases), list(activations)
+    weights, biases, activations = tuple(weights), tuple(biases), tuple(activations)
     n = len(weights)
     if not 1 <= n <= MAX_LAYERS or len(biases) != n or len(activations) != n:
         raise ValueError(f"fused_mlp: one bias (or None) and one activation for each of 1 to {MAX_LAYERS} weights")
@@ -277,10 +320,10 @@ def fused_mlp(x: torch.Tensor, weights, biases, activations) -> torch.Tensor:
             raise ValueError(f"fused_mlp: activations must be among {sorted(ACTIVATIONS)}, got {a!r}")
         _check_layer(cols, w, b, "fused_mlp")
         cols = w.shape[0]
-    acts = [ACTIVATIONS[a] for a in activations]
+    acts = tuple([ACTIVATIONS[a] for a in activations])
     if torch.is_grad_enabled() and (x.requires_grad or any(w.requires_grad for w in weights) or any(b is not None and b.requires_grad for b in biases)):
         return _FusedMLP.apply(x, acts, *weights, *biases)
-    return _mlp(x, weights, biases, acts, False)[2][-1]
+    return _mlp(x, weights, biases, acts, False)[2]
 
 
 _MODULES = {nn.ReLU: "relu", nn.Sigmoid: "sigmoid", nn.SiLU: "silu", nn.Identity: "none"}
