@@ -350,6 +350,7 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
 // Either way a lane has a row: bias, activation, residual; results go to its warp's staging rows, from which the warp writes 128
 // bytes of a row at a time.  Nobody waits for another warp.
 #define CAFE_PAIR_THREADS 320
+#define CAFE_PAIRS 74          // pairs of blocks that run at a time
 template <typename T, int BN> struct CafePairShape {
     typedef CafeTiles<T> L;
     typedef typename CafeSlopeOf<T>::type ST;
@@ -475,22 +476,53 @@ struct CafePairArgs {
     const float* sums;   // [sum_rows][gb_cols]: partial sums of a bias gradient, added up on the way
     int sum_rows, gb_cols;
     void* gb;
-    int share[75];
+    int share[CAFE_PAIRS + 1];
+    // fp32: the first product's depth in `splits` parts, whose sums go to `partial` ([part][rows][pitch]) for k_parts_join to add
+    int splits, pitch;
+    float* partial;
 };
 // A backward's two products are one launch.  The first one's tiles (the longer) go round the pairs; the second one's are handed out
 // so that all pairs end at about the same time, pair p has those from share[p] to share[p + 1]: 2048x1024x1024 takes the time of gW
 // alone (backward 84 us as two launches, 70 as one).
 struct CafePairTiles {
-    int first, step, own, from, all;   // tiles of the first product: first, first + step, .. `own` of them; of the second: from, from + 1, ..
+    int first, step, own, from, all;   // of the first product: first, first + step, .. `own` of them (part by part); of the second: from, from + 1, ..
     __device__ __forceinline__ CafePairTiles(const CafePairArgs& P, int pair, int pairs) {
+        const int units = P.job[0].tiles * P.splits;
         first = pair; step = pairs;
-        own = pair < P.job[0].tiles ? (P.job[0].tiles - pair + pairs - 1) / pairs : 0;
+        own = pair < units ? (units - pair + pairs - 1) / pairs : 0;
         from = P.share[pair];
         all = own + P.share[pair + 1] - from;
     }
     __device__ __forceinline__ int which(int n) const { return n >= own; }
-    __device__ __forceinline__ int tile(int n) const { return n < own ? first + n * step : from + n - own; }
+    __device__ __forceinline__ int tile(const CafePairArgs& P, int n) const { return n < own ? (first + n * step) % P.job[0].tiles : from + n - own; }
+    __device__ __forceinline__ int part(const CafePairArgs& P, int n) const { return n < own ? (first + n * step) / P.job[0].tiles : 0; }
+    // the turns [t0, t1) of the n-th tile
+    template <int BK> __device__ __forceinline__ void turns(const CafePairArgs& P, int n, int* t0, int* t1) const {
+        const int all_turns = (P.job[which(n)].depth + BK - 1) / BK;
+        *t0 = 0; *t1 = all_turns;
+        if (n < own && P.splits > 1) {
+            const int share = (all_turns + P.splits - 1) / P.splits;
+            *t0 = part(P, n) * share;
+            *t1 = min(all_turns, *t0 + share);
+        }
+    }
 };
+// the parts' sums of a product, added in order
+__global__ void __launch_bounds__(256) k_parts_join(const float* partial, int splits, int rows, int cols, int pitch, float* out, int64_t ldo) {
+    const int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x, per = pitch / 4, all = (int64_t)rows * pitch;
+    if (q >= rows * per) return;
+    const int64_t r = q / per;
+    const int c = (int)(q - r * per) * 4;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int p = 0; p < splits; ++p) {
+        const float4 y = __ldg(reinterpret_cast<const float4*>(partial + p * all + r * pitch + c));
+        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+    }
+    const float v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) if (c + j < cols) out[r * ldo + c + j] = v[j];
+}
 
 template <typename T, int BN>
 __global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) k_tiles_pair(const __grid_constant__ CafePairArgs P) {
@@ -539,12 +571,14 @@ __global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) k_tiles_pair(const __gri
         uint32_t phase = 1;   // (a fresh barrier's phase before its first counts as over)
         int64_t u = 0;
         for (int n = 0; n < list.all && fine; ++n) {
-            const int which = list.which(n), tile = list.tile(n);
+            const int which = list.which(n), tile = list.tile(P, n);
+            int t0, t1;
+            list.turns<L::BK>(P, n, &t0, &t1);
             const CafeJob& J = P.job[which];
             const CUtensorMap *ma = &P.a[which], *mb = &P.b[which];
             const int tm = tile / J.tiles_n, row0 = tm * 256 + rank * 128, col0 = (tile - tm * J.tiles_n) * BN + rank * (BN / 2);
             const int a_kc = J.a_kc, b_kc = J.b_kc;
-            for (int k0 = 0; k0 < J.depth; k0 += L::BK, ++u) {
+            for (int k0 = t0 * L::BK; k0 < t1 * L::BK; k0 += L::BK, ++u) {
                 if (!(fine = __all_sync(0xffffffffu, cafe_bar_wait(empty(s), phase, &bail)))) break;
                 const uint32_t a = base + s * Sh::stage, b = a + L::parts * Sh::a_part, bar = full(s);
                 if (cafe_elect()) {
@@ -571,8 +605,9 @@ __global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) k_tiles_pair(const __gri
             uint32_t phase = 0;
             bool fine = true;
             for (int n = 0; n < list.all && fine; ++n) {
-                const int turns = (P.job[list.which(n)].depth + L::BK - 1) / L::BK;
-                for (int t = 0; t < turns; ++t) {
+                int t0, t1;
+                list.turns<L::BK>(P, n, &t0, &t1);
+                for (int t = t0; t < t1; ++t) {
                     if (!(fine = cafe_bar_wait(full(s), phase, &bail))) break;
                     cafe_bar_arrive_at(cafe_cluster_map(full(s), 0));
                     if (++s == Sh::stages) { s = 0; phase ^= 1u; }
@@ -586,7 +621,9 @@ __global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) k_tiles_pair(const __gri
         uint32_t phase = 0, chunk_phase = 0;
         for (; n < list.all && fine; ++n) {
             const CafeJob& J = P.job[list.which(n)];
-            const int turns = (J.depth + L::BK - 1) / L::BK;
+            int t0, t1;
+            list.turns<L::BK>(P, n, &t0, &t1);
+            const int turns = t1 - t0;
             const uint32_t instr = cafe_mma_instr(L::type, 256, BN) | (J.a_kc ? 0u : 1u << 15) | (J.b_kc ? 0u : 1u << 16);
             const uint64_t da = J.a_kc ? cafe_operand<Sh::rowb>(base) : cafe_operand_mn(base, L::parts * L::BK * 128);
             const uint64_t db = J.b_kc ? cafe_operand<Sh::rowb>(base + L::parts * Sh::a_part) : cafe_operand_mn(base + L::parts * Sh::a_part, L::parts * L::BK * 128);
@@ -638,8 +675,7 @@ __global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) k_tiles_pair(const __gri
         uint32_t chunk_phase = 0;
         bool fine = true;
         if (P.sums) {
-            const int c = blockIdx.x * 256 + (int)threadIdx.x - 64;
-            if (c < P.gb_cols) {
+            for (int c = blockIdx.x * 256 + (int)threadIdx.x - 64; c < P.gb_cols; c += gridDim.x * 256) {
                 float x[4] = {0.f, 0.f, 0.f, 0.f};
                 int q = 0;
                 for (; q + 4 <= P.sum_rows; q += 4)
@@ -652,9 +688,11 @@ __global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) k_tiles_pair(const __gri
         }
         // fp32: every tile, the warp's half of the columns; 16 bits: every other tile, all of them
         for (int n = L::parts == 3 ? 0 : half; n < list.all; n += L::parts == 3 ? 1 : 2) {
-            const int tile = list.tile(n);
+            const int tile = list.tile(P, n);
             const CafeJob& J = P.job[list.which(n)];
-            const int turns = (J.depth + L::BK - 1) / L::BK;
+            int t0, t1;
+            list.turns<L::BK>(P, n, &t0, &t1);
+            const int turns = t1 - t0;
             const int g = n % Sh::sets, tm = tile / J.tiles_n, col0 = (tile - tm * J.tiles_n) * BN + (L::parts == 3 ? half * Sh::mine : 0);
             const int64_t row0 = (int64_t)tm * 256 + rank * 128 + rows;
             const int m = (int)max((int64_t)0, min((int64_t)32, J.rows - row0)), columns = max(0, min(Sh::mine, J.cols - col0));
@@ -716,12 +754,16 @@ __global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) k_tiles_pair(const __gri
                         const int64_t j = col0 + h + c;
                         if (nan && fine && lane < m) {
 #pragma unroll
-                            for (int q = 0; q < 16; ++q) if (z[q] != z[q] && j + q < J.cols) z[q] = cafe_plain_dot(J, row0 + lane, j + q, 0, J.depth);
+                            for (int q = 0; q < 16; ++q) if (z[q] != z[q] && j + q < J.cols) z[q] = cafe_plain_dot(J, row0 + lane, j + q, t0 * L::BK, min(J.depth, t1 * L::BK));
                         }
                         cafe_row_end<T, Sh::out_row, Sh::slope_row, false>(J, z, j, out, slopes, lane, c);
                     }
                     __syncwarp();
                     const int here = min(W, columns - h);
+                    if (P.splits > 1 && list.which(n) == 0)
+                        cafe_rows_out<float, W>(out, P.partial + ((int64_t)list.part(P, n) * J.rows + row0) * P.pitch + col0 + h, P.pitch, true, nullptr, 0, false, m,
+                                                min(W, P.pitch - col0 - h), lane);
+                    else
                     cafe_rows_out<T, W>(out, static_cast<T*>(J.out) + row0 * J.ldo + col0 + h, J.ldo, J.out_row,
                                         J.res ? static_cast<const T*>(J.res) + row0 * J.ldr + col0 + h : nullptr, J.ldr, J.res_row, m, here, lane);
                     if (J.slope_out)
@@ -827,6 +869,8 @@ static cudaError_t tiles_launch_bn(CafeTilesArgs& P, const TilesOperand& a, cons
 struct TilesProduct {
     CafeJob job;
     TilesOperand a, b;
+    int splits;         // parts of the depth whose sums go to `partial` first (pairs of blocks, fp32; else 1)
+    float* partial;
 };
 struct TilesSums {
     const float* at;
@@ -834,10 +878,22 @@ struct TilesSums {
     void* gb;
 };
 // what a pair's tile of a product takes, in the units of the estimates below
-template <typename T> static double tiles_pair_cost(const CafeJob& J, int bn) {
-    return (CafeTiles<T>::parts == 3 ? 1.2 : bn == 256 ? 2.7 : 2.2) * ((J.depth + CafeTiles<T>::BK - 1) / CafeTiles<T>::BK) + 3;
+template <typename T> static double tiles_pair_cost(const CafeJob& J, int bn, int splits) {
+    return (CafeTiles<T>::parts == 3 ? 1.2 : bn == 256 ? 2.7 : 2.2) * (((J.depth + CafeTiles<T>::BK - 1) / CafeTiles<T>::BK + splits - 1) / splits) + 3;
 }
-// The second product's tiles handed out to 74 pairs that have the first one's in turn: the least time in which all are done (by
+// Parts of the depth of a product that has so few tiles that clusters of eight blocks each leave SMs idle (gW of a narrow layer): two
+// rounds of all pairs, each part at least 32 turns and none empty.  fp32.  Backward of 47373x572x175 425 us without, 345 with;
+// 30000x256x256 212, 148; 4096x352x1024 (12 tiles) 79, 73; but 65536x479x1024 (16) 892, 962.
+static int tiles_splits(int rows, int cols, int depth) {
+    const int64_t tiles = (int64_t)((rows + 255) / 256) * ((cols + 127) / 128), turns = (depth + 31) / 32;
+    if (tiles > 12) return 1;
+    int64_t s = 2 * CAFE_PAIRS / tiles;
+    if (s > turns / 32) s = turns / 32;
+    while (s > 1 && ((turns + s - 1) / s) * (s - 1) >= turns) --s;
+    return s > 1 ? (int)s : 1;
+}
+static int64_t tiles_partial_bytes(int rows, int cols, int splits) { return splits > 1 ? (((int64_t)splits * rows * ((cols + 3) & ~3) * 4 + 255) & ~(int64_t)255) : 0; }
+// The second product's tiles handed out to the pairs that have the first one's in turn: the least time in which all are done (by
 // bisection), and who has how many (share may be null).
 static double tiles_share(int64_t tiles0, double cost0, int64_t tiles1, double cost1, int pairs, int* share) {
     double lo = 0, hi = cost0 * (double)((tiles0 + pairs - 1) / pairs) + cost1 * (double)((tiles1 + pairs - 1) / pairs);
@@ -867,27 +923,29 @@ template <typename T, int BN>
 static cudaError_t tiles_launch_pair(TilesProduct* q, int count, const TilesSums& sums, cudaStream_t st) {
     CafePairArgs P = {};
     P.count = count;
+    P.splits = q[0].splits; P.partial = q[0].partial; P.pitch = (q[0].job.cols + 3) & ~3;
     int tiles = 0;
     for (int i = 0; i < count; ++i) {
         CafeJob& J = q[i].job;
         if (!tiles_map<T>(&P.a[i], q[i].a, J.a_kc, CAFE_LIN_BM) || !tiles_map<T>(&P.b[i], q[i].b, J.b_kc, BN / 2)) return cudaErrorInvalidValue;
         J.tiles_n = (J.cols + BN - 1) / BN;
         J.tiles = ((J.rows + 255) / 256) * J.tiles_n;
-        tiles += J.tiles;
+        tiles += J.tiles * (i ? 1 : P.splits);
         P.job[i] = J;
     }
-    int pairs = tiles < 74 ? tiles : 74;
-    if (sums.at) {
-        P.sums = sums.at; P.sum_rows = sums.rows; P.gb_cols = sums.cols; P.gb = sums.gb;
-        const int least = (sums.cols + 511) / 512;   // (256 columns a block)
-        pairs = pairs < least ? least : pairs;
-    }
-    if (count == 2) tiles_share(P.job[0].tiles, tiles_pair_cost<T>(P.job[0], BN), P.job[1].tiles, tiles_pair_cost<T>(P.job[1], BN), pairs, P.share);
+    const int pairs = tiles < CAFE_PAIRS ? tiles : CAFE_PAIRS;
+    P.sums = sums.at; P.sum_rows = sums.rows; P.gb_cols = sums.cols; P.gb = sums.gb;
+    if (count == 2)
+        tiles_share(P.job[0].tiles * P.splits, tiles_pair_cost<T>(P.job[0], BN, P.splits), P.job[1].tiles, tiles_pair_cost<T>(P.job[1], BN, 1), pairs, P.share);
     constexpr int bytes = CafePairShape<T, BN>::bytes;
     static std::atomic<uint64_t> allowed{0};
     const cudaError_t e = dense_allow_shared((const void*)k_tiles_pair<T, BN>, bytes, &allowed);
     if (e != cudaSuccess) return e;
-    return dense_start<true>(k_tiles_pair<T, BN>, dim3(2u * pairs), CAFE_PAIR_THREADS, bytes, 2, st, P);
+    const cudaError_t r = dense_start<true>(k_tiles_pair<T, BN>, dim3(2u * pairs), CAFE_PAIR_THREADS, bytes, 2, st, P);
+    if (r != cudaSuccess || P.splits == 1) return r;
+    const CafeJob& J = P.job[0];
+    return dense_start<false>(k_parts_join, dim3((unsigned)(((int64_t)J.rows * P.pitch / 4 + 255) / 256)), 256, 0, 1, st, (const float*)P.partial, P.splits, J.rows,
+                              J.cols, P.pitch, (float*)J.out, J.ldo);
 }
 // Pairs of blocks through tile after tile, or two blocks an SM and clusters that share a tile's depth: whichever estimate is less,
 // in turns of a 128 x 128 tile at the tensor cores' full rate.  A pair's turn takes 1.2 (fp32) or, 256 columns wide, 2.7 (16 bits)
@@ -910,17 +968,18 @@ template <typename T> static double tiles_estimate_clusters(const CafeJob& J, in
     return best;
 }
 template <typename T> static double tiles_estimate_pairs(const TilesProduct* q, int count, int bn) {
-    double cost[2];
+    double cost[2], join = 0;
     int64_t tiles[2];
     for (int i = 0; i < count; ++i) {
         const CafeJob& J = q[i].job;
         if (J.depth == 0 || J.cols == 0) return 1e300;
-        cost[i] = tiles_pair_cost<T>(J, bn);
-        tiles[i] = (int64_t)((J.rows + 255) / 256) * ((J.cols + bn - 1) / bn);
+        const int splits = q[i].splits;
+        cost[i] = tiles_pair_cost<T>(J, bn, splits);
+        tiles[i] = (int64_t)((J.rows + 255) / 256) * ((J.cols + bn - 1) / bn) * splits;
+        if (splits > 1) join += 8 + 1e-6 * splits * J.rows * J.cols;
     }
-    if (count == 1) return (double)((tiles[0] + 73) / 74) * cost[0] + 14;
-    const int a = cost[0] < cost[1];
-    return tiles_share(tiles[a], cost[a], tiles[!a], cost[!a], 74, nullptr) + 14;
+    if (count == 1) return (double)((tiles[0] + CAFE_PAIRS - 1) / CAFE_PAIRS) * cost[0] + 14 + join;
+    return tiles_share(tiles[0], cost[0], tiles[1], cost[1], CAFE_PAIRS, nullptr) + 14 + join;
 }
 template <typename T>
 static cudaError_t tiles_launch_clusters(const TilesProduct& q, int splits, const TilesSums& sums, cudaStream_t st) {
@@ -955,10 +1014,11 @@ static cudaError_t tiles_launch(TilesProduct* q, int count, const TilesSums& sum
         }
         return tiles_launch_pair<T, 128>(p, n, s, st);
     };
-    if (count == 2 && tiles_estimate_pairs<T>(q, 2, bn) < apart) {
-        if (q[1].job.depth > q[0].job.depth) { const TilesProduct t = q[0]; q[0] = q[1]; q[1] = t; }
-        return pair(q, 2, sums);
-    }
+    // (longer tiles first, but the parts are always the first product's)
+    if (count == 2 && q[0].splits == 1 && q[1].job.depth > q[0].job.depth) {
+        TilesProduct t[2] = {q[1], q[0]};
+        if (tiles_estimate_pairs<T>(t, 2, bn) < apart) return pair(t, 2, sums);
+    } else if (count == 2 && tiles_estimate_pairs<T>(q, 2, bn) < apart) return pair(q, 2, sums);
     for (int i = 0; i < count; ++i) {
         const cudaError_t e = each[i] < 1e300 ? pair(q + i, 1, i ? none : sums) : tiles_launch_clusters<T>(q[i], splits[i], i ? none : sums, st);
         if (e != cudaSuccess) return e;
@@ -1026,6 +1086,7 @@ int64_t cafe_tiles_backward_work(const CafeBackward& f, int dtype) {
     if (f.slope_kind != CAFE_SLOPE_NONE || !tiles_in_place(dtype, f.gy, f.ldg)) need += tiles_bytes(parts, f.M, f.N);
     if (f.gx && !tiles_in_place(dtype, f.w, f.ldw)) need += tiles_bytes(parts, f.N, f.K);
     if (f.gw && !tiles_in_place(dtype, f.x, f.ldx)) need += tiles_bytes(parts, f.M, f.K);
+    if (f.gw && dtype == CAFE_F32) need += tiles_partial_bytes(f.N, f.K, tiles_splits(f.N, f.K, f.M));
     if (f.gb) need += tiles_round((int64_t)((f.M + cafe_parts_rows(f.M, f.N) - 1) / cafe_parts_rows(f.M, f.N)) * f.N * 4);
     return need;
 }
@@ -1037,7 +1098,7 @@ static cudaError_t tiles_forward(const CafeForward& f, int dtype, const CafeJob&
     const TilesOperand w = tiles_operand<T>(&parts, &work, dtype, f.w, f.ldw, f.N, f.K, nullptr, 0, CAFE_SLOPE_NONE, nullptr);
     cudaError_t e = tiles_parts<T>(parts, st);
     if (e != cudaSuccess) return e;
-    TilesProduct q = {job, x, w};
+    TilesProduct q = {job, x, w, 1, nullptr};
     return tiles_launch<T>(&q, 1, TilesSums{}, st);
 }
 template <typename T>
@@ -1058,11 +1119,13 @@ static cudaError_t tiles_backward(const CafeBackward& f, int dtype, const CafeJo
     TilesProduct q[2];
     int count = 0;
     if (gw) {   // (without gW wanted: no columns, no depth, the bias gradient alone)
-        q[count] = {*gw, g, x};
+        const int splits = f.gw && dtype == CAFE_F32 ? tiles_splits(f.N, f.K, f.M) : 1;
+        q[count] = {*gw, g, x, splits, (float*)work};
+        work += tiles_partial_bytes(f.N, f.K, splits);
         if (!f.gw) q[count].job.depth = 0;
         ++count;
     }
-    if (gx) q[count++] = {*gx, g, w};
+    if (gx) q[count++] = {*gx, g, w, 1, nullptr};
     return tiles_launch<T>(q, count, f.gb ? TilesSums{sums, sum_rows, f.N, f.gb} : TilesSums{}, st);
 }
 cudaError_t cafe_tiles_forward(const CafeForward& f, int dtype, const CafeJob& job, void* work, cudaStream_t st) {
