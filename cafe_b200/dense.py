@@ -67,10 +67,12 @@ def _rows(t: torch.Tensor, cols: int, repeated: bool = False):
 
 
 def _check(x, tensors, what):
-    if not x.is_cuda or x.dtype not in DTYPES:
+    dtype = x.dtype
+    if not x.is_cuda or dtype not in DTYPES:
         raise ValueError(f"{what} needs CUDA tensors of fp32, bf16 or fp16")
+    device = x.get_device()
     for t in tensors:
-        if t is not None and (t.dtype != x.dtype or t.device != x.device):
+        if t is not None and (t.dtype is not dtype or not t.is_cuda or t.get_device() != device):
             raise ValueError(f"{what}: all tensors must have one type and be on one device")
 
 

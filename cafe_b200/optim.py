@@ -31,7 +31,7 @@ class AdamW(torch.optim.Optimizer):
     state_bits = 32 keeps exp_avg and exp_avg_sq in fp32.  state_bits = 8 keeps a byte per element for exp_avg and one for the
     root of exp_avg_sq, plus a byte per 256 elements for each; they are rounded at random (by `seed`, the tensor's place among
     the parameters, the step and the element), so that moments which change by less than a code's step still move on average.
-    A gradient that is not finite makes its block of 256 moments not a number.
+    A gradient that is not finite, or whose square is not, makes its block of 256 moments not a number.
 
     A step counts on the device and reads nothing back, so it can be captured into a CUDA graph; lr and the other settings are
     then those of the capture, and the optimizer's state has to exist before it (one step outside).  Parameters without a
@@ -80,20 +80,27 @@ class AdamW(torch.optim.Optimizer):
         return s
 
     def _launches(self):
-        """Parameters with a gradient, by what one call takes: {(group, device, type): [(number, p, gradient, state)]}."""
-        found, number = {}, 0
+        """Parameters with a gradient, by what one call takes: {(group, device, type): (parameters, gradients, states, numbers)}."""
+        found, number, state = {}, 0, self.state
         for i, group in enumerate(self.param_groups):
+            key = rows = None
             for p in group["params"]:
                 g = p.grad
                 if g is not None:
                     if g.is_sparse:
                         raise RuntimeError("AdamW does not take sparse gradients")
-                    if g.stride() != p.stride():
+                    if not (g.is_contiguous() and p.is_contiguous()) and g.stride() != p.stride():
                         g = torch.empty_like(p, memory_format=torch.preserve_format).copy_(g)
-                    s = self.state[p]
+                    s = state[p]
                     if "step" not in s:
                         s = self._start(p)
-                    found.setdefault((i, p.device, p.dtype), []).append((number, p, g, s))
+                    if key != (p.device, p.dtype):
+                        key = (p.device, p.dtype)
+                        rows = found.setdefault((i, *key), ([], [], [], []))
+                    rows[0].append(p)
+                    rows[1].append(g)
+                    rows[2].append(s)
+                    rows[3].append(number)
                 number += 1
         return found
 
@@ -103,24 +110,28 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        lib = _lib.load()
-        for (i, device, dtype), rows in self._launches().items():
+        lib, packed = _lib.load(), self.state_bits == 8
+        for (i, device, dtype), (params, grads, states, numbers) in self._launches().items():
             group = self.param_groups[i]
             self._check_settings(group)
             ticket = self._ticket.get(device)
             if ticket is None:
                 ticket = self._ticket[device] = torch.zeros(1, dtype=torch.int32, device=device)
-            n, packed = len(rows), self.state_bits == 8
+            n = len(params)
             vp = ctypes.c_void_p * n
-            names = _CODES if packed else ("exp_avg", "exp_avg_sq")
-            state = {k: vp(*[s[k].data_ptr() for _, _, _, s in rows]) for k in ("step",) + names}
+            m = vp(*[s["exp_avg"].data_ptr() for s in states])
+            if packed:
+                v, mtop, vtop = (vp(*[s[name].data_ptr() for s in states]) for name in ("root_avg_sq", "exp_avg_top", "root_avg_sq_top"))
+            else:
+                v, mtop, vtop = vp(*[s["exp_avg_sq"].data_ptr() for s in states]), None, None
             with _on(device) as stream:
-                _lib.check(lib.cafe_adamw_step(
-                    n, vp(*[p.data_ptr() for _, p, _, _ in rows]), vp(*[g.data_ptr() for _, _, g, _ in rows]), state["exp_avg"],
-                    state["root_avg_sq" if packed else "exp_avg_sq"], state.get("exp_avg_top"), state.get("root_avg_sq_top"), state["step"],
-                    (ctypes.c_int64 * n)(*[p.numel() for _, p, _, _ in rows]), (ctypes.c_int32 * n)(*[k for k, _, _, _ in rows]), DTYPES[dtype],
-                    self.state_bits, group["lr"], *group["betas"], group["eps"], group["weight_decay"], self.seed, ticket.data_ptr(), stream),
-                    "cafe_adamw_step")
+                status = lib.cafe_adamw_step(
+                    n, vp(*[p.data_ptr() for p in params]), vp(*[g.data_ptr() for g in grads]), m, v, mtop, vtop,
+                    vp(*[s["step"].data_ptr() for s in states]), (ctypes.c_int64 * n)(*[p.numel() for p in params]), (ctypes.c_int32 * n)(*numbers),
+                    DTYPES[dtype], self.state_bits, group["lr"], *group["betas"], group["eps"], group["weight_decay"], self.seed,
+                    ticket.data_ptr(), stream)
+            if status:
+                _lib.check(status, "cafe_adamw_step")
         return loss
 
     @torch.no_grad()
@@ -137,11 +148,19 @@ class AdamW(torch.optim.Optimizer):
         for device, ps in by_device.items():
             n = len(ps)
             vp = ctypes.c_void_p * n
-            values = [torch.empty_like(p, dtype=torch.bfloat16, memory_format=torch.preserve_format) for p in ps + ps]
-            codes = [vp(*[self.state[p][name].data_ptr() for p in ps]) for name in _CODES]
+            sizes = [p.numel() for p in ps]
+            if all(k % 8 == 0 for k in sizes[:-1]) and all(p.is_contiguous() for p in ps):   # one allocation, every tensor on 16 bytes
+                values = []
+                for _ in range(2):
+                    flat = torch.empty(sum(sizes), dtype=torch.bfloat16, device=device)
+                    values += torch._utils._unflatten_dense_tensors(flat, ps)
+            else:
+                values = [torch.empty_like(p, dtype=torch.bfloat16, memory_format=torch.preserve_format) for p in ps + ps]
+            states = [self.state[p] for p in ps]
+            codes = [vp(*[s[name].data_ptr() for s in states]) for name in _CODES]
+            at = [v.data_ptr() for v in values]
             with _on(device) as stream:
-                _lib.check(_lib.load().cafe_adamw_moments(n, *codes, (ctypes.c_int64 * n)(*[p.numel() for p in ps]),
-                                                          vp(*[v.data_ptr() for v in values[:n]]), vp(*[v.data_ptr() for v in values[n:]]), stream),
+                _lib.check(_lib.load().cafe_adamw_moments(n, *codes, (ctypes.c_int64 * n)(*sizes), vp(*at[:n]), vp(*at[n:]), stream),
                            "cafe_adamw_moments")
             out.update(zip(ps, zip(values[:n], values[n:])))
         return [out[p] for p in params]
