@@ -46,6 +46,9 @@ class AdamW(torch.optim.Optimizer):
         self._ticket = {}
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
+    def __getstate__(self):   # (torch's has the settings and the state alone: copies and pickles need the rest)
+        return {**super().__getstate__(), "state_bits": self.state_bits, "seed": self.seed, "_ticket": {}}
+
     @staticmethod
     def _check_settings(group):
         if isinstance(group["lr"], torch.Tensor):

@@ -292,6 +292,29 @@ def test_state_dict_round_trip(bits):
         other.load_state_dict(kept)
 
 
+def test_copies_and_pickles():
+    import copy
+    import pickle
+    import torch
+    from cafe_b200 import AdamW
+    net = torch.nn.Linear(33, 9).cuda()
+    opt = AdamW(net.parameters(), state_bits=8, seed=3)
+    for p in net.parameters():
+        p.grad = torch.ones_like(p)
+    opt.step()
+    for again in (copy.deepcopy((net, opt)), pickle.loads(pickle.dumps((net, opt)))):
+        n2, o2 = again
+        assert (o2.state_bits, o2.seed) == (8, 3)
+        for p in n2.parameters():
+            p.grad = torch.ones_like(p)
+        o2.step()
+    for p in net.parameters():
+        p.grad = torch.ones_like(p)
+    opt.step()
+    for a, b in zip(net.parameters(), n2.parameters()):
+        assert torch.equal(a, b)
+
+
 def test_captured_steps_count_on():
     import torch
     from cafe_b200 import AdamW
