@@ -885,7 +885,8 @@ int cafe_mlp_backward(int layers, const int* widths, int M, const void* gy_dev, 
     CafeBackward f[CAFE_MLP_MAX_LAYERS];
     for (int l = layers - 1; l >= 0; --l) {
         const bool last = l == layers - 1;
-        const int kind = acts[l] == CAFE_ACT_NONE ? CAFE_SLOPE_NONE : slope_dev && slope_dev[l] ? CAFE_SLOPE_VALUES : CAFE_SLOPE_OUTPUT;
+        const bool plain = acts[l] == CAFE_ACT_NONE || M == 0 || widths[l + 1] == 0;   // (a layer without outputs has no slope either)
+        const int kind = plain ? CAFE_SLOPE_NONE : slope_dev && slope_dev[l] ? CAFE_SLOPE_VALUES : CAFE_SLOPE_OUTPUT;
         if (kind == CAFE_SLOPE_OUTPUT && acts[l] != CAFE_ACT_RELU) return CAFE_ERR_ARG;
         const int64_t ldn = (widths[l + 1] + 7) & ~7, ldk = (widths[l] + 7) & ~7;
         f[l] = {last ? gy_dev : half[l & 1], kind == CAFE_SLOPE_VALUES ? slope_dev[l] : y_dev[l], l ? y_dev[l - 1] : x_dev, w_dev[l],

@@ -1029,14 +1029,15 @@ static cudaError_t tiles_launch(TilesProduct* q, int count, const TilesSums& sum
 static int64_t tiles_round(int64_t bytes) { return (bytes + 255) & ~(int64_t)255; }
 static int64_t tiles_pitch(int cols) { return (cols + 7) & ~7; }
 static int64_t tiles_bytes(int parts, int rows, int cols) { return tiles_round((int64_t)parts * rows * tiles_pitch(cols) * 2); }
-static bool tiles_in_place(int dtype, const void* p, int64_t ld) { return dtype != CAFE_F32 && ((uintptr_t)p & 15) == 0 && ld % 8 == 0; }
+// (one row that stands for all, pitch 0, is laid out like any other that copies cannot read)
+static bool tiles_in_place(int dtype, const void* p, int64_t ld, int cols) { return dtype != CAFE_F32 && ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && ld >= cols; }
 
 // an operand: in place, or laid out at *work by a job of the next k_parts launch
 template <typename T>
 static TilesOperand tiles_operand(CafeParts* P, char** work, int dtype, const void* src, int64_t ld, int rows, int cols, const void* slope, int64_t lds,
                                   int kind, float* sums) {
     typedef CafeTiles<T> L;
-    const bool in_place = kind == CAFE_SLOPE_NONE && tiles_in_place(dtype, src, ld);
+    const bool in_place = kind == CAFE_SLOPE_NONE && tiles_in_place(dtype, src, ld, cols);
     TilesOperand o = {src, ld, 0, rows, cols};
     if (in_place && !sums) return o;
     CafePartsJob& J = P->job[P->count++];
@@ -1077,15 +1078,15 @@ static bool tiles_large(int M, int N, int K, int64_t least) {
 int64_t cafe_tiles_forward_work(const CafeForward& f, int dtype) {
     if (!tiles_large(f.M, f.N, f.K, CAFE_TILES_LEAST)) return 0;
     const int parts = dtype == CAFE_F32 ? 3 : 1;
-    return 256 + (tiles_in_place(dtype, f.x, f.ldx) ? 0 : tiles_bytes(parts, f.M, f.K)) + (tiles_in_place(dtype, f.w, f.ldw) ? 0 : tiles_bytes(parts, f.N, f.K));
+    return 256 + (tiles_in_place(dtype, f.x, f.ldx, f.K) ? 0 : tiles_bytes(parts, f.M, f.K)) + (tiles_in_place(dtype, f.w, f.ldw, f.K) ? 0 : tiles_bytes(parts, f.N, f.K));
 }
 int64_t cafe_tiles_backward_work(const CafeBackward& f, int dtype) {
     if (!tiles_large(f.M, f.N, f.K, CAFE_TILES_LEAST_BACK) || (!f.gx && !f.gw)) return 0;
     const int parts = dtype == CAFE_F32 ? 3 : 1;
     int64_t need = 256;
-    if (f.slope_kind != CAFE_SLOPE_NONE || !tiles_in_place(dtype, f.gy, f.ldg)) need += tiles_bytes(parts, f.M, f.N);
-    if (f.gx && !tiles_in_place(dtype, f.w, f.ldw)) need += tiles_bytes(parts, f.N, f.K);
-    if (f.gw && !tiles_in_place(dtype, f.x, f.ldx)) need += tiles_bytes(parts, f.M, f.K);
+    if (f.slope_kind != CAFE_SLOPE_NONE || !tiles_in_place(dtype, f.gy, f.ldg, f.N)) need += tiles_bytes(parts, f.M, f.N);
+    if (f.gx && !tiles_in_place(dtype, f.w, f.ldw, f.K)) need += tiles_bytes(parts, f.N, f.K);
+    if (f.gw && !tiles_in_place(dtype, f.x, f.ldx, f.K)) need += tiles_bytes(parts, f.M, f.K);
     if (f.gw && dtype == CAFE_F32) need += tiles_partial_bytes(f.N, f.K, tiles_splits(f.N, f.K, f.M));
     if (f.gb) need += tiles_round((int64_t)((f.M + cafe_parts_rows(f.M, f.N) - 1) / cafe_parts_rows(f.M, f.N)) * f.N * 4);
     return need;

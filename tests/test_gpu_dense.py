@@ -148,6 +148,13 @@ def test_empty_sizes():
         gx, gw, gb = torch.autograd.grad(y.sum(), [x, w, b])
         assert not gx.any() and not gw.any()
         assert torch.equal(gb, (b > 0).float() * M)
+    x = torch.randn(5, 3, device="cuda", requires_grad=True)      # a layer of nothing between two others
+    w = [torch.randn(0, 3, device="cuda", requires_grad=True), torch.randn(2, 0, device="cuda", requires_grad=True)]
+    b = torch.randn(2, device="cuda", requires_grad=True)
+    y = fused_mlp(x, w, [None, b], ["gelu", "none"])
+    assert torch.equal(y, b.expand(5, 2))
+    gx, gb = torch.autograd.grad(y.sum(), [x, b])
+    assert not gx.any() and torch.equal(gb, torch.full_like(gb, 5))
     x = torch.randn(0, 3, device="cuda", requires_grad=True)
     w = [torch.randn(4, 3, device="cuda", requires_grad=True), torch.randn(2, 4, device="cuda", requires_grad=True)]
     grads = torch.autograd.grad(fused_mlp(x, w, [None, None], ["relu", "none"]).sum(), [x, *w])
@@ -218,6 +225,99 @@ def test_large_and_small_magnitudes():
         want, bound, *_ = ref.forward(x, w, None, "none", None, torch.float32)
         # (products below the smallest normal number may be flushed: six per term, 1.2e-38 each)
         ref.assert_within(fused_linear(x, w), want, bound + 90 * 6 * 1.2e-38, f"y at {sx} {sw}")
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("M,N,K", [(90, 40, 24), (2000, 512, 640)])
+def test_one_gradient_row_for_all(M, N, K, dtype):
+    import torch
+    from cafe_b200 import fused_linear
+    import dense_reference as ref
+    dt = getattr(torch, dtype)
+    x, w, b, _, gy = _make(M, N, K, dt, 47)
+    row = gy[:1].expand(M, N)
+    _, _, z, z_off = ref.forward(x, w, b, "silu", None, dt)
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+    got = torch.autograd.grad(fused_linear(*leaves, "silu"), leaves, row)
+    for a, (name, (value, far)) in zip(got, ref.backward(row, z, z_off, x, w, "silu", dt).items()):
+        ref.assert_within(a, value, far, name)
+
+
+def test_more_rows_than_the_laid_out_form_takes():
+    import torch
+    _check((1 << 20) + 77, 65, 64, torch.float32, "relu", seed=53)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("M,N,K", [(3, 50, 70), (130, 70, 90), (5000, 3, 37), (2500, 500, 450)])
+def test_what_lies_between_rows_is_left(M, N, K, dtype):
+    """The C entry points with outputs that are slices of wider tensors: nothing but the slices is written, and nothing past the
+    workspace that the library asked for."""
+    import torch
+    from cafe_b200 import _lib
+    import dense_reference as ref
+    dt, lib = getattr(torch, dtype), _lib.load()
+    t = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dt]
+    x, w, b, _, gy = _make(M, N, K, dt, 59)
+    st = torch.cuda.current_stream().cuda_stream
+    wide = lambda r, c: torch.full((r + 2, c + 5), 7.0, device="cuda", dtype=dt)   # noqa: E731
+    cut = lambda a, r, c: a[1:1 + r, 2:2 + c]                                      # noqa: E731
+    slope = torch.full((M + 2, N + 5), 7.0, device="cuda", dtype=torch.float16 if dt == torch.bfloat16 else torch.float32)
+    y, gx, gw, gb = wide(M, N), wide(M, K), wide(N, K), torch.full((N + 4,), 7.0, device="cuda", dtype=dt)
+    at = lambda a, r, c: cut(a, r, c).data_ptr()                                   # noqa: E731
+
+    def work(size):
+        return torch.full((size + 64,), 171, dtype=torch.uint8, device="cuda")
+    size = lib.cafe_linear_forward_work(x.data_ptr(), K, w.data_ptr(), K, M, N, K, t)
+    wf = work(size)
+    assert lib.cafe_linear_forward(x.data_ptr(), K, w.data_ptr(), K, b.data_ptr(), None, 0, M, N, K, t, 4, at(y, M, N), N + 5, at(slope, M, N), N + 5,
+                                   wf.data_ptr(), size, st) == 0
+    size = lib.cafe_linear_backward_work(gy.data_ptr(), N, 1, x.data_ptr(), K, w.data_ptr(), K, M, N, K, t, 1, 1, 1)
+    wb = work(size)
+    assert lib.cafe_linear_backward(gy.data_ptr(), N, at(slope, M, N), N + 5, 1, x.data_ptr(), K, w.data_ptr(), K, M, N, K, t, at(gx, M, K), K + 5,
+                                    at(gw, N, K), K + 5, gb[2:].data_ptr(), wb.data_ptr(), size, st) == 0
+    torch.cuda.synchronize()
+    assert bool((wf[-64:] == 171).all()) and bool((wb[-64:] == 171).all())
+    want, bound, z, z_off = ref.forward(x, w, b, "silu", None, dt)
+    ref.assert_within(cut(y, M, N), want, bound, "y")
+    back = ref.backward(gy, z, z_off, x, w, "silu", dt)
+    for name, got in (("gx", cut(gx, M, K)), ("gw", cut(gw, N, K)), ("gb", gb[2:2 + N])):
+        ref.assert_within(got, *back[name], name)
+    for a, r, c in ((y, M, N), (slope, M, N), (gx, M, K), (gw, N, K)):
+        cut(a, r, c).fill_(7.0)
+        assert bool((a == 7).all())
+    gb[2:2 + N] = 7
+    assert bool((gb == 7).all())
+
+
+def test_two_threads():
+    """Calls of different sizes from two threads, each on its own stream."""
+    import threading
+    import torch
+    from cafe_b200 import fused_linear
+    sizes = [(3000, 600, 500), (40, 130, 90)]
+    sets = [_make(M, N, K, torch.float32, 61 + i) for i, (M, N, K) in enumerate(sizes)]
+    want = [fused_linear(x, w, b, "gelu") for x, w, b, _, _ in sets]
+    torch.cuda.synchronize()
+    got, errors = [[], []], []
+
+    def go(i):
+        try:
+            x, w, b, _, _ = sets[i]
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(30):
+                    got[i].append(fused_linear(x, w, b, "gelu"))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:   # noqa: BLE001
+            errors.append(e)
+    threads = [threading.Thread(target=go, args=(i,)) for i in range(2)]
+    for q in threads:
+        q.start()
+    for q in threads:
+        q.join()
+    assert not errors, errors
+    for i in range(2):
+        assert all(torch.equal(a, want[i]) for a in got[i])
 
 
 def test_offsets_past_32_bits():
@@ -294,10 +394,11 @@ def test_fused_mlp_module_is_the_reference_mlp():
     assert all(p.grad is not None and p.grad.shape == p.shape for p in fused.parameters())
 
 
-def test_on_another_stream_and_two_calls_at_once():
+@pytest.mark.parametrize("M,N,K", [(150, 400, 300), (1500, 700, 900)])
+def test_on_another_stream_and_two_calls_at_once(M, N, K):
     import torch
     from cafe_b200 import fused_linear
-    x, w, b, _, gy = _make(1500, 400, 300, torch.float32, 31)
+    x, w, b, _, gy = _make(M, N, K, torch.float32, 31)
     want = fused_linear(x, w, b, "gelu")
     streams = [torch.cuda.Stream() for _ in range(2)]
     torch.cuda.synchronize()
@@ -317,7 +418,7 @@ def test_on_another_stream_and_two_calls_at_once():
 def test_repeated_calls_give_the_same_bits():
     import torch
     from cafe_b200 import fused_linear
-    for M, N, K in [(9000, 130, 70), (64, 512, 1000), (30000, 16, 40)]:
+    for M, N, K in [(9000, 130, 70), (64, 512, 1000), (30000, 16, 40), (20000, 200, 300), (2048, 1024, 1024)]:
         x, w, b, _, gy = _make(M, N, K, torch.float32, 37)
         leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
         first = None
@@ -328,16 +429,17 @@ def test_repeated_calls_give_the_same_bits():
             first = now
 
 
-def test_captured_and_replayed():
+@pytest.mark.parametrize("M,N,K", [(700, 130, 260), (3000, 640, 900)])
+def test_captured_and_replayed(M, N, K):
     """Two captured graphs of forward and backward, replayed in turn and on two streams at once with new inputs."""
     import torch
     from cafe_b200 import fused_linear, fused_mlp
     sets = []
     for seed in (41, 42):
-        x, w, b, _, gy = _make(700, 130, 260, torch.float32, seed)
-        w2 = torch.randn(40, 130, device="cuda") * 0.1
+        x, w, b, _, gy = _make(M, N, K, torch.float32, seed)
+        w2 = torch.randn(40, N, device="cuda") * 0.1
         x, w, b, w2 = (t.detach().clone().requires_grad_(True) for t in (x, w, b, w2))
-        gy = torch.randn(700, 40, device="cuda")
+        gy = torch.randn(M, 40, device="cuda")
 
         def go(x=x, w=w, b=b, w2=w2, gy=gy):
             y = fused_linear(fused_linear(x, w, b, "gelu"), w2)
