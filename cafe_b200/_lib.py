@@ -81,6 +81,7 @@ SIGNATURES = {
     "cafe_linear_backward": (c_int, [_vp, c_int64, _vp, c_int64, c_int, _vp, c_int64, _vp, c_int64, c_int, c_int, c_int, c_int, _vp,
                                      c_int64, _vp, c_int64, _vp, _vp, c_int64, _vp]),
     "cafe_linear_backward_work": (c_int64, [_vp, c_int64, c_int, _vp, c_int64, _vp, c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "cafe_linear_gave_up": (c_int, [_i32p]),
     "cafe_mlp_forward": (c_int, [c_int, _i32p, c_int, _vp, c_int64, POINTER(_vp), _i64p, POINTER(_vp), _i32p, c_int, POINTER(_vp), _i64p,
                                  POINTER(_vp), _vp, c_int64, _vp]),
     "cafe_mlp_forward_work": (c_int64, [c_int, _i32p, c_int, _vp, c_int64, POINTER(_vp), _i64p, c_int]),

@@ -269,3 +269,4 @@ int64_t cafe_tiles_forward_work(const CafeForward& f, int dtype);
 int64_t cafe_tiles_backward_work(const CafeBackward& f, int dtype);
 cudaError_t cafe_tiles_forward(const CafeForward& f, int dtype, const CafeJob& job, void* work, cudaStream_t st);
 cudaError_t cafe_tiles_backward(const CafeBackward& f, int dtype, const CafeJob* gw, const CafeJob* gx, void* work, cudaStream_t st);
+cudaError_t cafe_tiles_gave_up(int* flag);

@@ -36,7 +36,7 @@ template <typename T, int BN> struct CafeLinShape {
     static constexpr int tm_cols = CafeLin<T>::parts == 3 ? 2 * BN : BN;
 };
 
-__device__ int g_dense_gave_up;   // a wait ran out (its outputs are not numbers)
+__device__ int g_dense_gave_up;   // 1: a wait of k_linear ran out (its outputs are not numbers)
 
 // eight values along k of one row: fp32, or 16-bit values two to a register
 template <typename T> struct CafePiece { uint32_t v[4]; };
@@ -829,6 +829,15 @@ int cafe_linear_backward(const void* gy_dev, int64_t ldg, const void* slope_dev,
     if (!dense_type_ok(dtype) || !dense_backward_ok(f) || !dense_work_ok(work_dev, work_bytes)) return CAFE_ERR_ARG;
     cudaError_t e;
     DENSE_TYPED(dtype, e = dense_backward<T>(f, dtype, work_dev, work_bytes, (cudaStream_t)stream));
+    return dense_done(e);
+}
+
+int cafe_linear_gave_up(int* count) {
+    if (!count) return CAFE_ERR_ARG;
+    int mine = 0, tiles = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(&mine, g_dense_gave_up, sizeof mine);
+    if (e == cudaSuccess) e = cafe_tiles_gave_up(&tiles);
+    *count = mine + tiles;
     return dense_done(e);
 }
 

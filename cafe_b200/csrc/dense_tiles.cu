@@ -22,7 +22,8 @@ static __host__ __device__ constexpr int cafe_parts_rows(int rows, int cols) {
     return (int64_t)((rows + 127) / 128) * ((cols + CAFE_PARTS_COLS - 1) / CAFE_PARTS_COLS) >= 1024 ? 128 : 32;
 }
 
-__device__ int g_tiles_gave_up;   // a wait ran out (its outputs are not numbers)
+__device__ int g_tiles_gave_up;   // 1: a wait ran out (its outputs are not numbers)
+cudaError_t cafe_tiles_gave_up(int* flag) { return cudaMemcpyFromSymbol(flag, g_tiles_gave_up, sizeof *flag); }
 
 template <typename T> struct CafeTiles {
     static constexpr int parts = 1, BK = 64, type = 0;

@@ -62,15 +62,6 @@ __device__ __forceinline__ void cafe_tm_load16(uint32_t at, float* v) {
                  : "r"(at));
 }
 
-// and back
-__device__ __forceinline__ void cafe_tm_store16(uint32_t at, const float* v) {
-    const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at), "r"(r[0]), "r"(r[1]),
-                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
-                 "r"(r[14]), "r"(r[15]) : "memory");
-}
-__device__ __forceinline__ void cafe_tm_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
 // D[128 x N] (+)= A[128 x 16] B[N x 16]^T, operands in shared memory (descriptors), D in tensor memory
 __device__ __forceinline__ void cafe_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool add) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(instr), "r"((uint32_t)add) : "memory");

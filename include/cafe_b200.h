@@ -330,10 +330,10 @@ int cafe_dot_interaction_backward(const float* x_dev, const float* emb_dev, int6
  * z = x W^T + b, y = act(z) + res for x [M, K], W [N, K], rows `ld` elements apart (ld >= the row's length; elements of a
  * row are contiguous).  All tensors of a call have one type; sums are fp32.  bias, res and slope may be null; ldr = 0: one
  * row of res for all.  slope_dev receives act'(z) for the backward: fp16 beside bf16, else fp32.
- * M, N, K <= CAFE_LINEAR_MAX.  Outputs overlap nothing else of the call.  No host synchronisation, no device memory of its own: work_dev (16-byte aligned, free again once
- * the call's work on `stream` is done; two calls that may run at once need one each) lets large layers lay their operands out
- * first; the *_work functions give its bytes for a call's arguments (0: none needed).  With less, or null, the call computes the
- * same without. */
+ * M, N, K <= CAFE_LINEAR_MAX.  Outputs overlap nothing else of the call.  No host synchronisation, no device memory of its
+ * own: work_dev (16-byte aligned, free again once the call's work on `stream` is done; two calls that may run at once need one
+ * each) lets large layers lay their operands out first; the *_work functions give its bytes for a call's arguments (0: none
+ * needed).  With less, or null, the call takes kernels that need none: the same values, sums in other orders. */
 enum { CAFE_F32 = 0, CAFE_BF16 = 1, CAFE_F16 = 2 };
 enum { CAFE_ACT_NONE = 0, CAFE_ACT_RELU = 1, CAFE_ACT_SIGMOID = 2, CAFE_ACT_GELU = 3, CAFE_ACT_SILU = 4 };
 /* what slope_dev of a backward holds: nothing (no activation), act'(z), or y of a ReLU without residual (y > 0) */
@@ -351,6 +351,9 @@ int cafe_linear_backward(const void* gy_dev, int64_t ldg, const void* slope_dev,
                          void* gb_dev, void* work_dev, int64_t work_bytes, void* stream);
 int64_t cafe_linear_backward_work(const void* gy_dev, int64_t ldg, int slope_kind, const void* x_dev, int64_t ldx, const void* w_dev, int64_t ldw,
                                   int M, int N, int K, int dtype, int want_gx, int want_gw, int want_gb);
+/* Every wait inside these kernels has an end (about a second): if one runs out, what it waited for is stored as NaN.  *count: how
+ * many of the two kinds of kernel this has happened to on the current device since the library was loaded (waits for the device). */
+int cafe_linear_gave_up(int* count);
 /* `layers` layers one behind the other: layer l maps widths[l] to widths[l + 1] with acts[l]; its output goes to y_dev[l]
  * (pitch ldy[l]) and, where slope_dev[l] is not null, act'(z) to slope_dev[l] (same pitch). */
 int cafe_mlp_forward(int layers, const int* widths, int M, const void* x_dev, int64_t ldx, const void* const* w_dev, const int64_t* ldw,
