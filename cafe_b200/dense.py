@@ -102,6 +102,13 @@ def _contiguous(t):
     return t if t is None or t.is_contiguous() else t.contiguous()
 
 
+def _saved_rows(t, cols):
+    if t is None or t.is_contiguous():
+        return t, cols
+    t, _, ld = _rows(t, cols)
+    return t, ld
+
+
 def _linear(x, weight, bias, residual, act, keep):
     """The forward call: (x, weight as rows, y, what the backward needs of the activation)."""
     n, k = weight.shape
@@ -124,7 +131,7 @@ def _linear(x, weight, bias, residual, act, keep):
                                          _ptr(_work(size, x)), size, stream)
     if status:
         _lib.check(status, "cafe_linear_forward")
-    return x2, w2, y, slope, (m, n, k, ldx, ldw)
+    return x2, w2, y, slope, (m, n, k)
 
 
 class _FusedLinear(torch.autograd.Function):
@@ -146,12 +153,16 @@ class _FusedLinear(torch.autograd.Function):
 
 def _linear_backward(ctx, grad_y):
     x, w, slope = ctx.saved_tensors
-    m, n, k, ldx, ldw = ctx.sizes
+    m, n, k = ctx.sizes
     need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
     gx = gw = gb = None
     if need_x or need_w or need_b:
         g, _, ldg = _rows(grad_y, n, True)
         dtype, device = g.dtype, g.device
+        # (what was saved need not come back at the pitch that it was saved with)
+        x, ldx = _saved_rows(x, k)
+        w, ldw = _saved_rows(w, k)
+        slope = _contiguous(slope)
         if need_x:
             gx = torch.empty(ctx.shape, dtype=dtype, device=device)
         if need_w:
@@ -177,8 +188,8 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
                  residual: torch.Tensor | None = None) -> torch.Tensor:
     """act(x W^T + b) + residual.  x [..., K], weight [N, K], bias [N]; residual broadcasts to [..., N]; activation is one of
     none, relu, sigmoid, gelu (with erf) and silu.  x, weight and residual may be slices of wider tensors (any pitch
-    between rows).  For the backward the call keeps x, weight and, with an activation, its derivative (fp32 or fp16); of a ReLU
-    without residual the output."""
+    between rows).  For the backward the call keeps x, weight and, with an activation, its derivative (fp16 beside bf16, else
+    fp32); of a ReLU without residual the output."""
     _check(x, (weight, bias, residual), "fused_linear")
     if activation not in ACTIVATIONS:
         raise ValueError(f"fused_linear: activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
@@ -266,7 +277,7 @@ def _mlp(x, weights, biases, acts, keep):
                                       plan.slopes(base) if keep else None, _ptr(_work(size, x)), size, stream)
     if status:
         _lib.check(status, "cafe_mlp_forward")
-    return x2, ws, y, between, (plan, m, ldx, lds)
+    return x2, ws, y, between, (plan, m)
 
 
 class _FusedMLP(torch.autograd.Function):
@@ -285,8 +296,12 @@ class _FusedMLP(torch.autograd.Function):
 
 def _mlp_backward(ctx, grad_y):
     x, y, between, *ws = ctx.saved_tensors
-    plan, m, ldx, lds = ctx.sizes
+    plan, m = ctx.sizes
     n, need = plan.n, ctx.needs_input_grad
+    # (what was saved need not come back at the pitch that it was saved with)
+    x, ldx = _saved_rows(x, plan.widths[0])
+    ws, lds = _weight_rows(ws)
+    y, between = y.contiguous(), between.contiguous()
     g, _, ldg = _rows(grad_y, plan.widths[n], True)
     dtype, device = g.dtype, g.device
     gx = torch.empty(ctx.shape, dtype=dtype, device=device) if need[0] else None

@@ -290,6 +290,27 @@ def test_what_lies_between_rows_is_left(M, N, K, dtype):
     assert bool((gb == 7).all())
 
 
+@pytest.mark.parametrize("M,N,K", [(60, 40, 50), (1500, 500, 450)])
+def test_saved_tensors_that_come_back_at_another_pitch(M, N, K):
+    """save_on_cpu brings slices of wider tensors back without what lay between their rows."""
+    import torch
+    from cafe_b200 import fused_linear, fused_mlp
+    x, w, b, _, gy = _make(M, N, K, torch.float32, 67)
+    wide = lambda t: torch.cat([t, torch.full((t.shape[0], 3), float("nan"), device="cuda")], 1)[:, :t.shape[1]]   # noqa: E731
+    w2 = torch.randn(20, N, device="cuda")
+    calls = {"linear": (lambda x, w, b: fused_linear(x, w, b, "gelu"), [x, w, b], gy),
+             "relu": (lambda x, w, b: fused_linear(x, w, b, "relu"), [x, w, b], gy),
+             "mlp": (lambda x, w, b, w2: fused_mlp(x, [w, w2], [b, None], ["silu", "none"]), [x, w, b, w2], gy[:, :20].contiguous())}
+    for name, (call, leaves, grad) in calls.items():
+        leaves = [t.detach().requires_grad_(True) for t in leaves]
+        want = torch.autograd.grad(call(*leaves), leaves, grad)
+        sliced = [wide(t.detach()).requires_grad_(True) if t.dim() == 2 else t for t in leaves]
+        with torch.autograd.graph.save_on_cpu():
+            y = call(*sliced)
+        for a, e in zip(torch.autograd.grad(y, sliced, grad), want):
+            torch.testing.assert_close(a, e, rtol=1e-4, atol=1e-4)   # (other kernels may take a slice: sums of 1500 terms in other orders)
+
+
 def test_two_threads():
     """Calls of different sizes from two threads, each on its own stream."""
     import threading
@@ -487,3 +508,13 @@ def test_refusals_with_cuda_tensors():
     gx, = torch.autograd.grad(fused_linear(lx, w, b, "gelu").sum(), lx, create_graph=True)
     with pytest.raises(RuntimeError):
         gx.sum().backward()
+
+
+def test_no_wait_has_run_out():
+    """Last of the file: the count of waits that ran out in all that ran before."""
+    import ctypes
+    from cafe_b200 import _lib
+    count = ctypes.c_int32(-1)
+    assert _lib.load().cafe_linear_gave_up(ctypes.byref(count)) == 0
+    assert count.value == 0
+    assert _lib.load().cafe_linear_gave_up(None) == 1
