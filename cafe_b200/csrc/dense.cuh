@@ -85,41 +85,19 @@ struct CafeJobs {
 __device__ __forceinline__ void cafe_put16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
-// A(i, k) B(j, k) added up in the plain order, for sums that the split operands turned into a NaN: an infinite part times a
-// lower part that is zero is one, where infinity times the whole number is not
-static __device__ __noinline__ float cafe_plain_dot(const CafeJob& J, int64_t i, int64_t j, int k0, int k1) {
-    const float *a = static_cast<const float*>(J.a), *b = static_cast<const float*>(J.b), *s = static_cast<const float*>(J.as);
-    float sum = 0.f;
-    for (int64_t k = k0; k < k1 && sum == sum; ++k) {
-        float x = __ldg(a + (J.a_kc ? i * J.lda + k : k * J.lda + i));
-        if (J.slope_kind != CAFE_SLOPE_NONE) {
-            const float t = __ldg(s + (J.a_kc ? i * J.ldas + k : k * J.ldas + i));
-            x = J.slope_kind == CAFE_SLOPE_VALUES ? x * t : t > 0.f ? x : 0.f;
-        }
-        sum += x * __ldg(b + (J.b_kc ? j * J.ldb + k : k * J.ldb + j));
-    }
-    return sum;
-}
+// The large sums of split operands and the others joined.  Of infinite operands the large sums alone are right: the lower parts of an
+// infinity are NaN, and times a lower part that is zero it would be one too.  (An infinity times a number below 2^-133, whose upper
+// part is zero, becomes NaN.)
+__device__ __forceinline__ float cafe_join_sums(float large, float rest) { return fabsf(large) < INFINITY ? large + rest : large; }
+// fp32 for splitting: every NaN with its upper bits set (an upper part that is cut off must not become an infinity)
+__device__ __forceinline__ float cafe_quiet(float x) { return x + 0.f; }
 
 // ---- the end of a product --------------------------------------------------------------------------------------------
-// A thread's 4 * QUADS consecutive columns of row r of the block's sums to shared memory; a NaN of split operands is looked into.
-template <bool SPLIT, int N>
-__device__ __forceinline__ void cafe_sums_put(const CafeJob& J, const float* acc, uint32_t at, int64_t row, int64_t col, int k0, int k1, bool look) {
-    bool nan = false;
+// A thread's N consecutive columns of a row of the block's sums to shared memory.
+template <int N> __device__ __forceinline__ void cafe_sums_put(const float* acc, uint32_t at) {
 #pragma unroll
-    for (int c = 0; c < N; c += 4) {
+    for (int c = 0; c < N; c += 4)
         cafe_put16(at + 4 * c, __float_as_uint(acc[c]), __float_as_uint(acc[c + 1]), __float_as_uint(acc[c + 2]), __float_as_uint(acc[c + 3]));
-        if (SPLIT) nan |= !(acc[c] == acc[c]) | !(acc[c + 1] == acc[c + 1]) | !(acc[c + 2] == acc[c + 2]) | !(acc[c + 3] == acc[c + 3]);
-    }
-    if (SPLIT && nan && look && row < J.rows)
-        for (int c = 0; c < N && col + c < J.cols; ++c) {
-            float v;
-            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at + 4 * c) : "memory");
-            if (v != v) {
-                v = cafe_plain_dot(J, row, col + c, k0, k1);
-                asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + 4 * c), "f"(v) : "memory");
-            }
-        }
 }
 // Four neighbouring elements of the residual (row i, columns j ..), as they lie.
 template <typename T> struct CafeQuad { alignas(4 * sizeof(T)) T v[4]; };

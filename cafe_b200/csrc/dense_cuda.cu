@@ -96,7 +96,7 @@ __device__ __forceinline__ void cafe_piece_store(const CafePiece<float>& p, uint
     uint32_t h[4], m[4], l[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const float x = p.v[2 * j], y = p.v[2 * j + 1];
+        const float x = cafe_quiet(p.v[2 * j]), y = cafe_quiet(p.v[2 * j + 1]);
         h[j] = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
         const float xm = x - __uint_as_float(__float_as_uint(x) & 0xffff0000u), ym = y - __uint_as_float(__float_as_uint(y) & 0xffff0000u);
         m[j] = __byte_perm(__float_as_uint(xm), __float_as_uint(ym), 0x7632);
@@ -338,7 +338,16 @@ __global__ void __launch_bounds__(CAFE_LIN_THREADS, 1) k_linear(const __grid_con
             fine = cafe_bar_wait(all_done, 0, &bail) && fine;
             cafe_tc_after();
             fine = __all_sync(0xffffffffu, fine);
-            if (L::parts == 3 && fine) take(from + BN, false);
+            if (L::parts == 3 && fine) {
+#pragma unroll
+                for (int c = 0; c < half_cols; c += 16) {
+                    float v[16];
+                    cafe_tm_load16(from + BN + c, v);
+                    cafe_tm_wait_load();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[c + i] = cafe_join_sums(acc[c + i], v[i]);
+                }
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < half_cols; ++i) acc[i] = 0.f;
@@ -357,8 +366,7 @@ __global__ void __launch_bounds__(CAFE_LIN_THREADS, 1) k_linear(const __grid_con
     // ---- the block's sums to shared memory, and what belongs at the end
     if (warp >= 8) {
         const int r = (warp & 3) * 32 + lane, c0 = (warp - 8) / 4 * half_cols;
-        cafe_sums_put<L::parts == 3, half_cols>(J, acc, base + (uint32_t)(r * (BN + 4) + c0) * 4u, row0 + r, col0 + c0, t0 * L::BK,
-                                                min(J.depth, (t0 + turns) * L::BK), !bail);
+        cafe_sums_put<half_cols>(acc, base + (uint32_t)(r * (BN + 4) + c0) * 4u);
     }
     if (splits > 1) cafe_cluster_sync(); else __syncthreads();
     cafe_finish<T, BN>(J, base, row0, col0, rank, splits, CAFE_LIN_THREADS);

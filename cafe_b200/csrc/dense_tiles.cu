@@ -103,6 +103,8 @@ __global__ void __launch_bounds__(256) k_parts(const __grid_constant__ CafeParts
                 *out = *reinterpret_cast<const uint4*>(o);
             } else {
 #pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = cafe_quiet(v[j]);
+#pragma unroll
                 for (int p = 0; p < 3; ++p) {   // the next 8 bits of each, cut off
                     uint32_t o[4];
 #pragma unroll
@@ -292,7 +294,16 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
             fine = cafe_bar_wait(all_done, 0, &bail) && fine;
             cafe_tc_after();
             fine = __all_sync(0xffffffffu, fine);
-            if (fine && turns > 0) take(from + BN, false);
+            if (fine && turns > 0) {
+#pragma unroll
+                for (int c = 0; c < BN; c += 16) {
+                    float v[16];
+                    cafe_tm_load16(from + BN + c, v);
+                    cafe_tm_wait_load();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[c + i] = cafe_join_sums(acc[c + i], v[i]);
+                }
+            }
         } else {
             fine = cafe_bar_wait(all_done, 0, &bail);
             cafe_tc_after();
@@ -314,7 +325,7 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
 #pragma unroll
                     for (int i = 0; i < BN; ++i) acc[i] = __uint_as_float(0x7fffffffu);
                 }
-                cafe_sums_put<true, BN>(J, acc, at, row0 + r, col0, t0 * L::BK, min(J.depth, (t0 + turns) * L::BK), ok);
+                cafe_sums_put<BN>(acc, at);
             } else {
 #pragma unroll
                 for (int c = 0; c < 128; c += 32) {
@@ -325,7 +336,7 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
 #pragma unroll
                         for (int i = 0; i < 32; ++i) acc[i] = ok ? 0.f : __uint_as_float(0x7fffffffu);
                     }
-                    cafe_sums_put<false, 32>(J, acc, at + 4 * c, 0, 0, 0, 0, false);
+                    cafe_sums_put<32>(acc, at + 4 * c);
                 }
             }
         }
@@ -726,7 +737,14 @@ __global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) k_tiles_pair(const __gri
                 fine = __all_sync(0xffffffffu, fine);
                 if (fine) {
                     take(from, between == 0);
-                    take(from + BN, false);
+#pragma unroll
+                    for (int c = 0; c < Sh::mine; c += 16) {
+                        float v[16];
+                        cafe_tm_load16(from + BN + c, v);
+                        cafe_tm_wait_load();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) acc[c + i] = cafe_join_sums(acc[c + i], v[i]);
+                    }
                 } else {
 #pragma unroll
                     for (int i = 0; i < Sh::mine; ++i) acc[i] = __uint_as_float(0x7fffffffu);
@@ -745,19 +763,12 @@ __global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) k_tiles_pair(const __gri
 #pragma unroll 1
                     for (int c = 0; c < W; c += 16) {
                         float z[16];
-                        bool nan = false;
 #pragma unroll
                         for (int q = 0; q < 16; q += 4) {
                             const uint4 x = cafe_get16(cafe_staged<128>(out, lane, (c + q) / 4));
                             z[q] = __uint_as_float(x.x); z[q + 1] = __uint_as_float(x.y); z[q + 2] = __uint_as_float(x.z); z[q + 3] = __uint_as_float(x.w);
-                            nan |= !(z[q] == z[q]) | !(z[q + 1] == z[q + 1]) | !(z[q + 2] == z[q + 2]) | !(z[q + 3] == z[q + 3]);
                         }
-                        const int64_t j = col0 + h + c;
-                        if (nan && fine && lane < m) {
-#pragma unroll
-                            for (int q = 0; q < 16; ++q) if (z[q] != z[q] && j + q < J.cols) z[q] = cafe_plain_dot(J, row0 + lane, j + q, t0 * L::BK, min(J.depth, t1 * L::BK));
-                        }
-                        cafe_row_end<T, Sh::out_row, Sh::slope_row, false>(J, z, j, out, slopes, lane, c);
+                        cafe_row_end<T, Sh::out_row, Sh::slope_row, false>(J, z, col0 + h + c, out, slopes, lane, c);
                     }
                     __syncwarp();
                     const int here = min(W, columns - h);

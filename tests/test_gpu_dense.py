@@ -214,6 +214,24 @@ def test_infinities_and_nans(act, M):
     assert float((got.double() - want)[fine].abs().max()) < 1e-4
 
 
+@pytest.mark.parametrize("M,N,K", [(900, 40, 50), (60000, 150, 96), (5000, 300, 400)])
+def test_gradients_that_are_not_finite(M, N, K):
+    """An infinite gradient reaches its row of gx and of gW with the signs that the sums give it; a NaN with nothing but its lowest
+    bit set (whose upper half alone would be an infinity) stays one."""
+    import torch
+    from cafe_b200 import fused_linear
+    x, w, _, _, gy = _make(M, N, K, torch.float32, 71)
+    x, w = x.sign() * 1.5, w.sign() * 0.25            # (few bits: lower parts that are zero)
+    gy[M // 2, 3], gy[7, 20] = float("inf"), -float("inf")
+    gy.view(torch.int32)[11, 9] = 0x7f800001
+    leaves = [t.detach().requires_grad_(True) for t in (x, w)]
+    gx, gw = torch.autograd.grad(fused_linear(*leaves), leaves, gy)
+    for got, want in ((gx, gy.double() @ w.double()), (gw, gy.double().t() @ x.double())):
+        assert torch.equal(got.isnan(), want.isnan())
+        inf = want.isinf()
+        assert torch.equal(got.isinf(), inf) and torch.equal(got[inf].double(), want[inf])
+
+
 def test_large_and_small_magnitudes():
     """Products far from 1: every part of a split operand keeps its place."""
     import torch
