@@ -1,8 +1,9 @@
-"""Builds libcafe_b200.so in-tree with nvcc for sm_100a.
+"""Builds libcafe_b200.so in-tree with nvcc for sm_100a, and _dense_torch.so with g++.
 
     python -m cafe_b200.build [--force]
 
-The library is a plain C-ABI shared object (include/cafe_b200.h); nothing here links against torch.
+The library is a plain C-ABI shared object (include/cafe_b200.h) that does not link against torch.  _dense_torch.so, the
+autograd nodes of the dense layers, links against it and torch.
 """
 from __future__ import annotations
 
@@ -16,6 +17,8 @@ CSRC = PKG / "csrc"
 SO = PKG / "libcafe_b200.so"
 SOURCES = ["sketch_cuda.cu", "embed_cuda.cu", "sigmod_cuda.cu", "interact_cuda.cu", "dense_cuda.cu", "dense_tiles.cu", "adamw_cuda.cu", "ref_abi.cu", "prof.cu"]
 HEADERS = ["cafe_types.h", "cafe_internal.h", "sketch_core.cuh", "sketch_engine.h", "radix_sort.cuh", "cafe_float.cuh", "tcgen05.cuh", "dense.cuh"]
+TORCH_SO = PKG / "_dense_torch.so"
+TORCH_SOURCE = CSRC / "dense_torch.cpp"
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
               "--expt-relaxed-constexpr"]
 # the sketch arithmetic must not be contracted into fused multiply-adds: counts are compared bit for bit
@@ -67,5 +70,28 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     return SO
 
 
+def build_torch(force: bool = False) -> Path:
+    """The extension module cafe_b200._dense_torch (after build(): it is linked against the library)."""
+    deps = [TORCH_SOURCE, PKG.parent / "include" / "cafe_b200.h", Path(__file__)]
+    if not force and TORCH_SO.exists() and all(d.stat().st_mtime <= TORCH_SO.stat().st_mtime for d in deps):
+        return TORCH_SO
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    nvcc = Path(_nvcc())
+    cuda = [f"-I{nvcc.parent.parent / 'include'}"] if nvcc.is_absolute() else []
+    # (g++ itself, whatever CXX says: a second libstdc++ linked into the module would crash on the first formatted message)
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[f"-I{p}" for p in cpp_extension.include_paths()], *cuda, f"-I{sysconfig.get_paths()['include']}", str(TORCH_SOURCE), "-o", str(TORCH_SO),
+           *[f"-L{p}" for p in cpp_extension.library_paths()], f"-L{PKG}", "-Wl,-rpath,$ORIGIN", f"-l:{SO.name}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
+           "-ltorch", "-ltorch_python"]
+    r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on {TORCH_SOURCE.name}:\n{r.stdout}")
+    return TORCH_SO
+
+
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose="-v" in sys.argv))
+    print(build_torch(force="--force" in sys.argv))

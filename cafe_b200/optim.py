@@ -6,7 +6,28 @@ import ctypes
 import torch
 
 from . import _lib
-from .dense import DTYPES, _on
+from .sketch import _stream
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)   # (without the checks of the public form)
+
+
+class _on:
+    """The tensors' device as the current one; `as` its current stream."""
+    __slots__ = ("other",)
+
+    def __init__(self, device):
+        self.other = None if device.index == _get_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.other is not None:
+            self.other.__enter__()
+        return _stream()
+
+    def __exit__(self, *args):
+        if self.other is not None:
+            self.other.__exit__(*args)
+
 
 BLOCK = 256   # elements that share the exponent of their 8-bit moments
 _CODES = ("exp_avg", "exp_avg_top", "root_avg_sq", "root_avg_sq_top")

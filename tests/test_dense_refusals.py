@@ -78,3 +78,20 @@ def test_python_refusals_on_cpu_tensors():
     for bad in [dict(lr=-1), dict(betas=(0.9, 1.0)), dict(eps=-1e-8), dict(weight_decay=-1), dict(state_bits=16), dict(lr=float("nan"))]:
         with pytest.raises(ValueError):
             cafe_b200.AdamW([], **bad)
+
+
+def test_torch_entry_points_without_a_gpu():
+    """The messages of the extension module are formatted and come as ValueError."""
+    import torch
+    from cafe_b200 import fused_linear, fused_mlp
+    x, w = torch.zeros(4, 6), torch.zeros(5, 6)
+    with pytest.raises(ValueError, match="needs CUDA tensors"):
+        fused_linear(x, w)
+    with pytest.raises(ValueError, match="1 to 32 weights"):
+        fused_mlp(x, [], [], [])
+    with pytest.raises(ValueError, match="1 to 32 weights"):
+        fused_mlp(x, [w], [], ["relu"])
+    with pytest.raises(ValueError, match="activation"):
+        fused_linear(x, w, activation="tanh")
+    with pytest.raises(TypeError):
+        fused_linear(x, None)

@@ -148,6 +148,12 @@ def test_empty_sizes():
         gx, gw, gb = torch.autograd.grad(y.sum(), [x, w, b])
         assert not gx.any() and not gw.any()
         assert torch.equal(gb, (b > 0).float() * M)
+    x = torch.randn(2, 3, 0, device="cuda", requires_grad=True)   # no depth, more than two axes
+    w, b = torch.randn(4, 0, device="cuda", requires_grad=True), torch.randn(4, device="cuda", requires_grad=True)
+    y = fused_linear(x, w, b, "relu")
+    assert torch.equal(y, b.clamp(min=0).expand(2, 3, 4))
+    gb, = torch.autograd.grad(y.sum(), [b])
+    assert torch.equal(gb, 6.0 * (b > 0))
     x = torch.randn(5, 3, device="cuda", requires_grad=True)      # a layer of nothing between two others
     w = [torch.randn(0, 3, device="cuda", requires_grad=True), torch.randn(2, 0, device="cuda", requires_grad=True)]
     b = torch.randn(2, device="cuda", requires_grad=True)
@@ -526,6 +532,46 @@ def test_refusals_with_cuda_tensors():
     gx, = torch.autograd.grad(fused_linear(lx, w, b, "gelu").sum(), lx, create_graph=True)
     with pytest.raises(RuntimeError):
         gx.sum().backward()
+
+
+@pytest.mark.parametrize("call", ["relu", "gelu", "mlp"])
+def test_as_a_node_of_the_graph(call):
+    """A second backward needs retain_graph, what was saved must not have been written to, nothing is left behind."""
+    import gc
+    import torch
+    from cafe_b200 import fused_linear, fused_mlp
+    x, w, b, _, gy = _make(70, 60, 50, torch.float32, 73)
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+
+    def forward():
+        x, w, b = leaves
+        return fused_mlp(x, [w], [b], ["silu"]) if call == "mlp" else fused_linear(x, w, b, call)
+    y = forward()
+    first = torch.autograd.grad(y, leaves, gy, retain_graph=True)
+    again = torch.autograd.grad(y, leaves, gy)
+    assert all(torch.equal(p, q) for p, q in zip(first, again))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y, leaves, gy)
+    y = forward()
+    with torch.no_grad():
+        leaves[1].mul_(2)
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(y, leaves, gy)
+    y = forward()
+    gw, = torch.autograd.grad(y, leaves[1], gy)
+    assert torch.isfinite(gw).all()
+    assert "Fused" in y.grad_fn.name()
+    del y, gw, first, again
+    gc.collect()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for _ in range(20):
+        y = forward()
+        torch.autograd.grad(y, leaves, gy)
+        forward()
+    del y
+    gc.collect()
+    assert torch.cuda.memory_allocated() == before
 
 
 def test_no_wait_has_run_out():
