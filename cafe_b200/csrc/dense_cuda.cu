@@ -436,11 +436,14 @@ static int dense_done(cudaError_t e) {
 }
 
 // ---- a few rows against many -------------------------------------------------------------------------------------------
-// y for at most 16 rows of x (one request to score), or of W (a last layer of one output): each of the many rows is read once,
-// in plain fp32 multiply-adds; tiles of 128 would mostly be padding.  A block takes eight of the many rows at a time for every warp
-// that has a share of k of its own: `kw` warps divide k among them, the others take further rows.  A lane has four k of eight
-// many and FEW few rows at a time, so 8 + FEW loads feed 32 FEW multiply-adds; sums of a warp's lanes are halved and exchanged
-// until each lane holds FEW / 4 of them (FEW >= 4), sums of the kw warps are added in their order through shared memory.
+// y for at most 16 rows of x (one request to score), or of W (a last layer of one output): each of the many rows is read once, or
+// twice where there are more than eight few, in plain fp32 multiply-adds; tiles of 128 would mostly be padding.  A block takes eight
+// of the many rows at a time for every warp that has a share of k of its own: `kw` warps divide k among them, the others take
+// further rows.  A lane has four k of eight many and FEW few rows at a time, so 8 + FEW loads feed 32 FEW multiply-adds; sums of a
+// warp's lanes are halved and exchanged until each lane holds FEW / 4 of them (FEW >= 4), sums of the kw warps are added in their
+// order through shared memory.  Bound by latency (a chain of launch, loads, exchange) until the many rows are a few MB, then by
+// their bytes: 1024x1024 1 row 2.9 us, 8 rows 5.2, 16 rows 6.1 (sixteen few at a time, one block an SM: 7.5); 4096x4096, in L2, 11 us
+// (6.1 TB/s), 25, 52 (73).
 struct CafeFew {
     const void *few, *many, *bias, *res;
     int64_t ldf, ldm, ldr, ldo, lds;
@@ -467,12 +470,13 @@ template <typename T> __device__ __forceinline__ void cafe_few_load(const T* p, 
     }
 }
 template <typename T, int FEW>
-__global__ void __launch_bounds__(256) k_few(const CafeFew P) {
+__global__ void __launch_bounds__(256, FEW == 1 ? 3 : 2) k_few(const CafeFew P) {
     typedef typename CafeSlopeOf<T>::type ST;
     constexpr int N = CAFE_FEW_MANY * FEW;
     __shared__ float part[8][N];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int groups = 8 / P.kw, group = warp / P.kw, kpart = warp % P.kw;
+    const int few0 = blockIdx.y * FEW, nfew = P.nfew - few0;   // (of this block; at least one)
     const int64_t per_block = (int64_t)groups * CAFE_FEW_MANY, first = blockIdx.x * per_block + group * CAFE_FEW_MANY;
     cafe_next_may_start();
     // k in steps of 128, shared out among kw warps
@@ -480,25 +484,34 @@ __global__ void __launch_bounds__(256) k_few(const CafeFew P) {
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = 0.f;
     if (first < P.nmany) {
-        const T* few = static_cast<const T*>(P.few);
+        const T* few = static_cast<const T*>(P.few) + few0 * P.ldf;
         const T* many = static_cast<const T*>(P.many) + first * P.ldm;
         const int last = (int)min((int64_t)CAFE_FEW_MANY, P.nmany - first) - 1;
-        for (int k = kpart * 128; k < P.depth; k += P.kw * 128) {
-            const int left = P.depth - k;
-            float w[CAFE_FEW_MANY][4];
+        float w[CAFE_FEW_MANY][4];
+        auto load_many = [&](int k) {
 #pragma unroll
-            for (int c = 0; c < CAFE_FEW_MANY; ++c) cafe_few_load(many + min(c, last) * P.ldm + k, P.vec, lane, left, w[c]);
+            for (int c = 0; c < CAFE_FEW_MANY; ++c) cafe_few_load(many + min(c, last) * P.ldm + k, P.vec, lane, P.depth - k, w[c]);
+        };
+        int k = kpart * 128;
+        // (weights of a layer that follows one of its call were there before the call: they are fetched while that one ends)
+        if (!P.few_is_row) cafe_wait_for_earlier();
+        if (k < P.depth) load_many(k);
+        if (P.few_is_row) cafe_wait_for_earlier();
+        while (k < P.depth) {
+            const int left = P.depth - k;
 #pragma unroll
             for (int f = 0; f < FEW; ++f) {
                 float x[4];
-                cafe_few_load(few + min(f, P.nfew - 1) * P.ldf + k, P.vec, lane, left, x);
+                cafe_few_load(few + min(f, nfew - 1) * P.ldf + k, P.vec, lane, left, x);
 #pragma unroll
                 for (int c = 0; c < CAFE_FEW_MANY; ++c)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) acc[f * CAFE_FEW_MANY + c] += x[j] * w[c][j];
             }
+            k += P.kw * 128;
+            if (k < P.depth) load_many(k);
         }
-    }
+    } else cafe_wait_for_earlier();
     // halving exchange: after it lane l holds, at acc[i], the whole sum number (l >> SH) * (N >> LG) + i
     constexpr int LG = N >= 32 ? 5 : N == 16 ? 4 : 3;   // halvings that leave something to halve
 #pragma unroll
@@ -525,10 +538,10 @@ __global__ void __launch_bounds__(256) k_few(const CafeFew P) {
         // neighbouring threads write neighbouring outputs
         const int f = P.few_is_row ? q / CAFE_FEW_MANY : q % FEW, c = P.few_is_row ? q % CAFE_FEW_MANY : q / FEW;
         const int64_t many = blockIdx.x * per_block + g * CAFE_FEW_MANY + c;
-        if (f >= P.nfew || many >= P.nmany) continue;
+        if (f >= nfew || many >= P.nmany) continue;
         float z = 0.f;
         for (int w = 0; w < P.kw; ++w) z += part[g * P.kw + w][f * CAFE_FEW_MANY + c];
-        const int64_t i = P.few_is_row ? f : many, j = P.few_is_row ? many : f;
+        const int64_t i = P.few_is_row ? few0 + f : many, j = P.few_is_row ? many : few0 + f;
         float d = 1.f;
         if (P.bias) z += cafe_to_float(__ldg(static_cast<const T*>(P.bias) + j));
         if (P.act != CAFE_ACT_NONE) z = cafe_act(z, P.act, &d);
@@ -538,7 +551,7 @@ __global__ void __launch_bounds__(256) k_few(const CafeFew P) {
     }
 }
 template <typename T>
-static cudaError_t dense_few(const CafeForward& f, cudaStream_t st) {
+static cudaError_t dense_few(const CafeForward& f, bool follows, cudaStream_t st) {
     CafeFew P = {};
     P.few_is_row = f.M <= f.N;
     const bool r = P.few_is_row;
@@ -553,10 +566,11 @@ static cudaError_t dense_few(const CafeForward& f, cudaStream_t st) {
     while (P.kw < 8 && P.kw * 128 < f.K && (int64_t)P.nmany * P.kw < 148 * 16 * 8 * 8) P.kw *= 2;
     const int per_block = 8 / P.kw * CAFE_FEW_MANY;
     const unsigned grid = (unsigned)((P.nmany + per_block - 1) / per_block);
-    if (P.nfew <= 1) return dense_start<false>(k_few<T, 1>, dim3(grid), 256, 0, 1, st, P);
-    if (P.nfew <= 4) return dense_start<false>(k_few<T, 4>, dim3(grid), 256, 0, 1, st, P);
-    if (P.nfew <= 8) return dense_start<false>(k_few<T, 8>, dim3(grid), 256, 0, 1, st, P);
-    return dense_start<false>(k_few<T, 16>, dim3(grid), 256, 0, 1, st, P);
+    auto start = [&](void (*kernel)(CafeFew), unsigned few) {
+        const dim3 g(grid, (P.nfew + few - 1) / few);
+        return follows ? dense_start<true>(kernel, g, 256, 0, 1, st, P) : dense_start<false>(kernel, g, 256, 0, 1, st, P);
+    };
+    return P.nfew <= 1 ? start(k_few<T, 1>, 1) : P.nfew <= 4 ? start(k_few<T, 4>, 4) : start(k_few<T, 8>, 8);
 }
 
 // The backward of a layer of at most 16 outputs: gx = gz W is a sum of few outer products, gW = gz^T x a few long sums, both bound
@@ -714,10 +728,11 @@ static cudaError_t dense_few_back(const CafeBackward& f, void* work, cudaStream_
     return dense_start<false>(k_few_join<T>, dim3((unsigned)(((int64_t)f.N * (f.K + 1) + 31) / 32)), 256, 0, 1, st, (const float*)P.part, blocks, f.N, f.K, f.gw, f.ldgw, f.gb);
 }
 
+// `follows`: the kernel before it in the stream is that of the layer before it in the same call, of as few rows
 template <typename T>
-static cudaError_t dense_forward(const CafeForward& f, int dtype, void* work, int64_t work_bytes, cudaStream_t st) {
+static cudaError_t dense_forward(const CafeForward& f, int dtype, bool follows, void* work, int64_t work_bytes, cudaStream_t st) {
     if (f.M == 0 || f.N == 0) return cudaSuccess;
-    if (f.M <= CAFE_FEW_MOST || f.N <= CAFE_FEW_MOST) return dense_few<T>(f, st);
+    if (f.M <= CAFE_FEW_MOST || f.N <= CAFE_FEW_MOST) return dense_few<T>(f, follows, st);
     CafeJobs P = {};
     CafeJob& J = P.job[0];
     P.count = 1;
@@ -816,7 +831,7 @@ int cafe_linear_forward(const void* x_dev, int64_t ldx, const void* w_dev, int64
     const CafeForward f = {x_dev, w_dev, bias_dev, res_dev, ldx, ldw, ldr, M, N, K, act, y_dev, slope_dev, ldy, lds};
     if (!dense_type_ok(dtype) || !dense_forward_ok(f) || !dense_work_ok(work_dev, work_bytes)) return CAFE_ERR_ARG;
     cudaError_t e;
-    DENSE_TYPED(dtype, e = dense_forward<T>(f, dtype, work_dev, work_bytes, (cudaStream_t)stream));
+    DENSE_TYPED(dtype, e = dense_forward<T>(f, dtype, false, work_dev, work_bytes, (cudaStream_t)stream));
     return dense_done(e);
 }
 
@@ -871,7 +886,10 @@ int cafe_mlp_forward(int layers, const int* widths, int M, const void* x_dev, in
         if (!dense_forward_ok(f[l])) return CAFE_ERR_ARG;
     }
     cudaError_t e = cudaSuccess;
-    for (int l = 0; l < layers && e == cudaSuccess; ++l) DENSE_TYPED(dtype, e = dense_forward<T>(f[l], dtype, work_dev, work_bytes, (cudaStream_t)stream));
+    for (int l = 0; l < layers && e == cudaSuccess; ++l) {
+        const bool follows = l > 0 && M <= CAFE_FEW_MOST && widths[l] > 0;
+        DENSE_TYPED(dtype, e = dense_forward<T>(f[l], dtype, follows, work_dev, work_bytes, (cudaStream_t)stream));
+    }
     return dense_done(e);
 }
 
