@@ -5,7 +5,9 @@
 //
 // A warp takes blocks of 256 consecutive elements of a tensor, eight per lane, over the tensors of the launch laid end to
 // end; everything is read and written once: 28 bytes an element with fp32 parameters and moments, 16 with 8-bit moments,
-// and those bytes are what bounds it.  Arithmetic is fp32, rounded to the parameter's type once, at the store.
+// and those bytes are what bounds it, but for 8-bit moments, whose codes take as long.  67 M elements: fp32 parameters with
+// 32-bit moments 338 us (5.6 TB/s), with 8-bit ones 261 (4.1), bf16 238 (6.2) and 273.  Arithmetic is fp32, rounded to the
+// parameter's type once, at the store.
 //
 // 8-bit moments.  The 256 elements of a block share an exponent `top` (one byte); an element's code keeps four bits of its
 // exponent relative to that and S bits of its mantissa: S = 3 and a sign for m, S = 4 for the root of v (which is what the

@@ -575,7 +575,7 @@ static cudaError_t dense_few(const CafeForward& f, bool follows, cudaStream_t st
 
 // The backward of a layer of at most 16 outputs: gx = gz W is a sum of few outer products, gW = gz^T x a few long sums, both bound
 // by the bytes of x and gx, which are read and written once here, in plain fp32 multiply-adds (2048 x 256 -> 1: 36 us as tiles of 128
-// that are padding).  A block has 256 columns of k, a thread four of them and every other row of the block's rows; sums of
+// that are padding, 8 and 5 by the two kernels here).  A block has 256 columns of k, a thread four of them and every other row of the block's rows; sums of
 // blocks' rows go to `part` and k_few_join adds them in order.
 struct CafeFewBack {
     const void *gy, *slope, *x, *w;
