@@ -1,5 +1,5 @@
-// dense_torch.cpp -- fused_linear and fused_mlp as nodes of torch's autograd graph: checks, allocations and the calls of the C
-// entry points (dense_cuda.cu) without the interpreter.  A backward that runs in Python is called by the engine's thread, which waits
+// dense_torch.cpp -- fused_linear and fused_mlp as nodes of torch's autograd graph, and AdamW's calls: checks, allocations and the calls
+// of the C entry points (dense_cuda.cu, adamw_cuda.cu) without the interpreter.  A backward that runs in Python is called by the engine's thread, which waits
 // for the interpreter's lock: linear 128x367x512 with its backward, whose kernels take 20 us, took 115 us a pass that way.
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -91,10 +91,12 @@ struct LinearNode : Node {
 
     std::string name() const override { return "FusedLinearBackward"; }
     void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
         x.reset_data(); w.reset_data(); slope.reset_data();
         freed = true;
     }
     variable_list apply(variable_list&& grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
         TORCH_CHECK(!freed, k_twice);
         const Tensor& gy = grads[0];
         variable_list result(4);
@@ -220,11 +222,13 @@ struct MlpNode : Node {
 
     std::string name() const override { return "FusedMLPBackward"; }
     void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
         x.reset_data(); y.reset_data(); between.reset_data();
         for (SavedVariable& v : w) v.reset_data();
         freed = true;
     }
     variable_list apply(variable_list&& grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
         TORCH_CHECK(!freed, k_twice);
         const Tensor& gy = grads[0];
         const int n = (int)plan.acts.size();
@@ -330,9 +334,84 @@ Tensor mlp(const Tensor& x, const std::vector<Tensor>& w, const std::vector<Mayb
     return y;
 }
 
+// ---- AdamW -----------------------------------------------------------------------------------------------------------
+std::vector<void*> pointers(const std::vector<Tensor>& t) {
+    std::vector<void*> p;
+    p.reserve(t.size());
+    for (const Tensor& x : t) p.push_back(const_cast<void*>(x.const_data_ptr()));
+    return p;
+}
+// a parameter's memory may have been exchanged since its moments were made
+void check_moments(const Tensor& p, const Tensor& m) {
+    TORCH_CHECK(p.is_cuda() && type_of(p) >= 0, "AdamW: a parameter has become ", p.scalar_type(), " on ", p.device());
+    TORCH_CHECK(m.numel() == p.numel() && m.device() == p.device() && p.is_non_overlapping_and_dense(),
+                "AdamW: a parameter has changed its size, device or layout since its moments were made");
+}
+// one step of parameters of one type on one device; mtop and vtop are empty with 32-bit moments
+void adamw_step(const std::vector<Tensor>& p, std::vector<Tensor> g, const std::vector<Tensor>& m, const std::vector<Tensor>& v, const std::vector<Tensor>& mtop,
+                const std::vector<Tensor>& vtop, const std::vector<Tensor>& step, const std::vector<int>& index, double lr, double beta1, double beta2, double eps,
+                double weight_decay, uint32_t seed, const Tensor& ticket) {
+    at::NoGradGuard plain_values;
+    const c10::cuda::CUDAGuard device(ticket.device());
+    const size_t n = p.size();
+    std::vector<int64_t> numel(n);
+    for (size_t i = 0; i < n; ++i) {
+        check_moments(p[i], m[i]);
+        TORCH_CHECK(g[i].scalar_type() == p[i].scalar_type(), "AdamW: a gradient of ", g[i].scalar_type(), " for a parameter of ", p[i].scalar_type());
+        if (!(g[i].is_contiguous() && p[i].is_contiguous()) && g[i].strides() != p[i].strides()) {
+            const Tensor same = at::empty_like(p[i]);
+            same.copy_(g[i]);
+            g[i] = same;
+        }
+        numel[i] = p[i].numel();
+    }
+    const std::vector<void*> gs = pointers(g), ms = pointers(mtop), vs = pointers(vtop), steps = pointers(step);
+    const bool packed = !mtop.empty();
+    check_status(cafe_adamw_step((int)n, pointers(p).data(), gs.data(), pointers(m).data(), pointers(v).data(), packed ? (uint8_t* const*)ms.data() : nullptr,
+                                 packed ? (uint8_t* const*)vs.data() : nullptr, (int64_t* const*)steps.data(), numel.data(), index.data(), type_of(p[0]), packed ? 8 : 32,
+                                 lr, beta1, beta2, eps, weight_decay, seed, static_cast<int*>(ticket.mutable_data_ptr()), c10::cuda::getCurrentCUDAStream().stream()),
+                 "cafe_adamw_step");
+    for (const Tensor& t : p)   // (a backward that has saved one of them must say so)
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+// the values of 8-bit moments of parameters on one device, (m, root of v) of each
+std::vector<std::pair<Tensor, Tensor>> adamw_moments(const std::vector<Tensor>& p, const std::vector<Tensor>& m, const std::vector<Tensor>& mtop, const std::vector<Tensor>& r,
+                                                     const std::vector<Tensor>& rtop) {
+    at::NoGradGuard plain_values;
+    const c10::cuda::CUDAGuard device(p[0].device());
+    const size_t n = p.size();
+    std::vector<int64_t> numel(n);
+    int64_t all = 0;
+    bool together = true;   // one allocation, every tensor on 16 bytes
+    for (size_t i = 0; i < n; ++i) {
+        check_moments(p[i], m[i]);
+        together &= p[i].is_contiguous() && all % 8 == 0;
+        all += numel[i] = p[i].numel();
+    }
+    const auto options = p[0].options().dtype(at::kBFloat16);
+    std::vector<std::pair<Tensor, Tensor>> out(n);
+    std::vector<void*> mo(n), ro(n);
+    Tensor flat_m, flat_r;
+    if (together) { flat_m = at::empty({all}, options); flat_r = at::empty({all}, options); }
+    int64_t at = 0;
+    for (size_t i = 0; i < n; ++i) {
+        if (together) out[i] = {flat_m.as_strided(p[i].sizes(), p[i].strides(), at), flat_r.as_strided(p[i].sizes(), p[i].strides(), at)};
+        else out[i] = {at::empty_like(p[i], options), at::empty_like(p[i], options)};
+        at += numel[i];
+        mo[i] = out[i].first.mutable_data_ptr();
+        ro[i] = out[i].second.mutable_data_ptr();
+    }
+    const std::vector<void*> mc = pointers(m), mt = pointers(mtop), rc = pointers(r), rt = pointers(rtop);
+    check_status(cafe_adamw_moments((int)n, (const uint8_t* const*)mc.data(), (const uint8_t* const*)mt.data(), (const uint8_t* const*)rc.data(), (const uint8_t* const*)rt.data(),
+                                    numel.data(), mo.data(), ro.data(), c10::cuda::getCurrentCUDAStream().stream()), "cafe_adamw_moments");
+    return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_dense_torch, m) {
     m.def("linear", &linear, pybind11::call_guard<pybind11::gil_scoped_release>());
     m.def("mlp", &mlp, pybind11::call_guard<pybind11::gil_scoped_release>());
+    m.def("adamw_step", &adamw_step, pybind11::call_guard<pybind11::gil_scoped_release>());
+    m.def("adamw_moments", &adamw_moments, pybind11::call_guard<pybind11::gil_scoped_release>());
 }

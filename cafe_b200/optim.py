@@ -1,34 +1,11 @@
 """AdamW over all tensors of a model in one launch (csrc/adamw_cuda.cu), moments in 32 bits or in 8."""
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
-from . import _lib
-from .sketch import _stream
+from .dense import _dense_torch
 
-DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)   # (without the checks of the public form)
-
-
-class _on:
-    """The tensors' device as the current one; `as` its current stream."""
-    __slots__ = ("other",)
-
-    def __init__(self, device):
-        self.other = None if device.index == _get_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.other is not None:
-            self.other.__enter__()
-        return _stream()
-
-    def __exit__(self, *args):
-        if self.other is not None:
-            self.other.__exit__(*args)
-
-
+DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 BLOCK = 256   # elements that share the exponent of their 8-bit moments
 _CODES = ("exp_avg", "exp_avg_top", "root_avg_sq", "root_avg_sq_top")
 
@@ -113,8 +90,6 @@ class AdamW(torch.optim.Optimizer):
                 if g is not None:
                     if g.is_sparse:
                         raise RuntimeError("AdamW does not take sparse gradients")
-                    if not (g.is_contiguous() and p.is_contiguous()) and g.stride() != p.stride():
-                        g = torch.empty_like(p, memory_format=torch.preserve_format).copy_(g)
                     s = state[p]
                     if "step" not in s:
                         s = self._start(p)
@@ -134,28 +109,16 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        lib, packed = _lib.load(), self.state_bits == 8
-        for (i, device, dtype), (params, grads, states, numbers) in self._launches().items():
+        names = ("exp_avg", "root_avg_sq", "exp_avg_top", "root_avg_sq_top") if self.state_bits == 8 else ("exp_avg", "exp_avg_sq")
+        for (i, device, _), (params, grads, states, numbers) in self._launches().items():
             group = self.param_groups[i]
             self._check_settings(group)
             ticket = self._ticket.get(device)
             if ticket is None:
                 ticket = self._ticket[device] = torch.zeros(1, dtype=torch.int32, device=device)
-            n = len(params)
-            vp = ctypes.c_void_p * n
-            m = vp(*[s["exp_avg"].data_ptr() for s in states])
-            if packed:
-                v, mtop, vtop = (vp(*[s[name].data_ptr() for s in states]) for name in ("root_avg_sq", "exp_avg_top", "root_avg_sq_top"))
-            else:
-                v, mtop, vtop = vp(*[s["exp_avg_sq"].data_ptr() for s in states]), None, None
-            with _on(device) as stream:
-                status = lib.cafe_adamw_step(
-                    n, vp(*[p.data_ptr() for p in params]), vp(*[g.data_ptr() for g in grads]), m, v, mtop, vtop,
-                    vp(*[s["step"].data_ptr() for s in states]), (ctypes.c_int64 * n)(*[p.numel() for p in params]), (ctypes.c_int32 * n)(*numbers),
-                    DTYPES[dtype], self.state_bits, group["lr"], *group["betas"], group["eps"], group["weight_decay"], self.seed,
-                    ticket.data_ptr(), stream)
-            if status:
-                _lib.check(status, "cafe_adamw_step")
+            m, v, *tops = ([s[name] for s in states] for name in names)
+            _dense_torch.adamw_step(params, grads, m, v, *(tops or ([], [])), [s["step"] for s in states], numbers, group["lr"], *group["betas"],
+                                    group["eps"], group["weight_decay"], self.seed, ticket)
         return loss
 
     @torch.no_grad()
@@ -169,24 +132,9 @@ class AdamW(torch.optim.Optimizer):
         for p in params:
             by_device.setdefault(p.device, []).append(p)
         out = {}
-        for device, ps in by_device.items():
-            n = len(ps)
-            vp = ctypes.c_void_p * n
-            sizes = [p.numel() for p in ps]
-            if all(k % 8 == 0 for k in sizes[:-1]) and all(p.is_contiguous() for p in ps):   # one allocation, every tensor on 16 bytes
-                values = []
-                for _ in range(2):
-                    flat = torch.empty(sum(sizes), dtype=torch.bfloat16, device=device)
-                    values += torch._utils._unflatten_dense_tensors(flat, ps)
-            else:
-                values = [torch.empty_like(p, dtype=torch.bfloat16, memory_format=torch.preserve_format) for p in ps + ps]
+        for ps in by_device.values():
             states = [self.state[p] for p in ps]
-            codes = [vp(*[s[name].data_ptr() for s in states]) for name in _CODES]
-            at = [v.data_ptr() for v in values]
-            with _on(device) as stream:
-                _lib.check(_lib.load().cafe_adamw_moments(n, *codes, (ctypes.c_int64 * n)(*sizes), vp(*at[:n]), vp(*at[n:]), stream),
-                           "cafe_adamw_moments")
-            out.update(zip(ps, zip(values[:n], values[n:])))
+            out.update(zip(ps, _dense_torch.adamw_moments(ps, *([s[name] for s in states] for name in _CODES))))
         return [out[p] for p in params]
 
     def state_dict(self):

@@ -341,6 +341,52 @@ def test_captured_steps_count_on():
             AdamW(c).step()
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_parameters_exchanged_behind_it(bits):
+    """A parameter whose memory is not what its moments were made for is refused before anything is launched."""
+    import torch
+    from cafe_b200 import AdamW
+
+    def fresh():
+        p = torch.nn.Parameter(torch.randn(40, 30, device="cuda"))
+        opt = AdamW([p], state_bits=bits)
+        p.grad = torch.randn_like(p)
+        opt.step()
+        return p, opt
+    for change in (lambda t: t.cpu(), lambda t: t.double(), lambda t: torch.cat([t, t]), lambda t: torch.cat([t, t], 1)[:, :30]):
+        p, opt = fresh()
+        p.grad = None
+        p.data = change(p.data)
+        p.grad = torch.randn_like(p)
+        with pytest.raises(RuntimeError):
+            opt.step()
+    p, opt = fresh()            # another floating type of the same size goes on with the same moments
+    p.grad = None
+    p.data = p.data.bfloat16()
+    p.grad = torch.randn_like(p)
+    opt.step()
+    assert torch.isfinite(p).all()
+    if hasattr(p, "grad_dtype"):
+        p, opt = fresh()
+        p.grad = None
+        p.grad_dtype = torch.bfloat16
+        p.grad = torch.randn(40, 30, device="cuda", dtype=torch.bfloat16)
+        with pytest.raises(RuntimeError):
+            opt.step()
+
+
+def test_a_step_between_forward_and_backward_is_noticed():
+    import torch
+    from cafe_b200 import AdamW
+    p = torch.nn.Parameter(torch.randn(40, 30, device="cuda"))
+    opt = AdamW([p])
+    y = (p * p).sum()
+    p.grad = torch.ones_like(p)
+    opt.step()
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.backward()
+
+
 def test_refusals():
     import torch
     from cafe_b200 import AdamW
