@@ -3,7 +3,7 @@
     python -m cafe_b200.build [--force]
 
 The library is a plain C-ABI shared object (include/cafe_b200.h) that does not link against torch.  _dense_torch.so, the
-autograd nodes of the dense layers, links against it and torch.
+autograd nodes of the dense layers and AdamW's calls, links against it and torch.
 """
 from __future__ import annotations
 
