@@ -31,8 +31,6 @@ import torch.nn as nn
 from torch.autograd.profiler import record_function
 
 from . import _lib, sizing, synthetic
-from .dense import FusedMLP, fused_linear
-from .optim import AdamW
 from .sketch import _stream
 from .sk_embedding_bag import SKEmbeddingGroup
 
@@ -67,7 +65,10 @@ def create_mlp(ln, sigmoid_layer: int, rng: np.random.Generator, fused: bool = F
         lin.bias.data = torch.from_numpy(rng.normal(0.0, np.sqrt(1 / m), size=m).astype(np.float32))
         layers.append(lin)
         layers.append(nn.Sigmoid() if i == sigmoid_layer else nn.ReLU())
-    return FusedMLP(*layers) if fused else nn.Sequential(*layers)
+    if fused:
+        from .dense import FusedMLP   # (the stock model needs no autograd extension)
+        return FusedMLP(*layers)
+    return nn.Sequential(*layers)
 
 
 class CafeEmbeddingLayer(nn.Module):
@@ -329,6 +330,7 @@ class DCNNet(nn.Module):
                 x1 = z * (x1 @ w) + b
             both = torch.cat([self.deep(z), x1], dim=1)
             if self.fused_mlp:
+                from .dense import fused_linear
                 return fused_linear(both, self.last.weight, self.last.bias, "sigmoid")
             return torch.sigmoid(self.last(both))
 
@@ -352,6 +354,7 @@ class TableSGDDenseAdamW:
         of_tables = {id(p) for p in model.emb.parameters()}
         tables = [p for p in mine if id(p) in of_tables]
         self.tables = torch.optim.SGD([dict(params=tables)], lr=lr)
+        from .optim import AdamW
         self.dense = AdamW([p for p in mine if id(p) not in of_tables], lr=dense_lr, state_bits=state_bits, **adamw)
 
     @property

@@ -352,7 +352,8 @@ int cafe_linear_backward(const void* gy_dev, int64_t ldg, const void* slope_dev,
 int64_t cafe_linear_backward_work(const void* gy_dev, int64_t ldg, int slope_kind, const void* x_dev, int64_t ldx, const void* w_dev, int64_t ldw,
                                   int M, int N, int K, int dtype, int want_gx, int want_gw, int want_gb);
 /* Every wait inside these kernels has an end (about a second): if one runs out, what it waited for is stored as NaN.  *count: how
- * many of the two kinds of kernel this has happened to on the current device since the library was loaded (waits for the device). */
+ * many of the two kinds of kernel this has happened to on the current device since the library was loaded (waits for the
+ * device; not while a stream of it is being captured). */
 int cafe_linear_gave_up(int* count);
 /* `layers` layers one behind the other: layer l maps widths[l] to widths[l + 1] with acts[l]; its output goes to y_dev[l]
  * (pitch ldy[l]) and, where slope_dev[l] is not null, act'(z) to slope_dev[l] (same pitch). */
