@@ -60,10 +60,27 @@ template <int N> __device__ __forceinline__ void cafe_act_all(float* z, int act,
 #undef CAFE_ACT_CASE
 }
 
-// the derivative kept for the backward, always finer than the type it multiplies, so that gz's own rounding stays the only
-// one that counts: fp16 (11 bits; it lies in [-0.2, 1.2]) beside bf16 (8 bits), else fp32
+// The derivative kept for the backward: fp32, or beside bf16 a code of 16 bits.  bf16 gradients have the exponents of fp32 (a sigmoid
+// under a cross-entropy meets gy = -1 / y, so that a derivative of 1e-35 still counts), which fp16 alone has not: it is zero below
+// 2^-25, where gz = -1 became 0 from z = -17.5 on.  No derivative reaches 2 (they lie in [-0.2, 1.2]), so the codes of fp16 from 2 on are free and
+// hold the bf16 codes of what is below 2^-17 (at most 0x3700, added to 0x4000).  Error: 2^-11 of the value down to 2^-14, 2^-25 down to 2^-17, where
+// that is 2^-8 of it, and 2^-8 of it below, down to bf16's own smallest numbers; gz's rounding to bf16 has 2^-8.
+struct CafeSlope16 { uint16_t code; };
+template <> __device__ __forceinline__ float cafe_to_float<CafeSlope16>(CafeSlope16 x) {
+    const uint32_t m = x.code & 0x7fffu;
+    const float low = __uint_as_float((x.code & 0x8000u) << 16 | (m - 0x4000u) << 16);
+    return m - 0x4000u < 0x3c00u ? low : __half2float(__ushort_as_half(x.code));   // (from 0x7c00 on: not a number)
+}
+template <> __device__ __forceinline__ CafeSlope16 cafe_from_float<CafeSlope16>(float x) {
+    const uint16_t low = (uint16_t)(__bfloat16_as_ushort(__float2bfloat16_rn(x)) + 0x4000u);
+    return CafeSlope16{fabsf(x) < 0x1p-17f ? low : __half_as_ushort(__float2half_rn(x))};
+}
 template <typename T> struct CafeSlopeOf { typedef float type; };
-template <> struct CafeSlopeOf<__nv_bfloat16> { typedef __half type; };
+template <> struct CafeSlopeOf<__nv_bfloat16> { typedef CafeSlope16 type; };
+
+// a load through the read-only path
+template <typename T> __device__ __forceinline__ T cafe_ldg(const T* p) { return __ldg(p); }
+template <> __device__ __forceinline__ CafeSlope16 cafe_ldg<CafeSlope16>(const CafeSlope16* p) { return CafeSlope16{__ldg(&p->code)}; }
 
 struct CafeJob {
     const void *a, *as, *b;

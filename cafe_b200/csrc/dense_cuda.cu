@@ -69,7 +69,7 @@ __device__ __forceinline__ void cafe_piece_load(CafePiece<T>& p, const T* src, i
         } else { p.v[0] = x.x; p.v[1] = x.y; p.v[2] = x.z; p.v[3] = x.w; }
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) cafe_piece_set<T>(p, j, FULL || j < left ? __ldg(src + (KC ? (int64_t)j : j * ld)) : cafe_from_float<T>(0.f));
+        for (int j = 0; j < 8; ++j) cafe_piece_set<T>(p, j, FULL || j < left ? cafe_ldg(src + (KC ? (int64_t)j : j * ld)) : cafe_from_float<T>(0.f));
     }
 }
 template <typename T, typename S>
@@ -608,7 +608,7 @@ __global__ void __launch_bounds__(128) k_few_back(const CafeFewBack P) {
 #pragma unroll
         for (int n = 0; n < FEW; ++n) {
             float v = n < P.N ? cafe_to_float(__ldg(static_cast<const T*>(P.gy) + m * P.ldg + n)) : 0.f;
-            if (n < P.N && P.kind == CAFE_SLOPE_VALUES) v *= cafe_to_float(__ldg(static_cast<const ST*>(P.slope) + m * P.lds + n));
+            if (n < P.N && P.kind == CAFE_SLOPE_VALUES) v *= cafe_to_float(cafe_ldg(static_cast<const ST*>(P.slope) + m * P.lds + n));
             else if (n < P.N && P.kind == CAFE_SLOPE_OUTPUT) v = cafe_to_float(__ldg(static_cast<const T*>(P.slope) + m * P.lds + n)) > 0.f ? v : 0.f;
             g[n] = v;
             gb[n] += v;

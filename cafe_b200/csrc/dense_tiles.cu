@@ -58,7 +58,7 @@ template <typename T> __device__ __forceinline__ void cafe_read8(const T* p, int
         for (int j = 0; j < 8; ++j) v[j] = cafe_to_float(x[j]);
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = j < n ? cafe_to_float(__ldg(p + j)) : 0.f;
+        for (int j = 0; j < 8; ++j) v[j] = j < n ? cafe_to_float(cafe_ldg(p + j)) : 0.f;
     }
 }
 // Bound by its bytes: fp32 4 in (8 with a slope) and 6 out an element (17.8 M elements of x and W 27 us, 6.5 TB/s with what stays in L2).
@@ -401,7 +401,7 @@ __device__ __forceinline__ void cafe_rows_out(uint32_t at, E* to, int64_t ld, bo
             if (add16 && whole) *reinterpret_cast<uint4*>(y) = __ldg(reinterpret_cast<const uint4*>(p));
             else {
 #pragma unroll
-                for (int q = 0; q < each; ++q) y[q] = c * each + q < n ? __ldg(p + q) : cafe_from_float<E>(0.f);
+                for (int q = 0; q < each; ++q) y[q] = c * each + q < n ? cafe_ldg(p + q) : cafe_from_float<E>(0.f);
             }
         }
         *reinterpret_cast<uint4*>(x) = cafe_get16(cafe_staged<ROW>(at, r, c));

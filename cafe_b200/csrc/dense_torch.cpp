@@ -25,7 +25,7 @@ int type_of(const Tensor& t) {
         default: return -1;
     }
 }
-at::ScalarType slope_type(at::ScalarType t) { return t == at::kBFloat16 ? at::kHalf : at::kFloat; }
+at::ScalarType slope_type(at::ScalarType t) { return t == at::kBFloat16 ? at::kShort : at::kFloat; }   // (codes of 16 bits, see the header)
 void check_status(int status, const char* where) {
     if (status == CAFE_OK) return;
     TORCH_CHECK(status != CAFE_ERR_CUDA, where, ": ", cafe_last_error());

@@ -29,8 +29,8 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
                  residual: torch.Tensor | None = None) -> torch.Tensor:
     """act(x W^T + b) + residual.  x [..., K], weight [N, K], bias [N]; residual broadcasts to [..., N]; activation is one of
     none, relu, sigmoid, gelu (with erf) and silu.  x, weight and residual may be slices of wider tensors (any pitch
-    between rows).  For the backward the call keeps x, weight and, with an activation, its derivative (fp16 beside bf16, else
-    fp32); of a ReLU without residual the output."""
+    between rows).  For the backward the call keeps x, weight and, with an activation, its derivative (16 bits beside bf16, with
+    the range of bf16, else fp32); of a ReLU without residual the output."""
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"fused_linear: activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")

@@ -329,7 +329,8 @@ int cafe_dot_interaction_backward(const float* x_dev, const float* emb_dev, int6
 /* ---- dense layers (the MLPs around the embedding path: dlrm_s_pytorch.py:213-251, dcn.py:410-422) ------------------
  * z = x W^T + b, y = act(z) + res for x [M, K], W [N, K], rows `ld` elements apart (ld >= the row's length; elements of a
  * row are contiguous).  All tensors of a call have one type; sums are fp32.  bias, res and slope may be null; ldr = 0: one
- * row of res for all.  slope_dev receives act'(z) for the backward: fp16 beside bf16, else fp32.
+ * row of res for all.  slope_dev receives act'(z) for the backward: fp32, or 16 bits an element beside bf16: fp16, whose codes from 2
+ * on (0x4000 + c, and the sign) stand for what is below 2^-17 in magnitude, as the bf16 code c.
  * M, N, K <= CAFE_LINEAR_MAX.  Outputs overlap nothing else of the call.  No host synchronisation, no device memory of its
  * own: work_dev (16-byte aligned, free again once the call's work on `stream` is done; two calls that may run at once need one
  * each) lets large layers lay their operands out first; the *_work functions give its bytes for a call's arguments (0: none
