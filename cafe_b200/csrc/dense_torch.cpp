@@ -341,22 +341,57 @@ std::vector<void*> pointers(const std::vector<Tensor>& t) {
     for (const Tensor& x : t) p.push_back(const_cast<void*>(x.const_data_ptr()));
     return p;
 }
-// a parameter's memory may have been exchanged since its moments were made
-void check_moments(const Tensor& p, const Tensor& m) {
+// Whether elements of these sizes and strides lie one behind the other in the order of their indexes.
+bool row_major(at::IntArrayRef sizes, at::IntArrayRef strides) {
+    int64_t at = 1;
+    for (const int64_t n : sizes) if (n == 0) return true;
+    for (size_t i = sizes.size(); i-- > 0;) {
+        if (sizes[i] == 1) continue;
+        if (strides[i] != at) return false;
+        at *= sizes[i];
+    }
+    return true;
+}
+// Whether p's k-th element in memory is also the k-th of these: both row-major, or the same axes (but for those of one element).
+bool same_order(const Tensor& p, at::IntArrayRef sizes, at::IntArrayRef strides) {
+    if (row_major(p.sizes(), p.strides())) return row_major(sizes, strides);
+    size_t j = 0;
+    for (int64_t i = 0; i < p.dim(); ++i) {
+        if (p.size(i) == 1) continue;
+        while (j < sizes.size() && sizes[j] == 1) ++j;
+        if (j == sizes.size() || sizes[j] != p.size(i) || strides[j] != p.stride(i)) return false;
+        ++j;
+    }
+    while (j < sizes.size() && sizes[j] == 1) ++j;
+    return j == sizes.size();
+}
+// A parameter's memory may have been exchanged since its moments were made.  `layout`: of 8-bit moments, whose codes lie flat, the
+// parameter's sizes and strides then (host, [2, axes]); 32-bit moments have their own.
+void check_moments(const Tensor& p, const Tensor& m, const Tensor* layout) {
     TORCH_CHECK(p.is_cuda() && type_of(p) >= 0, "AdamW: a parameter has become ", p.scalar_type(), " on ", p.device());
     TORCH_CHECK(m.numel() == p.numel() && m.device() == p.device() && p.is_non_overlapping_and_dense(),
                 "AdamW: a parameter has changed its size, device or layout since its moments were made");
+    bool same;
+    if (layout) {
+        TORCH_CHECK(layout->device().is_cpu() && layout->scalar_type() == at::kLong && layout->dim() == 2 && layout->size(0) == 2 && layout->is_contiguous(),
+                    "AdamW: the layout of a state is not what it was made as");
+        const int64_t* const at = layout->const_data_ptr<int64_t>();
+        const size_t axes = (size_t)layout->size(1);
+        same = same_order(p, {at, axes}, {at + axes, axes});
+    } else same = same_order(p, m.sizes(), m.strides());
+    TORCH_CHECK(same, "AdamW: a parameter's elements lie in another order than when its moments were made",
+                layout ? "" : " (load_state_dict(state_dict()) lays the moments out anew)");
 }
-// one step of parameters of one type on one device; mtop and vtop are empty with 32-bit moments
+// one step of parameters of one type on one device; mtop, vtop and layout are empty with 32-bit moments
 void adamw_step(const std::vector<Tensor>& p, std::vector<Tensor> g, const std::vector<Tensor>& m, const std::vector<Tensor>& v, const std::vector<Tensor>& mtop,
-                const std::vector<Tensor>& vtop, const std::vector<Tensor>& step, const std::vector<int>& index, double lr, double beta1, double beta2, double eps,
+                const std::vector<Tensor>& vtop, const std::vector<Tensor>& layout, const std::vector<Tensor>& step, const std::vector<int>& index, double lr, double beta1, double beta2, double eps,
                 double weight_decay, uint32_t seed, const Tensor& ticket) {
     at::NoGradGuard plain_values;
     const c10::cuda::CUDAGuard device(ticket.device());
     const size_t n = p.size();
     std::vector<int64_t> numel(n);
     for (size_t i = 0; i < n; ++i) {
-        check_moments(p[i], m[i]);
+        check_moments(p[i], m[i], layout.empty() ? nullptr : &layout[i]);
         TORCH_CHECK(g[i].scalar_type() == p[i].scalar_type(), "AdamW: a gradient of ", g[i].scalar_type(), " for a parameter of ", p[i].scalar_type());
         if (!(g[i].is_contiguous() && p[i].is_contiguous()) && g[i].strides() != p[i].strides()) {
             const Tensor same = at::empty_like(p[i]);
@@ -376,7 +411,7 @@ void adamw_step(const std::vector<Tensor>& p, std::vector<Tensor> g, const std::
 }
 // the values of 8-bit moments of parameters on one device, (m, root of v) of each
 std::vector<std::pair<Tensor, Tensor>> adamw_moments(const std::vector<Tensor>& p, const std::vector<Tensor>& m, const std::vector<Tensor>& mtop, const std::vector<Tensor>& r,
-                                                     const std::vector<Tensor>& rtop) {
+                                                     const std::vector<Tensor>& rtop, const std::vector<Tensor>& layout) {
     at::NoGradGuard plain_values;
     const c10::cuda::CUDAGuard device(p[0].device());
     const size_t n = p.size();
@@ -384,7 +419,7 @@ std::vector<std::pair<Tensor, Tensor>> adamw_moments(const std::vector<Tensor>& 
     int64_t all = 0;
     bool together = true;   // one allocation, every tensor on 16 bytes
     for (size_t i = 0; i < n; ++i) {
-        check_moments(p[i], m[i]);
+        check_moments(p[i], m[i], &layout[i]);
         together &= p[i].is_contiguous() && all % 8 == 0;
         all += numel[i] = p[i].numel();
     }

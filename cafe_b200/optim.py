@@ -22,6 +22,21 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
+def _layout(p: torch.Tensor) -> torch.Tensor:
+    """p's sizes and strides: the order in which a flat array of codes goes through its elements."""
+    return torch.tensor([tuple(p.shape), tuple(p.stride())], dtype=torch.int64)
+
+
+def _order(layout):
+    """What two layouts whose elements come in the same order have in common: None if row-major, else their axes."""
+    sizes, strides = layout.tolist()
+    axes, at, rows = [(n, s) for n, s in zip(sizes, strides) if n != 1], 1, True
+    for n, s in reversed(axes):
+        rows &= s == at
+        at *= n
+    return None if rows or 0 in sizes else axes
+
+
 class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's update (decoupled weight decay, both moments corrected for their start at zero) for CUDA parameters
     of fp32, bf16 or fp16, computed in fp32.
@@ -33,7 +48,8 @@ class AdamW(torch.optim.Optimizer):
 
     A step counts on the device and reads nothing back, so it can be captured into a CUDA graph; lr and the other settings are
     then those of the capture, and the optimizer's state has to exist before it (one step outside).  Parameters without a
-    gradient keep their moments and their step count.  Sparse gradients are refused."""
+    gradient keep their moments and their step count.  Sparse gradients are refused, and so is a parameter whose elements have come to
+    lie in another order than its moments (another memory format, exchanged .data)."""
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, state_bits: int = 32,
                  seed: int = 0):
@@ -46,6 +62,13 @@ class AdamW(torch.optim.Optimizer):
 
     def __getstate__(self):   # (torch's has the settings and the state alone: copies and pickles need the rest)
         return {**super().__getstate__(), "state_bits": self.state_bits, "seed": self.seed, "_ticket": {}}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if self.state_bits == 8:   # (pickles without layouts: the parameter came with its codes)
+            for p, s in self.state.items():
+                if isinstance(p, torch.Tensor) and "step" in s:
+                    s.setdefault("layout", _layout(p))
 
     @staticmethod
     def _check_settings(group):
@@ -78,6 +101,7 @@ class AdamW(torch.optim.Optimizer):
             n = p.numel()
             for name in _CODES:
                 s[name] = torch.zeros(-(-n // BLOCK) if name.endswith("top") else n, dtype=torch.uint8, device=p.device)
+            s["layout"] = _layout(p)
         return s
 
     def _launches(self):
@@ -117,8 +141,9 @@ class AdamW(torch.optim.Optimizer):
             if ticket is None:
                 ticket = self._ticket[device] = torch.zeros(1, dtype=torch.int32, device=device)
             m, v, *tops = ([s[name] for s in states] for name in names)
-            _dense_torch.adamw_step(params, grads, m, v, *(tops or ([], [])), [s["step"] for s in states], numbers, group["lr"], *group["betas"],
-                                    group["eps"], group["weight_decay"], self.seed, ticket)
+            _dense_torch.adamw_step(params, grads, m, v, *(tops or ([], [])), [s["layout"] for s in states] if tops else [],
+                                    [s["step"] for s in states], numbers, group["lr"], *group["betas"], group["eps"], group["weight_decay"],
+                                    self.seed, ticket)
         return loss
 
     @torch.no_grad()
@@ -134,14 +159,16 @@ class AdamW(torch.optim.Optimizer):
         out = {}
         for ps in by_device.values():
             states = [self.state[p] for p in ps]
-            out.update(zip(ps, _dense_torch.adamw_moments(ps, *([s[name] for s in states] for name in _CODES))))
+            out.update(zip(ps, _dense_torch.adamw_moments(ps, *([s[name] for s in states] for name in (*_CODES, "layout")))))
         return [out[p] for p in params]
 
     def state_dict(self):
         return {**super().state_dict(), "state_bits": self.state_bits, "seed": self.seed}
 
     def load_state_dict(self, state_dict):
-        """Takes a state_dict of this class.  Moments keep their own type (torch would give them the parameter's)."""
+        """Takes a state_dict of this class.  Moments keep their own type (torch would give them the parameter's); those of 32 bits
+        are laid out as the parameter is, codes of 8 bits have to lie in the parameter's order of elements (`layout` in the
+        state; row-major where it is missing)."""
         if state_dict.get("state_bits", self.state_bits) != self.state_bits:
             raise ValueError(f"the state is in {state_dict['state_bits']} bits, this optimizer's in {self.state_bits}")
         names = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else _CODES
@@ -158,7 +185,10 @@ class AdamW(torch.optim.Optimizer):
                     want = p.numel() if not name.endswith("top") else -(-p.numel() // BLOCK)
                     if s[name].numel() != want:
                         raise ValueError(f"{name} of parameter {k} has {s[name].numel()} elements, {want} are needed")
-        super().load_state_dict({k: v for k, v in state_dict.items() if k in ("state", "param_groups")})
+                if self.state_bits == 8 and _order(s["layout"] if "layout" in s else _layout(torch.empty(p.shape, device="meta"))) != _order(_layout(p)):
+                    raise ValueError(f"the codes of parameter {k} go through its elements in another order than the parameter's")
+        super().load_state_dict(dict(state={k: {n: v for n, v in s.items() if n != "layout"} for k, s in state_dict["state"].items()},
+                                     param_groups=state_dict["param_groups"]))
         self.seed = state_dict.get("seed", self.seed)
         for k, p in zip(places, params):
             s = state_dict["state"].get(k)
@@ -170,3 +200,5 @@ class AdamW(torch.optim.Optimizer):
                     mine[name] = torch.empty_like(p, dtype=torch.float32, memory_format=torch.preserve_format).copy_(s[name].reshape(p.shape))
                 else:
                     mine[name] = s[name].reshape(-1).to(device=p.device, dtype=torch.uint8, copy=True)
+            if self.state_bits == 8:
+                mine["layout"] = _layout(p)
