@@ -1,10 +1,12 @@
 // dense_torch.cpp -- fused_linear and fused_mlp as nodes of torch's autograd graph, and AdamW's calls: checks, allocations and the calls
 // of the C entry points (dense_cuda.cu, adamw_cuda.cu) without the interpreter.  A backward that runs in Python is called by the engine's thread, which waits
 // for the interpreter's lock: linear 128x367x512 with its backward, whose kernels take 20 us, took 115 us a pass that way.
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include "../../include/cafe_b200.h"
@@ -53,7 +55,17 @@ void* out(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr
 // Workspace of one call, from torch's allocator: free again in the stream's order.
 Tensor workspace(int64_t size, const Tensor& like) { return size > 0 ? at::empty({size}, like.options().dtype(at::kByte)) : Tensor(); }
 
+// Outputs are allocated here and filled through pointers, which neither a forward derivative nor a recording of torch's calls sees:
+// the one would read as zero, the other would replay the allocation alone.
+void check_first_order_eager(const char* what, const Tensor& x, c10::ArrayRef<const Tensor*> others) {
+    bool dual = x._fw_grad(0).defined();
+    for (const Tensor* t : others) dual |= t && t->defined() && t->_fw_grad(0).defined();
+    TORCH_CHECK_NOT_IMPLEMENTED(!dual, what, " has no forward-mode derivative");
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing() && !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY), what,
+                                " cannot be recorded by a trace");
+}
 void check_tensors(const char* what, const Tensor& x, c10::ArrayRef<const Tensor*> others) {
+    check_first_order_eager(what, x, others);
     TORCH_CHECK_VALUE(x.is_cuda() && type_of(x) >= 0, what, " needs CUDA tensors of fp32, bf16 or fp16");
     for (const Tensor* t : others)
         TORCH_CHECK_VALUE(!t || (t->is_cuda() && t->scalar_type() == x.scalar_type() && t->get_device() == x.get_device()), what,

@@ -6,7 +6,8 @@ FusedMLP       the Sequential of Linear and activation modules that the referenc
                (dlrm_s_pytorch.py:213-251), computed by fused_mlp; same parameters, same state_dict
 
 Tensors are CUDA tensors of one type (fp32, bf16 or fp16); sums are fp32.  Kernels go to the current stream of the tensors'
-device.  The gradients are those of first order: differentiating them again raises.  Captured into a CUDA graph, forward and
+device.  The gradients are those of first order: differentiating them again raises, and so do forward-mode derivatives
+and calls that a trace (torch.jit.trace, make_fx) records.  Captured into a CUDA graph, forward and
 backward follow torch's rules for whole-network capture (warm-up on a side stream, no autograd graph of the same leaves alive
 from outside the capture)."""
 from __future__ import annotations

@@ -1,0 +1,32 @@
+"""What the dense entry points refuse because they could not do it right; no GPU needed."""
+import pytest
+
+
+def test_forward_derivatives_are_refused():
+    import torch
+    import torch.autograd.forward_ad as fwad
+    from cafe_b200 import fused_linear, fused_mlp
+    x, w, b = torch.randn(3, 4), torch.randn(2, 4), torch.randn(2)
+    r = torch.randn(3, 2)
+    with fwad.dual_level():
+        dual = lambda t: fwad.make_dual(t, torch.ones_like(t))   # noqa: E731
+        for call in (lambda: fused_linear(dual(x), w, b), lambda: fused_linear(x, dual(w), b), lambda: fused_linear(x, w, dual(b)),
+                     lambda: fused_linear(x, w, b, "relu", dual(r)), lambda: fused_mlp(dual(x), [w], [b], ["relu"]),
+                     lambda: fused_mlp(x, [dual(w)], [None], ["relu"]), lambda: fused_mlp(x, [w], [dual(b)], ["relu"])):
+            with pytest.raises(NotImplementedError, match="forward"):
+                call()
+        with pytest.raises(ValueError, match="needs CUDA tensors"):   # (none of them dual: the next check's turn)
+            fused_linear(x, w, b)
+
+
+def test_traces_are_refused():
+    import torch
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from cafe_b200 import fused_linear, fused_mlp
+    x, w = torch.randn(3, 4), torch.randn(2, 4)
+    for call in (lambda x: fused_linear(x, w), lambda x: fused_mlp(x, [w], [None], ["silu"])):
+        with pytest.raises(NotImplementedError, match="trace"):
+            torch.jit.trace(call, (x,), check_trace=False)
+        with pytest.raises(NotImplementedError, match="trace"):
+            make_fx(call)(x)
+
