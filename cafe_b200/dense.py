@@ -58,8 +58,17 @@ def _module_activation(m: nn.Module) -> str:
     return _MODULES[type(m)]
 
 
+def _check_plain(m: nn.Module) -> None:
+    """FusedMLP takes what a module holds without calling it: what would run in a call of it must not be passed by."""
+    if m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks:
+        raise ValueError(f"FusedMLP does not call its modules: {m} has hooks (as of prune or weight_norm) that would not run")
+    if "forward" in m.__dict__:
+        raise ValueError(f"FusedMLP does not call its modules: {m} has a forward of its own that would not run")
+
+
 class FusedMLP(nn.Sequential):
-    """nn.Sequential of nn.Linear layers, each followed by an activation module or none, computed by fused_mlp."""
+    """nn.Sequential of nn.Linear layers, each followed by an activation module or none, computed by fused_mlp.  Its modules hold the
+    parameters and are not called: one with hooks is refused, when it comes in and in every call."""
 
     def __init__(self, *layers):
         super().__init__(*layers)
@@ -68,6 +77,7 @@ class FusedMLP(nn.Sequential):
     def _plan(self):
         linears, acts = [], []
         for m in self._modules.values():
+            _check_plain(m)
             if type(m) is nn.Linear:
                 linears.append(m)
                 acts.append(None)

@@ -1,4 +1,4 @@
-"""What the dense entry points refuse because they could not do it right; no GPU needed."""
+"""What the dense entry points and FusedMLP refuse because they could not do it right; no GPU needed."""
 import pytest
 
 
@@ -30,3 +30,41 @@ def test_traces_are_refused():
         with pytest.raises(NotImplementedError, match="trace"):
             make_fx(call)(x)
 
+
+def test_layers_with_hooks_are_refused():
+    """FusedMLP takes the weights of its modules without calling them, so what hangs on a call of one of them would be passed by."""
+    import torch
+    import torch.nn as nn
+    from torch.nn.utils import prune
+    from cafe_b200 import FusedMLP
+
+    def hook(*a):
+        return None
+    hooks = ["register_forward_hook", "register_forward_pre_hook", "register_full_backward_hook", "register_full_backward_pre_hook"]
+    for name in hooks:
+        for at in (0, 1, 2):
+            net = FusedMLP(nn.Linear(4, 3), nn.ReLU(), nn.Linear(3, 2))
+            handle = getattr(net[at], name)(hook)
+            with pytest.raises(ValueError, match="hook"):
+                net(torch.zeros(2, 4))
+            handle.remove()
+            with pytest.raises(ValueError, match="CUDA"):
+                net(torch.zeros(2, 4))
+    net = FusedMLP(nn.Linear(4, 3), nn.ReLU())
+    prune.l1_unstructured(net[0], "weight", 0.5)
+    with pytest.raises(ValueError, match="hook"):
+        net(torch.zeros(2, 4))
+    net = FusedMLP(nn.Linear(4, 3), nn.ReLU())
+    net[0].forward = lambda x: x
+    with pytest.raises(ValueError, match="forward"):
+        net(torch.zeros(2, 4))
+    normed = prune.identity(nn.Linear(4, 3), "weight")
+    with pytest.raises(ValueError, match="hook"):
+        FusedMLP(normed)
+    # hooks of the whole still run
+    seen = []
+    net = FusedMLP(nn.Linear(4, 3))
+    net.register_forward_pre_hook(lambda m, a: seen.append(1))
+    with pytest.raises(ValueError, match="CUDA"):
+        net(torch.zeros(2, 4))
+    assert seen == [1]
