@@ -225,7 +225,7 @@ struct Weights {
 };
 
 struct MlpNode : Node {
-    SavedVariable x, y, between;
+    SavedVariable x, y, between;   // y: where the last layer is a ReLU, whose derivative it tells
     std::vector<SavedVariable> w;
     Plan plan;
     int64_t m = 0;
@@ -253,7 +253,7 @@ struct MlpNode : Node {
             const Rows g(gy, plan.widths[n], true), xs(x.unpack(self), plan.widths[0]);
             Weights ws;
             for (SavedVariable& v : w) ws.add(v.unpack(self));
-            const Tensor ys = y.unpack(self).contiguous(), held = between.unpack(self).contiguous();
+            const Tensor held = between.unpack(self).contiguous(), ys = plan.acts[n - 1] == CAFE_ACT_RELU ? y.unpack(self).contiguous() : Tensor();
             std::vector<void*> gw(n, nullptr), gb(n, nullptr);
             if (task_should_compute_output(0)) result[0] = at::empty(shape, gy.options());
             for (int l = 0; l < n; ++l) {
@@ -261,7 +261,7 @@ struct MlpNode : Node {
                 if (task_should_compute_output(1 + n + l)) gb[l] = out(result[1 + n + l] = at::empty({plan.widths[l + 1]}, gy.options()));
             }
             char* const base = static_cast<char*>(const_cast<void*>(held.const_data_ptr()));
-            const std::vector<void*> outputs = plan.outputs(base, const_cast<void*>(ys.const_data_ptr())), slopes = plan.slopes(base);
+            const std::vector<void*> outputs = plan.outputs(base, const_cast<void*>(ptr(ys))), slopes = plan.slopes(base);
             const int t = type_of(gy);
             const int64_t size = cafe_mlp_backward_work(n, plan.widths.data(), m, g.ptr(), g.ld, xs.ptr(), xs.ld, ws.p.data(), ws.ld.data(), t);
             const Tensor work = workspace(size, gy);
@@ -341,7 +341,7 @@ Tensor mlp(const Tensor& x, const std::vector<Tensor>& w, const std::vector<Mayb
     }
     if (grad) {
         torch::autograd::set_history(y, node);
-        node->y = SavedVariable(y, true);
+        if (acts[n - 1] == CAFE_ACT_RELU) node->y = SavedVariable(y, true);
     }
     return y;
 }
