@@ -34,13 +34,13 @@ void check_status(int status, const char* where) {
     TORCH_CHECK(false, where, status == CAFE_ERR_ARG ? ": invalid argument" : ": failed");
 }
 
-// t as rows of `cols` contiguous elements at one pitch; other layouts are copied.  `repeated`: pitch 0 (a row that stands for all)
-// is one.
+// t as rows of `cols` contiguous elements at one pitch; other layouts are copied, and views that carry a sign (the imaginary part of a
+// conjugate) written out.  `repeated`: pitch 0 (a row that stands for all) is one.
 struct Rows {
     Tensor t;
     int64_t m = 0, ld = 0;
     Rows() = default;
-    Rows(const Tensor& given, int64_t cols, bool repeated = false) : t(given), m(1), ld(cols) {
+    Rows(const Tensor& given, int64_t cols, bool repeated = false) : t(given.resolve_neg()), m(1), ld(cols) {
         for (int64_t i = 0; i + 1 < given.dim(); ++i) m *= given.size(i);
         if (t.dim() != 2) t = t.reshape({m, cols});
         if (t.is_contiguous() || t.numel() == 0 || (m == 1 && t.stride(1) == 1)) return;
@@ -49,7 +49,7 @@ struct Rows {
     }
     const void* ptr() const { return t.defined() ? t.const_data_ptr() : nullptr; }
 };
-Tensor plain(const Maybe& t) { return t && t->defined() ? t->contiguous() : Tensor(); }
+Tensor plain(const Maybe& t) { return t && t->defined() ? t->contiguous().resolve_neg() : Tensor(); }
 const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void* out(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
 // Workspace of one call, from torch's allocator: free again in the stream's order.
@@ -405,6 +405,8 @@ void adamw_step(const std::vector<Tensor>& p, std::vector<Tensor> g, const std::
     for (size_t i = 0; i < n; ++i) {
         check_moments(p[i], m[i], layout.empty() ? nullptr : &layout[i]);
         TORCH_CHECK(g[i].scalar_type() == p[i].scalar_type(), "AdamW: a gradient of ", g[i].scalar_type(), " for a parameter of ", p[i].scalar_type());
+        TORCH_CHECK(!p[i].is_neg(), "AdamW: a parameter has become a view that carries a sign");
+        g[i] = g[i].resolve_neg();
         if (!(g[i].is_contiguous() && p[i].is_contiguous()) && g[i].strides() != p[i].strides()) {
             const Tensor same = at::empty_like(p[i]);
             same.copy_(g[i]);

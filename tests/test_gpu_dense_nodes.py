@@ -1,4 +1,4 @@
-"""fused_linear and fused_mlp as parts of a graph: what may be written to afterwards."""
+"""fused_linear and fused_mlp as parts of a graph: what may be written to afterwards, views that carry a sign."""
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -38,3 +38,48 @@ def test_an_output_of_no_use_is_not_kept():
     del y
     assert torch.cuda.memory_allocated() - before < 1 << 20, node   # (the output has 32 MB)
 
+
+def test_views_that_carry_a_sign():
+    """Tensors whose sign lies in their view (the imaginary part of a conjugate) are taken at their value, one column wide too."""
+    import torch
+    from cafe_b200 import fused_linear, fused_mlp
+    g = torch.Generator(device="cuda").manual_seed(4)
+
+    def signed(*shape):
+        t = torch._neg_view(torch.randn(*shape, device="cuda", generator=g))
+        assert t.is_neg()
+        return t
+    for M, N, K in ((40, 1, 1), (50, 30, 20)):
+        x, w, b, r, gy = signed(M, K), signed(N, K), signed(N), signed(M, N), signed(M, N)
+        plain = [(t + 0).detach() for t in (x, w, b, r, gy)]
+        assert not any(t.is_neg() for t in plain)
+        assert torch.equal(fused_linear(x, w, b, "silu", r), fused_linear(*plain[:3], "silu", plain[3]))
+        assert torch.equal(fused_mlp(x, [w], [b], ["gelu"]), fused_mlp(plain[0], [plain[1]], [plain[2]], ["gelu"]))
+        leaves = [t.requires_grad_(True) for t in plain[:4]]
+        for call in (lambda: fused_linear(*leaves[:3], "silu", leaves[3]), lambda: fused_mlp(leaves[0], [leaves[1]], [leaves[2]], ["gelu"])):
+            mine = leaves if "silu" in call.__code__.co_consts else leaves[:3]
+            got, want = torch.autograd.grad(call(), mine, gy), torch.autograd.grad(call(), mine, plain[4])
+            assert all(torch.equal(a, e) for a, e in zip(got, want))
+    # as a program meets it: through a conjugate of a complex number made of the output
+    x, w = torch.randn(40, 3, device="cuda", generator=g), torch.randn(1, 3, device="cuda", generator=g)
+    c = torch.randn(40, 1, dtype=torch.complex64, device="cuda", generator=g)
+    grads = []
+    for f in (lambda x, w: fused_linear(x, w), lambda x, w: x @ w.t()):
+        x1 = x.clone().requires_grad_(True)
+        y = f(x1, w)
+        (torch.complex(torch.zeros_like(y), y).conj() * c).abs().square().sum().backward()
+        (torch.complex(y.detach() * 0, f(x1, w)).conj() * c).imag.sum().backward()
+        grads.append(x1.grad)
+    torch.testing.assert_close(*grads, rtol=1e-5, atol=1e-6)
+
+
+def test_negative_views_as_gradients_of_adamw():
+    import torch
+    from cafe_b200 import AdamW
+    p, q = (torch.nn.Parameter(torch.ones(500, device="cuda")) for _ in range(2))
+    grad = torch.randn(500, device="cuda")
+    p.grad, q.grad = torch._neg_view(grad), -grad
+    a, b = AdamW([p]), AdamW([q])
+    a.step()
+    b.step()
+    assert torch.equal(p, q)
