@@ -394,6 +394,11 @@ void check_moments(const Tensor& p, const Tensor& m, const Tensor* layout) {
     TORCH_CHECK(same, "AdamW: a parameter's elements lie in another order than when its moments were made",
                 layout ? "" : " (load_state_dict(state_dict()) lays the moments out anew)");
 }
+// An array of the state is what the kernels read and write: `n` elements of a type, on p's device.
+void check_state(const Tensor& p, const Tensor& s, int64_t n, at::ScalarType type) {
+    TORCH_CHECK(s.numel() == n && s.scalar_type() == type && s.device() == p.device() && s.is_non_overlapping_and_dense(),
+                "AdamW: the moments or the step of a parameter are not what they were made as");
+}
 // one step of parameters of one type on one device; mtop, vtop and layout are empty with 32-bit moments
 void adamw_step(const std::vector<Tensor>& p, std::vector<Tensor> g, const std::vector<Tensor>& m, const std::vector<Tensor>& v, const std::vector<Tensor>& mtop,
                 const std::vector<Tensor>& vtop, const std::vector<Tensor>& layout, const std::vector<Tensor>& step, const std::vector<int>& index, double lr, double beta1, double beta2, double eps,
@@ -401,10 +406,21 @@ void adamw_step(const std::vector<Tensor>& p, std::vector<Tensor> g, const std::
     at::NoGradGuard plain_values;
     const c10::cuda::CUDAGuard device(ticket.device());
     const size_t n = p.size();
+    const bool packed = !mtop.empty();
     std::vector<int64_t> numel(n);
     for (size_t i = 0; i < n; ++i) {
         check_moments(p[i], m[i], layout.empty() ? nullptr : &layout[i]);
+        numel[i] = p[i].numel();
+        check_state(p[i], m[i], numel[i], packed ? at::kByte : at::kFloat);
+        check_state(p[i], v[i], numel[i], packed ? at::kByte : at::kFloat);
+        check_state(p[i], step[i], 1, at::kLong);
+        if (packed) {
+            check_state(p[i], mtop[i], (numel[i] + 255) / 256, at::kByte);
+            check_state(p[i], vtop[i], (numel[i] + 255) / 256, at::kByte);
+        } else check_moments(p[i], v[i], nullptr);
         TORCH_CHECK(g[i].scalar_type() == p[i].scalar_type(), "AdamW: a gradient of ", g[i].scalar_type(), " for a parameter of ", p[i].scalar_type());
+        TORCH_CHECK(g[i].sizes() == p[i].sizes() && g[i].device() == p[i].device(), "AdamW: a gradient of ", g[i].sizes(), " on ", g[i].device(),
+                    " for a parameter of ", p[i].sizes(), " on ", p[i].device());
         TORCH_CHECK(!p[i].is_neg(), "AdamW: a parameter has become a view that carries a sign");
         g[i] = g[i].resolve_neg();
         if (!(g[i].is_contiguous() && p[i].is_contiguous()) && g[i].strides() != p[i].strides()) {
@@ -412,10 +428,8 @@ void adamw_step(const std::vector<Tensor>& p, std::vector<Tensor> g, const std::
             same.copy_(g[i]);
             g[i] = same;
         }
-        numel[i] = p[i].numel();
     }
     const std::vector<void*> gs = pointers(g), ms = pointers(mtop), vs = pointers(vtop), steps = pointers(step);
-    const bool packed = !mtop.empty();
     check_status(cafe_adamw_step((int)n, pointers(p).data(), gs.data(), pointers(m).data(), pointers(v).data(), packed ? (uint8_t* const*)ms.data() : nullptr,
                                  packed ? (uint8_t* const*)vs.data() : nullptr, (int64_t* const*)steps.data(), numel.data(), index.data(), type_of(p[0]), packed ? 8 : 32,
                                  lr, beta1, beta2, eps, weight_decay, seed, static_cast<int*>(ticket.mutable_data_ptr()), c10::cuda::getCurrentCUDAStream().stream()),
@@ -434,6 +448,8 @@ std::vector<std::pair<Tensor, Tensor>> adamw_moments(const std::vector<Tensor>& 
     bool together = true;   // one allocation, every tensor on 16 bytes
     for (size_t i = 0; i < n; ++i) {
         check_moments(p[i], m[i], &layout[i]);
+        for (const Tensor* c : {&m[i], &r[i]}) check_state(p[i], *c, p[i].numel(), at::kByte);
+        for (const Tensor* c : {&mtop[i], &rtop[i]}) check_state(p[i], *c, (p[i].numel() + 255) / 256, at::kByte);
         together &= p[i].is_contiguous() && all % 8 == 0;
         all += numel[i] = p[i].numel();
     }

@@ -115,3 +115,30 @@ def test_codes_of_another_order_are_not_loaded():
     AdamW([third], state_bits=8).load_state_dict(kept)
     with pytest.raises(ValueError, match="order"):
         AdamW([q], state_bits=8).load_state_dict(kept)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_gradients_and_states_of_another_size_are_refused(bits):
+    """torch checks a gradient's size when it is set, but not when .data is exchanged behind it."""
+    import torch
+    from cafe_b200 import AdamW
+    for size in (5000, 3):
+        p = torch.nn.Parameter(torch.zeros(10, device="cuda"))
+        p.grad = torch.ones(10, device="cuda")
+        p.data = torch.zeros(size, device="cuda")
+        opt = AdamW([p], state_bits=bits)
+        with pytest.raises(RuntimeError, match="gradient"):
+            opt.step()
+        assert bool((p == 0).all())
+    for name in ("exp_avg", "exp_avg_sq", "step") if bits == 32 else ("exp_avg", "exp_avg_top", "root_avg_sq", "root_avg_sq_top", "step"):
+        p, opt = _fresh((40, 30), bits)
+        before = p.detach().clone()
+        for bad in (lambda t: t.reshape(-1)[:0], lambda t: t.double(), lambda t: t.cpu()):
+            kept = opt.state[p][name]
+            opt.state[p][name] = bad(kept)
+            with pytest.raises(RuntimeError, match="moments|order"):
+                opt.step()
+            opt.state[p][name] = kept
+        assert torch.equal(p, before)
+        opt.step()
+        assert not torch.equal(p, before)
