@@ -354,7 +354,8 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
 // Where there are tiles enough: two blocks, an SM each, work on tiles of 256 x BN, tile after tile.  Each fetches its own 128 rows of
 // A and half of B's, so an SM's boxes are half to three quarters of those of a block by itself, and the products no longer wait
 // for them (16384x1024x1024 in fp32: 48 KB for 768 cycles of products an SM came at 29 bytes a cycle, tensor cores busy 46 %).
-// Block 0 issues the products of both; block 1 tells it when its boxes are there.
+// Block 0 issues the products of both; the boxes of both complete on its barriers (no thread stands between a copy and the products
+// that read it).
 //
 // fp32: eight warps have 32 rows and half of the columns each.  They take the large sums out every 256 of k and everything when a
 // tile's products are done, into registers; tensor memory is then free for the next tile, whose products run while this one is
@@ -560,7 +561,7 @@ __global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) k_tiles_pair(const __gri
     const CafePairTiles list(P, pair, pairs);
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < Sh::stages; ++s) { cafe_bar_init(full(s), 2 - rank); cafe_bar_init(empty(s), 1); }   // (block 0: its boxes and the other's)
+        for (int s = 0; s < Sh::stages; ++s) { cafe_bar_init(full(s), 1); cafe_bar_init(empty(s), 1); }   // (full: block 0's, for the boxes of both)
         cafe_bar_init(chunk_full, 1);
         cafe_bar_init(chunk_taken, 2 * Sh::takers);
         for (int g = 0; g < 2; ++g) { cafe_bar_init(tile_full(g), 1); cafe_bar_init(tile_taken(g), 2 * Sh::takers); }
@@ -592,40 +593,30 @@ __global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) k_tiles_pair(const __gri
             const int a_kc = J.a_kc, b_kc = J.b_kc;
             for (int k0 = t0 * L::BK; k0 < t1 * L::BK; k0 += L::BK, ++u) {
                 if (!(fine = __all_sync(0xffffffffu, cafe_bar_wait(empty(s), phase, &bail)))) break;
-                const uint32_t a = base + s * Sh::stage, b = a + L::parts * Sh::a_part, bar = full(s);
+                const uint32_t a = base + s * Sh::stage, b = a + L::parts * Sh::a_part, bar = cafe_cluster_map(full(s), 0);
                 if (cafe_elect()) {
-                    cafe_bar_expect(bar, Sh::stage);
-                    if (a_kc) cafe_box_load(a, ma, k0, row0, 0, bar);
+                    if (rank == 0) cafe_bar_expect(full(s), 2 * Sh::stage);   // (block 1's bytes may come before: the phase waits for this arrival)
+                    if (a_kc) cafe_box_load2(a, ma, k0, row0, 0, bar);
                     else
 #pragma unroll
-                        for (int q = 0; q < CAFE_LIN_BM / 64; ++q) cafe_box_load(a + q * L::parts * L::BK * 128, ma, row0 + 64 * q, k0, 0, bar);
-                    if (b_kc) cafe_box_load(b, mb, k0, col0, 0, bar);
+                        for (int q = 0; q < CAFE_LIN_BM / 64; ++q) cafe_box_load2(a + q * L::parts * L::BK * 128, ma, row0 + 64 * q, k0, 0, bar);
+                    if (b_kc) cafe_box_load2(b, mb, k0, col0, 0, bar);
                     else
 #pragma unroll
-                        for (int q = 0; q < BN / 128; ++q) cafe_box_load(b + q * L::parts * L::BK * 128, mb, col0 + 64 * q, k0, 0, bar);
+                        for (int q = 0; q < BN / 128; ++q) cafe_box_load2(b + q * L::parts * L::BK * 128, mb, col0 + 64 * q, k0, 0, bar);
                 }
                 if (++s == Sh::stages) { s = 0; phase ^= 1u; }
             }
         }
-        if (!fine)   // given up: the copies in flight end before the block does
-            for (int64_t v = u > Sh::stages ? u - Sh::stages : 0; v < u; ++v)
-                for (int i = 0; i < (1 << 20) && !cafe_bar_try(full((int)(v % Sh::stages)), (uint32_t)(v / Sh::stages) & 1u); ++i) {}
-    } else if (warp == 1 && rank == 1) {
-        if (lane == 0) {
-            // ---- this block's boxes are there
-            int s = 0;
-            uint32_t phase = 0;
-            bool fine = true;
-            for (int n = 0; n < list.all && fine; ++n) {
-                int t0, t1;
-                list.turns<L::BK>(P, n, &t0, &t1);
-                for (int t = t0; t < t1; ++t) {
-                    if (!(fine = cafe_bar_wait(full(s), phase, &bail))) break;
-                    cafe_bar_arrive_at(cafe_cluster_map(full(s), 0));
-                    if (++s == Sh::stages) { s = 0; phase ^= 1u; }
-                }
-            }
+        if (!fine) {   // given up: the copies in flight end before the block does (block 1's complete at block 0: it waits 16 ms)
+            if (rank == 0) {
+                for (int64_t v = u > Sh::stages ? u - Sh::stages : 0; v < u; ++v)
+                    for (int i = 0; i < (1 << 20) && !cafe_bar_try(full((int)(v % Sh::stages)), (uint32_t)(v / Sh::stages) & 1u); ++i) {}
+            } else
+                for (int i = 0; i < (1 << 14); ++i) __nanosleep(1000);
         }
+    } else if (warp == 1 && rank == 1) {
+        // (block 0 issues)
     } else if (warp == 1) {
         // ---- products
         bool fine = true;
@@ -644,12 +635,12 @@ __global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) k_tiles_pair(const __gri
             const uint32_t ak = (J.a_kc ? 32 : 2048) >> 4, bk = (J.b_kc ? 32 : 2048) >> 4;
             const int g = n % Sh::sets;
             const uint32_t sums = tmem + g * Sh::tm_set;
-            if (n >= Sh::sets && !(fine = __all_sync(0xffffffffu, cafe_bar_wait(tile_taken(g), (uint32_t)(n / Sh::sets - 1) & 1u, &bail)))) break;
+            if (n >= Sh::sets && !(fine = __all_sync(0xffffffffu, cafe_bar_wait<true>(tile_taken(g), (uint32_t)(n / Sh::sets - 1) & 1u, &bail)))) break;
             int in_chunk = 0;
             for (int t = 0; t < turns; ++t) {
                 if (!(fine = __all_sync(0xffffffffu, cafe_bar_wait(full(s), phase, &bail)))) break;
                 if (L::parts == 3 && in_chunk == 0 && t > 0) {
-                    if (!(fine = __all_sync(0xffffffffu, cafe_bar_wait(chunk_taken, chunk_phase, &bail)))) break;
+                    if (!(fine = __all_sync(0xffffffffu, cafe_bar_wait<true>(chunk_taken, chunk_phase, &bail)))) break;
                     chunk_phase ^= 1u;
                 }
                 cafe_tc_after();
@@ -677,7 +668,7 @@ __global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) k_tiles_pair(const __gri
             if (cafe_elect()) cafe_mma_commit2(tile_full(g));
         }
         if (!fine)   // given up: products in flight end before the block does
-            for (int i = 0; i < (1 << 20) && !cafe_bar_try(tile_full(n % Sh::sets), (uint32_t)(n / Sh::sets) & 1u); ++i) {}
+            for (int i = 0; i < (1 << 20) && !cafe_bar_try<true>(tile_full(n % Sh::sets), (uint32_t)(n / Sh::sets) & 1u); ++i) {}
     } else {
         // ---- sums out of tensor memory and out of the block
         constexpr int W = Sh::cols;
@@ -724,7 +715,7 @@ __global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) k_tiles_pair(const __gri
                 };
                 const int between = turns > 0 ? (turns - 1) / CAFE_TILES_CHUNK : 0;   // chunks that do not end the tile
                 for (int c = 0; c < between && fine; ++c, chunk_phase ^= 1u) {
-                    fine = cafe_bar_wait(chunk_full, chunk_phase, &bail);
+                    fine = cafe_bar_wait<true>(chunk_full, chunk_phase, &bail);
                     cafe_tc_after();
                     fine = __all_sync(0xffffffffu, fine);
                     if (fine) take(from, c == 0);
@@ -732,7 +723,7 @@ __global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) k_tiles_pair(const __gri
                     __syncwarp();
                     if (lane == 0) cafe_bar_arrive_at(cafe_cluster_map(chunk_taken, 0));
                 }
-                if (fine) fine = cafe_bar_wait(tile_full(g), (uint32_t)(n / Sh::sets) & 1u, &bail);
+                if (fine) fine = cafe_bar_wait<true>(tile_full(g), (uint32_t)(n / Sh::sets) & 1u, &bail);
                 cafe_tc_after();
                 fine = __all_sync(0xffffffffu, fine);
                 if (fine) {
@@ -790,7 +781,7 @@ __global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) k_tiles_pair(const __gri
                     asm volatile("cp.async.commit_group;" ::: "memory");
                 };
                 residual(0);
-                if (fine) fine = cafe_bar_wait(tile_full(g), (uint32_t)(n / Sh::sets) & 1u, &bail);
+                if (fine) fine = cafe_bar_wait<true>(tile_full(g), (uint32_t)(n / Sh::sets) & 1u, &bail);
                 cafe_tc_after();
                 fine = __all_sync(0xffffffffu, fine);
 #pragma unroll 1

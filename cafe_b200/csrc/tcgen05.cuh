@@ -8,22 +8,27 @@ __device__ __forceinline__ uint32_t cafe_smem(const void* p) { return (uint32_t)
 
 __device__ __forceinline__ void cafe_bar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
 __device__ __forceinline__ void cafe_bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
-__device__ __forceinline__ bool cafe_bar_try(uint32_t bar, uint32_t parity) {
+// CLUSTER: for what the other block of a pair tells through this barrier about tensor memory.  Tensor memory is ordered by the tcgen05
+// fences on both sides (cafe_tc_before, cafe_tc_after) around the arrival and the wait, which therefore need no order of their own,
+// only the cluster's scope.
+template <bool CLUSTER = false> __device__ __forceinline__ bool cafe_bar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    if constexpr (CLUSTER)
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    else asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok;
 }
 // Waits for the phase of `parity` to end, but not for good: after about a second, or when another wait of the block has run
 // out (*bail), it gives up and says so.
-static __device__ __noinline__ bool cafe_bar_wait_on(uint32_t bar, uint32_t parity, volatile int* bail);
-__device__ __forceinline__ bool cafe_bar_wait(uint32_t bar, uint32_t parity, volatile int* bail) {
-    return cafe_bar_try(bar, parity) || cafe_bar_wait_on(bar, parity, bail);
-}
-static __device__ __noinline__ bool cafe_bar_wait_on(uint32_t bar, uint32_t parity, volatile int* bail) {
-    for (int i = 0; !cafe_bar_try(bar, parity); ++i) {
+template <bool CLUSTER> static __device__ __noinline__ bool cafe_bar_wait_on(uint32_t bar, uint32_t parity, volatile int* bail) {
+    for (int i = 0; !cafe_bar_try<CLUSTER>(bar, parity); ++i) {
         if (i > (1 << 20) || ((i & 255) == 255 && *bail)) { *bail = 1; return false; }
     }
     return true;
+}
+template <bool CLUSTER = false> __device__ __forceinline__ bool cafe_bar_wait(uint32_t bar, uint32_t parity, volatile int* bail) {
+    return cafe_bar_try<CLUSTER>(bar, parity) || cafe_bar_wait_on<CLUSTER>(bar, parity, bail);
 }
 
 // Launches that follow one another closely: the next kernel of the stream may start once all blocks of this one have, and does what
@@ -98,9 +103,9 @@ __device__ __forceinline__ void cafe_mma_commit2(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
 
-// An arrival at another block's barrier.  What it tells of is not in this thread's own writes (boxes that the copy engine has written,
-// tensor memory that has been read), so it needs no fence of the cluster's scope, which takes thousands of cycles.
-__device__ __forceinline__ void cafe_bar_arrive_at(uint32_t cluster_bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory"); }
+// An arrival at another block's barrier that tells of tensor memory having been read (cafe_bar_try's CLUSTER says what orders it; a
+// release of the cluster's scope would wait for this thread's own stores, thousands of cycles).
+__device__ __forceinline__ void cafe_bar_arrive_at(uint32_t cluster_bar) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory"); }
 
 __device__ __forceinline__ uint32_t cafe_cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ void cafe_cluster_sync() {
@@ -127,6 +132,10 @@ __device__ __forceinline__ void cafe_bar_expect(uint32_t bar, uint32_t bytes) { 
 // a box of a tensor (three axes, the innermost first) into shared memory; what lies outside the tensor becomes zero
 __device__ __forceinline__ void cafe_box_load(uint32_t to, const void* map, int x, int y, int z, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(to), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
+// The same into this block's shared memory, completing on a barrier of either block of a pair (an address in the cluster)
+__device__ __forceinline__ void cafe_box_load2(uint32_t to, const void* map, int x, int y, int z, uint32_t cluster_bar) {
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(to), "l"(map), "r"(x), "r"(y), "r"(z), "r"(cluster_bar) : "memory");
 }
 // The operand whose other index is contiguous: panels of 64 of them (128 bytes, pieces exchanged as above) x k, eight k a unit;
 // `panel` bytes from one panel to the next.
