@@ -837,6 +837,15 @@ static EncodeTiled tiles_encoder() {
     return f;
 }
 
+// The encoder asks for the calling thread's context, which a thread that has not called the runtime yet (the autograd engine's in its
+// first backward) does not have: setting the device that is current anyway makes it.
+static cudaError_t tiles_ready() {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess) e = cudaSetDevice(device);
+    return e != cudaSuccess ? e : tiles_encoder() ? cudaSuccess : cudaErrorNotSupported;
+}
+
 // an operand as the copies see it: rows x cols (cols contiguous), `parts` planes
 struct TilesOperand {
     const void* at;
@@ -1133,13 +1142,15 @@ static cudaError_t tiles_backward(const CafeBackward& f, int dtype, const CafeJo
     return tiles_launch<T>(q, count, f.gb ? TilesSums{sums, sum_rows, f.N, f.gb} : TilesSums{}, st);
 }
 cudaError_t cafe_tiles_forward(const CafeForward& f, int dtype, const CafeJob& job, void* work, cudaStream_t st) {
-    if (!tiles_encoder()) return cudaErrorNotSupported;
+    const cudaError_t e = tiles_ready();
+    if (e != cudaSuccess) return e;
     char* const at = (char*)(((uintptr_t)work + 255) & ~(uintptr_t)255);
     return dtype == CAFE_F32 ? tiles_forward<float>(f, dtype, job, at, st)
                              : dtype == CAFE_BF16 ? tiles_forward<__nv_bfloat16>(f, dtype, job, at, st) : tiles_forward<__half>(f, dtype, job, at, st);
 }
 cudaError_t cafe_tiles_backward(const CafeBackward& f, int dtype, const CafeJob* gw, const CafeJob* gx, void* work, cudaStream_t st) {
-    if (!tiles_encoder()) return cudaErrorNotSupported;
+    const cudaError_t e = tiles_ready();
+    if (e != cudaSuccess) return e;
     char* const at = (char*)(((uintptr_t)work + 255) & ~(uintptr_t)255);
     return dtype == CAFE_F32 ? tiles_backward<float>(f, dtype, gw, gx, at, st)
                              : dtype == CAFE_BF16 ? tiles_backward<__nv_bfloat16>(f, dtype, gw, gx, at, st) : tiles_backward<__half>(f, dtype, gw, gx, at, st);

@@ -1,4 +1,5 @@
-"""fused_linear and fused_mlp as parts of a graph: what may be written to afterwards, views that carry a sign."""
+"""fused_linear and fused_mlp as parts of a graph: what may be written to afterwards, views that carry a sign,
+threads that have made no CUDA call yet."""
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -83,3 +84,50 @@ def test_negative_views_as_gradients_of_adamw():
     a.step()
     b.step()
     assert torch.equal(p, q)
+
+
+def test_first_call_of_a_thread():
+    """A thread that has made no CUDA call of its own has no context, which the description of operands in place asks for.  Memory comes
+    from what the first pass left, so nothing else makes one."""
+    import threading
+    import torch
+    from cafe_b200 import fused_linear
+    x, w = (torch.randn(1024, 1024, device="cuda").bfloat16() for _ in range(2))
+    with torch.no_grad():
+        want = fused_linear(x, w)
+        spare = fused_linear(x, w)
+        torch.cuda.synchronize()
+        del spare
+        got = []
+
+        def call():
+            with torch.no_grad():
+                try:
+                    got.append(fused_linear(x, w))
+                except RuntimeError as e:
+                    got.append(e)
+        for _ in range(2):
+            t = threading.Thread(target=call)
+            t.start()
+            t.join()
+    assert not isinstance(got[0], Exception), got[0]
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want) and torch.equal(got[1], want)
+
+
+def test_first_backward_of_a_process():
+    import subprocess
+    import sys
+    from pathlib import Path
+    program = """
+import torch
+from cafe_b200 import fused_linear
+x, w, gy = (torch.randn(1024, 1024, device="cuda").bfloat16() for _ in range(3))
+w.requires_grad_(True)
+gw, = torch.autograd.grad(fused_linear(x, w), w, gy)
+want = gy.double().t() @ x.double()
+assert float((gw.double() - want).norm() / want.norm()) < 2.0 ** -8
+print("fine")
+"""
+    r = subprocess.run([sys.executable, "-c", program], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True, timeout=300)
+    assert r.stdout.strip() == "fine", r.stderr[-2000:]
