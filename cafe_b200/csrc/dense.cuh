@@ -106,6 +106,10 @@ __device__ __forceinline__ void cafe_put16(uint32_t at, uint32_t a, uint32_t b, 
 // infinity are NaN, and times a lower part that is zero it would be one too.  (An infinity times a number below 2^-133, whose upper
 // part is zero, becomes NaN.)
 __device__ __forceinline__ float cafe_join_sums(float large, float rest) { return fabsf(large) < INFINITY ? large + rest : large; }
+// Split operands: after how many pieces of the large sums the others are taken out as well (pieces of 256 of k, so every 4096).  They
+// are 2^-8 of the result, but five products feed them and the tensor cores cut every addition off (CAFE_TILES_CHUNK's comment has
+// the figures).
+#define CAFE_LIN_LOW 16
 // fp32 for splitting: every NaN with its upper bits set (an upper part that is cut off must not become an infinity)
 __device__ __forceinline__ float cafe_quiet(float x) { return x + 0.f; }
 

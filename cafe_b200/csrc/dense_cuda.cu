@@ -291,12 +291,23 @@ __global__ void __launch_bounds__(CAFE_LIN_THREADS, 1) k_linear(const __grid_con
                 for (int i = 0; i < 16; ++i) acc[c + i] = first ? v[i] : acc[c + i] + v[i];
             }
         };
+        auto join = [&]() {   // fp32: the other sums
+#pragma unroll
+            for (int c = 0; c < half_cols; c += 16) {
+                float v[16];
+                cafe_tm_load16(from + BN + c, v);
+                cafe_tm_wait_load();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[c + i] = cafe_join_sums(acc[c + i], v[i]);
+            }
+        };
         constexpr uint32_t instr = cafe_mma_instr(L::type, CAFE_LIN_BM, BN);
         const int chunks = (turns + L::chunk - 1) / L::chunk;
         bool fine = true;
         for (int c = 0; c < chunks && fine; ++c) {
             if (warp == 8) {
                 const int end = min(turns, (c + 1) * L::chunk);
+                const bool low = L::parts == 3 && (c + 1) % CAFE_LIN_LOW == 0 && c < chunks - 1;
                 if (c > 0) fine = __all_sync(0xffffffffu, cafe_bar_wait(acc_empty, (uint32_t)(c - 1) & 1u, &bail));
                 for (int t = c * L::chunk; t < end && fine; ++t) {
                     const int s = t % Sh::stages;
@@ -307,7 +318,7 @@ __global__ void __launch_bounds__(CAFE_LIN_THREADS, 1) k_linear(const __grid_con
 #pragma unroll
                         for (int k = 0; k < L::BK / 16; ++k)
                             cafe_mma(tmem, cafe_operand<Sh::rowb>(a + 32 * k), cafe_operand<Sh::rowb>(b + 32 * k), instr, t > c * L::chunk || k > 0);
-                        if (t == end - 1) cafe_mma_commit(acc_full);
+                        if (t == end - 1 && !low) cafe_mma_commit(acc_full);
                         if constexpr (L::parts == 3) {
 #pragma unroll
                             for (int q = 0; q < 5; ++q) {
@@ -315,8 +326,9 @@ __global__ void __launch_bounds__(CAFE_LIN_THREADS, 1) k_linear(const __grid_con
 #pragma unroll
                                 for (int k = 0; k < L::BK / 16; ++k)
                                     cafe_mma(tmem + BN, cafe_operand<Sh::rowb>(a + ia[q] * Sh::a_part + 32 * k),
-                                             cafe_operand<Sh::rowb>(b + ib[q] * Sh::b_part + 32 * k), instr, t > 0 || q > 0 || k > 0);
+                                             cafe_operand<Sh::rowb>(b + ib[q] * Sh::b_part + 32 * k), instr, t % (L::chunk * CAFE_LIN_LOW) > 0 || q > 0 || k > 0);
                             }
+                            if (t == end - 1 && low) cafe_mma_commit(acc_full);
                         }
                         cafe_mma_commit(empty(s));
                     }
@@ -328,7 +340,9 @@ __global__ void __launch_bounds__(CAFE_LIN_THREADS, 1) k_linear(const __grid_con
             if (fine) fine = cafe_bar_wait(acc_full, (uint32_t)c & 1u, &bail);
             cafe_tc_after();
             __syncwarp();
-            if (__all_sync(0xffffffffu, fine)) take(from, c == 0); else fine = false;
+            fine = __all_sync(0xffffffffu, fine);
+            if (fine) take(from, c == 0);
+            if (L::parts == 3 && fine && (c + 1) % CAFE_LIN_LOW == 0 && c < chunks - 1) join();
             cafe_tc_before();
             __syncwarp();
             if (lane == 0) cafe_bar_arrive(acc_empty);
@@ -338,16 +352,7 @@ __global__ void __launch_bounds__(CAFE_LIN_THREADS, 1) k_linear(const __grid_con
             fine = cafe_bar_wait(all_done, 0, &bail) && fine;
             cafe_tc_after();
             fine = __all_sync(0xffffffffu, fine);
-            if (L::parts == 3 && fine) {
-#pragma unroll
-                for (int c = 0; c < half_cols; c += 16) {
-                    float v[16];
-                    cafe_tm_load16(from + BN + c, v);
-                    cafe_tm_wait_load();
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[c + i] = cafe_join_sums(acc[c + i], v[i]);
-                }
-            }
+            if (L::parts == 3 && fine) join();
         } else {
 #pragma unroll
             for (int i = 0; i < half_cols; ++i) acc[i] = 0.f;

@@ -31,11 +31,13 @@ template <typename T> struct CafeTiles {
 };
 template <> struct CafeTiles<__nv_bfloat16> { static constexpr int parts = 1, BK = 64, type = 1; typedef __nv_bfloat16 part; };
 template <> struct CafeTiles<float> { static constexpr int parts = 3, BK = 32, type = 1; typedef __nv_bfloat16 part; };
-// fp32: turns of 32 between two times that the large sums are taken out.  The tensor cores cut sums off, 2^-24 of them a turn on
-// average: relative error (norms; signed, all positive operands) of a depth of 2048 in one go 5.3e-7, 9.9e-7, in pieces of 256
-// 2.9e-7, 4.8e-7 (in plain fp32 8.1e-7, 7.0e-7); of 65 536 in one go 9.4e-6, 3.6e-5, in pieces 5.5e-7, 1.6e-6.  Pieces of 1024
-// were not measurably faster.
+// fp32: turns of 32 between two times that the large sums are taken out, and the others.  The tensor cores cut an instruction's products and
+// their sum off: in proportion to the depth, and towards zero.  Relative error (norms; signed, all positive operands) of a depth of 65 536
+// in one go 9.4e-6, 3.6e-5; with the large sums in pieces of 256 of k and the others in one go 2.6e-6, 1.1e-5 (131 072: 4.9e-6, 2.0e-5); with
+// the others in pieces of 4096 5.0e-7, 7.2e-7 (131 072: 5.8e-7, 7.5e-7; 4096: 3.0e-7, 2.1e-7), where plain fp32 has 4.6e-6, 3.7e-6.  Larger
+// pieces were not measurably faster.
 #define CAFE_TILES_CHUNK 8
+#define CAFE_TILES_LOW (CAFE_TILES_CHUNK * CAFE_LIN_LOW)   // turns between two times that the other sums are
 
 // ---- operands as parts ---------------------------------------------------------------------------------------------------
 struct CafePartsJob {
@@ -226,19 +228,20 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
             }
             cafe_tc_after();
             const uint64_t a = da + (uint32_t)(s * Sh::stage >> 4), b = db + (uint32_t)(s * Sh::stage >> 4);
-            const bool ends = in_chunk == CAFE_TILES_CHUNK - 1 || t == turns - 1;
+            const bool ends = in_chunk == CAFE_TILES_CHUNK - 1 || t == turns - 1, low = (t + 1) % CAFE_TILES_LOW == 0 && t < turns - 1;
             if (cafe_elect()) {
 #pragma unroll
                 for (int k = 0; k < L::BK / 16; ++k) cafe_mma(tmem, a + ak * k, b + bk * k, instr, in_chunk > 0 || k > 0);
                 if constexpr (L::parts == 3) {
-                    if (ends) cafe_mma_commit(acc_full);
+                    if (ends && !low) cafe_mma_commit(acc_full);
 #pragma unroll
                     for (int q = 0; q < 5; ++q) {
                         constexpr int ia[5] = {0, 1, 1, 0, 2}, ib[5] = {1, 0, 1, 2, 0};
 #pragma unroll
                         for (int k = 0; k < L::BK / 16; ++k)
-                            cafe_mma(tmem + BN, a + ia[q] * ap + ak * k, b + ib[q] * bp + bk * k, instr, t > 0 || q > 0 || k > 0);
+                            cafe_mma(tmem + BN, a + ia[q] * ap + ak * k, b + ib[q] * bp + bk * k, instr, t % CAFE_TILES_LOW > 0 || q > 0 || k > 0);
                     }
+                    if (low) cafe_mma_commit(acc_full);
                 }
                 cafe_mma_commit(empty(s));
             }
@@ -277,6 +280,16 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
                     for (int i = 0; i < 16; ++i) acc[c + i] = first ? v[i] : acc[c + i] + v[i];
                 }
             };
+            auto join = [&]() {   // the other sums
+#pragma unroll
+                for (int c = 0; c < BN; c += 16) {
+                    float v[16];
+                    cafe_tm_load16(from + BN + c, v);
+                    cafe_tm_wait_load();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[c + i] = cafe_join_sums(acc[c + i], v[i]);
+                }
+            };
             const int chunks = (turns + CAFE_TILES_CHUNK - 1) / CAFE_TILES_CHUNK;
             if (turns == 0) {
 #pragma unroll
@@ -287,6 +300,7 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
                 cafe_tc_after();
                 fine = __all_sync(0xffffffffu, fine);
                 if (fine) take(from, c == 0);
+                if (fine && (c + 1) % CAFE_LIN_LOW == 0 && c < chunks - 1) join();
                 cafe_tc_before();
                 __syncwarp();
                 if (lane == 0) cafe_bar_arrive(acc_empty);
@@ -294,16 +308,7 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
             fine = cafe_bar_wait(all_done, 0, &bail) && fine;
             cafe_tc_after();
             fine = __all_sync(0xffffffffu, fine);
-            if (fine && turns > 0) {
-#pragma unroll
-                for (int c = 0; c < BN; c += 16) {
-                    float v[16];
-                    cafe_tm_load16(from + BN + c, v);
-                    cafe_tm_wait_load();
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[c + i] = cafe_join_sums(acc[c + i], v[i]);
-                }
-            }
+            if (fine && turns > 0) join();
         } else {
             fine = cafe_bar_wait(all_done, 0, &bail);
             cafe_tc_after();
@@ -645,18 +650,20 @@ __global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) k_tiles_pair(const __gri
                 }
                 cafe_tc_after();
                 const uint64_t a = da + (uint32_t)(s * Sh::stage >> 4), b = db + (uint32_t)(s * Sh::stage >> 4);
+                const bool ends = in_chunk == CAFE_TILES_CHUNK - 1 && t < turns - 1, low = ends && (t + 1) % CAFE_TILES_LOW == 0;
                 if (cafe_elect()) {
 #pragma unroll
                     for (int k = 0; k < L::BK / 16; ++k) cafe_mma2(sums, a + ak * k, b + bk * k, instr, in_chunk > 0 || k > 0);
                     if constexpr (L::parts == 3) {
-                        if (in_chunk == CAFE_TILES_CHUNK - 1 && t < turns - 1) cafe_mma_commit2(chunk_full);
+                        if (ends && !low) cafe_mma_commit2(chunk_full);
 #pragma unroll
                         for (int q = 0; q < 5; ++q) {
                             constexpr int ia[5] = {0, 1, 1, 0, 2}, ib[5] = {1, 0, 1, 2, 0};
 #pragma unroll
                             for (int k = 0; k < L::BK / 16; ++k)
-                                cafe_mma2(sums + BN, a + ia[q] * ap + ak * k, b + ib[q] * bp + bk * k, instr, t > 0 || q > 0 || k > 0);
+                                cafe_mma2(sums + BN, a + ia[q] * ap + ak * k, b + ib[q] * bp + bk * k, instr, t % CAFE_TILES_LOW > 0 || q > 0 || k > 0);
                         }
+                        if (low) cafe_mma_commit2(chunk_full);
                     }
                     cafe_mma_commit2(empty(s));
                 }
@@ -713,12 +720,23 @@ __global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) k_tiles_pair(const __gri
                         for (int i = 0; i < 16; ++i) acc[c + i] = first_sums ? v[i] : acc[c + i] + v[i];
                     }
                 };
+                auto join = [&]() {   // the other sums
+#pragma unroll
+                    for (int c = 0; c < Sh::mine; c += 16) {
+                        float v[16];
+                        cafe_tm_load16(from + BN + c, v);
+                        cafe_tm_wait_load();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) acc[c + i] = cafe_join_sums(acc[c + i], v[i]);
+                    }
+                };
                 const int between = turns > 0 ? (turns - 1) / CAFE_TILES_CHUNK : 0;   // chunks that do not end the tile
                 for (int c = 0; c < between && fine; ++c, chunk_phase ^= 1u) {
                     fine = cafe_bar_wait<true>(chunk_full, chunk_phase, &bail);
                     cafe_tc_after();
                     fine = __all_sync(0xffffffffu, fine);
                     if (fine) take(from, c == 0);
+                    if (fine && (c + 1) % CAFE_LIN_LOW == 0) join();
                     cafe_tc_before();
                     __syncwarp();
                     if (lane == 0) cafe_bar_arrive_at(cafe_cluster_map(chunk_taken, 0));
@@ -728,14 +746,7 @@ __global__ void __launch_bounds__(CAFE_PAIR_THREADS, 1) k_tiles_pair(const __gri
                 fine = __all_sync(0xffffffffu, fine);
                 if (fine) {
                     take(from, between == 0);
-#pragma unroll
-                    for (int c = 0; c < Sh::mine; c += 16) {
-                        float v[16];
-                        cafe_tm_load16(from + BN + c, v);
-                        cafe_tm_wait_load();
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) acc[c + i] = cafe_join_sums(acc[c + i], v[i]);
-                    }
+                    join();
                 } else {
 #pragma unroll
                     for (int i = 0; i < Sh::mine; ++i) acc[i] = __uint_as_float(0x7fffffffu);
