@@ -37,6 +37,13 @@ template <> struct CafeTiles<float> { static constexpr int parts = 3, BK = 32, t
 // the others in pieces of 4096 5.0e-7, 7.2e-7 (131 072: 5.8e-7, 7.5e-7; 4096: 3.0e-7, 2.1e-7), where plain fp32 has 4.6e-6, 3.7e-6.  Larger
 // pieces were not measurably faster.
 #define CAFE_TILES_CHUNK 8
+template <typename T> static constexpr int cafe_tiles_chunk() { return CafeTiles<T>::parts == 3 ? CAFE_TILES_CHUNK : 4096 / CafeTiles<T>::BK; }
+// 16 bits: a tile's sums stay in tensor memory to the end, so a block adds over its share of the depth in one go, and what is cut off
+// grows with it: 6.3e-9 (bf16 5.8e-9) of a sum of positive products for each k, in cuBLAS's products as in these.  No block gets more
+// than loses a fifth of what rounding the result may change (2^-11 = 4.9e-4, bf16 3.9e-3): 1.0e-4 and 7.6e-4.  Longer depths are
+// shared by a cluster's blocks, and where eight are not enough (fp16 beyond 131 072) their sums are held in registers and taken out
+// every 4096 of k.
+template <typename T> static constexpr int cafe_tiles_depth() { return sizeof(T) == 4 ? 1 << 30 : CafeTiles<T>::type ? 1 << 17 : 1 << 14; }
 #define CAFE_TILES_LOW (CAFE_TILES_CHUNK * CAFE_LIN_LOW)   // turns between two times that the other sums are
 
 // ---- operands as parts ---------------------------------------------------------------------------------------------------
@@ -142,6 +149,7 @@ template <typename T, int BN> struct CafeTilesShape {
     static constexpr int bytes = (stage * stages > tile ? stage * stages : tile) + 1024;
     static constexpr int tm_cols = L::parts == 3 ? 2 * BN : BN;
 };
+#define CAFE_TILES_ROWS (1 << 20)   // of x that these kernels take
 struct CafeTilesArgs {
     CUtensorMap a, b;
     CafeJob job;
@@ -149,7 +157,8 @@ struct CafeTilesArgs {
     int sum_rows, splits;
 };
 
-template <typename T, int BN>
+// HOLD: the sums are taken out and added in registers on the way (fp32: always; 16 bits: depths too long for tensor memory, BN = 128).
+template <typename T, int BN, bool HOLD>
 __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_constant__ CafeTilesArgs P) {
     typedef CafeTiles<T> L;
     typedef CafeTilesShape<T, BN> Sh;
@@ -184,7 +193,8 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
     cafe_tc_after();
     const uint32_t tmem = tm_at;
 
-    constexpr int taken = L::parts == 3 ? BN : 32;
+    static_assert(HOLD ? BN == 128 : L::parts == 1, "sums held by a thread");
+    constexpr int taken = HOLD ? BN : 32, CHUNK = cafe_tiles_chunk<T>();
     float acc[taken];
     const uint32_t from = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     bool fine = true;
@@ -223,17 +233,17 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
         uint32_t phase = 0, chunk_phase = 1;
         for (int t = 0; t < turns; ++t) {
             if (!(fine = __all_sync(0xffffffffu, cafe_bar_wait(full(s), phase, &bail)))) break;
-            if (L::parts == 3 && in_chunk == 0 && t > 0) {
+            if (HOLD && in_chunk == 0 && t > 0) {
                 if (!(fine = __all_sync(0xffffffffu, cafe_bar_wait(acc_empty, chunk_phase & 1u, &bail)))) break;
             }
             cafe_tc_after();
             const uint64_t a = da + (uint32_t)(s * Sh::stage >> 4), b = db + (uint32_t)(s * Sh::stage >> 4);
-            const bool ends = in_chunk == CAFE_TILES_CHUNK - 1 || t == turns - 1, low = (t + 1) % CAFE_TILES_LOW == 0 && t < turns - 1;
+            const bool ends = in_chunk == CHUNK - 1 || t == turns - 1, low = L::parts == 3 && (t + 1) % CAFE_TILES_LOW == 0 && t < turns - 1;
             if (cafe_elect()) {
 #pragma unroll
                 for (int k = 0; k < L::BK / 16; ++k) cafe_mma(tmem, a + ak * k, b + bk * k, instr, in_chunk > 0 || k > 0);
+                if (HOLD && ends && !low) cafe_mma_commit(acc_full);
                 if constexpr (L::parts == 3) {
-                    if (ends && !low) cafe_mma_commit(acc_full);
 #pragma unroll
                     for (int q = 0; q < 5; ++q) {
                         constexpr int ia[5] = {0, 1, 1, 0, 2}, ib[5] = {1, 0, 1, 2, 0};
@@ -246,7 +256,7 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
                 cafe_mma_commit(empty(s));
             }
             ++in_chunk;
-            if (L::parts == 3 && ends) { in_chunk = 0; ++chunk_phase; }
+            if (HOLD && ends) { in_chunk = 0; ++chunk_phase; }
             if (++s == Sh::stages) { s = 0; phase ^= 1u; }
         }
         __syncwarp();
@@ -269,7 +279,7 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
             }
             __syncwarp();
         }
-        if constexpr (L::parts == 3) {
+        if constexpr (HOLD) {
             auto take = [&](uint32_t at, bool first) {
 #pragma unroll
                 for (int c = 0; c < BN; c += 16) {
@@ -280,7 +290,7 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
                     for (int i = 0; i < 16; ++i) acc[c + i] = first ? v[i] : acc[c + i] + v[i];
                 }
             };
-            auto join = [&]() {   // the other sums
+            auto join = [&]() {   // fp32: the other sums
 #pragma unroll
                 for (int c = 0; c < BN; c += 16) {
                     float v[16];
@@ -290,7 +300,7 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
                     for (int i = 0; i < 16; ++i) acc[c + i] = cafe_join_sums(acc[c + i], v[i]);
                 }
             };
-            const int chunks = (turns + CAFE_TILES_CHUNK - 1) / CAFE_TILES_CHUNK;
+            const int chunks = (turns + CHUNK - 1) / CHUNK;
             if (turns == 0) {
 #pragma unroll
                 for (int i = 0; i < BN; ++i) acc[i] = 0.f;
@@ -300,7 +310,7 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
                 cafe_tc_after();
                 fine = __all_sync(0xffffffffu, fine);
                 if (fine) take(from, c == 0);
-                if (fine && (c + 1) % CAFE_LIN_LOW == 0 && c < chunks - 1) join();
+                if (L::parts == 3 && fine && (c + 1) % CAFE_LIN_LOW == 0 && c < chunks - 1) join();
                 cafe_tc_before();
                 __syncwarp();
                 if (lane == 0) cafe_bar_arrive(acc_empty);
@@ -308,7 +318,7 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
             fine = cafe_bar_wait(all_done, 0, &bail) && fine;
             cafe_tc_after();
             fine = __all_sync(0xffffffffu, fine);
-            if (fine && turns > 0) join();
+            if (L::parts == 3 && fine && turns > 0) join();
         } else {
             fine = cafe_bar_wait(all_done, 0, &bail);
             cafe_tc_after();
@@ -325,7 +335,7 @@ __global__ void __launch_bounds__(CAFE_TILES_THREADS, 2) k_tiles(const __grid_co
             const int r = (warp & 3) * 32 + lane;
             const uint32_t at = base + (uint32_t)(r * 132) * 4u;
             const bool ok = fine && !bail;
-            if constexpr (L::parts == 3) {
+            if constexpr (HOLD) {
                 if (!ok) {
 #pragma unroll
                     for (int i = 0; i < BN; ++i) acc[i] = __uint_as_float(0x7fffffffu);
@@ -876,7 +886,7 @@ static bool tiles_map(CUtensorMap* map, const TilesOperand& o, int kc, int box) 
                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int BN>
+template <typename T, int BN, bool HOLD>
 static cudaError_t tiles_launch_bn(CafeTilesArgs& P, const TilesOperand& a, const TilesOperand& b, cudaStream_t st) {
     // (a bias gradient alone: no columns, no depth, nothing fetched)
     if (P.job.depth > 0 && (!tiles_map<T>(&P.a, a, P.job.a_kc, CAFE_LIN_BM) || !tiles_map<T>(&P.b, b, P.job.b_kc, BN))) return cudaErrorInvalidValue;
@@ -884,9 +894,9 @@ static cudaError_t tiles_launch_bn(CafeTilesArgs& P, const TilesOperand& a, cons
     P.job.tiles = ((P.job.rows + CAFE_LIN_BM - 1) / CAFE_LIN_BM) * P.job.tiles_n;
     constexpr int bytes = CafeTilesShape<T, BN>::bytes;
     static std::atomic<uint64_t> allowed{0};
-    const cudaError_t e = dense_allow_shared((const void*)k_tiles<T, BN>, bytes, &allowed);
+    const cudaError_t e = dense_allow_shared((const void*)k_tiles<T, BN, HOLD>, bytes, &allowed);
     if (e != cudaSuccess) return e;
-    return dense_start<false>(k_tiles<T, BN>, dim3((unsigned)(P.job.tiles * P.splits)), CAFE_TILES_THREADS, bytes, P.splits, st, P);
+    return dense_start<false>(k_tiles<T, BN, HOLD>, dim3((unsigned)(P.job.tiles * P.splits)), CAFE_TILES_THREADS, bytes, P.splits, st, P);
 }
 // One product of a call: its job, its operands, and for gW where the bias gradient's partial sums are
 struct TilesProduct {
@@ -970,6 +980,8 @@ static cudaError_t tiles_launch_pair(TilesProduct* q, int count, const TilesSums
     return dense_start<false>(k_parts_join, dim3((unsigned)(((int64_t)J.rows * P.pitch / 4 + 255) / 256)), 256, 0, 1, st, (const float*)P.partial, P.splits, J.rows,
                               J.cols, P.pitch, (float*)J.out, J.ldo);
 }
+// Whether the sums of a product are held in registers by k_tiles
+template <typename T> static bool tiles_held(int depth) { return CafeTiles<T>::parts == 3 || depth > 8ll * cafe_tiles_depth<T>(); }
 // Pairs of blocks through tile after tile, or two blocks an SM and clusters that share a tile's depth: whichever estimate is less,
 // in turns of a 128 x 128 tile at the tensor cores' full rate.  A pair's turn takes 1.2 (fp32) or, 256 columns wide, 2.7 (16 bits)
 // of these, a tile 3 more and a launch 14; two blocks on an SM share its tensor cores and wait for their boxes, 2.7 (fp32) or 3.3 a
@@ -978,12 +990,14 @@ static cudaError_t tiles_launch_pair(TilesProduct* q, int count, const TilesSums
 // blocks run at a time in clusters of 1, 2, 4 and 8 (what the device says).
 template <typename T> static double tiles_estimate_clusters(const CafeJob& J, int* splits) {
     constexpr bool split = CafeTiles<T>::parts == 3;
-    const int bn = !split && J.cols > 128 ? 256 : 128;
+    const bool hold = tiles_held<T>(J.depth);
+    const int bn = !split && !hold && J.cols > 128 ? 256 : 128;
     const int64_t tiles = (int64_t)((J.rows + CAFE_LIN_BM - 1) / CAFE_LIN_BM) * (J.cols > 0 ? (J.cols + bn - 1) / bn : 1);
     const int turns = (J.depth + CafeTiles<T>::BK - 1) / CafeTiles<T>::BK;
     static const int room[4] = {296, 296, 284, 264};
     double best = 1e300;
     for (int s = 0; s < 4; ++s) {
+        if (!hold && ((turns + (1 << s) - 1) >> s) * (int64_t)CafeTiles<T>::BK > cafe_tiles_depth<T>()) continue;
         const int64_t blocks = tiles << s, rounds = (blocks + room[s] - 1) / room[s];
         const double est = (double)rounds * ((blocks > 148 ? split ? 2.7 : 3.3 : split ? 1.7 : 2.0) * (bn / 128) * ((turns + (1 << s) - 1) >> s) + 14 + s);
         if (est < best * 0.999) { best = est; *splits = 1 << s; }
@@ -995,7 +1009,7 @@ template <typename T> static double tiles_estimate_pairs(const TilesProduct* q, 
     int64_t tiles[2];
     for (int i = 0; i < count; ++i) {
         const CafeJob& J = q[i].job;
-        if (J.depth == 0 || J.cols == 0) return 1e300;
+        if (J.depth == 0 || J.cols == 0 || J.depth > cafe_tiles_depth<T>()) return 1e300;
         const int splits = q[i].splits;
         cost[i] = tiles_pair_cost<T>(J, bn, splits);
         tiles[i] = (int64_t)((J.rows + 255) / 256) * ((J.cols + bn - 1) / bn) * splits;
@@ -1010,10 +1024,11 @@ static cudaError_t tiles_launch_clusters(const TilesProduct& q, int splits, cons
     P.job = q.job;
     P.splits = splits;
     P.sums = sums.at; P.sum_rows = sums.rows;
-    if constexpr (CafeTiles<T>::parts == 1) {
-        if (q.job.cols > 128) return tiles_launch_bn<T, 256>(P, q.a, q.b, st);
+    if constexpr (CafeTiles<T>::parts == 3 || CAFE_TILES_ROWS > 8ll * cafe_tiles_depth<T>()) {   // (no others are that deep)
+        if (tiles_held<T>(q.job.depth)) return tiles_launch_bn<T, 128, true>(P, q.a, q.b, st);
     }
-    return tiles_launch_bn<T, 128>(P, q.a, q.b, st);
+    if constexpr (CafeTiles<T>::parts == 1) return q.job.cols > 128 ? tiles_launch_bn<T, 256, false>(P, q.a, q.b, st) : tiles_launch_bn<T, 128, false>(P, q.a, q.b, st);
+    return cudaErrorNotSupported;
 }
 // `count` products; the partial sums, if any, belong to the first
 template <typename T>
@@ -1093,9 +1108,8 @@ static cudaError_t tiles_parts(const CafeParts& P, cudaStream_t st) {
 // 28 us by this file, 21 by dense_cuda.cu's kernel, backward 45 and 50) that are no narrow strips.
 #define CAFE_TILES_LEAST (1ll << 29)
 #define CAFE_TILES_LEAST_BACK (1ll << 27)
-// (Sums over more than 2^17 of k in one go, 2^20 over the blocks of a cluster, would lose bits of a 16-bit result.)
 static bool tiles_large(int M, int N, int K, int64_t least) {
-    return (int64_t)M * N * K >= least && M >= 128 && N >= 64 && K >= 64 && M <= 1 << 20 && N <= 1 << 17 && K <= 1 << 17;
+    return (int64_t)M * N * K >= least && M >= 128 && N >= 64 && K >= 64 && M <= CAFE_TILES_ROWS && N <= 1 << 17 && K <= 1 << 17;
 }
 
 int64_t cafe_tiles_forward_work(const CafeForward& f, int dtype) {

@@ -66,3 +66,15 @@ def test_16_bit_norms(product, M, N, K, dtype):
     for positive in (True, False):
         _, norm = _error(product, M, N, K, dt, positive)
         assert norm < 1.25 * torch.finfo(dt).eps / 2, (positive, norm)
+
+
+@pytest.mark.parametrize("M,N,K", [(16384, 1024, 2048), (65536, 1024, 2048), (131072, 1024, 2048), (3 << 17, 1024, 512), (1 << 18, 512, 2048), (1 << 20, 256, 256)])
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_16_bit_long_sums_of_one_sign(M, N, K, dtype):
+    """gW over many rows, all products positive: what is cut off adds up, 6.3e-9 of the sum for each row that is added in one go, so that no
+    more than a fifth of what rounding the result may change is lost: 1.0e-4 in fp16, 7.6e-4 in bf16 (and a fifth of that for other
+    values than the comment's).  Beside it the mean of n independent roundings, half a step / sqrt(3 n), 6 standard deviations."""
+    import torch
+    dt = getattr(torch, dtype)
+    mean, _ = _error("gw", M, N, K, dt, True)
+    assert abs(mean) < (1.0e-4 if dtype == "float16" else 7.6e-4) * 1.2 + 6 * torch.finfo(dt).eps / 2 / (3 * 128 * 128) ** 0.5, mean
