@@ -19,6 +19,7 @@ SOURCES = ["sketch_cuda.cu", "embed_cuda.cu", "sigmod_cuda.cu", "interact_cuda.c
 HEADERS = ["cafe_types.h", "cafe_internal.h", "sketch_core.cuh", "sketch_engine.h", "radix_sort.cuh", "cafe_float.cuh", "tcgen05.cuh", "dense.cuh"]
 TORCH_SO = PKG / "_dense_torch.so"
 TORCH_SOURCE = CSRC / "dense_torch.cpp"
+TORCH_RECORD = PKG / "build" / "_dense_torch.built_for"   # what TORCH_SO was built for: it loads with no other torch or python
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
               "--expt-relaxed-constexpr"]
 # the sketch arithmetic must not be contracted into fused multiply-adds: counts are compared bit for bit
@@ -72,8 +73,11 @@ def build(force: bool = False, verbose: bool = False) -> Path:
 
 def build_torch(force: bool = False) -> Path:
     """The extension module cafe_b200._dense_torch (after build(): it is linked against the library)."""
+    from importlib.metadata import version
+    built_for = f"torch {version('torch')}, python {sys.version}"
     deps = [TORCH_SOURCE, PKG.parent / "include" / "cafe_b200.h", Path(__file__)]
-    if not force and TORCH_SO.exists() and all(d.stat().st_mtime <= TORCH_SO.stat().st_mtime for d in deps):
+    if not force and TORCH_SO.exists() and all(d.stat().st_mtime <= TORCH_SO.stat().st_mtime for d in deps) and \
+            TORCH_RECORD.exists() and TORCH_RECORD.read_text() == built_for:
         return TORCH_SO
     import sysconfig
 
@@ -89,6 +93,8 @@ def build_torch(force: bool = False) -> Path:
     r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed on {TORCH_SOURCE.name}:\n{r.stdout}")
+    TORCH_RECORD.parent.mkdir(exist_ok=True)
+    TORCH_RECORD.write_text(built_for)
     return TORCH_SO
 
 
