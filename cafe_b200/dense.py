@@ -2,6 +2,7 @@
 
 fused_linear   y = act(x W^T + b) + residual, differentiable
 fused_mlp      a run of such layers as one node of the autograd graph: one call per direction
+gave_up        whether a bounded wait inside the kernels has ever run out (outputs are then not numbers)
 FusedMLP       the Sequential of Linear and activation modules that the reference's create_mlp builds
                (dlrm_s_pytorch.py:213-251), computed by fused_mlp; same parameters, same state_dict
 
@@ -11,6 +12,9 @@ and calls that a trace (torch.jit.trace, make_fx) records.  Captured into a CUDA
 backward follow torch's rules for whole-network capture (warm-up on a side stream, no autograd graph of the same leaves alive
 from outside the capture)."""
 from __future__ import annotations
+
+import contextlib
+import ctypes
 
 import torch
 import torch.nn as nn
@@ -45,6 +49,16 @@ def fused_mlp(x: torch.Tensor, weights, biases, activations) -> torch.Tensor:
     if None in acts:
         raise ValueError(f"fused_mlp: activations must be among {sorted(ACTIVATIONS)}, got {list(activations)!r}")
     return _dense_torch.mlp(x, list(weights), list(biases), acts)
+
+
+def gave_up(device=None) -> int:
+    """How many of the two kinds of kernel here have, since the library was loaded, ended a wait that ran out on this device (0: none).  Every
+    wait inside them has an end, about a second; what it waited for is then stored as NaN, and this says that the NaN came from
+    there.  Waits for the device; not while a stream of it is being captured."""
+    count = ctypes.c_int32(0)
+    with torch.cuda.device(device) if device is not None else contextlib.nullcontext():
+        _lib.check(_lib.load().cafe_linear_gave_up(ctypes.byref(count)), "cafe_linear_gave_up")
+    return count.value
 
 
 _MODULES = {nn.ReLU: "relu", nn.Sigmoid: "sigmoid", nn.SiLU: "silu", nn.Identity: "none"}

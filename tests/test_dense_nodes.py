@@ -68,3 +68,22 @@ def test_layers_with_hooks_are_refused():
     with pytest.raises(ValueError, match="CUDA"):
         net(torch.zeros(2, 4))
     assert seen == [1]
+
+
+def test_waits_that_ran_out_are_told(monkeypatch):
+    """What the library counts reaches the caller, and so does its error."""
+    import types
+    import pytest
+    from cafe_b200 import CafeError, dense
+
+    def library(status, kinds):
+        def gave_up(count):
+            count._obj.value = kinds
+            return status
+        return types.SimpleNamespace(cafe_linear_gave_up=gave_up, cafe_last_error=lambda: b"no device")
+    for kinds in (0, 1, 2):
+        monkeypatch.setattr(dense._lib, "load", lambda: library(0, kinds))
+        assert dense.gave_up() == kinds
+    monkeypatch.setattr(dense._lib, "load", lambda: library(dense._lib.ERR_CUDA, 0))
+    with pytest.raises(CafeError):
+        dense.gave_up()
