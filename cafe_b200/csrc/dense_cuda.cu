@@ -923,7 +923,9 @@ int cafe_mlp_backward(int layers, const int* widths, int M, const void* gy_dev, 
     if (!dense_work_ok(work_dev, work_bytes)) return CAFE_ERR_ARG;
     char* const half[2] = {(char*)work_dev, (char*)work_dev + half_bytes};
     CafeBackward f[CAFE_MLP_MAX_LAYERS];
-    for (int l = layers - 1; l >= 0; --l) {
+    int first = gx_dev ? 0 : layers;   // the lowest layer that a gradient is wanted of: below it nothing is computed
+    for (int l = layers - 1; l >= 0; --l) if (gw_dev[l] || gb_dev[l]) first = l < first ? l : first;
+    for (int l = layers - 1; l >= first; --l) {
         const bool last = l == layers - 1;
         const bool plain = acts[l] == CAFE_ACT_NONE || M == 0 || widths[l + 1] == 0;   // (a layer without outputs has no slope either)
         const int kind = plain ? CAFE_SLOPE_NONE : slope_dev && slope_dev[l] ? CAFE_SLOPE_VALUES : CAFE_SLOPE_OUTPUT;
@@ -931,11 +933,11 @@ int cafe_mlp_backward(int layers, const int* widths, int M, const void* gy_dev, 
         const int64_t ldn = (widths[l + 1] + 7) & ~7, ldk = (widths[l] + 7) & ~7;
         f[l] = {last ? gy_dev : half[l & 1], kind == CAFE_SLOPE_VALUES ? slope_dev[l] : y_dev[l], l ? y_dev[l - 1] : x_dev, w_dev[l],
                 last ? ldg : ldn, ldy[l], l ? ldy[l - 1] : ldx, ldw[l], kind, M, widths[l + 1], widths[l],
-                l ? half[(l - 1) & 1] : gx_dev, gw_dev[l], gb_dev[l], l ? ldk : ldgx, widths[l]};
+                l > first ? half[(l - 1) & 1] : l ? nullptr : gx_dev, gw_dev[l], gb_dev[l], l ? ldk : ldgx, widths[l]};
         if (!dense_backward_ok(f[l])) return CAFE_ERR_ARG;
     }
     cudaError_t e = cudaSuccess;
-    for (int l = layers - 1; l >= 0 && e == cudaSuccess; --l)
+    for (int l = layers - 1; l >= first && e == cudaSuccess; --l)
         DENSE_TYPED(dtype, e = dense_backward<T>(f[l], dtype, half[1] + half_bytes, work_bytes - 2 * half_bytes, (cudaStream_t)stream));
     return dense_done(e);
 }

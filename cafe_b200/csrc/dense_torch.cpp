@@ -219,14 +219,17 @@ struct Weights {
     std::vector<const void*> p;
     std::vector<int64_t> ld;
     void add(const Tensor& w) {
-        const Rows r(w, w.size(1));
+        const Rows r = w.defined() ? Rows(w, w.size(1)) : Rows();
         t.push_back(r.t); p.push_back(r.ptr()); ld.push_back(r.ld);
     }
 };
 
 struct MlpNode : Node {
-    SavedVariable x, y, between;   // y: where the last layer is a ReLU, whose derivative it tells
+    // y: where the last layer is a ReLU, whose derivative it tells; x and each of w: where a gradient that can be asked for needs it
+    SavedVariable x, y, between;
     std::vector<SavedVariable> w;
+    std::vector<bool> has_w;
+    bool has_x = false;
     Plan plan;
     int64_t m = 0;
     std::vector<int64_t> shape;
@@ -250,9 +253,9 @@ struct MlpNode : Node {
             const auto self = shared_from_this();
             at::NoGradGuard plain_values;
             const c10::cuda::CUDAGuard device(gy.device());
-            const Rows g(gy, plan.widths[n], true), xs(x.unpack(self), plan.widths[0]);
+            const Rows g(gy, plan.widths[n], true), xs = has_x ? Rows(x.unpack(self), plan.widths[0]) : Rows();
             Weights ws;
-            for (SavedVariable& v : w) ws.add(v.unpack(self));
+            for (int l = 0; l < n; ++l) ws.add(has_w[l] ? w[l].unpack(self) : Tensor());
             const Tensor held = between.unpack(self).contiguous(), ys = plan.acts[n - 1] == CAFE_ACT_RELU ? y.unpack(self).contiguous() : Tensor();
             std::vector<void*> gw(n, nullptr), gb(n, nullptr);
             if (task_should_compute_output(0)) result[0] = at::empty(shape, gy.options());
@@ -334,9 +337,15 @@ Tensor mlp(const Tensor& x, const std::vector<Tensor>& w, const std::vector<Mayb
             node->plan = plan;
             node->m = xs.m;
             node->shape.assign(x.sizes().begin(), x.sizes().end());
-            node->x = SavedVariable(xs.t, false);
             node->between = SavedVariable(between, false);
-            for (const Tensor& v : ws.t) node->w.emplace_back(v, false);
+            node->has_x = w[0].requires_grad();
+            if (node->has_x) node->x = SavedVariable(xs.t, false);
+            bool below = x.requires_grad();   // (a layer's weight carries the gradient on to what lies below it)
+            for (int l = 0; l < n; ++l) {
+                node->has_w.push_back(below);
+                node->w.push_back(below ? SavedVariable(ws.t[l], false) : SavedVariable());
+                below |= w[l].requires_grad() || (b[l] && b[l]->requires_grad());
+            }
         }
     }
     if (grad) {

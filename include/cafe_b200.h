@@ -364,7 +364,8 @@ int cafe_mlp_forward(int layers, const int* widths, int M, const void* x_dev, in
 int64_t cafe_mlp_forward_work(int layers, const int* widths, int M, const void* x_dev, int64_t ldx, const void* const* w_dev, const int64_t* ldw, int dtype);
 /* Its backward: a layer without slope_dev[l] has no activation or a ReLU (taken from y_dev[l]; the last layer's y is read for that
  * alone and may be null otherwise).  gw_dev[l] is [widths[l + 1], widths[l]] contiguous; gx_dev, gw_dev[l] and gb_dev[l] may be
- * null.  work_dev also holds the gradients between the layers (two of M x the widest of them): less than that is refused. */
+ * null, and so may x_dev and w_dev[l] where no gradient that is wanted needs them.  work_dev also holds the gradients between the
+ * layers (two of M x the widest of them): less than that is refused. */
 int64_t cafe_mlp_backward_work(int layers, const int* widths, int M, const void* gy_dev, int64_t ldg, const void* x_dev, int64_t ldx,
                                const void* const* w_dev, const int64_t* ldw, int dtype);
 int cafe_mlp_backward(int layers, const int* widths, int M, const void* gy_dev, int64_t ldg, const void* x_dev, int64_t ldx,

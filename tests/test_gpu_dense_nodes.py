@@ -131,3 +131,48 @@ print("fine")
 """
     r = subprocess.run([sys.executable, "-c", program], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True, timeout=300)
     assert r.stdout.strip() == "fine", r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("M,widths", [(40, [30, 20, 10]), (70, [33, 40, 5]), (700, [300, 400, 600])])
+def test_what_an_mlp_keeps(M, widths):
+    """Whichever gradients are wanted, they are right, and the same tensors may be written to before the backward as with the layers one
+    by one: a weight whose input needs no gradient is not needed, nor x where the first weight is frozen."""
+    import itertools
+    import torch
+    from cafe_b200 import fused_mlp
+    g = torch.Generator(device="cuda").manual_seed(9)
+    r = lambda *s: torch.randn(s, device="cuda", generator=g) * 0.2   # noqa: E731
+    values = [r(M, widths[0]), r(widths[1], widths[0]), r(widths[1]), r(widths[2], widths[1]), r(widths[2])]
+    gy = r(M, widths[2])
+    act = torch.nn.functional.silu
+
+    def fused(x, w0, b0, w1, b1):
+        return fused_mlp(x, [w0, w1], [b0, b1], ["silu", "none"])
+
+    def stock(x, w0, b0, w1, b1):
+        return act(x @ w0.t() + b0) @ w1.t() + b1
+    for wanted in itertools.product((False, True), repeat=5):
+        if not any(wanted):
+            continue
+        grads = []
+        for f in (fused, stock):
+            leaves = [v.double() if f is stock else v.clone() for v in values]
+            leaves = [v.requires_grad_(n) for v, n in zip(leaves, wanted)]
+            grads.append(torch.autograd.grad(f(*leaves), [v for v in leaves if v.requires_grad], gy.to(leaves[0].dtype)))
+        for a, e in zip(*grads):
+            # (norms: one layer's sums and evaluations are a few units of 2^-23 each)
+            assert float((a.double() - e).norm() / e.norm()) < 1e-5, wanted
+        for changed in range(5):
+            raised = []
+            for f in (fused, stock):
+                leaves = [v.clone().requires_grad_(n) for v, n in zip(values, wanted)]
+                y = f(*leaves)
+                with torch.no_grad():
+                    leaves[changed].mul_(2)
+                try:
+                    y.backward(gy)
+                    raised.append(False)
+                except RuntimeError as e:
+                    assert "inplace" in str(e)
+                    raised.append(True)
+            assert raised[0] == raised[1], (wanted, changed, raised)
