@@ -141,6 +141,9 @@ class AdamW(torch.optim.Optimizer):
             if ticket is None:
                 ticket = self._ticket[device] = torch.zeros(1, dtype=torch.int32, device=device)
             m, v, *tops = ([s[name] for s in states] for name in names)
+            for s in states if tops else ():
+                if s["layout"].is_cuda:   # (moved there with the rest of a state)
+                    s["layout"] = s["layout"].cpu()
             _dense_torch.adamw_step(params, grads, m, v, *(tops or ([], [])), [s["layout"] for s in states] if tops else [],
                                     [s["step"] for s in states], numbers, group["lr"], *group["betas"], group["eps"], group["weight_decay"],
                                     self.seed, ticket)
@@ -159,6 +162,8 @@ class AdamW(torch.optim.Optimizer):
         out = {}
         for ps in by_device.values():
             states = [self.state[p] for p in ps]
+            for s in states:
+                s["layout"] = s["layout"].cpu()
             out.update(zip(ps, _dense_torch.adamw_moments(ps, *([s[name] for s in states] for name in (*_CODES, "layout")))))
         return [out[p] for p in params]
 

@@ -142,3 +142,29 @@ def test_gradients_and_states_of_another_size_are_refused(bits):
         assert torch.equal(p, before)
         opt.step()
         assert not torch.equal(p, before)
+
+
+def test_states_that_a_trainer_moves():
+    """Loops that move every tensor of a state to the parameter's device take the layouts along."""
+    import torch
+    p, opt = _fresh((40, 30), 8)
+    q, other = _fresh((40, 30), 8)
+    for s in opt.state.values():
+        for k, t in s.items():
+            s[k] = t.cuda()
+    assert torch.equal(opt.moments()[0][0], other.moments()[0][0])
+    for s in opt.state.values():
+        for k, t in s.items():
+            s[k] = t.cuda()
+    p.grad = torch.randn_like(p)
+    q.grad = p.grad.clone()
+    opt.step()
+    other.step()
+    assert torch.equal(p, q)
+    for size in ((0, 3), ()):            # nothing, and a number
+        e = torch.nn.Parameter(torch.ones(size, device="cuda"))
+        e.grad = torch.ones(size, device="cuda")
+        opt = type(opt)([e], state_bits=8)
+        opt.step()
+        opt.step()
+        assert int(opt.state[e]["step"]) == 2 and opt.moments()[0][0].shape == e.shape

@@ -176,3 +176,13 @@ def test_what_an_mlp_keeps(M, widths):
                     assert "inplace" in str(e)
                     raised.append(True)
             assert raised[0] == raised[1], (wanted, changed, raised)
+
+
+def test_tensors_without_memory_are_refused():
+    import torch
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from cafe_b200 import fused_linear
+    with FakeTensorMode():
+        x, w = torch.empty(4, 8, device="cuda"), torch.empty(5, 8, device="cuda")
+        with pytest.raises(RuntimeError):
+            fused_linear(x, w)
