@@ -49,6 +49,8 @@ struct CafeAdamwScalars {
     int* ticket;
 };
 
+// A bijection of 32 bits: xorshifts by 16, 15, 16 between two odd multipliers, which Christopher Wellons found by searching for the least
+// bias ("Prospecting for Hash Functions", nullprogram.com, 2018).
 __device__ __forceinline__ uint32_t cafe_mix32(uint32_t x) {
     x ^= x >> 16; x *= 0x7FEB352Du; x ^= x >> 15; x *= 0x846CA68Bu; x ^= x >> 16;
     return x;

@@ -483,8 +483,7 @@ __device__ __forceinline__ void cafe_row_end(const CafeJob& J, float* z, int64_t
 #pragma unroll
         for (int p = 0; p < 16; p += slope_each) {
             alignas(16) ST x[slope_each];
-#pragma unroll
-            for (int q = 0; q < slope_each; ++q) x[q] = cafe_from_float<ST>(d[p + q]);
+            cafe_slopes<slope_each>(d + p, x);
             const uint4 y = *reinterpret_cast<const uint4*>(x);
             cafe_put16(cafe_staged<SLOPE_ROW>(slopes, r, (c + p) / slope_each), y.x, y.y, y.z, y.w);
         }
