@@ -27,6 +27,14 @@ def _layout(p: torch.Tensor) -> torch.Tensor:
     return torch.tensor([tuple(p.shape), tuple(p.stride())], dtype=torch.int64)
 
 
+def _layouts(states) -> list:
+    found = [s["layout"] for s in states]
+    for i, t in enumerate(found):
+        if t.is_cuda:   # (moved there with the rest of a state)
+            found[i] = states[i]["layout"] = t.cpu()
+    return found
+
+
 def _order(layout):
     """What two layouts whose elements come in the same order have in common: None if row-major, else their axes."""
     sizes, strides = layout.tolist()
@@ -141,10 +149,7 @@ class AdamW(torch.optim.Optimizer):
             if ticket is None:
                 ticket = self._ticket[device] = torch.zeros(1, dtype=torch.int32, device=device)
             m, v, *tops = ([s[name] for s in states] for name in names)
-            for s in states if tops else ():
-                if s["layout"].is_cuda:   # (moved there with the rest of a state)
-                    s["layout"] = s["layout"].cpu()
-            _dense_torch.adamw_step(params, grads, m, v, *(tops or ([], [])), [s["layout"] for s in states] if tops else [],
+            _dense_torch.adamw_step(params, grads, m, v, *(tops or ([], [])), _layouts(states) if tops else [],
                                     [s["step"] for s in states], numbers, group["lr"], *group["betas"], group["eps"], group["weight_decay"],
                                     self.seed, ticket)
         return loss
@@ -162,9 +167,7 @@ class AdamW(torch.optim.Optimizer):
         out = {}
         for ps in by_device.values():
             states = [self.state[p] for p in ps]
-            for s in states:
-                s["layout"] = s["layout"].cpu()
-            out.update(zip(ps, _dense_torch.adamw_moments(ps, *([s[name] for s in states] for name in (*_CODES, "layout")))))
+            out.update(zip(ps, _dense_torch.adamw_moments(ps, *([s[name] for s in states] for name in _CODES), _layouts(states))))
         return [out[p] for p in params]
 
     def state_dict(self):
