@@ -9,7 +9,8 @@
 //
 // k_tiles: a block makes 128 x BN outputs; one thread fetches, one issues products, four warps take the sums out (and meanwhile
 // add up the bias gradient).  Two blocks share an SM, so that one's end runs beside the other's products; two stages of 48 KB
-// each.  Blocks of a cluster share the depth of a tile as in dense_cuda.cu.
+// each.  Held sums leave 40 of a thread's 168 registers for the rest: 492 bytes of spill stores and 352 of loads in fp32, 172 and 112 in
+// fp16; k_tiles_pair in fp32 48 and 116.  Blocks of a cluster share the depth of a tile as in dense_cuda.cu.
 #include <cuda.h>
 
 #include "dense.cuh"
@@ -915,7 +916,9 @@ template <typename T> static double tiles_pair_cost(const CafeJob& J, int bn, in
 }
 // Parts of the depth of a product that has so few tiles that clusters of eight blocks each leave SMs idle (gW of a narrow layer): two
 // rounds of all pairs, each part at least 32 turns and none empty.  fp32.  Backward of 47373x572x175 425 us without, 345 with;
-// 30000x256x256 212, 148; 4096x352x1024 (12 tiles) 79, 73; but 65536x479x1024 (16) 892, 962.
+// 30000x256x256 212, 148; 4096x352x1024 (12 tiles) 79, 73; but 65536x479x1024 (16) 892, 962.  From 13 to 20 tiles at 2048 to 65 536 rows there
+// is no rule: without and with, 15 tiles (768x640) 62, 42 at 2048 and 222, 219 at 16 384; 16 (1024x512) 61, 56 and 228, 290; 20
+// (1024x640) 45, 69 and 292, 283.
 static int tiles_splits(int rows, int cols, int depth) {
     const int64_t tiles = (int64_t)((rows + 255) / 256) * ((cols + 127) / 128), turns = (depth + 31) / 32;
     if (tiles > 12) return 1;

@@ -104,7 +104,7 @@ __device__ __forceinline__ void cafe_mma_commit2(uint32_t bar) {
 }
 
 // An arrival at another block's barrier that tells of tensor memory having been read (cafe_bar_try's CLUSTER says what orders it; a
-// release of the cluster's scope would wait for this thread's own stores, thousands of cycles).
+// release of the cluster's scope costs a fence each time: one for every box took 16384x1024x4096 in bf16 from 106 to 240 us).
 __device__ __forceinline__ void cafe_bar_arrive_at(uint32_t cluster_bar) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory"); }
 
 __device__ __forceinline__ uint32_t cafe_cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
