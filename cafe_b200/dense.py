@@ -91,7 +91,6 @@ class FusedMLP(nn.Sequential):
     def _plan(self):
         linears, acts = [], []
         for m in self._modules.values():
-            _check_plain(m)
             if type(m) is nn.Linear:
                 linears.append(m)
                 acts.append(None)
@@ -99,6 +98,7 @@ class FusedMLP(nn.Sequential):
                 raise ValueError("FusedMLP: every activation follows a Linear layer")
             else:
                 acts[-1] = _module_activation(m)
+            _check_plain(m)
         return linears, [a or "none" for a in acts]
 
     def forward(self, x):
