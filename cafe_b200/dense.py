@@ -35,7 +35,9 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     """act(x W^T + b) + residual.  x [..., K], weight [N, K], bias [N]; residual broadcasts to [..., N]; activation is one of
     none, relu, sigmoid, gelu (with erf) and silu.  x, weight and residual may be slices of wider tensors (any pitch
     between rows).  For the backward the call keeps x, weight and, with an activation, its derivative (16 bits beside bf16, with
-    the range of bf16, else fp32); of a ReLU without residual the output."""
+    the range of bf16, else fp32); of a ReLU without residual the output.  In
+    16 bits the gradient of the pre-activation is rounded to the tensors' type before its two products, as by torch's own layers (in
+    fp16 it overflows with a gradient above 58 000 where a GELU's or SiLU's derivative is above 1)."""
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"fused_linear: activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
